@@ -31,6 +31,10 @@ CFLAGS = [
     # no implicit a*b+c -> fma: elementwise stages round like the reference's
     # separate torch ops; fused multiply-adds are written as fmaf explicitly
     "-ffp-contract=off",
+    # no packed fp32 instructions (v_pk_add / mul / fma_f32): the compiler forms
+    # them by itself from scalar float code, and some forms have given wrong
+    # results on this GPU; the rounding of the scalar forms is the same
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
     "-Wno-unused-function",
     f"-I{ROOT / 'include'}",
