@@ -515,6 +515,31 @@ class IqnHeadBwdFusedDesc(C.Structure):
 
 
 # name -> (restype, argtypes)
+class GatedMlpDesc(C.Structure):
+    _fields_ = (
+        [(f, vp) for f in ("x", "Wg", "Wu", "Wd", "bg", "bu", "bd", "y", "g", "u", "dy",
+                           "dx", "dWg", "dWu", "dWd", "dbg", "dbu", "dbd")]
+        + [(f, C.c_int64) for f in ("rows", "n_in", "n_hidden", "n_out", "members", "ldx", "sx",
+                                    "ldWg", "sWg", "ldWu", "sWu", "ldWd", "sWd", "lddy", "sdy")]
+        + [("dtype", C.c_int32), ("act", C.c_int32), ("ws", vp), ("ws_bytes", C.c_int64)])
+
+
+class LinearXentDesc(C.Structure):
+    _fields_ = (
+        [(f, vp) for f in ("x", "W", "b", "target", "loss", "lse", "out", "scale", "gloss",
+                           "dx", "dW", "db")]
+        + [(f, C.c_int64) for f in ("rows", "n_in", "vocab", "ldx", "ldW", "ignore_index")]
+        + [("dtype", C.c_int32), ("reduction", C.c_int32), ("ws", vp), ("ws_bytes", C.c_int64)])
+
+
+class LayerNormDesc(C.Structure):
+    _fields_ = (
+        [(f, vp) for f in ("x", "w", "b", "y", "mean", "rstd", "dy", "dx", "dw", "db")]
+        + [(f, C.c_int64) for f in ("rows", "n", "members", "ldx", "sx", "lddy", "sdy")]
+        + [("eps", C.c_double), ("dtype", C.c_int32), ("wtype", C.c_int32), ("ws", vp),
+           ("ws_bytes", C.c_int64)])
+
+
 _SIGNATURES = {
     "d3a_abi_version": (C.c_int, []),
     "d3a_last_error": (C.c_char_p, []),
@@ -618,6 +643,15 @@ _SIGNATURES = {
     "d3a_td3bc_actor_input": (C.c_int, [C.POINTER(Td3bcActorDesc), vp]),
     "d3a_td3bc_actor_seed": (C.c_int, [C.POINTER(Td3bcActorDesc), vp]),
     "d3a_td3bc_actor_head": (C.c_int, [C.POINTER(Td3bcActorDesc), vp]),
+    "d3a_gated_mlp_workspace": (C.c_int, [C.POINTER(GatedMlpDesc), C.c_int32, C.POINTER(C.c_int64)]),
+    "d3a_gated_mlp": (C.c_int, [C.POINTER(GatedMlpDesc), vp]),
+    "d3a_gated_mlp_bwd": (C.c_int, [C.POINTER(GatedMlpDesc), vp]),
+    "d3a_linear_xent_workspace": (C.c_int, [C.POINTER(LinearXentDesc), C.c_int32, C.POINTER(C.c_int64)]),
+    "d3a_linear_xent": (C.c_int, [C.POINTER(LinearXentDesc), vp]),
+    "d3a_linear_xent_bwd": (C.c_int, [C.POINTER(LinearXentDesc), vp]),
+    "d3a_layer_norm_workspace": (C.c_int, [C.POINTER(LayerNormDesc), C.c_int32, C.POINTER(C.c_int64)]),
+    "d3a_layer_norm": (C.c_int, [C.POINTER(LayerNormDesc), vp]),
+    "d3a_layer_norm_bwd": (C.c_int, [C.POINTER(LayerNormDesc), vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,295 @@
+// The gated feed-forward block, forward and backward, of every ensemble member:
+//
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) * u,  y = h Wd^T + bd
+//   dh = dy Wd,  dg = dh * u * act'(g),  du = dh * act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
+//
+// All six products are tiles of mm.hpp, bound by the matrix cores for many
+// rows.  The first forward launch stages gate and up weights as one B tile
+// whose waves hold the same 32 columns of both, so activation and product
+// happen on the accumulators; the backward's first launch forms dh and, from
+// the kept g and u, dg, du and h in its epilogue.  Kept between the two: g and
+// u in the tensors' type (their rounding to bfloat16 is no coarser than that of
+// the products' own bfloat16 operands dg, du and h).
+#include "mm_host.hpp"
+#include "../../include/d3rlpy_amd.h"
+
+namespace d3a {
+namespace {
+
+using namespace mm;
+
+// act(g) and act'(g)
+template <bool FAST>
+__device__ __forceinline__ void activation(int act, float g, float& a, float& da) {
+  if (act == D3A_ACT_RELU) {
+    a = fmaxf(g, 0.f);
+    if (g != g) a = g;
+    da = g > 0.f ? 1.f : 0.f;
+  } else if (act == D3A_ACT_GELU) {
+    const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    a = g * cdf;
+    da = cdf + g * (FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g)) * 0.3989422804014327f;
+  } else {
+    const float e = FAST ? __expf(-g) : expf(-g);
+    const float s = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+    a = g * s;
+    da = s * (1.f + g * (1.f - s));
+  }
+}
+
+template <class T, int NP>
+struct GatedEpi {
+  T *g, *u;        // kept pre-activations, [batch][M] rows of ld, or null
+  __bf16* h;       // planes [NP][batch][M] rows of ld
+  int64_t ld, s_part;
+  const T *bg, *bu;
+  int64_t s_bias;
+  int32_t act;
+
+  template <class C>
+  __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
+    each4<C, 0, 1>(acc, t, [&](int m, int n, float* v, int i, int, int q) {
+      if (n >= ld) return;
+      float up[4], h4[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        up[r] = acc[i][1][4 * q + r];
+        if (bg) v[r] += (float)bg[t.batch * s_bias + min(n + r, t.N - 1)];
+        if (bu) up[r] += (float)bu[t.batch * s_bias + min(n + r, t.N - 1)];
+        float a, da;
+        activation<NP == 1>(act, v[r], a, da);
+        h4[r] = n + r < t.N ? a * up[r] : 0.f;
+      }
+      const int64_t at = ((int64_t)t.batch * t.M + m) * ld + n;
+      if (g) {
+        store4(g + at, v);
+        store4(u + at, up);
+      }
+      store_planes<NP>(h + at, s_part, h4);
+    });
+  }
+};
+
+template <class T, int NP>
+struct GatedBwdEpi {
+  const T *g, *u;
+  __bf16 *dg, *du, *h;  // planes, rows of ld
+  int64_t ld, s_part;
+  int32_t act;
+
+  template <class C>
+  __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
+    each4<C>(acc, t, [&](int m, int n, float* v, int, int, int) {
+      if (n >= ld) return;
+      const int64_t at = ((int64_t)t.batch * t.M + m) * ld + n;
+      float g4[4], u4[4], h4[4];
+      load4(g + at, g4);
+      load4(u + at, u4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float a, da;
+        activation<NP == 1>(act, g4[r], a, da);
+        const bool on = n + r < t.N;
+        h4[r] = on ? a * u4[r] : 0.f;
+        g4[r] = on ? v[r] * u4[r] * da : 0.f;
+        u4[r] = on ? v[r] * a : 0.f;
+      }
+      store_planes<NP>(dg + at, s_part, g4);
+      store_planes<NP>(du + at, s_part, u4);
+      store_planes<NP>(h + at, s_part, h4);
+    });
+  }
+};
+
+int check(const d3a_gated_mlp_desc* d, bool bwd) {
+  D3A_CHECK_ARG(d, "gated_mlp: null descriptor");
+  D3A_CHECK_ARG(d->dtype == D3A_F32 || d->dtype == D3A_BF16, "gated_mlp: dtype must be float32 or bfloat16");
+  D3A_CHECK_ARG(d->act >= D3A_ACT_SILU && d->act <= D3A_ACT_RELU, "gated_mlp: unknown activation");
+  D3A_CHECK_ARG(d->rows >= 0 && d->members >= 1 && d->n_in >= 1 && d->n_hidden >= 1 && d->n_out >= 1,
+                "gated_mlp: sizes must be positive");
+  const int64_t top = (1LL << 31) - 4096;
+  D3A_CHECK_ARG(d->rows < top && d->n_in < top && d->n_hidden < top && d->n_out < top &&
+                    d->members <= 65535,
+                "gated_mlp: size too large");
+  D3A_CHECK_ARG(d->ldx >= d->n_in && d->ldWg >= d->n_in && d->ldWu >= d->n_in && d->ldWd >= d->n_hidden,
+                "gated_mlp: row stride smaller than the row");
+  D3A_CHECK_ARG(d->Wg && d->Wu && d->Wd, "gated_mlp: null weight");
+  if (d->rows > 0) D3A_CHECK_ARG(d->x && (bwd ? d->dy != nullptr : d->y != nullptr), "gated_mlp: null operand");
+  D3A_CHECK_ARG((d->g == nullptr) == (d->u == nullptr), "gated_mlp: g and u go together");
+  const uintptr_t kept = reinterpret_cast<uintptr_t>(d->g) | reinterpret_cast<uintptr_t>(d->u);
+  D3A_CHECK_ARG((kept & 15) == 0, "gated_mlp: g and u must be 16-byte aligned");
+  if (bwd) {
+    D3A_CHECK_ARG(d->g || d->rows == 0, "gated_mlp: the backward needs the forward's g and u");
+    D3A_CHECK_ARG(d->lddy >= d->n_out, "gated_mlp: row stride smaller than the row");
+  }
+  return 0;
+}
+
+// run (stream given) or measure (ws null): the same walk over the workspace
+template <class T, int NP>
+int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
+  Packer<T, NP> pack(ws);
+  const Operand x = pack.operand(d.x, d.ldx, C > 1 ? d.sx : 0, C, R, D);
+  const bool apart = d.ldWg != d.ldWu || (C > 1 && d.sWg != d.sWu) ||
+                     (reinterpret_cast<uintptr_t>(d.Wg) & 15) || (reinterpret_cast<uintptr_t>(d.Wu) & 15);
+  const Operand wg = pack.operand(d.Wg, d.ldWg, C > 1 ? d.sWg : 0, C, F, D, apart);
+  const Operand wu = pack.operand(d.Wu, d.ldWu, C > 1 ? d.sWu : 0, C, F, D, apart);
+  const Operand wd = pack.operand(d.Wd, d.ldWd, C > 1 ? d.sWd : 0, C, O, F);
+  Operand h{};
+  h.p = ws.take<__bf16>(NP * C * R * F8);
+  h.ld = F8;
+  h.s_batch = R * F8;
+  h.s_part = C * R * F8;
+
+  Launch<GatedEpi<T, NP>> L{};
+  L.n = 1;
+  Problem& p = L.p[0];
+  p.a = x;
+  p.b = wg;
+  p.b2 = wu.p;
+  p.M = (int32_t)R;
+  p.N = (int32_t)F;
+  p.K = (int32_t)D;
+  p.batch = (int32_t)C;
+  p.n_outer = p.n_inner = p.splits = 1;
+  GatedEpi<T, NP>& e = L.e[0];
+  e.g = static_cast<T*>(d.g);
+  e.u = static_cast<T*>(d.u);
+  e.h = const_cast<__bf16*>(h.p);
+  e.ld = F8;
+  e.s_part = h.s_part;
+  e.bg = static_cast<const T*>(d.bg);
+  e.bu = static_cast<const T*>(d.bu);
+  e.s_bias = F;
+  e.act = d.act;
+
+  Products<T, NP> down;
+  down.add(h, wd, R, O, F, C, 1, 1, d.y, O, R * O, d.bd, O);
+  down.reserve(ws, d.bd == nullptr);
+  *bytes = ws.used;
+  if (dry || R == 0) return 0;
+  if (pack.launch(stream) != 0) return -1;
+  if (run<NP, false, false, true>(L, choose<NP>(L, true), stream, "gated_mlp") != 0) return -1;
+  return down.template launch<false, false>(stream, "gated_mlp");
+}
+
+template <class T, int NP>
+int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
+  const bool hidden = d.dx || d.dWg || d.dWu || d.dWd || d.dbg || d.dbu;
+  Packer<T, NP> pack(ws);
+  Operand dy{}, x{}, wd{}, wg{}, wu{};
+  if (hidden) {
+    dy = pack.operand(d.dy, d.lddy, C > 1 ? d.sdy : 0, C, R, O);
+    wd = pack.operand(d.Wd, d.ldWd, C > 1 ? d.sWd : 0, C, O, F);
+  }
+  if (d.dWg || d.dWu) x = pack.operand(d.x, d.ldx, C > 1 ? d.sx : 0, C, R, D);
+  if (d.dx) {
+    const bool apart = d.ldWg != d.ldWu || (C > 1 && d.sWg != d.sWu) ||
+                       (reinterpret_cast<uintptr_t>(d.Wg) & 15) || (reinterpret_cast<uintptr_t>(d.Wu) & 15);
+    wg = pack.operand(d.Wg, d.ldWg, C > 1 ? d.sWg : 0, C, F, D, apart);
+    wu = pack.operand(d.Wu, d.ldWu, C > 1 ? d.sWu : 0, C, F, D, apart);
+  }
+  const int64_t plane = C * R * F8;
+  Operand dg{};
+  dg.p = hidden ? ws.take<__bf16>(3 * NP * plane) : nullptr;  // dg, du, h
+  dg.ld = F8;
+  dg.s_batch = R * F8;
+  dg.s_part = plane;
+  Operand du = dg, h = dg;
+  du.p += NP * plane;
+  h.p += 2 * NP * plane;
+
+  Launch<GatedBwdEpi<T, NP>> L{};
+  L.n = 1;
+  Problem& p = L.p[0];
+  p.a = dy;
+  p.b = wd;
+  p.M = (int32_t)R;
+  p.N = (int32_t)F;
+  p.K = (int32_t)O;
+  p.batch = (int32_t)C;
+  p.n_outer = p.n_inner = p.splits = 1;
+  GatedBwdEpi<T, NP>& e = L.e[0];
+  e.g = static_cast<const T*>(d.g);
+  e.u = static_cast<const T*>(d.u);
+  e.dg = const_cast<__bf16*>(dg.p);
+  e.du = const_cast<__bf16*>(du.p);
+  e.h = const_cast<__bf16*>(h.p);
+  e.ld = F8;
+  e.s_part = plane;
+  e.act = d.act;
+
+  Products<T, NP> dx, dw;
+  if (d.dx) {
+    // K runs over the gate's and the up's hidden units (and, for an x that the
+    // members share, over the members)
+    Operand a = dg, b = wg;
+    a.s_inner = du.p - dg.p;
+    b.s_inner = reinterpret_cast<const __bf16*>(wu.p) - wg.p;
+    const bool shared = C > 1 && d.sx == 0;
+    if (shared) {
+      a.s_outer = a.s_batch;
+      b.s_outer = b.s_batch;
+      a.s_batch = b.s_batch = 0;
+    }
+    dx.add(a, b, R, D, F, shared ? 1 : C, shared ? C : 1, 2, d.dx, D, shared ? 0 : R * D, nullptr, 0);
+    dx.reserve(ws, true);
+  }
+  if (d.dWg) dw.add(dg, x, F, D, R, C, 1, 1, d.dWg, D, F * D, nullptr, 0);
+  if (d.dWu) dw.add(du, x, F, D, R, C, 1, 1, d.dWu, D, F * D, nullptr, 0);
+  if (d.dWd) dw.add(dy, h, O, F, R, C, 1, 1, d.dWd, F, O * F, nullptr, 0);
+  dw.reserve(ws, true);
+  Colsum<T, __bf16, NP> cs;
+  if (d.dbg) cs.add(dg.p, F8, R * F8, plane, R, F, C, d.dbg, F);
+  if (d.dbu) cs.add(du.p, F8, R * F8, plane, R, F, C, d.dbu, F);
+  cs.reserve(ws);
+  Colsum<T, T, 1> csd;
+  if (d.dbd) csd.add(static_cast<const T*>(d.dy), d.lddy, C > 1 ? d.sdy : 0, 0, R, O, C, d.dbd, O);
+  csd.reserve(ws);
+  *bytes = ws.used;
+  if (dry) return 0;
+  if (hidden && R > 0) {
+    if (pack.launch(stream) != 0) return -1;
+    if (run<NP, false, true, false>(L, choose<NP>(L, false), stream, "gated_mlp_bwd") != 0) return -1;
+    if (dx.template launch<false, true>(stream, "gated_mlp_bwd") != 0) return -1;
+  }
+  if (dw.template launch<true, true>(stream, "gated_mlp_bwd") != 0) return -1;
+  if (cs.launch(stream) != 0) return -1;
+  return csd.launch(stream);
+}
+
+int call(const d3a_gated_mlp_desc* d, bool bwd, bool dry, hipStream_t stream, int64_t* bytes) {
+  Arena ws{dry ? nullptr : static_cast<char*>(d->ws)};
+  if (d->dtype == D3A_F32)
+    return bwd ? backward<float, 3>(*d, ws, dry, stream, bytes) : forward<float, 3>(*d, ws, dry, stream, bytes);
+  return bwd ? backward<__bf16, 1>(*d, ws, dry, stream, bytes) : forward<__bf16, 1>(*d, ws, dry, stream, bytes);
+}
+
+int entry(const d3a_gated_mlp_desc* d, bool bwd, void* stream) {
+  if (check(d, bwd) != 0) return -1;
+  int64_t need = 0;
+  if (call(d, bwd, true, nullptr, &need) != 0) return -1;
+  D3A_CHECK_ARG(need == 0 || (d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 255) == 0),
+                "gated_mlp: workspace of %lld bytes (256-byte aligned) needed", (long long)need);
+  return call(d, bwd, false, static_cast<hipStream_t>(stream), &need);
+}
+
+}  // namespace
+}  // namespace d3a
+
+extern "C" {
+
+int d3a_gated_mlp_workspace(const d3a_gated_mlp_desc* d, int32_t backward, int64_t* bytes) {
+  if (d3a::check(d, backward != 0) != 0) return -1;
+  D3A_CHECK_ARG(bytes, "gated_mlp: null size");
+  return d3a::call(d, backward != 0, true, nullptr, bytes);
+}
+
+int d3a_gated_mlp(const d3a_gated_mlp_desc* d, void* stream) { return d3a::entry(d, false, stream); }
+
+int d3a_gated_mlp_bwd(const d3a_gated_mlp_desc* d, void* stream) { return d3a::entry(d, true, stream); }
+
+}  // extern "C"

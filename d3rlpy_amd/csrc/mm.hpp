@@ -1,0 +1,457 @@
+// Tiled matrix products on the bf16 matrix cores with the epilogue fused, the
+// core of the gated block (gated.hip) and of the linear cross entropy
+// (xent.hip).
+//
+//   D(m, n) = sum over segments and k of A(m, k) B(n, k)
+//
+// An operand is either k-contiguous (element (r, k) at p + r * ld + k) or
+// row-contiguous (p + k * ld + r); the tile of either goes from memory to LDS
+// without passing registers (16 bytes a lane), and a row-contiguous tile is
+// transposed by the LDS reads.  A bfloat16 operand has one plane; a float32
+// operand is given as its exact three-way bf16 split (three planes, pack.hpp
+// layout), and a k step then takes the six part products that matter, smallest
+// first: fp32 accuracy at six bf16 products a term.
+//
+// 16-byte pieces outside the operand (rows past its end, ks past K) read as
+// zero through the buffer resource's range check, so M, N and K are free; the
+// contiguous axis of an operand is a multiple of 8 elements long and 16-byte
+// aligned (the caller packs one that is not).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "common.hpp"
+
+namespace d3a {
+namespace mm {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+
+struct Operand {
+  const __bf16* p;
+  int64_t ld;
+  int64_t s_batch, s_outer, s_inner, s_part;  // elements
+};
+
+// One product of a launch.  K is one segment's length; the sum runs over
+// n_outer * n_inner segments at offsets o * s_outer + i * s_inner of both
+// operands.  splits > 1: workgroup split s sums its share of the k tiles
+// (the epilogue writes a partial).
+struct Problem {
+  Operand a, b;
+  const __bf16* b2;  // dual products: the second B (b's strides), else null
+  int32_t M, N, K;
+  int32_t batch, n_outer, n_inner, splits;
+  int32_t tiles_m, tiles_n, first;  // set by plan()
+};
+
+constexpr int kMaxProblems = 3;
+
+template <class Epi>
+struct Launch {
+  Problem p[kMaxProblems];
+  Epi e[kMaxProblems];
+  int32_t n, total;
+};
+
+// BM x BN output tile, BK deep k tiles, WM x WN waves, NP planes an operand
+template <int BM_, int BN_, int BK_, int WM_, int WN_, int NP_>
+struct Config {
+  static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, NP = NP_;
+  static constexpr int NW = WM * WN, THREADS = 64 * NW;
+  static constexpr int TM = BM / WM, TN = BN / WN;  // a wave's tile
+  static constexpr int MT = TM / 32, NT = TN / 32;
+};
+
+struct Tile {
+  int m0, n0;            // first row / column of this wave's part
+  int batch, split, lane;
+  int M, N;
+};
+
+constexpr unsigned kOutside = 0x80000000u;  // = the resource's extent
+
+// Rows x BK tile of one operand: where each lane's pieces come from and go to.
+// T: row-contiguous operand.  ROWS: tile rows; NW: waves that load it.
+template <int ROWS, int BK, int NP, int NW, bool T>
+struct Loader {
+  static constexpr int PER_PART = ROWS * BK / 512;  // wave instructions a plane
+  static constexpr int NJ = NP * PER_PART / NW;     // of each wave
+  static_assert(NP * PER_PART % NW == 0 && ROWS * BK % 512 == 0, "tile split");
+  static constexpr int LANES = T ? ROWS / 8 : BK / 8;  // lanes a line of the tile
+  static constexpr int LINES = 64 / LANES;             // lines an instruction
+  static_assert(LANES <= 64, "line length");
+
+  unsigned off[NJ];  // byte offset from the tile's base, or kOutside
+  int kk;            // k-contiguous: the first k of the lane's piece
+  int sel;           // dual: bit j set = instruction j reads the second matrix
+
+  // k-contiguous lines are rows of BK; the 16-byte piece c of row r sits at
+  // piece c ^ swz(r), so eight rows' pieces of one k cover all banks.
+  // Row-contiguous lines are ks of ROWS; 32-byte unit u of k sits at
+  // u ^ (k & 3), so a transposed read's four ks cover all banks.
+  static __device__ __forceinline__ int swz(int r) {
+    return BK == 64 ? (r & 7) : ((r >> 1) & 3);
+  }
+
+  template <bool DUAL>
+  __device__ __forceinline__ void init(int w, int lane, int row0, int rows, int64_t ld) {
+    sel = 0;
+    const int line0 = lane / LANES, c = lane % LANES;
+    kk = T ? 0 : 8 * (c ^ swz(line0));
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int q = (j * NW + w) % PER_PART, line = q * LINES + line0;
+      if constexpr (T) {
+        const int cc = c ^ ((line & 3) << 1);
+        off[j] = row0 + 8 * cc < rows ? (unsigned)(line * ld * 2) + 16u * cc : kOutside;
+      } else {
+        int row = line;
+        if constexpr (DUAL) {
+          sel |= ((q * LINES / 32) & 1) << j;
+          row = (line / 64) * 32 + line % 32;
+        }
+        // (swz(line) depends on the lane alone: LINES is 8 or 16)
+        off[j] = row0 + row < rows ? (unsigned)(row * ld * 2) + 2u * kk : kOutside;
+      }
+    }
+  }
+
+  // p: the tile's first element (plane 0); k_left: ks of the segment from the
+  // tile's first on
+  template <bool DUAL>
+  __device__ __forceinline__ void load(char* lds, int w, int lane, const __bf16* p, const __bf16* p2,
+                                       int64_t s_part, int k_left) const {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int part = NP == 1 ? 0 : (j * NW + w) / PER_PART;
+      const __bf16* base = DUAL && ((sel >> j) & 1) ? p2 : p;
+      base += part * s_part;
+      const int k = T ? ((j * NW + w) % PER_PART) * LINES + lane / LANES : kk;
+      const unsigned o = k < k_left ? off[j] : kOutside;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<__bf16*>(base), (short)0, (int)kOutside, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(lds + (j * NW + w) * 1024), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+// Fragments of a tile in LDS: 32 rows x 16 ks for v_mfma_f32_32x32x16_bf16,
+// lane l holding row l % 32, ks 8 (l / 32) .. + 7 of the step.
+template <int ROWS, int BK, bool T>
+struct Frag {
+  // byte offset of plane `part`, rows rb .. rb + 31 (rb a multiple of 32), step s
+  static __device__ __forceinline__ bf16x8 get(const char* lds, int part, int rb, int s, int lane) {
+    const char* base = lds + part * (ROWS * BK * 2);
+    if constexpr (!T) {
+      const int r = lane & 31, c = 2 * s + (lane >> 5);
+      const int x = BK == 64 ? (r & 7) : ((r >> 1) & 3);
+      return *reinterpret_cast<const bf16x8*>(base + (rb + r) * (BK * 2) + ((c ^ x) << 4));
+    } else {
+      // a 16-lane group reads a 4 (k) x 16 (row) block: lane 4 q + p of it
+      // addresses k q, rows 4 p .. 4 p + 3, and receives row `lane & 15`'s ks
+      const int G = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+      const int k = 16 * s + 8 * (G >> 1) + q;
+      const int unit = (rb / 16 + (G & 1)) ^ q;
+      const char* a = base + k * (ROWS * 2) + unit * 32 + p * 8;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(a));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) i16x4*)(a + 4 * (ROWS * 2)));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// A wave's products of one staged k tile.  The B rows are the MFMA's first
+// operand, so a lane ends with one output row m (lane % 32) and runs of four
+// consecutive columns n.
+template <class C, bool AT, bool BT>
+__device__ __forceinline__ void compute(const char* sa, const char* sb, int wm, int wn, int lane,
+                                        f32x16 (&acc)[C::MT][C::NT]) {
+#pragma unroll
+  for (int s = 0; s < C::BK / 16; ++s) {
+    bf16x8 a[C::MT][C::NP], b[C::NT][C::NP];
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int p = 0; p < C::NP; ++p)
+        b[j][p] = Frag<C::BN, C::BK, BT>::get(sb, p, wn * C::TN + 32 * j, s, lane);
+#pragma unroll
+    for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+      for (int p = 0; p < C::NP; ++p)
+        a[i][p] = Frag<C::BM, C::BK, AT>::get(sa, p, wm * C::TM + 32 * i, s, lane);
+    if constexpr (C::NP == 1) {
+#pragma unroll
+      for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j) acc[i][j] = mma(b[j][0], a[i][0], acc[i][j]);
+    } else {
+      // (2,0) (1,1) (0,2) (1,0) (0,1) (0,0): the six products of the split
+      // above 2^-24 of the leading one, smallest first
+      constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+      for (int t = 0; t < 6; ++t)
+#pragma unroll
+        for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+          for (int j = 0; j < C::NT; ++j) acc[i][j] = mma(b[j][pb[t]], a[i][pa[t]], acc[i][j]);
+    }
+  }
+}
+
+template <class C, bool AT, bool BT, bool DUAL, class Epi>
+__global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) {
+  static_assert(!DUAL || (C::TN == 64 && !BT), "dual: a wave's columns are 32 of each matrix");
+  __shared__ __attribute__((aligned(1024))) char sa0[C::NP * C::BM * C::BK * 2];
+  __shared__ __attribute__((aligned(1024))) char sb0[C::NP * C::BN * C::BK * 2];
+  __shared__ __attribute__((aligned(1024))) char sa1[C::NP * C::BM * C::BK * 2];
+  __shared__ __attribute__((aligned(1024))) char sb1[C::NP * C::BN * C::BK * 2];
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = w / C::WN, wn = w % C::WN;
+
+  // workgroups go to the eight XCDs in turn: give each XCD a run of
+  // neighbouring tiles, whose operand rows then meet in its L2
+  int id = blockIdx.x;
+  {
+    const int q = L.total / 8, r = L.total % 8, x = id % 8;
+    id = id / 8 + x * q + (x < r ? x : r);
+  }
+  int pi = 0;
+  while (pi + 1 < L.n && id >= L.p[pi + 1].first) ++pi;
+  const Problem& P = L.p[pi];
+  id -= P.first;
+  const int per = P.tiles_m * P.tiles_n;
+  const int bs = id / per, batch = bs % P.batch, split = bs / P.batch;
+  id %= per;
+  constexpr int GM = 8;  // and the run is a block of GM tile rows
+  const int group = id / (GM * P.tiles_n), in = id % (GM * P.tiles_n);
+  const int gm = min(P.tiles_m - group * GM, GM);
+  const int m0 = (group * GM + in % gm) * C::BM;
+  const int n0 = (in / gm) * (DUAL ? C::BN / 2 : C::BN);
+
+  Loader<C::BM, C::BK, C::NP, C::NW, AT> la;
+  Loader<C::BN, C::BK, C::NP, C::NW, BT> lb;
+  la.template init<false>(w, lane, m0, P.M, P.a.ld);
+  lb.template init<DUAL>(w, lane, n0, P.N, P.b.ld);
+
+  const int kt_seg = max((P.K + C::BK - 1) / C::BK, 1);  // K = 0: one empty tile
+  const int T = kt_seg * P.n_outer * P.n_inner;
+  int t = (int)((int64_t)T * split / P.splits);
+  const int t_end = (int)((int64_t)T * (split + 1) / P.splits);
+  int seg = t / kt_seg;
+  const int64_t a_row = AT ? (int64_t)m0 : (int64_t)m0 * P.a.ld;
+  const int64_t b_row = BT ? (int64_t)n0 : (int64_t)n0 * P.b.ld;
+  const int64_t a_k = AT ? P.a.ld * C::BK : C::BK, b_k = BT ? P.b.ld * C::BK : C::BK;
+
+  // the next k tile: its first elements, and the ks its segment has left
+  const __bf16 *pa, *pb;
+  int left;
+  const int64_t b2 = DUAL ? P.b2 - P.b.p : 0;
+  const int n_inner = P.n_inner, K = P.K;
+  const int64_t a_part = P.a.s_part, b_part = P.b.s_part;
+  auto enter = [&](int kt) {
+    const int o = seg / n_inner, i = seg - o * n_inner;
+    pa = P.a.p + batch * P.a.s_batch + o * P.a.s_outer + i * P.a.s_inner + a_row + kt * a_k;
+    pb = P.b.p + batch * P.b.s_batch + o * P.b.s_outer + i * P.b.s_inner + b_row + kt * b_k;
+    left = K - kt * C::BK;
+  };
+  enter(t % kt_seg);
+  auto load = [&](char* sa, char* sb) {
+    la.template load<false>(sa, w, lane, pa, nullptr, a_part, left);
+    lb.template load<DUAL>(sb, w, lane, pb, pb + b2, b_part, left);
+    pa += a_k;
+    pb += b_k;
+    left -= C::BK;
+    if (left <= 0) {
+      ++seg;
+      enter(0);
+    }
+  };
+
+  f32x16 acc[C::MT][C::NT];
+#pragma unroll
+  for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  // two buffers: the barrier ends the reads of one and the loads of the other
+  if (t < t_end) {
+    load(sa0, sb0);
+    do {
+      __syncthreads();
+      if (t + 1 < t_end) load(sa1, sb1);
+      compute<C, AT, BT>(sa0, sb0, wm, wn, lane, acc);
+      __syncthreads();
+      if (t + 2 < t_end) load(sa0, sb0);
+      if (t + 1 < t_end) compute<C, AT, BT>(sa1, sb1, wm, wn, lane, acc);
+      t += 2;
+    } while (t < t_end);
+  }
+
+  Tile tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N};
+  L.e[pi].template run<C>(acc, tile);
+}
+
+// ---- host -------------------------------------------------------------------
+template <class C, bool DUAL, class Epi>
+int plan(Launch<Epi>& L) {
+  int64_t total = 0;
+  for (int i = 0; i < L.n; ++i) {
+    Problem& p = L.p[i];
+    const int bn = DUAL ? C::BN / 2 : C::BN;
+    p.tiles_m = (p.M + C::BM - 1) / C::BM;
+    p.tiles_n = (p.N + bn - 1) / bn;
+    p.first = (int32_t)total;
+    total += (int64_t)p.tiles_m * p.tiles_n * p.batch * p.splits;
+    if (total >= (1 << 30)) {
+      set_error("product has too many tiles");
+      return -1;
+    }
+  }
+  L.total = (int32_t)total;
+  return 0;
+}
+
+template <class C, bool AT, bool BT, bool DUAL, class Epi>
+int launch(Launch<Epi>& L, hipStream_t stream, const char* what) {
+  if (plan<C, DUAL>(L) != 0) return -1;
+  if (L.total == 0) return 0;
+  mm_kernel<C, AT, BT, DUAL, Epi><<<L.total, C::THREADS, 0, stream>>>(L);
+  D3A_LAUNCH_CHECK(what);
+  return 0;
+}
+
+// float4 <-> storage
+__device__ __forceinline__ void split3(float x, __bf16& p0, __bf16& p1, __bf16& p2) {
+  p0 = (__bf16)x;
+  const float r = x - (float)p0;
+  p1 = (__bf16)r;
+  p2 = (__bf16)(r - (float)p1);
+}
+
+// v[0..3] as columns n .. n + 3 of NP planes at row pointer `p` (n % 4 == 0,
+// the row padded to a multiple of 8 columns)
+template <int NP>
+__device__ __forceinline__ void store_planes(__bf16* p, int64_t s_part, const float v[4]) {
+  if constexpr (NP == 1) {
+    bf16x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (__bf16)v[i];
+    *reinterpret_cast<bf16x4*>(p) = o;
+  } else {
+    bf16x4 o[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __bf16 a, b, c;
+      split3(v[i], a, b, c);
+      o[0][i] = a;
+      o[1][i] = b;
+      o[2][i] = c;
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x4*>(p + q * s_part) = o[q];
+  }
+}
+
+__device__ __forceinline__ void store4(float* p, const float v[4]) {
+  *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ void store4(__bf16* p, const float v[4]) {
+  *reinterpret_cast<bf16x4*>(p) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+}
+__device__ __forceinline__ void load4(const float* p, float v[4]) {
+  const f32x4 x = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = x[i];
+}
+__device__ __forceinline__ void load4(const __bf16* p, float v[4]) {
+  const bf16x4 x = *reinterpret_cast<const bf16x4*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+}
+
+// every run of four columns of a wave's tile: f(m, n, v[4]) for m < M
+template <class C, int J0 = 0, int J1 = C::NT, class F>
+__device__ __forceinline__ void each4(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, F f) {
+#pragma unroll
+  for (int i = 0; i < C::MT; ++i) {
+    const int m = t.m0 + 32 * i + (t.lane & 31);
+#pragma unroll
+    for (int j = J0; j < J1; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = t.n0 + 32 * (j - J0) + 8 * q + 4 * (t.lane >> 5);
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r];
+        if (m < t.M) f(m, n, v, i, j, q);
+      }
+  }
+}
+
+// D (+ bias) in T, or an fp32 partial of a split / running sum over launches
+template <class T>
+struct StoreEpi {
+  T* out;           // [batch][M] rows of ld
+  int64_t ld, s_batch;
+  const T* bias;    // [batch][N] or null
+  int64_t s_bias;
+  float* sum;       // splits: [split][batch][M][N]; running sum: [M][N]
+  int32_t mode;     // 0 out = D, 1 partial, 2 sum = D, 3 sum += D, 4 out = sum + D
+  int32_t vec;      // out rows take four-wide stores
+
+  template <class C>
+  __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
+    each4<C>(acc, t, [&](int m, int n, float* v, int, int, int) {
+      if (n >= t.N) return;
+      if (mode == 1) {
+        float* s = sum + (((int64_t)t.split * gridDim_batch(t) + t.batch) * t.M + m) * t.N + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < t.N) s[r] = v[r];
+        return;
+      }
+      if (mode >= 2) {
+        float* s = sum + (int64_t)m * t.N + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < t.N) {
+            if (mode >= 3) v[r] += s[r];
+            if (mode <= 3) s[r] = v[r];
+          }
+        if (mode <= 3) return;
+      }
+      if (bias) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += (float)bias[t.batch * s_bias + min(n + r, t.N - 1)];
+      }
+      T* o = out + t.batch * s_batch + (int64_t)m * ld + n;
+      if (vec && n + 4 <= t.N) {
+        store4(o, v);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < t.N) o[r] = (T)v[r];
+      }
+    });
+  }
+  int32_t n_batch;
+  __device__ __forceinline__ int gridDim_batch(const Tile&) const { return n_batch; }
+};
+
+}  // namespace mm
+}  // namespace d3a

@@ -1,0 +1,380 @@
+// Host side of the products of mm.hpp, and the small passes around them:
+// packing an operand (float32: its exact three-way bf16 split; bfloat16: an
+// aligned copy of one that the tiles cannot read in place), column sums (bias
+// gradients) and the sum of split-k partials.
+#pragma once
+
+#include <algorithm>
+
+#include "mm.hpp"
+
+namespace d3a {
+namespace mm {
+
+inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Bump allocation over the caller's workspace; with a null base it measures.
+struct Arena {
+  char* base;
+  int64_t used = 0;
+  template <class T>
+  T* take(int64_t n) {
+    used = (used + 255) / 256 * 256;
+    T* p = reinterpret_cast<T*>(base ? base + used : nullptr);
+    used += n * (int64_t)sizeof(T);
+    return p;
+  }
+};
+
+// ---- packing ------------------------------------------------------------------
+struct PackJob {
+  const void* src;
+  __bf16* dst;             // [planes][batch][rows][round8(cols)], the tail zero
+  int64_t ld, s_batch;     // of src, elements
+  int64_t rows, cols, batch;
+};
+constexpr int kMaxPack = 6;
+struct PackJobs {
+  PackJob j[kMaxPack];
+  int64_t end[kMaxPack];  // running count of 8-wide pieces
+  int32_t n;
+};
+
+// One 8-wide piece a thread: 32 bytes (16) in, 48 (16) out; memory bound.
+template <class T, int NP>
+__global__ __launch_bounds__(256) void pack_kernel(const PackJobs J) {
+  int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int i = 0;
+  while (i < J.n && p >= J.end[i]) ++i;
+  if (i == J.n) return;
+  if (i > 0) p -= J.end[i - 1];
+  const PackJob& j = J.j[i];
+  const int64_t blocks = (j.cols + 7) / 8;
+  const int64_t row = p / blocks;  // batch * rows + r
+  const int c = (int)(p - row * blocks) * 8;
+  const int64_t b = row / j.rows, r = row - b * j.rows;
+  const T* s = static_cast<const T*>(j.src) + b * j.s_batch + r * j.ld + c;
+  float v[8];
+  if (c + 8 <= j.cols && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
+    if constexpr (sizeof(T) == 4) {
+      load4(s, v);
+      load4(s + 4, v + 4);
+    } else {
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(s);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? (float)s[k] : 0.f;
+  }
+  const int64_t s_part = j.batch * j.rows * blocks * 8;
+  __bf16* d = j.dst + row * blocks * 8 + c;
+  bf16x8 o[NP];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (NP == 1) {
+      o[0][k] = (__bf16)v[k];
+    } else {
+      __bf16 x, y, z;
+      split3(v[k], x, y, z);
+      o[0][k] = x;
+      o[1][k] = y;
+      o[2][k] = z;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < NP; ++q) *reinterpret_cast<bf16x8*>(d + q * s_part) = o[q];
+}
+
+// Collects what one call has to pack and launches it once.
+template <class T, int NP>
+struct Packer {
+  PackJobs jobs{};
+  Arena& ws;
+  explicit Packer(Arena& a) : ws(a) {}
+
+  // The operand planes of a [batch][rows][cols] array (s_batch 0: one shared
+  // batch), in place where the tiles can read it: one plane, 16-byte rows, and
+  // offsets within a tile that fit the resource.
+  Operand operand(const void* p, int64_t ld, int64_t s_batch, int64_t batch, int64_t rows,
+                  int64_t cols, bool force = false) {
+    Operand o{};
+    const int64_t c8 = round8(cols);
+    const int64_t nb = s_batch == 0 ? 1 : batch;
+    const bool in_place = NP == 1 && !force && cols % 8 == 0 && ld % 8 == 0 && s_batch % 8 == 0 &&
+                          (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld < (1 << 21);
+    if (in_place) {
+      o.p = static_cast<const __bf16*>(p);
+      o.ld = ld;
+      o.s_batch = s_batch;
+      return o;
+    }
+    __bf16* d = ws.take<__bf16>(NP * nb * rows * c8);
+    o.p = d;
+    o.ld = c8;
+    o.s_batch = s_batch == 0 ? 0 : rows * c8;
+    o.s_part = nb * rows * c8;
+    PackJob& j = jobs.j[jobs.n];
+    j = PackJob{p, d, ld, s_batch, rows, cols, nb};
+    jobs.end[jobs.n] = (jobs.n ? jobs.end[jobs.n - 1] : 0) + nb * rows * (c8 / 8);
+    ++jobs.n;
+    return o;
+  }
+
+  int launch(hipStream_t stream) {
+    if (jobs.n == 0 || jobs.end[jobs.n - 1] == 0) return 0;
+    const int64_t blocks = (jobs.end[jobs.n - 1] + 255) / 256;
+    if (blocks >= (1LL << 31)) {
+      set_error("operand too large to pack");
+      return -1;
+    }
+    pack_kernel<T, NP><<<(unsigned)blocks, 256, 0, stream>>>(jobs);
+    D3A_LAUNCH_CHECK("pack");
+    return 0;
+  }
+};
+
+// ---- column sums -----------------------------------------------------------------
+// out[b][c] = sum over rows of the value at [b][r][c]: NP planes added (planes
+// of an exact split), or one array of T.  Rows are cut into chunks whose fp32
+// sums a second pass adds in order, so the result does not depend on timing.
+template <class S>
+struct ColsumJob {
+  const S* src;
+  int64_t ld, s_batch, s_part;
+  void* out;       // T
+  int64_t s_out;   // elements between batches
+  int32_t rows, cols, batch;
+};
+constexpr int kMaxColsum = 3;
+template <class S>
+struct ColsumJobs {
+  ColsumJob<S> j[kMaxColsum];
+  float* part;      // [chunks][total columns]
+  int64_t first[kMaxColsum + 1];  // running count of batch * cols
+  int32_t n, chunks;
+};
+
+// a workgroup: 64 columns (one a lane) x its chunk of rows over four waves
+template <class S, int NP>
+__global__ __launch_bounds__(256) void colsum_kernel(const ColsumJobs<S> J) {
+  __shared__ float red[256];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  const bool on = c < J.first[J.n];
+  int i = 0;
+  while (i + 1 < J.n && c >= J.first[i + 1]) ++i;
+  const ColsumJob<S>& j = J.j[i];
+  const int64_t cc = on ? c - J.first[i] : 0;
+  const int64_t b = cc / j.cols, col = cc - b * j.cols;
+  const S* p = j.src + b * j.s_batch + col;
+  const int64_t per = (j.rows + J.chunks - 1) / J.chunks;
+  const int64_t r0 = per * blockIdx.y, r1 = min(r0 + per, (int64_t)j.rows);
+  float s = 0.f;
+  if (on)
+#pragma unroll 4
+    for (int64_t r = r0 + w; r < r1; r += 4) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = NP - 1; q >= 0; --q) v += (float)p[q * j.s_part + r * j.ld];
+      s += v;
+    }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (w == 0 && on)
+    J.part[(int64_t)blockIdx.y * J.first[J.n] + c] =
+        ((red[lane] + red[64 + lane]) + red[128 + lane]) + red[192 + lane];
+}
+
+template <class T, class S>
+__global__ __launch_bounds__(256) void colsum_finish(const ColsumJobs<S> J) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= J.first[J.n]) return;
+  float s = 0.f;
+  for (int k = 0; k < J.chunks; ++k) s += J.part[(int64_t)k * J.first[J.n] + c];
+  int i = 0;
+  while (i + 1 < J.n && c >= J.first[i + 1]) ++i;
+  const ColsumJob<S>& j = J.j[i];
+  const int64_t cc = c - J.first[i], b = cc / j.cols;
+  static_cast<T*>(j.out)[b * j.s_out + cc - b * j.cols] = (T)s;
+}
+
+template <class T, class S, int NP>
+struct Colsum {
+  ColsumJobs<S> jobs{};
+  void add(const S* src, int64_t ld, int64_t s_batch, int64_t s_part, int64_t rows, int64_t cols,
+           int64_t batch, void* out, int64_t s_out) {
+    ColsumJob<S>& j = jobs.j[jobs.n];
+    j = ColsumJob<S>{src, ld, s_batch, s_part, out, s_out, (int32_t)rows, (int32_t)cols, (int32_t)batch};
+    jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * cols;
+    ++jobs.n;
+    // about 1024 workgroups, chunks of at least 32 rows
+    const int64_t blocks = (jobs.first[jobs.n] + 63) / 64;
+    jobs.chunks = (int32_t)std::max<int64_t>(
+        1, std::min<int64_t>({1024 / std::max<int64_t>(blocks, 1), (rows + 31) / 32, 256}));
+  }
+  void reserve(Arena& ws) {
+    if (jobs.n) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n]);
+  }
+  int launch(hipStream_t stream) {
+    const int64_t cols = jobs.first[jobs.n];
+    if (jobs.n == 0 || cols == 0) return 0;
+    colsum_kernel<S, NP><<<dim3((unsigned)((cols + 63) / 64), jobs.chunks), 256, 0, stream>>>(jobs);
+    D3A_LAUNCH_CHECK("column sums");
+    colsum_finish<T, S><<<(unsigned)((cols + 255) / 256), 256, 0, stream>>>(jobs);
+    D3A_LAUNCH_CHECK("column sums");
+    return 0;
+  }
+};
+
+// ---- split-k partials -------------------------------------------------------------
+template <class T>
+struct SumJob {
+  const float* part;  // [splits][batch][M][N]
+  T* out;
+  int64_t ld, s_batch;
+  int64_t n;          // batch * M * N
+  int32_t M, N, splits;
+};
+template <class T>
+struct SumJobs {
+  SumJob<T> j[kMaxProblems];
+  int64_t end[kMaxProblems];
+  int32_t n;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
+  int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int i = 0;
+  while (i < J.n && e >= J.end[i]) ++i;
+  if (i == J.n) return;
+  if (i > 0) e -= J.end[i - 1];
+  const SumJob<T>& j = J.j[i];
+  float s = 0.f;
+  for (int k = 0; k < j.splits; ++k) s += j.part[k * j.n + e];
+  const int64_t row = e / j.N, n = e - row * j.N, b = row / j.M;
+  j.out[b * j.s_batch + (row - b * j.M) * j.ld + n] = (T)s;
+}
+
+// ---- tile choice --------------------------------------------------------------------
+// Three tiles: the large one reuses each staged byte most (128 or 85 products a
+// byte) and is taken where its workgroups fill most of the 256 CUs; the small
+// ones keep the chip busy on less.
+enum TileSize { kLarge, kMid, kSmall };
+
+template <int NP>
+struct Tiles;
+template <>
+struct Tiles<1> {
+  typedef Config<256, 256, 64, 2, 4, 1> Large;
+  typedef Config<128, 128, 64, 2, 2, 1> Mid;
+  typedef Config<64, 64, 64, 2, 1, 1> Small;
+};
+template <>
+struct Tiles<3> {
+  typedef Config<256, 128, 32, 4, 2, 3> Large;
+  typedef Config<128, 128, 32, 2, 2, 3> Mid;
+  typedef Config<64, 64, 32, 2, 1, 3> Small;
+};
+
+template <int NP, class Epi>
+int64_t count_tiles(const Launch<Epi>& L, TileSize s, bool dual) {
+  typedef Tiles<NP> X;
+  const int bm = s == kLarge ? X::Large::BM : s == kMid ? X::Mid::BM : X::Small::BM;
+  int bn = s == kLarge ? X::Large::BN : s == kMid ? X::Mid::BN : X::Small::BN;
+  if (dual) bn /= 2;
+  int64_t n = 0;
+  for (int i = 0; i < L.n; ++i)
+    n += (int64_t)((L.p[i].M + bm - 1) / bm) * ((L.p[i].N + bn - 1) / bn) * L.p[i].batch;
+  return n;
+}
+
+template <int NP, class Epi>
+TileSize choose(const Launch<Epi>& L, bool dual) {
+  if (count_tiles<NP>(L, kLarge, dual) >= 160) return kLarge;
+  if (count_tiles<NP>(L, kMid, dual) >= 160) return kMid;
+  return kSmall;
+}
+
+template <int NP, bool AT, bool BT, bool DUAL, class Epi>
+int run(Launch<Epi>& L, TileSize s, hipStream_t stream, const char* what) {
+  typedef Tiles<NP> X;
+  if (s == kLarge) return launch<typename X::Large, AT, BT, DUAL>(L, stream, what);
+  if (s == kMid) return launch<typename X::Mid, AT, BT, DUAL>(L, stream, what);
+  return launch<typename X::Small, AT, BT, DUAL>(L, stream, what);
+}
+
+// A launch of plain products D -> T (StoreEpi), with the k axis cut where the
+// tiles alone leave CUs idle and each cut keeps `kMinSteps` k tiles.
+template <class T, int NP>
+struct Products {
+  Launch<StoreEpi<T>> L{};
+  SumJobs<T> sums{};
+  TileSize size = kLarge;
+
+  void add(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, int64_t batch,
+           int64_t n_outer, int64_t n_inner, void* out, int64_t ld, int64_t s_batch,
+           const void* bias, int64_t s_bias) {
+    Problem& p = L.p[L.n];
+    p = Problem{};
+    p.a = a;
+    p.b = b;
+    p.M = (int32_t)M;
+    p.N = (int32_t)N;
+    p.K = (int32_t)K;
+    p.batch = (int32_t)batch;
+    p.n_outer = (int32_t)n_outer;
+    p.n_inner = (int32_t)n_inner;
+    p.splits = 1;
+    StoreEpi<T>& e = L.e[L.n];
+    e = StoreEpi<T>{};
+    e.out = static_cast<T*>(out);
+    e.ld = ld;
+    e.s_batch = s_batch;
+    e.bias = static_cast<const T*>(bias);
+    e.s_bias = s_bias;
+    e.n_batch = (int32_t)batch;
+    e.vec = ld % 4 == 0 && s_batch % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
+    ++L.n;
+  }
+
+  // after every add(): the tile, the splits and their partials
+  void reserve(Arena& ws, bool may_split) {
+    if (L.n == 0) return;
+    size = choose<NP>(L, false);
+    if (!may_split) return;
+    typedef Tiles<NP> X;
+    const int64_t tiles = count_tiles<NP>(L, size, false);
+    const int bk = size == kLarge ? X::Large::BK : size == kMid ? X::Mid::BK : X::Small::BK;
+    constexpr int64_t kMinSteps = 8;
+    for (int i = 0; i < L.n; ++i) {
+      Problem& p = L.p[i];
+      const int64_t steps = (int64_t)((p.K + bk - 1) / bk) * p.n_outer * p.n_inner;
+      const int64_t s = std::min<int64_t>({256 / std::max<int64_t>(tiles, 1), steps / kMinSteps, 16});
+      if (s < 2) continue;
+      p.splits = (int32_t)s;
+      StoreEpi<T>& e = L.e[i];
+      const int64_t n = (int64_t)p.batch * p.M * p.N;
+      e.sum = ws.take<float>(s * n);
+      e.mode = 1;
+      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits};
+      sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + n;
+      ++sums.n;
+    }
+  }
+
+  template <bool AT, bool BT>
+  int launch(hipStream_t stream, const char* what) {
+    if (L.n == 0) return 0;
+    if (run<NP, AT, BT, false>(L, size, stream, what) != 0) return -1;
+    if (sums.n == 0) return 0;
+    sum_kernel<T><<<(unsigned)((sums.end[sums.n - 1] + 255) / 256), 256, 0, stream>>>(sums);
+    D3A_LAUNCH_CHECK(what);
+    return 0;
+  }
+};
+
+}  // namespace mm
+}  // namespace d3a

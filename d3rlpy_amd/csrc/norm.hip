@@ -1,0 +1,515 @@
+// Layer norm, forward and backward, of rows of n values:
+//
+//   xh = (x - mean) rstd,  y = xh w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   t = dy w,  dx = rstd (t - mean(t) - xh mean(t xh))
+//   dw = sum over rows of dy xh,  db = sum over rows of dy
+//
+// Memory bound: forward reads x and writes y, backward reads x and dy and
+// writes dx.  A row is held in registers (by a wave, or by four where it is
+// long), so each value is read once and the variance is that of the centred
+// values; the backward's waves walk the rows and keep the columns' sums of dw
+// and db in registers, one partial a workgroup, which a second pass adds in
+// order.  Statistics and sums are float32.
+#include <algorithm>
+
+#include "mm_host.hpp"
+#include "../../include/d3rlpy_amd.h"
+
+namespace d3a {
+namespace {
+
+using mm::Arena;
+using mm::bf16x8;
+using mm::f32x4;
+
+// VEC values at p as float; VEC 1, or 16 bytes of T (and as many of another type)
+template <int VEC, class T>
+__device__ __forceinline__ void load_vec(const T* p, float* v) {
+  if constexpr (VEC == 1) {
+    v[0] = (float)p[0];
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) mm::load4(p + k, v + k);
+  } else {
+    static_assert(VEC == 8, "16 bytes");
+    const bf16x8 x = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
+  }
+}
+
+template <int VEC, class T>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+  if constexpr (VEC == 1) {
+    p[0] = (T)v[0];
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) mm::store4(p + k, v + k);
+  } else {
+    bf16x8 x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = (__bf16)v[k];
+    *reinterpret_cast<bf16x8*>(p) = x;
+  }
+}
+
+struct Args {
+  const void *x, *w, *b, *dy;
+  void *y, *dx, *dw, *db;
+  float *mean, *rstd, *part;
+  int64_t rows, members, ldx, sx, lddy, sdy;
+  int32_t n;
+  float eps;
+};
+
+// the sum over the WPR waves that hold a row
+template <int WPR>
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
+  if constexpr (WPR == 1) return wave_sum(v);
+  return block_sum(v, scratch);
+}
+
+// NCH pieces of VEC values a lane; WPR waves a row (1: four rows a workgroup)
+template <class T, class W, int VEC, int NCH, int WPR>
+__global__ __launch_bounds__(256) void norm_kernel(const Args A) {
+  __shared__ float scratch[4];
+  const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wid / WPR;
+  if (row >= A.rows * A.members) return;  // (WPR 4: the whole workgroup or none of it)
+  const int64_t c = row / A.rows, r = row - c * A.rows;
+  const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
+  const int l = (wid % WPR) * 64 + lane;
+  float v[NCH][VEC], s = 0.f;
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int col = (j * WPR * 64 + l) * VEC;
+    if (col < A.n) {
+      load_vec<VEC>(x + col, v[j]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[j][k] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s += v[j][k];
+  }
+  const float mean = row_sum<WPR>(s, scratch) / (float)A.n;
+  s = 0.f;
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int col = (j * WPR * 64 + l) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      v[j][k] = col < A.n ? v[j][k] - mean : 0.f;
+      s = fmaf(v[j][k], v[j][k], s);
+    }
+  }
+  const float rstd = 1.f / sqrtf(row_sum<WPR>(s, scratch) / (float)A.n + A.eps);
+  if (A.mean && l == 0) {
+    A.mean[row] = mean;
+    A.rstd[row] = rstd;
+  }
+  T* y = static_cast<T*>(A.y) + row * A.n;
+  const W* w = static_cast<const W*>(A.w) + c * A.n;
+  const W* b = static_cast<const W*>(A.b) + c * A.n;
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int col = (j * WPR * 64 + l) * VEC;
+    if (col >= A.n) continue;
+    float wv[VEC], bv[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      wv[k] = 1.f;
+      bv[k] = 0.f;
+    }
+    if (A.w) load_vec<VEC>(w + col, wv);
+    if (A.b) load_vec<VEC>(b + col, bv);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[j][k] = fmaf(v[j][k] * rstd, wv[k], bv[k]);
+    store_vec<VEC>(y + col, v[j]);
+  }
+}
+
+// grid (workgroups, members): workgroup g of a member takes rows g, g + grid, ..
+// (times the rows it holds at once)
+template <class T, class W, int VEC, int NCH, int WPR>
+__global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
+  __shared__ float scratch[8];
+  __shared__ float cols[WPR == 1 ? 2 * NCH * VEC * 64 : 1];
+  const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int l = (wid % WPR) * 64 + lane;
+  const int64_t c = blockIdx.y;
+  const W* w = static_cast<const W*>(A.w) + c * A.n;
+  float wv[NCH][VEC], dw[NCH][VEC], db[NCH][VEC];
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int col = (j * WPR * 64 + l) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      wv[j][k] = 1.f;
+      dw[j][k] = db[j][k] = 0.f;
+    }
+    if (A.w && col < A.n) load_vec<VEC>(w + col, wv[j]);
+  }
+  const int64_t step = (int64_t)gridDim.x * (4 / WPR);
+  for (int64_t r = (int64_t)blockIdx.x * (4 / WPR) + wid / WPR; r < A.rows; r += step) {
+    const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
+    const T* dy = static_cast<const T*>(A.dy) + c * A.sdy + r * A.lddy;
+    const int64_t row = c * A.rows + r;
+    const float mean = A.mean[row], rstd = A.rstd[row];
+    float xh[NCH][VEC], t[NCH][VEC], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      const int col = (j * WPR * 64 + l) * VEC;
+      if (col < A.n) {
+        load_vec<VEC>(x + col, xh[j]);
+        load_vec<VEC>(dy + col, t[j]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          xh[j][k] = mean;
+          t[j][k] = 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        xh[j][k] = (xh[j][k] - mean) * rstd;
+        dw[j][k] = fmaf(t[j][k], xh[j][k], dw[j][k]);
+        db[j][k] += t[j][k];
+        t[j][k] *= wv[j][k];
+        s[0] += t[j][k];
+        s[1] = fmaf(t[j][k], xh[j][k], s[1]);
+      }
+    if (!A.dx) continue;
+    if constexpr (WPR == 1) {
+      s[0] = wave_sum(s[0]);
+      s[1] = wave_sum(s[1]);
+    } else {
+      block_sum_k<2>(s, scratch);
+    }
+    const float m0 = s[0] / (float)A.n, m1 = s[1] / (float)A.n;
+    T* dx = static_cast<T*>(A.dx) + row * A.n;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      const int col = (j * WPR * 64 + l) * VEC;
+      if (col >= A.n) continue;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) t[j][k] = rstd * (t[j][k] - m0 - xh[j][k] * m1);
+      store_vec<VEC>(dx + col, t[j]);
+    }
+  }
+  if (!A.part) return;
+  if constexpr (WPR == 1) {
+    // the four waves' sums, added in order
+    for (int q = 0; q < 4; ++q) {
+      if (wid == q) {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            const int at = (j * VEC + k) * 64 + lane;
+            cols[at] = q ? cols[at] + dw[j][k] : dw[j][k];
+            cols[NCH * VEC * 64 + at] = q ? cols[NCH * VEC * 64 + at] + db[j][k] : db[j][k];
+          }
+      }
+      __syncthreads();
+    }
+    if (wid != 0) return;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        dw[j][k] = cols[(j * VEC + k) * 64 + lane];
+        db[j][k] = cols[(NCH * VEC + j * VEC + k) * 64 + lane];
+      }
+  }
+  float* part = A.part + (c * gridDim.x + blockIdx.x) * 2 * A.n;
+#pragma unroll
+  for (int j = 0; j < NCH; ++j) {
+    const int col = (j * WPR * 64 + l) * VEC;
+    if (col >= A.n) continue;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      part[col + k] = dw[j][k];
+      part[A.n + col + k] = db[j][k];
+    }
+  }
+}
+
+// dw, db of a member: 64 of its 2 n columns a workgroup, the parts over its waves
+template <class W>
+__global__ __launch_bounds__(256) void norm_finish_kernel(const Args A, int32_t parts) {
+  __shared__ float red[256];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane, c = blockIdx.y;
+  const int64_t n = A.n;
+  float s = 0.f;
+  if (col < 2 * n) {
+    const float* p = A.part + c * parts * 2 * n + col;
+#pragma unroll 8
+    for (int k = wid; k < parts; k += 4) s += p[k * 2 * n];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (wid != 0 || col >= 2 * n) return;
+  s = ((red[lane] + red[64 + lane]) + red[128 + lane]) + red[192 + lane];
+  if (col < n) {
+    if (A.dw) static_cast<W*>(A.dw)[c * n + col] = (W)s;
+  } else {
+    if (A.db) static_cast<W*>(A.db)[c * n + col - n] = (W)s;
+  }
+}
+
+// rows too long for four waves' registers: a workgroup a row, in passes
+template <class T, class W>
+__global__ __launch_bounds__(256) void norm_long_kernel(const Args A) {
+  __shared__ float scratch[4];
+  const int64_t row = blockIdx.x, c = row / A.rows, r = row - c * A.rows;
+  const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
+  const W* w = static_cast<const W*>(A.w) + c * A.n;
+  const W* b = static_cast<const W*>(A.b) + c * A.n;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < A.n; i += 256) s += (float)x[i];
+  const float mean = block_sum(s, scratch) / (float)A.n;
+  s = 0.f;
+  for (int i = threadIdx.x; i < A.n; i += 256) {
+    const float v = (float)x[i] - mean;
+    s = fmaf(v, v, s);
+  }
+  const float rstd = 1.f / sqrtf(block_sum(s, scratch) / (float)A.n + A.eps);
+  if (A.mean && threadIdx.x == 0) {
+    A.mean[row] = mean;
+    A.rstd[row] = rstd;
+  }
+  T* y = static_cast<T*>(A.y) + row * A.n;
+  for (int i = threadIdx.x; i < A.n; i += 256)
+    y[i] = (T)fmaf(((float)x[i] - mean) * rstd, A.w ? (float)w[i] : 1.f, A.b ? (float)b[i] : 0.f);
+}
+
+template <class T, class W>
+__global__ __launch_bounds__(256) void norm_long_dx_kernel(const Args A) {
+  __shared__ float scratch[8];
+  const int64_t row = blockIdx.x, c = row / A.rows, r = row - c * A.rows;
+  const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
+  const T* dy = static_cast<const T*>(A.dy) + c * A.sdy + r * A.lddy;
+  const W* w = static_cast<const W*>(A.w) + c * A.n;
+  const float mean = A.mean[row], rstd = A.rstd[row];
+  float s[2] = {0.f, 0.f};
+  for (int i = threadIdx.x; i < A.n; i += 256) {
+    const float t = (float)dy[i] * (A.w ? (float)w[i] : 1.f);
+    s[0] += t;
+    s[1] = fmaf(t, ((float)x[i] - mean) * rstd, s[1]);
+  }
+  block_sum_k<2>(s, scratch);
+  const float m0 = s[0] / (float)A.n, m1 = s[1] / (float)A.n;
+  T* dx = static_cast<T*>(A.dx) + row * A.n;
+  for (int i = threadIdx.x; i < A.n; i += 256) {
+    const float t = (float)dy[i] * (A.w ? (float)w[i] : 1.f);
+    dx[i] = (T)(rstd * (t - m0 - ((float)x[i] - mean) * rstd * m1));
+  }
+}
+
+// partials of dw, db: 64 columns x a chunk of rows (grid x: columns, y: chunks, z: members)
+template <class T>
+__global__ __launch_bounds__(256) void norm_long_cols_kernel(const Args A) {
+  __shared__ float red[2][256];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane, c = blockIdx.z;
+  const int64_t per = (A.rows + gridDim.y - 1) / gridDim.y, r0 = per * blockIdx.y;
+  const int64_t r1 = min(r0 + per, A.rows);
+  float dw = 0.f, db = 0.f;
+  if (col < A.n)
+    for (int64_t r = r0 + wid; r < r1; r += 4) {
+      const int64_t row = c * A.rows + r;
+      const float x = (float)static_cast<const T*>(A.x)[c * A.sx + r * A.ldx + col];
+      const float t = (float)static_cast<const T*>(A.dy)[c * A.sdy + r * A.lddy + col];
+      dw = fmaf(t, (x - A.mean[row]) * A.rstd[row], dw);
+      db += t;
+    }
+  red[0][threadIdx.x] = dw;
+  red[1][threadIdx.x] = db;
+  __syncthreads();
+  if (wid != 0 || col >= A.n) return;
+  float* part = A.part + (c * gridDim.y + blockIdx.y) * 2 * A.n + col;
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+    part[q * A.n] = ((red[q][lane] + red[q][64 + lane]) + red[q][128 + lane]) + red[q][192 + lane];
+}
+
+// ---- host -------------------------------------------------------------------
+constexpr int kLong = 8192;  // values that four waves hold
+
+int check(const d3a_layer_norm_desc* d, bool bwd) {
+  D3A_CHECK_ARG(d, "layer_norm: null descriptor");
+  D3A_CHECK_ARG(d->dtype == D3A_F32 || d->dtype == D3A_BF16, "layer_norm: dtype must be float32 or bfloat16");
+  D3A_CHECK_ARG(d->wtype == d->dtype || d->wtype == D3A_F32,
+                "layer_norm: weight and bias must have x's dtype or be float32");
+  D3A_CHECK_ARG(d->rows >= 0 && d->members >= 1 && d->members <= 65535 && d->n >= 1,
+                "layer_norm: sizes must be positive");
+  D3A_CHECK_ARG(d->n < (1LL << 30) && d->rows < (1LL << 31) && d->rows * d->members < (1LL << 31),
+                "layer_norm: size too large");
+  D3A_CHECK_ARG(d->ldx >= d->n && (!bwd || d->lddy >= d->n), "layer_norm: row stride smaller than the row");
+  D3A_CHECK_ARG((d->mean == nullptr) == (d->rstd == nullptr), "layer_norm: mean and rstd go together");
+  if (d->rows > 0) {
+    D3A_CHECK_ARG(d->x && (bwd ? d->dy != nullptr : d->y != nullptr), "layer_norm: null operand");
+    D3A_CHECK_ARG(!bwd || d->mean, "layer_norm: the backward needs the forward's mean and rstd");
+  }
+  return 0;
+}
+
+Args args_of(const d3a_layer_norm_desc& d) {
+  Args a{};
+  a.x = d.x;
+  a.w = d.w;
+  a.b = d.b;
+  a.dy = d.dy;
+  a.y = d.y;
+  a.dx = d.dx;
+  a.dw = d.dw;
+  a.db = d.db;
+  a.mean = d.mean;
+  a.rstd = d.rstd;
+  a.rows = d.rows;
+  a.members = d.members;
+  a.ldx = d.ldx;
+  a.sx = d.sx;
+  a.lddy = d.lddy;
+  a.sdy = d.sdy;
+  a.n = (int32_t)d.n;
+  a.eps = (float)d.eps;
+  return a;
+}
+
+// every row of every array starts on 16 bytes and is whole 16-byte pieces
+bool aligned(const d3a_layer_norm_desc& d, bool bwd) {
+  const int64_t vec = d.dtype == D3A_F32 ? 4 : 8;
+  uintptr_t p = reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.w) |
+                reinterpret_cast<uintptr_t>(bwd ? d.dx : d.y) |
+                reinterpret_cast<uintptr_t>(bwd ? d.dy : d.b);
+  int64_t s = d.n | d.ldx | d.sx;
+  if (bwd) s |= d.lddy | d.sdy;
+  return (p & 15) == 0 && s % vec == 0;
+}
+
+// workgroups a member: enough to fill the chip (1024 over the members), each
+// wave at least one row
+int64_t bwd_blocks(const d3a_layer_norm_desc& d) {
+  const int64_t at_once = d.n > 2048 ? 1 : 4;
+  const int64_t most = std::max<int64_t>(1, 1024 / d.members);
+  return std::max<int64_t>(1, std::min((d.rows + at_once - 1) / at_once, most));
+}
+
+template <class T, class W, int VEC, int NCH, int WPR>
+int launch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, int64_t blocks, hipStream_t stream) {
+  if (bwd) {
+    norm_bwd_kernel<T, W, VEC, NCH, WPR><<<dim3((unsigned)blocks, (unsigned)d.members), 256, 0, stream>>>(a);
+  } else {
+    const int64_t rows = d.rows * d.members;
+    norm_kernel<T, W, VEC, NCH, WPR><<<(unsigned)((rows * WPR + 3) / 4), 256, 0, stream>>>(a);
+  }
+  D3A_LAUNCH_CHECK("layer_norm");
+  return 0;
+}
+
+// pieces of 16 bytes where every row allows them, else single values
+template <class T, class W>
+int dispatch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, int64_t blocks, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t n = d.n;
+  if (aligned(d, bwd)) {
+    if (n > 4096) return launch<T, W, V, 8192 / (256 * V), 4>(d, a, bwd, blocks, s);
+    if (n > 2048) return launch<T, W, V, 4096 / (256 * V), 4>(d, a, bwd, blocks, s);
+    if (n > 1024) return launch<T, W, V, 2048 / (64 * V), 1>(d, a, bwd, blocks, s);
+    if (n > 512) return launch<T, W, V, 1024 / (64 * V), 1>(d, a, bwd, blocks, s);
+    if (n > 256 || V == 8) return launch<T, W, V, 512 / (64 * V), 1>(d, a, bwd, blocks, s);
+    return launch<T, W, V, V == 8 ? 1 : 256 / (64 * V), 1>(d, a, bwd, blocks, s);
+  }
+  if (n > 4096) return launch<T, W, 1, 32, 4>(d, a, bwd, blocks, s);
+  if (n > 2048) return launch<T, W, 1, 16, 4>(d, a, bwd, blocks, s);
+  if (n > 1024) return launch<T, W, 1, 32, 1>(d, a, bwd, blocks, s);
+  if (n > 512) return launch<T, W, 1, 16, 1>(d, a, bwd, blocks, s);
+  return launch<T, W, 1, 8, 1>(d, a, bwd, blocks, s);
+}
+
+template <class T, class W>
+int forward(const d3a_layer_norm_desc& d, hipStream_t stream) {
+  const Args a = args_of(d);
+  if (d.rows == 0) return 0;
+  if (d.n <= kLong) return dispatch<T, W>(d, a, false, 0, stream);
+  norm_long_kernel<T, W><<<(unsigned)(d.rows * d.members), 256, 0, stream>>>(a);
+  D3A_LAUNCH_CHECK("layer_norm");
+  return 0;
+}
+
+int64_t long_chunks(const d3a_layer_norm_desc& d) {
+  const int64_t blocks = (d.n + 63) / 64 * d.members;
+  return std::max<int64_t>(1, std::min<int64_t>((d.rows + 31) / 32, 2048 / blocks));
+}
+
+template <class T, class W>
+int backward(const d3a_layer_norm_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  Args a = args_of(d);
+  const bool cols = d.dw || d.db, is_long = d.n > kLong;
+  const int64_t parts = is_long ? long_chunks(d) : bwd_blocks(d);
+  if (cols) a.part = ws.take<float>(d.members * parts * 2 * d.n);
+  *bytes = ws.used;
+  if (dry || (!cols && (!d.dx || d.rows == 0))) return 0;
+  if (is_long) {
+    if (d.dx && d.rows > 0) {
+      norm_long_dx_kernel<T, W><<<(unsigned)(d.rows * d.members), 256, 0, stream>>>(a);
+      D3A_LAUNCH_CHECK("layer_norm_bwd");
+    }
+    if (cols) {
+      norm_long_cols_kernel<T><<<dim3((unsigned)((d.n + 63) / 64), (unsigned)parts, (unsigned)d.members), 256, 0,
+                                 stream>>>(a);
+      D3A_LAUNCH_CHECK("layer_norm_bwd");
+    }
+  } else {
+    if (dispatch<T, W>(d, a, true, parts, stream) != 0) return -1;
+  }
+  if (!cols) return 0;
+  norm_finish_kernel<W><<<dim3((unsigned)((2 * d.n + 63) / 64), (unsigned)d.members), 256, 0, stream>>>(
+      a, (int32_t)parts);
+  D3A_LAUNCH_CHECK("layer_norm_bwd");
+  return 0;
+}
+
+int call_bwd(const d3a_layer_norm_desc* d, bool dry, hipStream_t stream, int64_t* bytes) {
+  Arena ws{dry ? nullptr : static_cast<char*>(d->ws)};
+  if (d->dtype == D3A_F32) return backward<float, float>(*d, ws, dry, stream, bytes);
+  if (d->wtype == D3A_F32) return backward<__bf16, float>(*d, ws, dry, stream, bytes);
+  return backward<__bf16, __bf16>(*d, ws, dry, stream, bytes);
+}
+
+}  // namespace
+}  // namespace d3a
+
+extern "C" {
+
+int d3a_layer_norm_workspace(const d3a_layer_norm_desc* d, int32_t backward, int64_t* bytes) {
+  if (d3a::check(d, backward != 0) != 0) return -1;
+  D3A_CHECK_ARG(bytes, "layer_norm: null size");
+  *bytes = 0;
+  return backward ? d3a::call_bwd(d, true, nullptr, bytes) : 0;
+}
+
+int d3a_layer_norm(const d3a_layer_norm_desc* d, void* stream) {
+  if (d3a::check(d, false) != 0) return -1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (d->dtype == D3A_F32) return d3a::forward<float, float>(*d, s);
+  if (d->wtype == D3A_F32) return d3a::forward<__bf16, float>(*d, s);
+  return d3a::forward<__bf16, __bf16>(*d, s);
+}
+
+int d3a_layer_norm_bwd(const d3a_layer_norm_desc* d, void* stream) {
+  if (d3a::check(d, true) != 0) return -1;
+  int64_t need = 0;
+  if (d3a::call_bwd(d, true, nullptr, &need) != 0) return -1;
+  D3A_CHECK_ARG(need == 0 || (d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 255) == 0),
+                "layer_norm: workspace of %lld bytes (256-byte aligned) needed", (long long)need);
+  return d3a::call_bwd(d, false, static_cast<hipStream_t>(stream), &need);
+}
+
+}  // extern "C"

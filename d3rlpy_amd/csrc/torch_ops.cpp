@@ -37,6 +37,15 @@
 //   squashed_gaussian_sample(mu, logstd, eps, lo, hi) / _backward
 //                                  SquashedNormalPolicy.sample_with_log_prob
 //                                  (distributions.py:112-135, policies.py:196-216)
+//   layer_norm(x, w, b, eps) / _backward
+//                                  torch.nn.LayerNorm over the last axis, of every
+//                                  ensemble member; float32 or bfloat16
+//   gated_mlp(x, Wg, Wu, Wd, ..)  / _backward
+//                                  (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd of
+//                                  every ensemble member; float32 or bfloat16
+//   linear_cross_entropy(x, W, target, b, ..) / _backward
+//                                  cross_entropy(x W^T + b, target) without the
+//                                  logits in memory; float32 or bfloat16
 //   cql_update_step(graph, state)  one whole CQLImpl update (CQL._update,
 //                                  algos/cql.py:234-258 over cql_impl.py:119-243,
 //                                  sac_impl.py, ddpg_impl.py): the step's HIP
@@ -48,9 +57,12 @@
 //                                  same for the TD3+BC, BCQ and DiscreteCQL Impls.
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
 
+#include <array>
 #include <cmath>
+#include <tuple>
 #include <vector>
 
 #include "d3rlpy_amd.h"
@@ -567,6 +579,485 @@ std::vector<at::Tensor> squashed_gaussian_sample_backward_meta(
   return {at::empty_like(mu), at::empty_like(mu)};
 }
 
+// ---- layer norm, gated feed-forward block, linear cross entropy ------------------
+// float32 or bfloat16 tensors on one device, whose current stream runs the call.
+using OptTensor = c10::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+const void* ptr_or_null(const OptTensor& t) { return given(t) ? t->data_ptr() : nullptr; }
+
+void* ptr_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+int32_t dtype_code(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", name,
+              " must be float32 or bfloat16, got ", t.scalar_type());
+  return t.scalar_type() == at::kFloat ? D3A_F32 : D3A_BF16;
+}
+
+void check_like(const at::Tensor& t, const at::Tensor& x, const char* op, const char* name) {
+  TORCH_CHECK(t.device() == x.device(), op, ": ", name, " is on ", t.device(), ", x on ", x.device());
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), op, ": ", name, " is ", t.scalar_type(), ", x ",
+              x.scalar_type());
+}
+
+void check_gpu(const at::Tensor& x, const char* op) {
+  TORCH_CHECK(x.is_cuda(), op, ": x must be a HIP (cuda) tensor");
+}
+
+// The rows of a [members][rows][n] array (members leading only where
+// `members` > 1), read in place where one row and one member stride say where
+// they are; copied otherwise.
+struct RowsOf {
+  at::Tensor t;
+  int64_t ld, s, rows;
+};
+
+RowsOf rows_of(const at::Tensor& t, int64_t members) {
+  const int64_t n = t.size(-1), lead = members > 1 ? 1 : 0;
+  RowsOf r;
+  r.rows = n > 0 ? t.numel() / (n * members) : 0;
+  bool in_place = t.dim() == 2 + lead && (t.stride(-1) == 1 || n == 1) &&
+                  (r.rows <= 1 || t.stride(-2) >= n);
+  if (in_place && lead) in_place = t.stride(0) > 0;
+  r.t = in_place ? t : t.contiguous();
+  r.ld = in_place && r.rows > 1 ? t.stride(-2) : n;
+  r.s = !lead ? 0 : in_place ? t.stride(0) : r.rows * n;
+  return r;
+}
+
+at::Tensor workspace(int64_t bytes, const at::Tensor& like) {
+  return at::empty({bytes}, like.options().dtype(at::kByte));
+}
+
+// x [.., n] (w [n]) or [members, .., n] (w [members, n]) -> rows, members
+int64_t norm_members(const at::Tensor& x, const OptTensor& w, const OptTensor& b) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "layer_norm: empty last dimension");
+  int64_t members = 1;
+  for (const OptTensor* p : {&w, &b}) {
+    if (!given(*p)) continue;
+    const at::Tensor& v = **p;
+    TORCH_CHECK(v.dim() == 1 || v.dim() == 2, "layer_norm: weight and bias [n] or [members, n]");
+    TORCH_CHECK(v.size(-1) == x.size(-1), "layer_norm: weight / bias of ", v.size(-1), " values, x rows of ",
+                x.size(-1));
+    TORCH_CHECK(v.device() == x.device(), "layer_norm: weight / bias on ", v.device(), ", x on ", x.device());
+    if (v.dim() == 2) {
+      TORCH_CHECK(x.dim() >= 2 && x.size(0) == v.size(0), "layer_norm: x [members, .., n] for weight [members, n]");
+      members = v.size(0);
+    }
+  }
+  if (given(w) && given(b))
+    TORCH_CHECK(w->sizes() == b->sizes() && w->scalar_type() == b->scalar_type(),
+                "layer_norm: weight and bias of one shape and dtype");
+  return members;
+}
+
+d3a_layer_norm_desc norm_desc(const at::Tensor& x, const RowsOf& rx, const OptTensor& w, const OptTensor& b,
+                              int64_t members, const at::Tensor& stats, double eps) {
+  d3a_layer_norm_desc d{};
+  d.dtype = dtype_code(x, "layer_norm", "x");
+  d.wtype = given(w) ? dtype_code(*w, "layer_norm", "weight")
+                     : given(b) ? dtype_code(*b, "layer_norm", "bias") : d.dtype;
+  d.x = rx.t.data_ptr();
+  d.w = ptr_or_null(w);
+  d.b = ptr_or_null(b);
+  d.rows = rx.rows;
+  d.n = x.size(-1);
+  d.members = members;
+  d.ldx = rx.ld;
+  d.sx = rx.s;
+  d.eps = eps;
+  if (stats.numel() > 0) {
+    d.mean = stats.data_ptr<float>();
+    d.rstd = d.mean + members * rx.rows;
+  }
+  return d;
+}
+
+OptTensor contig(const OptTensor& t) { return given(t) ? OptTensor(contig(*t)) : t; }
+
+// -> (y, stats [2, members, rows]: the rows' mean and 1 / standard deviation)
+std::tuple<at::Tensor, at::Tensor> layer_norm_hip(const at::Tensor& x, const OptTensor& w_in, const OptTensor& b_in,
+                                                  double eps) {
+  check_gpu(x, "layer_norm");
+  TORCH_CHECK(eps >= 0, "layer_norm: eps must not be negative");
+  const c10::DeviceGuard guard(x.device());
+  const OptTensor w = contig(w_in), b = contig(b_in);
+  const int64_t members = norm_members(x, w, b);
+  const RowsOf rx = rows_of(x, members);
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  at::Tensor stats = at::empty({2, members, rx.rows}, x.options().dtype(at::kFloat));
+  d3a_layer_norm_desc d = norm_desc(x, rx, w, b, members, stats, eps);
+  d.y = y.data_ptr();
+  check_rc(d3a_layer_norm(&d, cur_stream()), "d3rlpy_amd::layer_norm");
+  return {y, stats};
+}
+
+std::tuple<at::Tensor, at::Tensor> layer_norm_meta(const at::Tensor& x, const OptTensor& w, const OptTensor& b,
+                                                   double) {
+  const int64_t members = norm_members(x, w, b);
+  return {at::empty(x.sizes(), x.options()),
+          at::empty({2, members, x.numel() / (x.size(-1) * members)}, x.options().dtype(at::kFloat))};
+}
+
+// the gradients of x, w, b that `wanted` asks for; the others undefined
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_hip(
+    const at::Tensor& g, const at::Tensor& x, const OptTensor& w_in, const OptTensor& b_in,
+    const at::Tensor& stats, std::array<bool, 3> wanted) {
+  check_gpu(x, "layer_norm_backward");
+  check_like(g, x, "layer_norm_backward", "grad");
+  TORCH_CHECK(g.sizes() == x.sizes(), "layer_norm_backward: grad must have x's shape");
+  const c10::DeviceGuard guard(x.device());
+  const OptTensor w = contig(w_in), b = contig(b_in);
+  const int64_t members = norm_members(x, w, b);
+  const RowsOf rx = rows_of(x, members), rg = rows_of(g, members);
+  check_f32_gpu(stats, "stats");
+  TORCH_CHECK(stats.device() == x.device() && stats.numel() == 2 * members * rx.rows,
+              "layer_norm_backward: stats of another forward");
+  d3a_layer_norm_desc d = norm_desc(x, rx, w, b, members, stats, 0.0);
+  d.dy = rg.t.data_ptr();
+  d.lddy = rg.ld;
+  d.sdy = rg.s;
+  at::Tensor dx, dw, db;
+  if (wanted[0]) dx = at::empty(x.sizes(), x.options());
+  if (wanted[1] && given(w)) dw = at::empty_like(*w);
+  if (wanted[2] && given(b)) db = at::empty_like(*b);
+  d.dx = ptr_or_null(dx);
+  d.dw = ptr_or_null(dw);
+  d.db = ptr_or_null(db);
+  check_rc(d3a_layer_norm_workspace(&d, 1, &d.ws_bytes), "d3rlpy_amd::layer_norm_backward");
+  at::Tensor ws;
+  if (d.ws_bytes > 0) {
+    ws = workspace(d.ws_bytes, x);
+    d.ws = ws.data_ptr();
+  }
+  check_rc(d3a_layer_norm_bwd(&d, cur_stream()), "d3rlpy_amd::layer_norm_backward");
+  return {dx, dw, db};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_meta(
+    const at::Tensor&, const at::Tensor& x, const OptTensor& w, const OptTensor& b, const at::Tensor&,
+    std::array<bool, 3> wanted) {
+  at::Tensor dx, dw, db;
+  if (wanted[0]) dx = at::empty(x.sizes(), x.options());
+  if (wanted[1] && given(w)) dw = at::empty_like(*w);
+  if (wanted[2] && given(b)) db = at::empty_like(*b);
+  return {dx, dw, db};
+}
+
+int32_t activation_code(c10::string_view a) {
+  if (a == "silu") return D3A_ACT_SILU;
+  if (a == "gelu") return D3A_ACT_GELU;
+  if (a == "relu") return D3A_ACT_RELU;
+  TORCH_CHECK(false, "gated_mlp: activation must be 'silu', 'gelu' or 'relu', got '", std::string(a), "'");
+}
+
+// the sizes of a gated block, checked
+struct Gated {
+  int64_t members, rows, n_in, n_hidden, n_out;
+  bool shared;                 // one x for all members
+  std::vector<int64_t> y_shape;
+};
+
+Gated gated_shape(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu, const at::Tensor& Wd,
+                  const OptTensor& bg, const OptTensor& bu, const OptTensor& bd) {
+  Gated s;
+  const bool single = Wg.dim() == 2;
+  TORCH_CHECK(single || Wg.dim() == 3, "gated_mlp: Wg [hidden, in] or [members, hidden, in]");
+  TORCH_CHECK(Wu.sizes() == Wg.sizes(), "gated_mlp: Wu must have Wg's shape");
+  TORCH_CHECK(Wd.dim() == Wg.dim() && Wd.size(-1) == Wg.size(-2) && (single || Wd.size(0) == Wg.size(0)),
+              "gated_mlp: Wd [out, hidden] or [members, out, hidden]");
+  s.members = single ? 1 : Wg.size(0);
+  s.n_in = Wg.size(-1);
+  s.n_hidden = Wg.size(-2);
+  s.n_out = Wd.size(-2);
+  TORCH_CHECK(s.members >= 1 && s.n_in >= 1 && s.n_hidden >= 1 && s.n_out >= 1, "gated_mlp: empty weight");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == s.n_in, "gated_mlp: x has ", x.dim() ? x.size(-1) : 0,
+              " features, Wg expects ", s.n_in);
+  s.shared = !single && x.dim() == 2;
+  TORCH_CHECK(single || s.shared || (x.dim() >= 3 && x.size(0) == s.members),
+              "gated_mlp: x [rows, in] or [members, .., in] for weights of ", s.members, " members");
+  s.rows = x.numel() / s.n_in / (single || s.shared ? 1 : s.members);
+  s.y_shape = x.sizes().vec();
+  s.y_shape.back() = s.n_out;
+  if (s.shared) s.y_shape.insert(s.y_shape.begin(), s.members);
+  const int64_t width[3] = {s.n_hidden, s.n_hidden, s.n_out};
+  const OptTensor* bias[3] = {&bg, &bu, &bd};
+  for (int i = 0; i < 3; ++i)
+    if (given(*bias[i]))
+      TORCH_CHECK((*bias[i])->dim() == Wg.dim() - 1 && (*bias[i])->size(-1) == width[i] &&
+                      (single || (*bias[i])->size(0) == s.members),
+                  "gated_mlp: a bias must be [n] or [members, n] of its layer");
+  return s;
+}
+
+struct GatedCall {
+  RowsOf x, wg, wu, wd, dy;
+  OptTensor bg, bu, bd;
+  d3a_gated_mlp_desc d{};
+};
+
+void gated_call(GatedCall& c, const Gated& s, const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                c10::string_view act) {
+  check_like(Wg, x, "gated_mlp", "Wg");
+  check_like(Wu, x, "gated_mlp", "Wu");
+  check_like(Wd, x, "gated_mlp", "Wd");
+  if (given(bg)) check_like(*bg, x, "gated_mlp", "bg");
+  if (given(bu)) check_like(*bu, x, "gated_mlp", "bu");
+  if (given(bd)) check_like(*bd, x, "gated_mlp", "bd");
+  // (weights of one member [1, f, d] are read as [f, d])
+  const int64_t C = s.members;
+  c.x = s.shared ? rows_of(x, 1) : rows_of(C == 1 && x.dim() > 2 ? x.reshape({s.rows, s.n_in}) : x, C);
+  auto weight = [&](const at::Tensor& w) { return rows_of(C == 1 && w.dim() == 3 ? w.squeeze(0) : w, C); };
+  c.wg = weight(Wg);
+  c.wu = weight(Wu);
+  c.wd = weight(Wd);
+  c.bg = contig(bg);
+  c.bu = contig(bu);
+  c.bd = contig(bd);
+  d3a_gated_mlp_desc& d = c.d;
+  d.dtype = dtype_code(x, "gated_mlp", "x");
+  d.act = activation_code(act);
+  d.rows = s.rows;
+  d.n_in = s.n_in;
+  d.n_hidden = s.n_hidden;
+  d.n_out = s.n_out;
+  d.members = C;
+  d.x = c.x.t.data_ptr();
+  d.ldx = c.x.ld;
+  d.sx = s.shared ? 0 : c.x.s;
+  d.Wg = c.wg.t.data_ptr();
+  d.ldWg = c.wg.ld;
+  d.sWg = c.wg.s;
+  d.Wu = c.wu.t.data_ptr();
+  d.ldWu = c.wu.ld;
+  d.sWu = c.wu.s;
+  d.Wd = c.wd.t.data_ptr();
+  d.ldWd = c.wd.ld;
+  d.sWd = c.wd.s;
+  d.bg = ptr_or_null(c.bg);
+  d.bu = ptr_or_null(c.bu);
+  d.bd = ptr_or_null(c.bd);
+}
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// -> (y, pre [2, members, rows, hidden rounded up to 8]: g and u; empty unless `keep`)
+std::tuple<at::Tensor, at::Tensor> gated_mlp_hip(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                                                 const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
+                                                 const OptTensor& bd, c10::string_view act, bool keep) {
+  check_gpu(x, "gated_mlp");
+  const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
+  const c10::DeviceGuard guard(x.device());
+  GatedCall c;
+  gated_call(c, s, x, Wg, Wu, Wd, bg, bu, bd, act);
+  at::Tensor y = at::empty(s.y_shape, x.options());
+  at::Tensor pre = keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options())
+                        : at::empty({0}, x.options());
+  c.d.y = y.data_ptr();
+  if (pre.numel() > 0) {
+    c.d.g = pre.select(0, 0).data_ptr();
+    c.d.u = pre.select(0, 1).data_ptr();
+  }
+  check_rc(d3a_gated_mlp_workspace(&c.d, 0, &c.d.ws_bytes), "d3rlpy_amd::gated_mlp");
+  const at::Tensor ws = workspace(c.d.ws_bytes, x);
+  c.d.ws = ws.data_ptr();
+  check_rc(d3a_gated_mlp(&c.d, cur_stream()), "d3rlpy_amd::gated_mlp");
+  return {y, pre};
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_mlp_meta(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                                                  const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
+                                                  const OptTensor& bd, c10::string_view act, bool keep) {
+  const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
+  activation_code(act);
+  return {at::empty(s.y_shape, x.options()),
+          keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options()) : at::empty({0}, x.options())};
+}
+
+using Seven = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+std::array<at::Tensor, 7> gated_grads(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                                      const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
+                                      const OptTensor& bd, const std::array<bool, 7>& wanted) {
+  std::array<at::Tensor, 7> o;
+  const at::Tensor* t[4] = {&x, &Wg, &Wu, &Wd};
+  const OptTensor* b[3] = {&bg, &bu, &bd};
+  for (int i = 0; i < 4; ++i)
+    if (wanted[i]) o[i] = at::empty(t[i]->sizes(), t[i]->options());
+  for (int i = 0; i < 3; ++i)
+    if (wanted[4 + i] && given(*b[i])) o[4 + i] = at::empty((*b[i])->sizes(), (*b[i])->options());
+  return o;
+}
+
+// the gradients of x, Wg, Wu, Wd, bg, bu, bd that `wanted` asks for; the others undefined
+Seven gated_mlp_backward_hip(const at::Tensor& g, const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                             const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                             const at::Tensor& pre, c10::string_view act, std::array<bool, 7> wanted) {
+  check_gpu(x, "gated_mlp_backward");
+  const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
+  check_like(g, x, "gated_mlp_backward", "grad");
+  check_like(pre, x, "gated_mlp_backward", "pre");
+  TORCH_CHECK(g.sizes() == at::IntArrayRef(s.y_shape), "gated_mlp_backward: grad must have the output's shape");
+  TORCH_CHECK(pre.is_contiguous() && pre.numel() == 2 * s.members * s.rows * round8(s.n_hidden),
+              "gated_mlp_backward: pre of a forward with keep = True");
+  const c10::DeviceGuard guard(x.device());
+  GatedCall c;
+  gated_call(c, s, x, Wg, Wu, Wd, bg, bu, bd, act);
+  c.dy = rows_of(s.members == 1 ? g.reshape({s.rows, s.n_out}) : g, s.members);
+  c.d.dy = c.dy.t.data_ptr();
+  c.d.lddy = c.dy.ld;
+  c.d.sdy = c.dy.s;
+  if (pre.numel() > 0) {
+    c.d.g = pre.data_ptr();
+    c.d.u = pre.select(0, 1).data_ptr();
+  }
+  std::array<at::Tensor, 7> o = gated_grads(x, Wg, Wu, Wd, bg, bu, bd, wanted);
+  void** to[7] = {&c.d.dx, &c.d.dWg, &c.d.dWu, &c.d.dWd, &c.d.dbg, &c.d.dbu, &c.d.dbd};
+  for (int i = 0; i < 7; ++i) *to[i] = ptr_or_null(o[i]);
+  check_rc(d3a_gated_mlp_workspace(&c.d, 1, &c.d.ws_bytes), "d3rlpy_amd::gated_mlp_backward");
+  const at::Tensor ws = workspace(c.d.ws_bytes, x);
+  c.d.ws = ws.data_ptr();
+  check_rc(d3a_gated_mlp_bwd(&c.d, cur_stream()), "d3rlpy_amd::gated_mlp_backward");
+  return {o[0], o[1], o[2], o[3], o[4], o[5], o[6]};
+}
+
+Seven gated_mlp_backward_meta(const at::Tensor&, const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                              const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                              const at::Tensor&, c10::string_view, std::array<bool, 7> wanted) {
+  std::array<at::Tensor, 7> o = gated_grads(x, Wg, Wu, Wd, bg, bu, bd, wanted);
+  return {o[0], o[1], o[2], o[3], o[4], o[5], o[6]};
+}
+
+int32_t reduction_code(c10::string_view r) {
+  if (r == "none") return 0;
+  if (r == "mean") return 1;
+  if (r == "sum") return 2;
+  TORCH_CHECK(false, "linear_cross_entropy: reduction must be 'none', 'mean' or 'sum', got '", std::string(r), "'");
+}
+
+void xent_shape(const at::Tensor& x, const at::Tensor& W, const at::Tensor& target, const OptTensor& b) {
+  TORCH_CHECK(W.dim() == 2 && W.size(0) >= 1 && W.size(1) >= 1, "linear_cross_entropy: W [vocab, in]");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == W.size(1), "linear_cross_entropy: x has ",
+              x.dim() ? x.size(-1) : 0, " features, W expects ", W.size(1));
+  TORCH_CHECK(target.sizes() == x.sizes().slice(0, x.dim() - 1),
+              "linear_cross_entropy: one target for each row of x");
+  TORCH_CHECK(target.scalar_type() == at::kLong, "linear_cross_entropy: target must be int64");
+  if (given(b)) TORCH_CHECK(b->dim() == 1 && b->size(0) == W.size(0), "linear_cross_entropy: b [vocab]");
+}
+
+struct XentCall {
+  RowsOf x, w;
+  OptTensor b;
+  at::Tensor target;
+  d3a_linear_xent_desc d{};
+};
+
+void xent_call(XentCall& c, const at::Tensor& x, const at::Tensor& W, const at::Tensor& target, const OptTensor& b,
+               int64_t ignore, c10::string_view reduction) {
+  xent_shape(x, W, target, b);
+  check_like(W, x, "linear_cross_entropy", "W");
+  if (given(b)) check_like(*b, x, "linear_cross_entropy", "b");
+  TORCH_CHECK(target.device() == x.device(), "linear_cross_entropy: target is on ", target.device(), ", x on ",
+              x.device());
+  c.x = rows_of(x.dim() == 2 ? x : x.reshape({target.numel(), x.size(-1)}), 1);
+  c.w = rows_of(W, 1);
+  c.b = contig(b);
+  c.target = contig(target);
+  d3a_linear_xent_desc& d = c.d;
+  d.dtype = dtype_code(x, "linear_cross_entropy", "x");
+  d.reduction = reduction_code(reduction);
+  d.x = c.x.t.data_ptr();
+  d.W = c.w.t.data_ptr();
+  d.b = ptr_or_null(c.b);
+  d.target = c.target.data_ptr<int64_t>();
+  d.rows = c.x.rows;
+  d.n_in = W.size(1);
+  d.vocab = W.size(0);
+  d.ldx = c.x.ld;
+  d.ldW = c.w.ld;
+  d.ignore_index = ignore;
+}
+
+// -> (loss [..] or [], lse [..], scale [1]: the factor of a row's gradient)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_hip(
+    const at::Tensor& x, const at::Tensor& W, const at::Tensor& target, const OptTensor& b, int64_t ignore,
+    c10::string_view reduction) {
+  check_gpu(x, "linear_cross_entropy");
+  const c10::DeviceGuard guard(x.device());
+  XentCall c;
+  xent_call(c, x, W, target, b, ignore, reduction);
+  const auto f = x.options().dtype(at::kFloat);
+  at::Tensor rows = at::empty(target.sizes(), f), lse = at::empty(target.sizes(), f), scale = at::empty({1}, f);
+  at::Tensor out = c.d.reduction == 0 ? rows : at::empty({}, f);
+  c.d.loss = rows.data_ptr<float>();
+  c.d.lse = lse.data_ptr<float>();
+  c.d.scale = scale.data_ptr<float>();
+  c.d.out = out.data_ptr<float>();
+  check_rc(d3a_linear_xent_workspace(&c.d, 0, &c.d.ws_bytes), "d3rlpy_amd::linear_cross_entropy");
+  const at::Tensor ws = workspace(c.d.ws_bytes, x);
+  c.d.ws = ws.data_ptr();
+  check_rc(d3a_linear_xent(&c.d, cur_stream()), "d3rlpy_amd::linear_cross_entropy");
+  return {out, lse, scale};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_meta(
+    const at::Tensor& x, const at::Tensor& W, const at::Tensor& target, const OptTensor& b, int64_t,
+    c10::string_view reduction) {
+  xent_shape(x, W, target, b);
+  const auto f = x.options().dtype(at::kFloat);
+  return {reduction_code(reduction) == 0 ? at::empty(target.sizes(), f) : at::empty({}, f),
+          at::empty(target.sizes(), f), at::empty({1}, f)};
+}
+
+// the gradients of x, W, b that `wanted` asks for; the others undefined
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backward_hip(
+    const at::Tensor& g_in, const at::Tensor& x, const at::Tensor& W, const at::Tensor& target, const OptTensor& b,
+    const at::Tensor& lse, const at::Tensor& scale, int64_t ignore, c10::string_view reduction,
+    std::array<bool, 3> wanted) {
+  check_gpu(x, "linear_cross_entropy_backward");
+  const c10::DeviceGuard guard(x.device());
+  XentCall c;
+  xent_call(c, x, W, target, b, ignore, reduction);
+  const at::Tensor g = contig(g_in);
+  check_f32_gpu(g, "grad");
+  check_f32_gpu(lse, "lse");
+  check_f32_gpu(scale, "scale");
+  TORCH_CHECK(g.device() == x.device() && lse.device() == x.device() && scale.device() == x.device(),
+              "linear_cross_entropy_backward: tensors on several devices");
+  TORCH_CHECK(lse.numel() == c.d.rows && scale.numel() == 1 && g.numel() == (c.d.reduction == 0 ? c.d.rows : 1),
+              "linear_cross_entropy_backward: grad of the loss, lse and scale of its forward");
+  c.d.gloss = g.data_ptr<float>();
+  c.d.lse = lse.data_ptr<float>();
+  c.d.scale = scale.data_ptr<float>();
+  // (written by the forward alone)
+  c.d.loss = c.d.lse;
+  c.d.out = c.d.scale;
+  at::Tensor dx, dW, db;
+  if (wanted[0]) dx = at::empty(x.sizes(), x.options());
+  if (wanted[1]) dW = at::empty(W.sizes(), W.options());
+  if (wanted[2] && given(b)) db = at::empty(b->sizes(), b->options());
+  c.d.dx = ptr_or_null(dx);
+  c.d.dW = ptr_or_null(dW);
+  c.d.db = ptr_or_null(db);
+  check_rc(d3a_linear_xent_workspace(&c.d, 1, &c.d.ws_bytes), "d3rlpy_amd::linear_cross_entropy_backward");
+  const at::Tensor ws = workspace(c.d.ws_bytes, x);
+  c.d.ws = ws.data_ptr();
+  check_rc(d3a_linear_xent_bwd(&c.d, cur_stream()), "d3rlpy_amd::linear_cross_entropy_backward");
+  return {dx, dW, db};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backward_meta(
+    const at::Tensor&, const at::Tensor& x, const at::Tensor& W, const at::Tensor&, const OptTensor& b,
+    const at::Tensor&, const at::Tensor&, int64_t, c10::string_view, std::array<bool, 3> wanted) {
+  at::Tensor dx, dW, db;
+  if (wanted[0]) dx = at::empty(x.sizes(), x.options());
+  if (wanted[1]) dW = at::empty(W.sizes(), W.options());
+  if (wanted[2] && given(b)) db = at::empty(b->sizes(), b->options());
+  return {dx, dW, db};
+}
+
 // the captured update pipeline (a hipGraphExec_t owned by the caller's
 // torch.cuda.CUDAGraph, CUDAGraph.raw_cuda_graph_exec()) launched on the
 // current stream.  The graph draws its noise from the library's own Philox
@@ -605,6 +1096,19 @@ TORCH_LIBRARY(d3rlpy_amd, m) {
         "float max_logstd) -> Tensor[]");
   m.def("squashed_gaussian_sample_backward(Tensor grad_action, Tensor grad_log_prob, Tensor mu, "
         "Tensor logstd, Tensor eps, float min_logstd, float max_logstd) -> Tensor[]");
+  m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
+  m.def("layer_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, "
+        "bool[3] wanted) -> (Tensor, Tensor, Tensor)");
+  m.def("gated_mlp(Tensor x, Tensor Wg, Tensor Wu, Tensor Wd, Tensor? bg, Tensor? bu, Tensor? bd, "
+        "str activation, bool keep) -> (Tensor, Tensor)");
+  m.def("gated_mlp_backward(Tensor grad, Tensor x, Tensor Wg, Tensor Wu, Tensor Wd, Tensor? bg, "
+        "Tensor? bu, Tensor? bd, Tensor pre, str activation, bool[7] wanted) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy(Tensor x, Tensor W, Tensor target, Tensor? b, int ignore_index, "
+        "str reduction) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_cross_entropy_backward(Tensor grad, Tensor x, Tensor W, Tensor target, Tensor? b, "
+        "Tensor lse, Tensor scale, int ignore_index, str reduction, bool[3] wanted) -> "
+        "(Tensor, Tensor, Tensor)");
   m.def("cql_update_step(int graph_exec, Tensor(a!)[] state) -> ()");
   m.def("update_step(int graph_exec, Tensor(a!)[] state) -> ()");
 }
@@ -628,6 +1132,12 @@ TORCH_LIBRARY_IMPL(d3rlpy_amd, CUDA, m) {
   m.impl("iqn_cos_embed_backward", &iqn_cos_embed_backward_hip);
   m.impl("squashed_gaussian_sample", &squashed_gaussian_sample_hip);
   m.impl("squashed_gaussian_sample_backward", &squashed_gaussian_sample_backward_hip);
+  m.impl("layer_norm", &layer_norm_hip);
+  m.impl("layer_norm_backward", &layer_norm_backward_hip);
+  m.impl("gated_mlp", &gated_mlp_hip);
+  m.impl("gated_mlp_backward", &gated_mlp_backward_hip);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_hip);
+  m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_hip);
   m.impl("cql_update_step", &update_step_hip);
   m.impl("update_step", &update_step_hip);
 }
@@ -651,4 +1161,10 @@ TORCH_LIBRARY_IMPL(d3rlpy_amd, Meta, m) {
   m.impl("iqn_cos_embed_backward", &iqn_cos_embed_backward_meta);
   m.impl("squashed_gaussian_sample", &squashed_gaussian_sample_meta);
   m.impl("squashed_gaussian_sample_backward", &squashed_gaussian_sample_backward_meta);
+  m.impl("layer_norm", &layer_norm_meta);
+  m.impl("layer_norm_backward", &layer_norm_backward_meta);
+  m.impl("gated_mlp", &gated_mlp_meta);
+  m.impl("gated_mlp_backward", &gated_mlp_backward_meta);
+  m.impl("linear_cross_entropy", &linear_cross_entropy_meta);
+  m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_meta);
 }

@@ -1,0 +1,365 @@
+// Softmax cross entropy of a linear head over a large vocabulary, forward and
+// backward, without the logits in memory:
+//
+//   z = x W^T + b,  lse_r = log sum_v exp z_rv,  loss_r = lse_r - z_r,target
+//   dz_rv = (exp(z_rv - lse_r) - [v = target_r]) dloss_r
+//   dx = dz W,  dW = dz^T x,  db_v = sum_r dz_rv
+//
+// Forward: the tiles of mm.hpp over (rows, vocabulary); a tile's epilogue
+// reduces each of its rows to (max, sum of exp(z - max)) and picks the
+// target's logit, and a second pass joins the tiles of a row.  Backward: the
+// logits again, a piece of the vocabulary at a time, whose epilogue writes dz
+// of the piece in the operand layout of the two products that follow; the
+// piece is cut so that dz stays within kPieceBytes.  All products are bound by
+// the matrix cores.
+//
+// A row whose target is ignore_index has loss 0 and no gradient, whatever its
+// logits are; a row whose target is outside the vocabulary has loss NaN and a
+// NaN gradient.
+#include "mm_host.hpp"
+#include "../../include/d3rlpy_amd.h"
+
+namespace d3a {
+namespace {
+
+using namespace mm;
+
+constexpr int64_t kPieceBytes = 512LL << 20;
+
+template <int NP>
+__device__ __forceinline__ float exp_(float x) {
+  // (one bfloat16 plane: 2 ulp of the hardware exponential are far below dz's
+  // own rounding, and below the float32 sum's)
+  return NP == 1 ? __expf(x) : expf(x);
+}
+
+// (max, sum of exp(z - max)) of a + b; an empty side has max -inf, sum 0
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float a = m == top ? s : s * expf(m - top);
+  const float b = m2 == top ? s2 : s2 * expf(m2 - top);
+  m = top;
+  s = a + b;
+}
+
+// One (max, sum) a row and wave column; z of the target.
+template <class T, int NP>
+struct LsePartEpi {
+  const T* bias;
+  const int64_t* target;
+  float2* part;     // [columns of waves][M]
+  float* ztarget;   // [M]
+  int32_t v0;       // vocabulary index of column 0
+  int32_t wave_cols;  // columns a wave covers
+
+  template <class C>
+  __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
+#pragma unroll
+    for (int i = 0; i < C::MT; ++i) {
+      const int m = t.m0 + 32 * i + (t.lane & 31);
+      const int64_t want = m < t.M ? target[m] - v0 : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int n = t.n0 + 32 * j + 8 * (r / 4) + 4 * (t.lane >> 5) + r % 4;
+          float v = acc[i][j][r];
+          if (bias) v += (float)bias[min(n, t.N - 1)];
+          if (n == want && n < t.N) ztarget[m] = v;
+          v = n < t.N ? v : -INFINITY;
+          acc[i][j][r] = v;
+          top = fmaxf(top, v);
+        }
+      // a row of -inf alone: any finite reference gives its sum of 0
+      const float ref = top == -INFINITY ? 0.f : top;
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += exp_<NP>(acc[i][j][r] - ref);
+      const float m2 = __shfl_xor(top, 32), s2 = __shfl_xor(s, 32);
+      join(top, s, m2, s2);
+      // (a wave past the last column has no part)
+      if (t.lane < 32 && m < t.M && t.n0 < t.N)
+        part[(int64_t)(t.n0 / wave_cols) * t.M + m] = make_float2(top, s);
+    }
+  }
+};
+
+// Joins a row's parts: 32 rows x 8 groups of parts a workgroup.
+__global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32_t parts, int32_t rows,
+                                                       const float* ztarget, const int64_t* target,
+                                                       int64_t vocab, int64_t ignore, float* lse,
+                                                       float* loss) {
+  __shared__ float2 red[256];
+  const int r = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  float m = -INFINITY, s = 0.f;
+  if (r < rows)
+    for (int p = g; p < parts; p += 8) {
+      const float2 v = part[(int64_t)p * rows + r];
+      join(m, s, v.x, v.y);
+    }
+  red[threadIdx.x] = make_float2(m, s);
+  __syncthreads();
+  if (g != 0 || r >= rows) return;
+  for (int k = 1; k < 8; ++k) {
+    const float2 v = red[32 * k + threadIdx.x];
+    join(m, s, v.x, v.y);
+  }
+  const float l = m + logf(s);
+  const int64_t t = target[r];
+  lse[r] = l;
+  loss[r] = t == ignore ? 0.f : t >= 0 && t < vocab ? l - ztarget[r] : NAN;
+}
+
+// The sum of the rows' losses (mean: over the counted rows, at least one), and
+// the factor of each row's gradient.  One workgroup: fixed order, float64.
+__global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* loss, const int64_t* target,
+                                                           int64_t ignore, int32_t rows, int32_t mean,
+                                                           float* out, float* scale) {
+  __shared__ double ps[16];
+  __shared__ int pn[16];
+  double s = 0.0;
+  int n = 0;
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    s += (double)loss[r];
+    n += target[r] != ignore;
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o);
+    n += __shfl_xor(n, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    ps[threadIdx.x >> 6] = s;
+    pn[threadIdx.x >> 6] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  s = 0.0;
+  n = 0;
+  for (int k = 0; k < 16; ++k) {
+    s += ps[k];
+    n += pn[k];
+  }
+  const double by = mean ? (double)max(n, 1) : 1.0;
+  out[0] = (float)(s / by);
+  scale[0] = (float)(1.0 / by);
+}
+
+// dz of a piece of the vocabulary, as operand planes
+template <class T, int NP>
+struct DzEpi {
+  const T* bias;
+  const int64_t* target;
+  const float *lse, *gloss, *scale;  // scale: null = 1
+  int64_t s_gloss;                   // 1 (a row's own) or 0 (one for all)
+  int64_t ignore, vocab;
+  __bf16* dz;                        // planes, rows of ld
+  int64_t ld, s_part;
+  int32_t v0;
+
+  template <class C>
+  __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
+    const float by = scale ? scale[0] : 1.f;
+#pragma unroll
+    for (int i = 0; i < C::MT; ++i) {
+      const int m = t.m0 + 32 * i + (t.lane & 31);
+      if (m >= t.M) continue;
+      const int64_t y = target[m];
+      const bool on = y != ignore;
+      const float l = lse[m];
+      const float g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
+      const int64_t want = y - v0;
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = t.n0 + 32 * j + 8 * q + 4 * (t.lane >> 5);
+          if (n >= ld) continue;
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float z = acc[i][j][4 * q + r];
+            if (bias) z += (float)bias[min(n + r, t.N - 1)];
+            const float d = (exp_<NP>(z - l) - (n + r == want ? 1.f : 0.f)) * g;
+            v[r] = on && n + r < t.N ? d : 0.f;
+          }
+          store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
+        }
+    }
+  }
+};
+
+int check(const d3a_linear_xent_desc* d, bool bwd) {
+  D3A_CHECK_ARG(d, "linear_cross_entropy: null descriptor");
+  D3A_CHECK_ARG(d->dtype == D3A_F32 || d->dtype == D3A_BF16,
+                "linear_cross_entropy: dtype must be float32 or bfloat16");
+  D3A_CHECK_ARG(d->reduction >= 0 && d->reduction <= 2, "linear_cross_entropy: unknown reduction");
+  D3A_CHECK_ARG(d->rows >= 0 && d->n_in >= 1 && d->vocab >= 1, "linear_cross_entropy: sizes must be positive");
+  const int64_t top = (1LL << 31) - 4096;
+  D3A_CHECK_ARG(d->rows < top && d->n_in < top && d->vocab < top, "linear_cross_entropy: size too large");
+  D3A_CHECK_ARG(d->ldx >= d->n_in && d->ldW >= d->n_in, "linear_cross_entropy: row stride smaller than the row");
+  D3A_CHECK_ARG(d->W, "linear_cross_entropy: null weight");
+  if (d->rows > 0)
+    D3A_CHECK_ARG(d->x && d->target && d->lse && d->loss, "linear_cross_entropy: null operand");
+  D3A_CHECK_ARG(d->reduction == 0 || (d->out && d->scale), "linear_cross_entropy: a reduction needs out and scale");
+  if (bwd) D3A_CHECK_ARG(d->gloss || d->rows == 0, "linear_cross_entropy: null gradient");
+  return 0;
+}
+
+template <int NP>
+int wave_columns(TileSize s) {
+  typedef Tiles<NP> X;
+  return s == kLarge ? X::Large::TN : s == kMid ? X::Mid::TN : X::Small::TN;
+}
+
+template <class T, int NP>
+int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t R = d.rows, D = d.n_in, V = d.vocab;
+  Packer<T, NP> pack(ws);
+  Launch<LsePartEpi<T, NP>> L{};
+  L.n = 1;
+  Problem& p = L.p[0];
+  p.a = pack.operand(d.x, d.ldx, 0, 1, R, D);
+  p.b = pack.operand(d.W, d.ldW, 0, 1, V, D);
+  p.M = (int32_t)R;
+  p.N = (int32_t)V;
+  p.K = (int32_t)D;
+  p.batch = p.n_outer = p.n_inner = p.splits = 1;
+  const TileSize size = choose<NP>(L, false);
+  const int cols = wave_columns<NP>(size);
+  const int64_t parts = (V + cols - 1) / cols;
+  LsePartEpi<T, NP>& e = L.e[0];
+  e.bias = static_cast<const T*>(d.b);
+  e.target = d.target;
+  e.part = ws.take<float2>(parts * R);
+  e.ztarget = ws.take<float>(R);
+  e.wave_cols = cols;
+  *bytes = ws.used;
+  if (dry) return 0;
+  if (R > 0) {
+    if (pack.launch(stream) != 0) return -1;
+    if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy") != 0) return -1;
+    lse_join_kernel<<<(unsigned)((R + 31) / 32), 256, 0, stream>>>(
+        e.part, (int32_t)parts, (int32_t)R, e.ztarget, d.target, V, d.ignore_index, d.lse, d.loss);
+    D3A_LAUNCH_CHECK("linear_cross_entropy");
+  }
+  if (d.reduction != 0) {
+    loss_reduce_kernel<<<1, 1024, 0, stream>>>(d.loss, d.target, d.ignore_index, (int32_t)R,
+                                               d.reduction == 1, d.out, d.scale);
+    D3A_LAUNCH_CHECK("linear_cross_entropy");
+  }
+  return 0;
+}
+
+template <class T, int NP>
+int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t R = d.rows, D = d.n_in, V = d.vocab;
+  if (!d.dx && !d.dW && !d.db) {
+    *bytes = 0;
+    return 0;
+  }
+  Packer<T, NP> pack(ws);
+  const Operand x = pack.operand(d.x, d.ldx, 0, 1, R, D);
+  const Operand w = pack.operand(d.W, d.ldW, 0, 1, V, D);
+  // pieces of equal size, multiples of the widest tile
+  int64_t piece = std::max<int64_t>(kPieceBytes / (2 * NP * std::max<int64_t>(R, 1)), 256);
+  const int64_t n_pieces = (V + piece - 1) / piece;
+  piece = std::min<int64_t>(V, ((V + n_pieces - 1) / n_pieces + 255) / 256 * 256);
+  const int64_t ld = round8(piece);
+  Operand dz{};
+  dz.p = ws.take<__bf16>(NP * R * ld);
+  dz.ld = ld;
+  dz.s_part = R * ld;
+  float* sum = n_pieces > 1 && d.dx ? ws.take<float>(R * D) : nullptr;
+  const int64_t keep = ws.used;
+  if (!dry && R > 0 && pack.launch(stream) != 0) return -1;
+  for (int64_t v0 = 0, k = 0; v0 < V; v0 += piece, ++k) {
+    // (the pieces reuse one workspace: a stream runs them in order)
+    ws.used = keep;
+    const int64_t n = std::min(piece, V - v0);
+    const bool last = v0 + n == V;
+    Launch<DzEpi<T, NP>> L{};
+    L.n = 1;
+    Problem& p = L.p[0];
+    p.a = x;
+    p.b = w;
+    p.b.p += v0 * w.ld;
+    p.M = (int32_t)R;
+    p.N = (int32_t)n;
+    p.K = (int32_t)D;
+    p.batch = p.n_outer = p.n_inner = p.splits = 1;
+    DzEpi<T, NP>& e = L.e[0];
+    e.bias = d.b ? static_cast<const T*>(d.b) + v0 : nullptr;
+    e.target = d.target;
+    e.lse = d.lse;
+    e.gloss = d.gloss;
+    e.scale = d.reduction == 1 ? d.scale : nullptr;
+    e.s_gloss = d.reduction == 0 ? 1 : 0;
+    e.ignore = d.ignore_index;
+    e.vocab = V;
+    e.dz = const_cast<__bf16*>(dz.p);
+    e.ld = ld;
+    e.s_part = dz.s_part;
+    e.v0 = (int32_t)v0;
+
+    Products<T, NP> dx, dw;
+    if (d.dx) {
+      dx.add(dz, p.b, R, D, n, 1, 1, 1, d.dx, D, 0, nullptr, 0);
+      if (n_pieces > 1) {
+        dx.L.e[0].sum = sum;
+        dx.L.e[0].mode = last ? 4 : k == 0 ? 2 : 3;
+      }
+      dx.reserve(ws, n_pieces == 1);
+    }
+    if (d.dW) dw.add(dz, x, n, D, R, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0);
+    dw.reserve(ws, true);
+    Colsum<T, __bf16, NP> cs;
+    if (d.db) cs.add(dz.p, ld, 0, dz.s_part, R, n, 1, static_cast<T*>(d.db) + v0, 0);
+    cs.reserve(ws);
+    *bytes = std::max(*bytes, ws.used);
+    if (dry) continue;
+    if (R > 0) {
+      if (run<NP, false, false, false>(L, choose<NP>(L, false), stream, "linear_cross_entropy_bwd") != 0) return -1;
+      if (dx.template launch<false, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
+    }
+    if (dw.template launch<true, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
+    if (cs.launch(stream) != 0) return -1;
+  }
+  return 0;
+}
+
+int call(const d3a_linear_xent_desc* d, bool bwd, bool dry, hipStream_t stream, int64_t* bytes) {
+  Arena ws{dry ? nullptr : static_cast<char*>(d->ws)};
+  *bytes = 0;
+  if (d->dtype == D3A_F32)
+    return bwd ? backward<float, 3>(*d, ws, dry, stream, bytes) : forward<float, 3>(*d, ws, dry, stream, bytes);
+  return bwd ? backward<__bf16, 1>(*d, ws, dry, stream, bytes) : forward<__bf16, 1>(*d, ws, dry, stream, bytes);
+}
+
+int entry(const d3a_linear_xent_desc* d, bool bwd, void* stream) {
+  if (check(d, bwd) != 0) return -1;
+  int64_t need = 0;
+  if (call(d, bwd, true, nullptr, &need) != 0) return -1;
+  D3A_CHECK_ARG(need == 0 || (d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 255) == 0),
+                "linear_cross_entropy: workspace of %lld bytes (256-byte aligned) needed", (long long)need);
+  return call(d, bwd, false, static_cast<hipStream_t>(stream), &need);
+}
+
+}  // namespace
+}  // namespace d3a
+
+extern "C" {
+
+int d3a_linear_xent_workspace(const d3a_linear_xent_desc* d, int32_t backward, int64_t* bytes) {
+  if (d3a::check(d, backward != 0) != 0) return -1;
+  D3A_CHECK_ARG(bytes, "linear_cross_entropy: null size");
+  return d3a::call(d, backward != 0, true, nullptr, bytes);
+}
+
+int d3a_linear_xent(const d3a_linear_xent_desc* d, void* stream) { return d3a::entry(d, false, stream); }
+
+int d3a_linear_xent_bwd(const d3a_linear_xent_desc* d, void* stream) { return d3a::entry(d, true, stream); }
+
+}  // extern "C"

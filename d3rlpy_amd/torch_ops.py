@@ -12,7 +12,8 @@ There is no fallback: a missing library raises.
     q = ops.mlp_forward(x, [W0, W1, W2], [b0, b1, b2])
 
 The differentiable wrappers below (``linear``, ``logsumexp``, ``td_mse_loss``,
-``quantile_huber_loss``, ``iqn_cos_embed``, ``squashed_gaussian_sample``) let a
+``quantile_huber_loss``, ``iqn_cos_embed``, ``squashed_gaussian_sample``,
+``layer_norm``, ``gated_mlp``, ``linear_cross_entropy``) let a
 reference-shaped torch module — the Q functions, policy and losses of
 d3rlpy/models/torch and algos/torch — run its forward AND backward on the HIP
 kernels under ordinary ``loss.backward()``; tests/test_torch_ops.py checks a
@@ -21,8 +22,10 @@ CQL critic / SAC actor / QR / IQN loss written this way against the oracle.
 from __future__ import annotations
 
 import os
+from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libd3rlpy_amd_torch.so")
 _loaded = False
@@ -179,3 +182,96 @@ def squashed_gaussian_sample(mu, logstd, eps, min_logstd: float = -20.0,
     the noise given: raw = mu + eps * exp(clamp(logstd)) (policies.py:196-216,
     distributions.py:112-135); log_prob [B, 1]."""
     return _SquashedGaussian.apply(mu, logstd, eps, min_logstd, max_logstd)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps: float):
+        y, stats = load().layer_norm(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, stats = ctx.saved_tensors
+        return *load().layer_norm_backward(g, x, weight, bias, stats,
+                                           ctx.needs_input_grad[:3]), None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of ``x``
+    (torch.nn.LayerNorm's, var the mean of the centred squares).
+
+    ``x`` [.., n] with ``weight`` / ``bias`` [n], or [members, .., n] with
+    [members, n] (every member its own); float32 or bfloat16, the weights in
+    ``x``'s dtype or float32 and either may be None.  Statistics are float32."""
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+class _GatedMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, Wg, Wu, Wd, bg, bu, bd, activation: str, keep: bool):
+        y, pre = load().gated_mlp(x, Wg, Wu, Wd, bg, bu, bd, activation, keep)
+        ctx.activation = activation
+        ctx.save_for_backward(x, Wg, Wu, Wd, bg, bu, bd, pre)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, Wg, Wu, Wd, bg, bu, bd, pre = ctx.saved_tensors
+        return *load().gated_mlp_backward(g, x, Wg, Wu, Wd, bg, bu, bd, pre, ctx.activation,
+                                          ctx.needs_input_grad[:7]), None, None
+
+
+def gated_mlp(x: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, Wd: torch.Tensor,
+              bg: Optional[torch.Tensor] = None, bu: Optional[torch.Tensor] = None,
+              bd: Optional[torch.Tensor] = None, activation: str = "silu") -> torch.Tensor:
+    """The gated feed-forward block (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd.
+
+    ``Wg``, ``Wu`` [hidden, in] and ``Wd`` [out, hidden] with ``x`` [.., in], or
+    every ensemble member in the same launches: weights [members, ..], biases
+    [members, n], ``x`` [members, .., in] or one [rows, in] for all members
+    (-> [members, rows, out]).  ``activation``: 'silu', 'gelu' (the erf form) or
+    'relu'.  float32 (products to float32 accuracy) or bfloat16 (sums in
+    float32), one dtype for all.  Where a gradient is wanted the forward keeps
+    both pre-activations for the backward."""
+    wants = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, Wg, Wu, Wd, bg, bu, bd))
+    return _GatedMlp.apply(x, Wg, Wu, Wd, bg, bu, bd, activation, wants)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, W, target, b, ignore_index: int, reduction: str):
+        loss, lse, scale = load().linear_cross_entropy(x, W, target, b, ignore_index, reduction)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        ctx.save_for_backward(x, W, target, b, lse, scale)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, W, target, b, lse, scale = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dW, db = load().linear_cross_entropy_backward(
+            g, x, W, target, b, lse, scale, ctx.ignore_index, ctx.reduction,
+            (need[0], need[1], need[3]))
+        return dx, dW, None, db, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, target: torch.Tensor,
+                         b: Optional[torch.Tensor] = None, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """torch.nn.functional.cross_entropy(x @ W.T + b, target) of a head over a
+    large vocabulary (discrete or tokenised actions) without the logits in
+    memory: forward keeps each row's logsumexp, backward forms them again, a
+    piece of the vocabulary at a time.
+
+    ``x`` [.., in], ``W`` [vocab, in], ``b`` [vocab] or None, float32 or
+    bfloat16; ``target`` [..] int64.  The loss is float32.  A row whose target
+    is ``ignore_index`` has loss 0 and no gradient; 'mean' is over the other
+    rows (0 where there are none).  A target outside the vocabulary gives NaN."""
+    return _LinearCrossEntropy.apply(x, W, target, b, ignore_index, reduction)

@@ -1348,6 +1348,94 @@ typedef struct d3a_iqn_head_bwd_fused_desc {
 } d3a_iqn_head_bwd_fused_desc;
 int d3a_iqn_head_bwd_fused(const d3a_iqn_head_bwd_fused_desc* d, void* stream);
 
+/* ---- layers and losses of larger policies: layer norm, the gated feed-forward
+ *      block, the softmax cross entropy of a linear head.  Tensors are float32
+ *      or bfloat16 (D3A_F32 / D3A_BF16; 16-bit storage, sums and statistics in
+ *      float32); `ws` is scratch of at least the size that the matching
+ *      *_workspace call reports for the same descriptor (256-byte aligned, owned
+ *      by the call until its kernels have run). ------------------------------- */
+#define D3A_F32 0
+#define D3A_BF16 1
+
+#define D3A_ACT_SILU 0 /* g / (1 + exp(-g))                   */
+#define D3A_ACT_GELU 1 /* g (1 + erf(g / sqrt 2)) / 2          */
+#define D3A_ACT_RELU 2 /* max(g, 0); derivative 0 at g = 0     */
+
+/* The gated block of every ensemble member c:
+ *   g = x_c Wg_c^T + bg_c, u = x_c Wu_c^T + bu_c, y_c = (act(g) * u) Wd_c^T + bd_c
+ * x_c rows at x + c * sx + r * ldx (sx = 0 with members > 1: one x for all),
+ * Wg / Wu [members][n_hidden][n_in] and Wd [members][n_out][n_hidden] with row
+ * strides ldW* and member strides sW*; biases [members][n] contiguous or NULL;
+ * y [members][rows][n_out] contiguous.  g, u: NULL, or [members][rows] rows of
+ * n_hidden rounded up to 8, kept for the backward.
+ * The backward reads x, the weights, g, u and dy (lddy, sdy) and writes the
+ * gradients whose pointers are given, contiguous in their tensor's shape; dx of
+ * an x that the members share is the sum over them.  It does not read y. */
+typedef struct d3a_gated_mlp_desc {
+  const void *x, *Wg, *Wu, *Wd;
+  const void *bg, *bu, *bd;
+  void *y, *g, *u;
+  const void* dy;
+  void *dx, *dWg, *dWu, *dWd, *dbg, *dbu, *dbd;
+  int64_t rows, n_in, n_hidden, n_out, members;
+  int64_t ldx, sx, ldWg, sWg, ldWu, sWu, ldWd, sWd, lddy, sdy;
+  int32_t dtype, act;
+  void* ws;
+  int64_t ws_bytes;
+} d3a_gated_mlp_desc;
+int d3a_gated_mlp_workspace(const d3a_gated_mlp_desc* desc, int32_t backward, int64_t* bytes);
+int d3a_gated_mlp(const d3a_gated_mlp_desc* desc, void* stream);
+int d3a_gated_mlp_bwd(const d3a_gated_mlp_desc* desc, void* stream);
+
+/* Softmax cross entropy of a linear head, the logits never kept:
+ *   z = x W^T + b (W [vocab][n_in] rows of ldW; b [vocab] or NULL),
+ *   lse[r] = log sum exp z[r], loss[r] = lse[r] - z[r][target[r]];
+ * target[r] = ignore_index: loss 0, no gradient; target outside [0, vocab):
+ * loss and gradient NaN.  reduction 0 none, 1 mean over the rows that are not
+ * ignored (0 where there is none), 2 sum; 1 and 2 write out[0] and scale[0] (the
+ * factor of a row's gradient, read by the backward).  loss and lse [rows] are
+ * written always.
+ * The backward reads x, W, b, target, lse, scale and gloss ([rows] with
+ * reduction 0, else [1]) and writes the gradients whose pointers are given:
+ * dx [rows][n_in], dW [vocab][n_in], db [vocab], contiguous. */
+typedef struct d3a_linear_xent_desc {
+  const void *x, *W, *b;
+  const int64_t* target;
+  float *loss, *lse, *out, *scale;
+  const float* gloss;
+  void *dx, *dW, *db;
+  int64_t rows, n_in, vocab, ldx, ldW, ignore_index;
+  int32_t dtype, reduction;
+  void* ws;
+  int64_t ws_bytes;
+} d3a_linear_xent_desc;
+int d3a_linear_xent_workspace(const d3a_linear_xent_desc* desc, int32_t backward, int64_t* bytes);
+int d3a_linear_xent(const d3a_linear_xent_desc* desc, void* stream);
+int d3a_linear_xent_bwd(const d3a_linear_xent_desc* desc, void* stream);
+
+/* Layer norm over the last axis, forward and backward:
+ *   y = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ * x [members][rows] rows of n at member stride sx, row stride ldx; w, b
+ * [members][n] contiguous (either may be NULL: 1, 0); y and dx contiguous; mean,
+ * rstd [members][rows] float32 (NULL in a forward without a backward).  dtype:
+ * x, y, dy, dx; wtype: w, b, dw, db (dtype, or float32).  The backward writes
+ * the gradients whose pointers are given. */
+typedef struct d3a_layer_norm_desc {
+  const void *x, *w, *b;
+  void* y;
+  float *mean, *rstd;
+  const void* dy;
+  void *dx, *dw, *db;
+  int64_t rows, n, members, ldx, sx, lddy, sdy;
+  double eps;
+  int32_t dtype, wtype;
+  void* ws;
+  int64_t ws_bytes;
+} d3a_layer_norm_desc;
+int d3a_layer_norm_workspace(const d3a_layer_norm_desc* desc, int32_t backward, int64_t* bytes);
+int d3a_layer_norm(const d3a_layer_norm_desc* desc, void* stream);
+int d3a_layer_norm_bwd(const d3a_layer_norm_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,439 @@
+"""layer_norm, gated_mlp and linear_cross_entropy of torch_ops against their
+float64 forms, each output within the bound that its roundings give
+(policy_layer_helpers): sizes from one row up, odd ones, strides, members,
+masked rows, infinities, replays, streams."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from policy_layer_helpers import gated_reference, norm_reference, within, xent_reference
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def T():
+    from d3rlpy_amd import torch_ops
+    return torch_ops
+
+
+def rnd(seed, *shape, dtype=F32, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale + shift).to(dtype).to(DEV)
+
+
+def check(got, ref, keys=None):
+    for k in keys or ref:
+        within(got[k], *ref[k], k)
+
+
+# ------------------------------------------------------------------ layer norm
+def run_norm(T, x, w, b, dy, eps=1e-5):
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    y = T.layer_norm(*leaves, eps)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    return {"y": y, "x": dx, "weight": dw, "bias": db}
+
+
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 64), (3, 17), (257, 256), (1000, 257), (5, 513),
+                                    (130, 1024), (33, 1537), (9, 2048), (6, 2049), (7, 4100),
+                                    (5, 8192), (3, 8193), (70, 12288), (4100, 24)])
+@pytest.mark.parametrize("dtype,wtype", [(F32, F32), (BF16, BF16), (BF16, F32)])
+def test_layer_norm(T, rows, n, dtype, wtype):
+    x = rnd(1, rows, n, dtype=dtype, scale=2.0, shift=0.7)
+    w, b = rnd(2, n, dtype=wtype, scale=0.3, shift=1.0), rnd(3, n, dtype=wtype)
+    dy = rnd(4, rows, n, dtype=dtype)
+    check(run_norm(T, x, w, b, dy), norm_reference(x, w, b, 1e-5, dy))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [96, 300, 9000])
+def test_layer_norm_members(T, dtype, n):
+    C, R = 3, 37
+    x, dy = rnd(1, C, R, n, dtype=dtype), rnd(4, C, R, n, dtype=dtype)
+    w, b = rnd(2, C, n, dtype=dtype), rnd(3, C, n, dtype=dtype)
+    ref = norm_reference(x, w[:, None], b[:, None], 1e-5, dy)
+    check(run_norm(T, x, w, b, dy), ref)
+
+
+def test_layer_norm_strides_and_leading_axes(T):
+    x = rnd(1, 6, 50, 128, dtype=BF16)
+    w, b, dy = rnd(2, 64), rnd(3, 64), rnd(4, 6, 50, 64, dtype=BF16)
+    for v in (x[:, :, :64], x[:, :, 64:], x[:, :, 1:65], x[:, :, ::2]):
+        ref = norm_reference(v, w, b, 1e-5, dy)
+        got = run_norm(T, v, w, b, dy)
+        assert got["y"].is_contiguous()
+        ref["weight"] = tuple(t.sum(0) for t in ref["weight"])
+        ref["bias"] = tuple(t.sum(0) for t in ref["bias"])
+        # 300 rows in all where the bound counted 50 a slice: the same sums
+        check(got, ref)
+    flat = x[0, :, :64]  # rows 128 apart
+    ref = norm_reference(flat, w, b, 1e-5, dy[0])
+    check(run_norm(T, flat, w, b, dy[0]), ref)
+    # a gradient that is one value expanded, and rows of a transposed array
+    one = torch.ones((), device=DEV, dtype=BF16).expand(50, 64)
+    check(run_norm(T, flat, w, b, one), norm_reference(flat, w, b, 1e-5, one))
+    tr = rnd(5, 64, 50, dtype=BF16).t()
+    check(run_norm(T, tr, w, b, dy[0]), norm_reference(tr, w, b, 1e-5, dy[0]))
+
+
+def test_layer_norm_without_weight_or_rows(T):
+    x = rnd(1, 9, 40).requires_grad_(True)
+    dy = rnd(2, 9, 40)
+    one, zero = torch.ones(40, device=DEV), torch.zeros(40, device=DEV)
+    y = T.layer_norm(x)
+    (dx,) = torch.autograd.grad(y, [x], dy)
+    ref = norm_reference(x, one, zero, 1e-5, dy)
+    check({"y": y, "x": dx}, ref, ("y", "x"))
+    w, b = one.clone().requires_grad_(True), zero.clone().requires_grad_(True)
+    none = torch.empty(0, 40, device=DEV, requires_grad=True)
+    y = T.layer_norm(none, w, b)
+    grads = torch.autograd.grad(y, [none, w, b], torch.empty_like(y))
+    assert y.shape == (0, 40) and grads[0].shape == (0, 40)
+    assert not grads[1].any() and not grads[2].any()
+    # one gradient alone
+    (dw,) = torch.autograd.grad(T.layer_norm(x.detach(), w, b), [w], dy)
+    within(dw, *ref["weight"], "weight")
+
+
+def test_layer_norm_constant_and_bad_rows(T):
+    x = rnd(1, 4, 100)
+    x[1] = 3.0
+    x[2, 7] = float("inf")
+    x[3, 9] = float("nan")
+    w, b = torch.ones(100, device=DEV), torch.zeros(100, device=DEV)
+    y = T.layer_norm(x, w, b)
+    assert torch.isfinite(y[:2]).all() and y[2:].isnan().all()
+    within(y[:2], *(t[:2] for t in norm_reference(x, w, b, 1e-5, x)["y"]), "y")
+
+
+# ------------------------------------------------------------------ gated block
+def gated_params(C, R, D, F, O, dtype, bias, shared=False):
+    lead = (C,) if C else ()
+    p = {"x": rnd(1, *(() if shared else lead), R, D, dtype=dtype),
+         "Wg": rnd(2, *lead, F, D, dtype=dtype, scale=D ** -0.5),
+         "Wu": rnd(3, *lead, F, D, dtype=dtype, scale=D ** -0.5),
+         "Wd": rnd(4, *lead, O, F, dtype=dtype, scale=F ** -0.5)}
+    if bias:
+        p |= {"bg": rnd(5, *lead, F, dtype=dtype, scale=0.3),
+              "bu": rnd(6, *lead, F, dtype=dtype, scale=0.3),
+              "bd": rnd(7, *lead, O, dtype=dtype, scale=0.3)}
+    return p, rnd(8, *lead, R, O, dtype=dtype)
+
+
+def run_gated(T, p, dy, activation):
+    q = {k: v.detach().requires_grad_(True) for k, v in p.items()}
+    y = T.gated_mlp(q["x"], q["Wg"], q["Wu"], q["Wd"], q.get("bg"), q.get("bu"), q.get("bd"),
+                    activation=activation)
+    grads = torch.autograd.grad(y, list(q.values()), dy)
+    return {"y": y} | dict(zip(q, grads))
+
+
+SIZES = [(1, 8, 8, 8), (1, 1, 1, 1), (2, 3, 5, 7), (5, 64, 32, 48), (17, 40, 72, 24),
+         (33, 129, 100, 65), (64, 256, 130, 256), (65, 72, 520, 71), (200, 256, 512, 256),
+         (333, 130, 1000, 129)]
+
+
+@pytest.mark.parametrize("R,D,F,O", SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("activation,bias", [("silu", False), ("gelu", True), ("relu", True)])
+def test_gated_mlp(T, R, D, F, O, dtype, activation, bias):
+    p, dy = gated_params(0, R, D, F, O, dtype, bias)
+    check(run_gated(T, p, dy, activation), gated_reference(p, dy, activation))
+
+
+# enough tiles for the larger ones
+@pytest.mark.parametrize("R,D,F,O", [(2560, 192, 1280, 130), (3000, 136, 2056, 264),
+                                     (4100, 264, 4100, 2100)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gated_mlp_large_tiles(T, R, D, F, O, dtype):
+    p, dy = gated_params(0, R, D, F, O, dtype, False)
+    check(run_gated(T, p, dy, "silu"), gated_reference(p, dy, "silu"))
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("R,D,F,O", [(1, 17, 40, 3), (40, 24, 100, 33), (300, 128, 512, 128)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gated_mlp_members(T, R, D, F, O, dtype, shared):
+    p, dy = gated_params(3, R, D, F, O, dtype, True, shared)
+    got = run_gated(T, p, dy, "silu")
+    assert got["y"].shape == (3, R, O)
+    check(got, gated_reference(p, dy, "silu", shared))
+
+
+def test_gated_mlp_strides(T):
+    R, D, F, O = 50, 64, 96, 40
+    p, dy = gated_params(0, R, D, F, O, BF16, False)
+    ref = gated_reference(p, dy, "silu")
+
+    def wide(t, by, off):  # the same values in rows `by` longer, `off` in
+        big = torch.full((t.shape[0], t.shape[1] + by), 7.0, device=DEV, dtype=t.dtype)
+        big[:, off:off + t.shape[1]] = t
+        return big[:, off:off + t.shape[1]]
+
+    for by, off in ((64, 0), (64, 8), (24, 16), (3, 1), (5, 0)):
+        v = {k: wide(t, by, off) for k, t in p.items()}
+        check(run_gated(T, v, wide(dy, by, off), "silu"), ref)
+    # gate and up as halves of one array, down transposed, x rows far apart
+    both = torch.cat([p["Wg"], p["Wu"]])
+    v = {"x": wide(p["x"], 1000, 8), "Wg": both[:F], "Wu": both[F:], "Wd": p["Wd"].t().contiguous().t()}
+    check(run_gated(T, v, dy, "silu"), ref)
+    # three leading axes, an expanded gradient
+    x3 = {"x": p["x"].view(5, 10, D)} | {k: p[k] for k in ("Wg", "Wu", "Wd")}
+    got = run_gated(T, x3, dy.view(5, 10, O), "silu")
+    assert got["y"].shape == (5, 10, O) and got["x"].shape == (5, 10, D)
+    check({k: t.reshape(ref[k][0].shape) for k, t in got.items()}, ref)
+    one = torch.ones((), device=DEV, dtype=BF16).expand(R, O)
+    check(run_gated(T, p, one, "silu"), gated_reference(p, one, "silu"))
+
+
+def test_gated_mlp_one_gradient_and_no_rows(T):
+    p, dy = gated_params(0, 20, 24, 40, 16, F32, True)
+    ref = gated_reference(p, dy, "silu")
+    for k in p:
+        q = {n: t.detach().requires_grad_(n == k) for n, t in p.items()}
+        y = T.gated_mlp(q["x"], q["Wg"], q["Wu"], q["Wd"], q["bg"], q["bu"], q["bd"])
+        (d,) = torch.autograd.grad(y, [q[k]], dy)
+        within(d, *ref[k], k)
+    p["x"], dy = p["x"][:0], dy[:0]
+    got = run_gated(T, p, dy, "silu")
+    assert got["y"].shape == (0, 16) and got["x"].shape == (0, 24)
+    assert not any(bool(got[k].any()) for k in got if k not in ("y", "x"))
+
+
+def test_gated_mlp_rows_do_not_mix(T):
+    """A row of infinities spoils its own outputs and no other row's."""
+    p, _ = gated_params(0, 70, 40, 72, 24, BF16, False)
+    args = (p["Wg"], p["Wu"], p["Wd"])
+    y = T.gated_mlp(p["x"], *args)
+    x = p["x"].clone()
+    x[33] = float("inf")
+    z = T.gated_mlp(x, *args)
+    keep = torch.arange(70, device=DEV) != 33
+    assert torch.equal(y[keep], z[keep]) and not torch.isfinite(z[33]).all()
+
+
+# ------------------------------------------------------------- linear cross entropy
+def run_xent(T, x, W, b, target, reduction, g, ignore=-100):
+    q = {"x": x.detach().requires_grad_(True), "W": W.detach().requires_grad_(True)}
+    if b is not None:
+        q["b"] = b.detach().requires_grad_(True)
+    loss = T.linear_cross_entropy(q["x"], q["W"], target, q.get("b"), ignore, reduction)
+    grads = torch.autograd.grad(loss, list(q.values()),
+                                g if torch.is_tensor(g) else torch.full_like(loss, g))
+    return {"loss": loss} | dict(zip(q, grads))
+
+
+def xent_inputs(R, D, V, dtype, bias, pad=0.2):
+    gen = torch.Generator().manual_seed(R * 7 + V)
+    t = torch.randint(0, V, (R,), generator=gen)
+    t[torch.rand(R, generator=gen) < pad] = -100
+    return (rnd(1, R, D, dtype=dtype), rnd(2, V, D, dtype=dtype, scale=2 * D ** -0.5),
+            rnd(3, V, dtype=dtype) if bias else None, t.to(DEV))
+
+
+@pytest.mark.parametrize("R,D,V", [(1, 1, 1), (1, 8, 2), (3, 17, 5), (8, 64, 1000), (33, 100, 257),
+                                   (65, 40, 130), (130, 256, 64), (257, 33, 1031),
+                                   (700, 128, 2050)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("reduction,bias", [("mean", False), ("sum", True), ("none", True)])
+def test_linear_cross_entropy(T, R, D, V, dtype, reduction, bias):
+    x, W, b, t = xent_inputs(R, D, V, dtype, bias)
+    g = rnd(9, R) if reduction == "none" else 0.7
+    check(run_xent(T, x, W, b, t, reduction, g), xent_reference(x, W, b, t, -100, reduction, g))
+
+
+@pytest.mark.parametrize("R,D,V", [(4000, 136, 4099), (2049, 72, 10007)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_cross_entropy_large_tiles(T, R, D, V, dtype):
+    x, W, b, t = xent_inputs(R, D, V, dtype, True)
+    check(run_xent(T, x, W, b, t, "mean", 1.0), xent_reference(x, W, b, t, -100, "mean", 1.0))
+
+
+def test_linear_cross_entropy_pieces(T):
+    """A vocabulary in several pieces (float32: 6 bytes a logit, 512 MiB a
+    piece), the last one odd, is the sum of its pieces."""
+    x, W, b, t = xent_inputs(6000, 24, 33001, F32, True)
+    check(run_xent(T, x, W, b, t, "mean", 1.0), xent_reference(x, W, b, t, -100, "mean", 1.0))
+
+
+def test_linear_cross_entropy_masked_rows(T):
+    x, W, b, t = xent_inputs(40, 24, 77, F32, True)
+    t[:] = -100
+    for reduction in ("mean", "sum", "none"):
+        got = run_xent(T, x, W, b, t, reduction, 1.0)
+        assert not any(bool(v.any()) for v in got.values())
+    # another ignored value, one that is a class; and rows whose logits are not numbers
+    t = torch.arange(40, device=DEV) % 5
+    ref = xent_reference(x, W, b, t, 3, "mean", 1.0)
+    check(run_xent(T, x, W, b, t, "mean", 1.0, ignore=3), ref)
+    bad = x.clone()
+    bad[t == 3] = float("nan")
+    bad[8] = float("inf")  # (target 3)
+    got = run_xent(T, bad, W, b, t, "mean", 1.0, ignore=3)
+    check({k: got[k] for k in ("loss", "b")}, ref, ("loss", "b"))
+    assert torch.equal(got["x"][t == 3], torch.zeros_like(got["x"][t == 3]))
+
+
+def test_linear_cross_entropy_extreme_logits(T):
+    """Logits of the type's lowest value and of -inf (a masked action), and a
+    target outside the vocabulary."""
+    x, W, b, t = xent_inputs(30, 16, 70, F32, True, pad=0.0)
+    t = t % 35
+    b[35:50] = float("-inf")
+    b[50:] = torch.finfo(F32).min
+    cut = xent_reference(x, W[:35], b[:35], t, -100, "mean", 1.0)
+    got = run_xent(T, x, W, b, t, "mean", 1.0)
+    within(got["loss"], *cut["loss"], "loss")
+    within(got["x"], *cut["x"], "x")
+    within(got["W"][:35], *cut["W"], "W")
+    assert not got["W"][35:].any() and not got["b"][35:].any()
+    for wrong in (-1, 70, 1 << 40, -(1 << 40)):
+        u = t.clone()
+        u[4] = wrong
+        got = run_xent(T, x, W, b, u, "none", 1.0)
+        assert got["loss"][4].isnan() and got["x"][4].isnan().all()
+        rest = torch.arange(30, device=DEV) != 4
+        assert torch.isfinite(got["loss"][rest]).all() and torch.isfinite(got["x"][rest]).all()
+
+
+def test_linear_cross_entropy_shapes_and_strides(T):
+    x, W, b, t = xent_inputs(48, 40, 90, BF16, True)
+    ref = xent_reference(x, W, b, t, -100, "mean", 1.0)
+    got = run_xent(T, x.view(4, 12, 40), W, b, t.view(4, 12), "mean", 1.0)
+    assert got["x"].shape == (4, 12, 40)
+    got["x"] = got["x"].reshape(48, 40)
+    check(got, ref)
+    big = torch.full((48, 83), 5.0, device=DEV, dtype=BF16)
+    big[:, 3:43] = x
+    tied = rnd(11, 90, 80, dtype=BF16)
+    tied[:, 40:] = W
+    got = run_xent(T, big[:, 3:43], tied[:, 40:], b, t, "mean", 1.0)
+    check(got, ref)
+    none = run_xent(T, x[:0], W, b, t[:0], "mean", 1.0)
+    assert float(none["loss"]) == 0 and not none["W"].any() and not none["b"].any()
+
+
+# --------------------------------------------------------------- together, replays
+def block_step(T, q, tokens, target):
+    """A pre-norm gated residual block and a classification head: loss, gradients."""
+    x = q["emb"][tokens]
+    h = T.layer_norm(x, q["n1"], q["c1"])
+    x = x + T.gated_mlp(h, q["Wg"], q["Wu"], q["Wd"])
+    loss = T.linear_cross_entropy(T.layer_norm(x, q["n2"], q["c2"]), q["emb"], target)
+    return loss, torch.autograd.grad(loss, list(q.values()))
+
+
+def block_inputs(dtype):
+    V, D, F, R = 300, 64, 160, 90
+    gen = torch.Generator().manual_seed(5)
+    q = {"emb": torch.randn(V, D, generator=gen), "n1": torch.ones(D), "c1": torch.zeros(D),
+         "Wg": torch.randn(F, D, generator=gen) * D ** -0.5,
+         "Wu": torch.randn(F, D, generator=gen) * D ** -0.5,
+         "Wd": torch.randn(D, F, generator=gen) * F ** -0.5, "n2": torch.ones(D),
+         "c2": torch.zeros(D)}
+    q = {k: v.to(dtype).to(DEV).requires_grad_(True) for k, v in q.items()}
+    tokens = torch.randint(0, V, (R,), generator=gen).to(DEV)
+    target = torch.randint(0, V, (R,), generator=gen).to(DEV)
+    target[::7] = -100
+    return q, tokens, target
+
+
+def test_block_trains_as_in_float64(T):
+    """The three together, the embedding tied to the head: loss and gradients
+    against the same network in float64 torch.  Every stage is good to the
+    float32 bounds above; through three stages and a sum over 90 rows they
+    stay under 2e-5 of the largest gradient (2^-24 times some 300 chained
+    roundings)."""
+    q, tokens, target = block_inputs(F32)
+    loss, grads = block_step(T, q, tokens, target)
+    d = {k: v.detach().double().requires_grad_(True) for k, v in q.items()}
+    x = d["emb"][tokens]
+    D = x.shape[1]
+    nrm = torch.nn.functional.layer_norm
+    h = nrm(x, (D,), d["n1"], d["c1"])
+    g = h @ d["Wg"].t()
+    x = x + (g * torch.sigmoid(g) * (h @ d["Wu"].t())) @ d["Wd"].t()
+    ref = torch.nn.functional.cross_entropy(nrm(x, (D,), d["n2"], d["c2"]) @ d["emb"].t(), target)
+    want = torch.autograd.grad(ref, list(d.values()))
+    assert abs(float(loss) - float(ref)) <= 2e-5 * abs(float(ref))
+    for k, a, b in zip(q, grads, want):
+        assert float((a - b).abs().max()) <= 2e-5 * float(b.abs().max()), k
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_block_is_deterministic_and_replays(T, dtype):
+    """Bit-identical from run to run, on another stream, and in a captured
+    graph replayed between eager calls."""
+    q, tokens, target = block_inputs(dtype)
+    det = {k: v.detach() for k, v in q.items()}
+
+    def step():
+        # (forward and backward calls, not autograd: what a captured loop runs)
+        ops = T.load()
+        x = det["emb"][tokens]
+        h, s1 = ops.layer_norm(x, det["n1"], det["c1"], 1e-5)
+        y, pre = ops.gated_mlp(h, det["Wg"], det["Wu"], det["Wd"], None, None, None, "silu", True)
+        r, s2 = ops.layer_norm(x + y, det["n2"], det["c2"], 1e-5)
+        loss, lse, scale = ops.linear_cross_entropy(r, det["emb"], target, None, -100, "mean")
+        dr, demb, _ = ops.linear_cross_entropy_backward(
+            torch.ones_like(loss), r, det["emb"], target, None, lse, scale, -100, "mean",
+            [True, True, False])
+        dxy, dn2, dc2 = ops.layer_norm_backward(dr, x + y, det["n2"], det["c2"], s2, [True] * 3)
+        dh, dWg, dWu, dWd = ops.gated_mlp_backward(
+            dxy, h, det["Wg"], det["Wu"], det["Wd"], None, None, None, pre, "silu",
+            [True] * 4 + [False] * 3)[:4]
+        return [loss, demb, dn2, dc2, dh, dWg, dWu, dWd]
+
+    want = step()
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def test_gradients_against_differences(T):
+    """The losses' directional derivative, by central differences of the
+    float32 loss: steps of 1e-2 leave 1e-4 of curvature and 1e-5 of rounding
+    over 2e-2, so 2e-2 of the derivative's size."""
+    q, tokens, target = block_inputs(F32)
+    _, grads = block_step(T, q, tokens, target)
+    for k, g in zip(q, grads):
+        v = g / g.norm()
+        ends = []
+        for s in (1e-2, -1e-2):
+            with torch.no_grad():
+                moved = dict(q) | {k: q[k] + s * v}
+                x = moved["emb"][tokens]
+                h = T.layer_norm(x, moved["n1"], moved["c1"])
+                x = x + T.gated_mlp(h, moved["Wg"], moved["Wu"], moved["Wd"])
+                ends.append(float(T.linear_cross_entropy(
+                    T.layer_norm(x, moved["n2"], moved["c2"]), moved["emb"], target)))
+        slope = (ends[0] - ends[1]) / 2e-2
+        assert abs(slope - float(g.norm())) <= 2e-2 * max(float(g.norm()), 1e-2), (k, slope, float(g.norm()))
+
+
+def test_no_second_derivative(T):
+    x = rnd(1, 4, 8).requires_grad_(True)
+    (dx,) = torch.autograd.grad(T.layer_norm(x).sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
