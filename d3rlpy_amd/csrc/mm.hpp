@@ -72,7 +72,10 @@ struct Tile {
   int m0, n0;            // first row / column of this wave's part
   int batch, split, lane;
   int M, N;
+  char* slab;            // staged epilogues: the wave's own kSlab bytes of LDS
 };
+
+constexpr int kSlab = 32 * 64 * 4;  // 32 rows of a wave's 64 columns in float32
 
 constexpr unsigned kOutside = 0x80000000u;  // = the resource's extent
 
@@ -302,7 +305,13 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
     } while (t < t_end);
   }
 
-  Tile tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N};
+  Tile tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr};
+  if constexpr (Epi::kStaged) {
+    __syncthreads();  // the tiles are read: each wave takes a slab of the first buffer
+    constexpr int in_a = C::NP * C::BM * C::BK * 2 / kSlab;
+    static_assert(in_a + C::NP * C::BN * C::BK * 2 / kSlab >= C::NW, "slabs");
+    tile.slab = w < in_a ? sa0 + w * kSlab : sb0 + (w - in_a) * kSlab;
+  }
   L.e[pi].template run<C>(acc, tile);
 }
 
@@ -335,7 +344,7 @@ int launch(Launch<Epi>& L, hipStream_t stream, const char* what) {
   return 0;
 }
 
-// float4 <-> storage
+// the exact split of a float32 value in three bfloat16 parts
 __device__ __forceinline__ void split3(float x, __bf16& p0, __bf16& p1, __bf16& p2) {
   p0 = (__bf16)x;
   const float r = x - (float)p0;
@@ -343,114 +352,146 @@ __device__ __forceinline__ void split3(float x, __bf16& p0, __bf16& p1, __bf16& 
   p2 = (__bf16)(r - (float)p1);
 }
 
-// v[0..3] as columns n .. n + 3 of NP planes at row pointer `p` (n % 4 == 0,
-// the row padded to a multiple of 8 columns)
+// v[0..7] to NP planes at p (16-byte aligned)
 template <int NP>
-__device__ __forceinline__ void store_planes(__bf16* p, int64_t s_part, const float v[4]) {
-  if constexpr (NP == 1) {
-    bf16x4 o;
+__device__ __forceinline__ void store_planes(__bf16* p, int64_t s_part, const float v[8]) {
+  bf16x8 o[NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (__bf16)v[i];
-    *reinterpret_cast<bf16x4*>(p) = o;
-  } else {
-    bf16x4 o[3];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (NP == 1) {
+      o[0][i] = (__bf16)v[i];
+    } else {
       __bf16 a, b, c;
       split3(v[i], a, b, c);
       o[0][i] = a;
       o[1][i] = b;
       o[2][i] = c;
     }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x4*>(p + q * s_part) = o[q];
   }
+#pragma unroll
+  for (int q = 0; q < NP; ++q) *reinterpret_cast<bf16x8*>(p + q * s_part) = o[q];
 }
 
 __device__ __forceinline__ void store4(float* p, const float v[4]) {
   *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-}
-__device__ __forceinline__ void store4(__bf16* p, const float v[4]) {
-  *reinterpret_cast<bf16x4*>(p) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
 }
 __device__ __forceinline__ void load4(const float* p, float v[4]) {
   const f32x4 x = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = x[i];
 }
-__device__ __forceinline__ void load4(const __bf16* p, float v[4]) {
-  const bf16x4 x = *reinterpret_cast<const bf16x4*>(p);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
+__device__ __forceinline__ void store8(float* p, const float v[8]) {
+  store4(p, v);
+  store4(p + 4, v + 4);
+}
+__device__ __forceinline__ void store8(__bf16* p, const float v[8]) { store_planes<1>(p, 0, v); }
+__device__ __forceinline__ void load8(const float* p, float v[8]) {
+  load4(p, v);
+  load4(p + 4, v + 4);
 }
 
-// every run of four columns of a wave's tile: f(m, n, v[4]) for m < M
-template <class C, int J0 = 0, int J1 = C::NT, class F>
-__device__ __forceinline__ void each4(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, F f) {
+// A wave's tile, 32 rows at a time, turned in LDS from the matrix
+// instructions' layout (a lane holds one row's runs of four columns, 64 rows
+// apart in memory) to rows: f(m, n, v[8], up[8]) for m < M, with eight
+// consecutive columns n a lane and whole 128-byte rows a group of lanes, so that
+// the epilogue's loads and stores are 16 bytes a lane and contiguous.  Writing
+// straight from the layout cost the 8192 x 32768 x 1024 logits' gradient
+// 1220 us, of 620 without its stores.  DUAL: the wave's 32 columns of both
+// matrices, v and up.  16-byte piece c of row r sits at c ^ (r & 15).
+template <class C, bool DUAL, class F>
+__device__ __forceinline__ void each8(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, F f) {
+  static_assert(C::TN == 64, "slab");
+  const int row = t.lane & 31, half = t.lane >> 5;
 #pragma unroll
   for (int i = 0; i < C::MT; ++i) {
-    const int m = t.m0 + 32 * i + (t.lane & 31);
 #pragma unroll
-    for (int j = J0; j < J1; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n = t.n0 + 32 * (j - J0) + 8 * q + 4 * (t.lane >> 5);
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r];
-        if (m < t.M) f(m, n, v, i, j, q);
+        const int c = 8 * j + 2 * q + half;
+        const f32x16& a = acc[i][j];
+        *reinterpret_cast<f32x4*>(t.slab + row * 256 + ((c ^ (row & 15)) << 4)) =
+            f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
       }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    constexpr int LANES = DUAL ? 4 : 8;  // lanes a row
+#pragma unroll
+    for (int p = 0; p < 32 * LANES / 64; ++p) {
+      const int r = p * (64 / LANES) + t.lane / LANES, c = 2 * (t.lane % LANES);
+      float v[8], up[8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(t.slab + r * 256 + (((c + k) ^ (r & 15)) << 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * k + e] = x[e];
+        if constexpr (DUAL) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(t.slab + r * 256 + (((8 + c + k) ^ (r & 15)) << 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) up[4 * k + e] = y[e];
+        }
+      }
+      const int m = t.m0 + 32 * i + r, n = t.n0 + 4 * c;
+      if (m < t.M) f(m, n, v, up);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// D (+ bias) in T, or an fp32 partial of a split / running sum over launches
+// D (+ bias) in T, or a float32 partial of a split / running sum over launches
 template <class T>
 struct StoreEpi {
+  static constexpr bool kStaged = true;
   T* out;           // [batch][M] rows of ld
   int64_t ld, s_batch;
   const T* bias;    // [batch][N] or null
   int64_t s_bias;
   float* sum;       // splits: [split][batch][M][N]; running sum: [M][N]
   int32_t mode;     // 0 out = D, 1 partial, 2 sum = D, 3 sum += D, 4 out = sum + D
-  int32_t vec;      // out rows take four-wide stores
+  int32_t vec;      // out's rows are 16-byte aligned
+  int32_t n_batch;
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
-    each4<C>(acc, t, [&](int m, int n, float* v, int, int, int) {
+    const bool whole = t.N % 4 == 0;
+    each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
       if (n >= t.N) return;
-      if (mode == 1) {
-        float* s = sum + (((int64_t)t.split * gridDim_batch(t) + t.batch) * t.M + m) * t.N + n;
+      const int left = t.N - n;
+      if (mode != 0) {
+        float* s = sum + ((mode == 1 ? ((int64_t)t.split * n_batch + t.batch) * t.M : 0) + m) * t.N + n;
+        if (whole && left >= 8) {
+          if (mode >= 3) {
+            float o[8];
+            load8(s, o);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < t.N) s[r] = v[r];
-        return;
-      }
-      if (mode >= 2) {
-        float* s = sum + (int64_t)m * t.N + n;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < t.N) {
-            if (mode >= 3) v[r] += s[r];
-            if (mode <= 3) s[r] = v[r];
+            for (int r = 0; r < 8; ++r) v[r] += o[r];
           }
+          if (mode <= 3) store8(s, v);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r < left) {
+              if (mode >= 3) v[r] += s[r];
+              if (mode <= 3) s[r] = v[r];
+            }
+        }
         if (mode <= 3) return;
       }
       if (bias) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += (float)bias[t.batch * s_bias + min(n + r, t.N - 1)];
+        for (int r = 0; r < 8; ++r) v[r] += (float)bias[t.batch * s_bias + min(n + r, t.N - 1)];
       }
       T* o = out + t.batch * s_batch + (int64_t)m * ld + n;
-      if (vec && n + 4 <= t.N) {
-        store4(o, v);
+      if (vec && left >= 8) {
+        store8(o, v);
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < t.N) o[r] = (T)v[r];
+        for (int r = 0; r < 8; ++r)
+          if (r < left) o[r] = (T)v[r];
       }
     });
   }
-  int32_t n_batch;
-  __device__ __forceinline__ int gridDim_batch(const Tile&) const { return n_batch; }
 };
 
 }  // namespace mm

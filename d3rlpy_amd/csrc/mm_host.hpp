@@ -336,7 +336,7 @@ struct Products {
     e.bias = static_cast<const T*>(bias);
     e.s_bias = s_bias;
     e.n_batch = (int32_t)batch;
-    e.vec = ld % 4 == 0 && s_batch % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
+    e.vec = ld * sizeof(T) % 16 == 0 && s_batch * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     ++L.n;
   }
 

@@ -843,7 +843,7 @@ void gated_call(GatedCall& c, const Gated& s, const at::Tensor& x, const at::Ten
 
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// -> (y, pre [2, members, rows, hidden rounded up to 8]: g and u; empty unless `keep`)
+// -> (y, pre [2, members, rows, hidden rounded up to 8]: g and u in float32; empty unless `keep`)
 std::tuple<at::Tensor, at::Tensor> gated_mlp_hip(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
                                                  const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
                                                  const OptTensor& bd, c10::string_view act, bool keep) {
@@ -853,12 +853,12 @@ std::tuple<at::Tensor, at::Tensor> gated_mlp_hip(const at::Tensor& x, const at::
   GatedCall c;
   gated_call(c, s, x, Wg, Wu, Wd, bg, bu, bd, act);
   at::Tensor y = at::empty(s.y_shape, x.options());
-  at::Tensor pre = keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options())
-                        : at::empty({0}, x.options());
+  at::Tensor pre = keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options().dtype(at::kFloat))
+                        : at::empty({0}, x.options().dtype(at::kFloat));
   c.d.y = y.data_ptr();
   if (pre.numel() > 0) {
-    c.d.g = pre.select(0, 0).data_ptr();
-    c.d.u = pre.select(0, 1).data_ptr();
+    c.d.g = pre.data_ptr<float>();
+    c.d.u = c.d.g + pre.numel() / 2;
   }
   check_rc(d3a_gated_mlp_workspace(&c.d, 0, &c.d.ws_bytes), "d3rlpy_amd::gated_mlp");
   const at::Tensor ws = workspace(c.d.ws_bytes, x);
@@ -873,7 +873,7 @@ std::tuple<at::Tensor, at::Tensor> gated_mlp_meta(const at::Tensor& x, const at:
   const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
   activation_code(act);
   return {at::empty(s.y_shape, x.options()),
-          keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options()) : at::empty({0}, x.options())};
+          keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options().dtype(at::kFloat)) : at::empty({0}, x.options().dtype(at::kFloat))};
 }
 
 using Seven = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
@@ -898,9 +898,10 @@ Seven gated_mlp_backward_hip(const at::Tensor& g, const at::Tensor& x, const at:
   check_gpu(x, "gated_mlp_backward");
   const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
   check_like(g, x, "gated_mlp_backward", "grad");
-  check_like(pre, x, "gated_mlp_backward", "pre");
+  check_f32_gpu(pre, "pre");
+  TORCH_CHECK(pre.device() == x.device(), "gated_mlp_backward: pre is on ", pre.device(), ", x on ", x.device());
   TORCH_CHECK(g.sizes() == at::IntArrayRef(s.y_shape), "gated_mlp_backward: grad must have the output's shape");
-  TORCH_CHECK(pre.is_contiguous() && pre.numel() == 2 * s.members * s.rows * round8(s.n_hidden),
+  TORCH_CHECK(pre.numel() == 2 * s.members * s.rows * round8(s.n_hidden),
               "gated_mlp_backward: pre of a forward with keep = True");
   const c10::DeviceGuard guard(x.device());
   GatedCall c;
@@ -910,8 +911,8 @@ Seven gated_mlp_backward_hip(const at::Tensor& g, const at::Tensor& x, const at:
   c.d.lddy = c.dy.ld;
   c.d.sdy = c.dy.s;
   if (pre.numel() > 0) {
-    c.d.g = pre.data_ptr();
-    c.d.u = pre.select(0, 1).data_ptr();
+    c.d.g = pre.data_ptr<float>();
+    c.d.u = c.d.g + pre.numel() / 2;
   }
   std::array<at::Tensor, 7> o = gated_grads(x, Wg, Wu, Wd, bg, bu, bd, wanted);
   void** to[7] = {&c.d.dx, &c.d.dWg, &c.d.dWu, &c.d.dWd, &c.d.dbg, &c.d.dbu, &c.d.dbd};

@@ -45,6 +45,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // One (max, sum) a row and wave column; z of the target.
 template <class T, int NP>
 struct LsePartEpi {
+  static constexpr bool kStaged = false;
   const T* bias;
   const int64_t* target;
   float2* part;     // [columns of waves][M]
@@ -150,6 +151,7 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* loss, co
 // dz of a piece of the vocabulary, as operand planes
 template <class T, int NP>
 struct DzEpi {
+  static constexpr bool kStaged = true;
   const T* bias;
   const int64_t* target;
   const float *lse, *gloss, *scale;  // scale: null = 1
@@ -162,32 +164,21 @@ struct DzEpi {
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
     const float by = scale ? scale[0] : 1.f;
-#pragma unroll
-    for (int i = 0; i < C::MT; ++i) {
-      const int m = t.m0 + 32 * i + (t.lane & 31);
-      if (m >= t.M) continue;
+    each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
+      if (n >= ld) return;
       const int64_t y = target[m];
       const bool on = y != ignore;
       const float l = lse[m];
       const float g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
       const int64_t want = y - v0;
 #pragma unroll
-      for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = t.n0 + 32 * j + 8 * q + 4 * (t.lane >> 5);
-          if (n >= ld) continue;
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float z = acc[i][j][4 * q + r];
-            if (bias) z += (float)bias[min(n + r, t.N - 1)];
-            const float d = (exp_<NP>(z - l) - (n + r == want ? 1.f : 0.f)) * g;
-            v[r] = on && n + r < t.N ? d : 0.f;
-          }
-          store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
-        }
-    }
+      for (int r = 0; r < 8; ++r) {
+        if (bias) v[r] += (float)bias[min(n + r, t.N - 1)];
+        const float d = (exp_<NP>(v[r] - l) - (n + r == want ? 1.f : 0.f)) * g;
+        v[r] = on && n + r < t.N ? d : 0.f;
+      }
+      store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
+    });
   }
 };
 

@@ -1367,14 +1367,15 @@ int d3a_iqn_head_bwd_fused(const d3a_iqn_head_bwd_fused_desc* d, void* stream);
  * Wg / Wu [members][n_hidden][n_in] and Wd [members][n_out][n_hidden] with row
  * strides ldW* and member strides sW*; biases [members][n] contiguous or NULL;
  * y [members][rows][n_out] contiguous.  g, u: NULL, or [members][rows] rows of
- * n_hidden rounded up to 8, kept for the backward.
+ * n_hidden rounded up to 8 in float32, kept for the backward.
  * The backward reads x, the weights, g, u and dy (lddy, sdy) and writes the
  * gradients whose pointers are given, contiguous in their tensor's shape; dx of
  * an x that the members share is the sum over them.  It does not read y. */
 typedef struct d3a_gated_mlp_desc {
   const void *x, *Wg, *Wu, *Wd;
   const void *bg, *bu, *bd;
-  void *y, *g, *u;
+  void* y;
+  float *g, *u;
   const void* dy;
   void *dx, *dWg, *dWu, *dWd, *dbg, *dbu, *dbd;
   int64_t rows, n_in, n_hidden, n_out, members;

@@ -109,8 +109,8 @@ def gated_reference(p, dy, activation, shared=False):
     y = add(h @ _t(wd), "bd")
     out = {"y": (y, e_h @ _t(wd.abs()) + acc(F) * (h.abs() @ _t(wd.abs())) + (2 * U + ut) * y.abs())}
 
-    # the backward goes by g and u as kept in the tensors' type
-    e_g, e_u = e_g + ut * g.abs(), e_u + ut * u.abs()
+    # the backward goes by g and u as kept, in float32
+    e_g, e_u = e_g + U * g.abs(), e_u + U * u.abs()
     e_a = e_g * l1 + 8 * U * (a.abs() + g.abs())
     e_da = e_g * l2 + 16 * U * (1 + g.abs())
     if activation == "relu":  # a gate this near zero may fall on either side
