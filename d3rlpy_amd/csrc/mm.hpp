@@ -20,6 +20,9 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+#include <utility>
+
 #include "common.hpp"
 
 namespace d3a {
@@ -59,13 +62,15 @@ struct Launch {
   int32_t n, total;
 };
 
-// BM x BN output tile, BK deep k tiles, WM x WN waves, NP planes an operand
-template <int BM_, int BN_, int BK_, int WM_, int WN_, int NP_>
+// B x B output tile, BK deep k tiles in NB LDS buffers, WM x WN waves, NP
+// planes an operand
+template <int B_, int BK_, int NB_, int WM_, int WN_, int NP_>
 struct Config {
-  static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, NP = NP_;
+  static constexpr int BM = B_, BN = B_, BK = BK_, NB = NB_, WM = WM_, WN = WN_, NP = NP_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int TM = BM / WM, TN = BN / WN;  // a wave's tile
   static constexpr int MT = TM / 32, NT = TN / 32;
+  static constexpr int BYTES = NP * B_ * BK * 2;    // of one buffer of one operand
 };
 
 struct Tile {
@@ -94,24 +99,30 @@ struct Loader {
   int kk;            // k-contiguous: the first k of the lane's piece
   int sel;           // dual: bit j set = instruction j reads the second matrix
 
-  // k-contiguous lines are rows of BK; the 16-byte piece c of row r sits at
-  // piece c ^ swz(r), so eight rows' pieces of one k cover all banks.
-  // Row-contiguous lines are ks of ROWS; 32-byte unit u of k sits at
-  // u ^ (k & 3), so a transposed read's four ks cover all banks.
+  // LDS serves 256 bytes a cycle.  k-contiguous lines are rows of BK: piece c
+  // (16 bytes) of row r sits at c ^ swz(r), so that sixteen rows' pieces of one
+  // k cover all banks.  Row-contiguous lines are ks of ROWS: unit u (32 bytes) of
+  // k sits at u ^ unit_swz(k), so that the four ks x two units of half a
+  // transposed read do.
   static __device__ __forceinline__ int swz(int r) {
-    return BK == 64 ? (r & 7) : ((r >> 1) & 3);
+    return BK == 64 ? ((r >> 1) & 7) : BK == 32 ? ((r >> 2) & 3) : ((r >> 3) & 1);
+  }
+  static __device__ __forceinline__ int unit_swz(int k) {
+    return ROWS >= 128 ? (k & 3) << 1 : ((k >> 1) & 1) << 1;
   }
 
   template <bool DUAL>
   __device__ __forceinline__ void init(int w, int lane, int row0, int rows, int64_t ld) {
     sel = 0;
     const int line0 = lane / LANES, c = lane % LANES;
-    kk = T ? 0 : 8 * (c ^ swz(line0));
+    // (one k for all the lane's pieces: its lines are whole periods of swz apart)
+    static_assert(T || NW * LINES % 16 == 0, "period of swz");
+    kk = T ? 0 : 8 * (c ^ swz(w % PER_PART * LINES + line0));
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int q = (j * NW + w) % PER_PART, line = q * LINES + line0;
       if constexpr (T) {
-        const int cc = c ^ ((line & 3) << 1);
+        const int cc = c ^ (unit_swz(line) << 1);
         off[j] = row0 + 8 * cc < rows ? (unsigned)(line * ld * 2) + 16u * cc : kOutside;
       } else {
         int row = line;
@@ -119,7 +130,6 @@ struct Loader {
           sel |= ((q * LINES / 32) & 1) << j;
           row = (line / 64) * 32 + line % 32;
         }
-        // (swz(line) depends on the lane alone: LINES is 8 or 16)
         off[j] = row0 + row < rows ? (unsigned)(row * ld * 2) + 2u * kk : kOutside;
       }
     }
@@ -154,14 +164,14 @@ struct Frag {
     const char* base = lds + part * (ROWS * BK * 2);
     if constexpr (!T) {
       const int r = lane & 31, c = 2 * s + (lane >> 5);
-      const int x = BK == 64 ? (r & 7) : ((r >> 1) & 3);
+      const int x = Loader<ROWS, BK, 1, 1, false>::swz(r);
       return *reinterpret_cast<const bf16x8*>(base + (rb + r) * (BK * 2) + ((c ^ x) << 4));
     } else {
       // a 16-lane group reads a 4 (k) x 16 (row) block: lane 4 q + p of it
       // addresses k q, rows 4 p .. 4 p + 3, and receives row `lane & 15`'s ks
       const int G = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
       const int k = 16 * s + 8 * (G >> 1) + q;
-      const int unit = (rb / 16 + (G & 1)) ^ q;
+      const int unit = (rb / 16 + (G & 1)) ^ Loader<ROWS, BK, 1, 1, true>::unit_swz(q);
       const char* a = base + k * (ROWS * 2) + unit * 32 + p * 8;
       const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(a));
       const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -175,15 +185,14 @@ __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// A wave's products of one staged k tile.  The B rows are the MFMA's first
-// operand, so a lane ends with one output row m (lane % 32) and runs of four
-// consecutive columns n.
+// A wave's operands of one 16-deep step, and their products.  The B rows are
+// the MFMA's first operand, so a lane ends with one output row m (lane % 32)
+// and runs of four consecutive columns n.
 template <class C, bool AT, bool BT>
-__device__ __forceinline__ void compute(const char* sa, const char* sb, int wm, int wn, int lane,
-                                        f32x16 (&acc)[C::MT][C::NT]) {
-#pragma unroll
-  for (int s = 0; s < C::BK / 16; ++s) {
-    bf16x8 a[C::MT][C::NP], b[C::NT][C::NP];
+struct Step {
+  bf16x8 a[C::MT][C::NP], b[C::NT][C::NP];
+
+  __device__ __forceinline__ void read(const char* sa, const char* sb, int s, int wm, int wn, int lane) {
 #pragma unroll
     for (int j = 0; j < C::NT; ++j)
 #pragma unroll
@@ -194,32 +203,51 @@ __device__ __forceinline__ void compute(const char* sa, const char* sb, int wm, 
 #pragma unroll
       for (int p = 0; p < C::NP; ++p)
         a[i][p] = Frag<C::BM, C::BK, AT>::get(sa, p, wm * C::TM + 32 * i, s, lane);
-    if constexpr (C::NP == 1) {
+  }
+
+  __device__ __forceinline__ void products(f32x16 (&acc)[C::MT][C::NT]) const {
+    // (2,0) (1,1) (0,2) (1,0) (0,1) (0,0): the six products of the split
+    // above 2^-24 of the leading one, smallest first
+    constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+    for (int t = C::NP == 1 ? 5 : 0; t < 6; ++t)
 #pragma unroll
       for (int i = 0; i < C::MT; ++i)
 #pragma unroll
-        for (int j = 0; j < C::NT; ++j) acc[i][j] = mma(b[j][0], a[i][0], acc[i][j]);
-    } else {
-      // (2,0) (1,1) (0,2) (1,0) (0,1) (0,0): the six products of the split
-      // above 2^-24 of the leading one, smallest first
-      constexpr int pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
-#pragma unroll
-      for (int t = 0; t < 6; ++t)
-#pragma unroll
-        for (int i = 0; i < C::MT; ++i)
-#pragma unroll
-          for (int j = 0; j < C::NT; ++j) acc[i][j] = mma(b[j][pb[t]], a[i][pa[t]], acc[i][j]);
-    }
+        for (int j = 0; j < C::NT; ++j) acc[i][j] = mma(b[j][pb[t]], a[i][pa[t]], acc[i][j]);
   }
+};
+
+template <class F, int... I>
+__device__ __forceinline__ void each_of(const F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+// f(0), f(1), .. f(N - 1) with the number as a type
+template <int N, class F>
+__device__ __forceinline__ void static_for(const F& f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+template <class V>
+__device__ __forceinline__ V pick(bool c, V a, V b) {
+  return c ? a : b;
+}
+
+// all but the wave's last `N` loads have arrived, and every wave says so
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
 template <class C, bool AT, bool BT, bool DUAL, class Epi>
 __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) {
   static_assert(!DUAL || (C::TN == 64 && !BT), "dual: a wave's columns are 32 of each matrix");
-  __shared__ __attribute__((aligned(1024))) char sa0[C::NP * C::BM * C::BK * 2];
-  __shared__ __attribute__((aligned(1024))) char sb0[C::NP * C::BN * C::BK * 2];
-  __shared__ __attribute__((aligned(1024))) char sa1[C::NP * C::BM * C::BK * 2];
-  __shared__ __attribute__((aligned(1024))) char sb1[C::NP * C::BN * C::BK * 2];
+  // (arrays of their own, each named where it is used: so the compiler sees that
+  // the loads in flight go to other buffers than the reads)
+  constexpr int BYTES3 = C::NB == 4 ? C::BYTES : 16;
+  __shared__ __attribute__((aligned(1024))) char a0[C::BYTES], a1[C::BYTES], a2[C::BYTES], a3[BYTES3];
+  __shared__ __attribute__((aligned(1024))) char b0[C::BYTES], b1[C::BYTES], b2[C::BYTES], b3[BYTES3];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / C::WN, wn = w % C::WN;
@@ -251,36 +279,38 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
 
   const int kt_seg = max((P.K + C::BK - 1) / C::BK, 1);  // K = 0: one empty tile
   const int T = kt_seg * P.n_outer * P.n_inner;
-  int t = (int)((int64_t)T * split / P.splits);
-  const int t_end = (int)((int64_t)T * (split + 1) / P.splits);
+  const int share = T / P.splits, over = T % P.splits;
+  const int t = share * split + min(split, over), t_end = t + share + (split < over ? 1 : 0);
   int seg = t / kt_seg;
   const int64_t a_row = AT ? (int64_t)m0 : (int64_t)m0 * P.a.ld;
   const int64_t b_row = BT ? (int64_t)n0 : (int64_t)n0 * P.b.ld;
-  const int64_t a_k = AT ? P.a.ld * C::BK : C::BK, b_k = BT ? P.b.ld * C::BK : C::BK;
+  const int64_t a_k = AT ? P.a.ld * C::BK : (int64_t)C::BK, b_k = BT ? P.b.ld * C::BK : (int64_t)C::BK;
 
-  // the next k tile: its first elements, and the ks its segment has left
-  const __bf16 *pa, *pb;
-  int left;
-  const int64_t b2 = DUAL ? P.b2 - P.b.p : 0;
+  // the next k tile: its first elements, the ks its segment has left, and its
+  // place among the inner segments.  No branches: the loads' address work runs
+  // between the matrix instructions of one block.
   const int n_inner = P.n_inner, K = P.K;
-  const int64_t a_part = P.a.s_part, b_part = P.b.s_part;
-  auto enter = [&](int kt) {
-    const int o = seg / n_inner, i = seg - o * n_inner;
-    pa = P.a.p + batch * P.a.s_batch + o * P.a.s_outer + i * P.a.s_inner + a_row + kt * a_k;
-    pb = P.b.p + batch * P.b.s_batch + o * P.b.s_outer + i * P.b.s_inner + b_row + kt * b_k;
-    left = K - kt * C::BK;
-  };
-  enter(t % kt_seg);
-  auto load = [&](char* sa, char* sb) {
-    la.template load<false>(sa, w, lane, pa, nullptr, a_part, left);
-    lb.template load<DUAL>(sb, w, lane, pb, pb + b2, b_part, left);
-    pa += a_k;
-    pb += b_k;
-    left -= C::BK;
-    if (left <= 0) {
-      ++seg;
-      enter(0);
-    }
+  const int64_t a_part = P.a.s_part, b_part = P.b.s_part, b_up = DUAL ? P.b2 - P.b.p : 0;
+  int inner = seg % n_inner, left = K - t % kt_seg * C::BK, to_load = t_end - t;
+  const __bf16* pa = P.a.p + batch * P.a.s_batch + seg / n_inner * P.a.s_outer + inner * P.a.s_inner + a_row +
+                     t % kt_seg * a_k;
+  const __bf16* pb = P.b.p + batch * P.b.s_batch + seg / n_inner * P.b.s_outer + inner * P.b.s_inner + b_row +
+                     t % kt_seg * b_k;
+  // from a segment's last tile to the next segment's first
+  const int64_t a_in = P.a.s_inner - (kt_seg - 1) * a_k, b_in = P.b.s_inner - (kt_seg - 1) * b_k;
+  const int64_t a_out = a_in + P.a.s_outer - n_inner * P.a.s_inner;
+  const int64_t b_out = b_in + P.b.s_outer - n_inner * P.b.s_inner;
+  auto load = [&](char* sa, char* sb) __attribute__((always_inline)) {
+    const int k_left = to_load > 0 ? left : 0;  // past the last tile: zeros, which the waits count
+    la.template load<false>(sa, w, lane, pa, nullptr, a_part, k_left);
+    lb.template load<DUAL>(sb, w, lane, pb, pb + b_up, b_part, k_left);
+    const bool end = left <= C::BK, last = inner + 1 == n_inner;
+    // (by value: a choice between variables would be one between addresses)
+    pa += pick(end, pick(last, a_out, a_in), a_k);
+    pb += pick(end, pick(last, b_out, b_in), b_k);
+    left = pick(end, K, left - C::BK);
+    inner = pick(end, pick(last, 0, inner + 1), inner);
+    --to_load;
   };
 
   f32x16 acc[C::MT][C::NT];
@@ -291,26 +321,77 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  // two buffers: the barrier ends the reads of one and the loads of the other
+  // NB buffers in turn.  Iteration t's barrier says that tile t + 1 is there
+  // and tile t - 1 is read; then the loads of tile t + NB - 1 start, into the
+  // latter's buffer, and each step's operands are read while the step before
+  // it is in the matrix cores, across the tiles' border too.
+  constexpr int LPT = Loader<C::BM, C::BK, C::NP, C::NW, AT>::NJ + Loader<C::BN, C::BK, C::NP, C::NW, BT>::NJ;
+  constexpr int STEPS = C::BK / 16;
+  static_assert(C::NB == 3 || C::NB == 4, "buffers");
+  Step<C, AT, BT> f0, f1;
+  auto iteration = [&](const char* ca, const char* cb, const char* na, const char* nb, char* fa, char* fb,
+                       auto parity)
+                       __attribute__((always_inline)) {
+    arrive<(C::NB - 3) * LPT>();
+    static_for<STEPS>([&](auto step) __attribute__((always_inline)) {
+      constexpr int S = decltype(step)::value, P = (decltype(parity)::value + S) & 1;
+      Step<C, AT, BT>&now = P ? f1 : f0, &next = P ? f0 : f1;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (S == 0) load(fa, fb);
+      if constexpr (S + 1 < STEPS) next.read(ca, cb, S + 1, wm, wn, lane);
+      else next.read(na, nb, 0, wm, wn, lane);
+      now.products(acc);
+      // the step's products with the next step's reads, the far tile's loads
+      // and their address work spread between them
+      constexpr int MF = C::MT * C::NT * (C::NP == 1 ? 1 : 6);
+      constexpr int DS = (C::MT * (AT ? 2 : 1) + C::NT * (BT ? 2 : 1)) * C::NP;
+      static_for<MF>([&](auto mf) __attribute__((always_inline)) {
+        constexpr int k = decltype(mf)::value;
+        constexpr int ds = (k + 1) * DS / MF - k * DS / MF, vm = (k + 1) * LPT / MF - k * LPT / MF;
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (ds > 0) __builtin_amdgcn_sched_group_barrier(0x100, ds, 0);
+        if constexpr (S == 0) __builtin_amdgcn_sched_group_barrier(0x006, MF > 8 ? 4 : 6, 0);
+        if constexpr (S == 0 && vm > 0) __builtin_amdgcn_sched_group_barrier(0x010, vm, 0);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
   if (t < t_end) {
-    load(sa0, sb0);
+    load(a0, b0);
+    load(a1, b1);
+    if constexpr (C::NB == 4) load(a2, b2);
+    arrive<(C::NB - 2) * LPT>();
+    f0.read(a0, b0, 0, wm, wn, lane);
+    constexpr std::integral_constant<int, 0> even{};
+    constexpr std::integral_constant<int, STEPS & 1> odd{};
+    // (whole rounds of the buffers: the tiles past the last are zeros)
+    int n = t_end - t;
     do {
-      __syncthreads();
-      if (t + 1 < t_end) load(sa1, sb1);
-      compute<C, AT, BT>(sa0, sb0, wm, wn, lane, acc);
-      __syncthreads();
-      if (t + 2 < t_end) load(sa0, sb0);
-      if (t + 1 < t_end) compute<C, AT, BT>(sa1, sb1, wm, wn, lane, acc);
-      t += 2;
-    } while (t < t_end);
+      if constexpr (C::NB == 4) iteration(a0, b0, a1, b1, a3, b3, even);
+      else iteration(a0, b0, a1, b1, a2, b2, even);
+      iteration(a1, b1, a2, b2, a0, b0, odd);
+      if constexpr (C::NB == 4) {
+        iteration(a2, b2, a3, b3, a1, b1, even);
+        iteration(a3, b3, a0, b0, a2, b2, odd);
+      } else {
+        iteration(a2, b2, a0, b0, a1, b1, even);
+        if constexpr (STEPS & 1) {  // (odd counts of buffers and steps: the operand registers alternate)
+          iteration(a0, b0, a1, b1, a2, b2, odd);
+          iteration(a1, b1, a2, b2, a0, b0, even);
+          iteration(a2, b2, a0, b0, a1, b1, odd);
+        }
+      }
+      n -= C::NB == 3 && (STEPS & 1) ? 6 : C::NB;
+    } while (n > 0);
   }
 
   Tile tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr};
+  arrive<0>();  // nothing more arrives in LDS, and nobody reads it
   if constexpr (Epi::kStaged) {
-    __syncthreads();  // the tiles are read: each wave takes a slab of the first buffer
-    constexpr int in_a = C::NP * C::BM * C::BK * 2 / kSlab;
-    static_assert(in_a + C::NP * C::BN * C::BK * 2 / kSlab >= C::NW, "slabs");
-    tile.slab = w < in_a ? sa0 + w * kSlab : sb0 + (w - in_a) * kSlab;
+    constexpr int each = C::BYTES / kSlab;
+    static_assert(4 * each >= C::NW, "slabs");
+    char* s = w < each ? a0 : w < 2 * each ? b0 : w < 3 * each ? a1 : b1;
+    tile.slab = s + w % each * kSlab;
   }
   L.e[pi].template run<C>(acc, tile);
 }
