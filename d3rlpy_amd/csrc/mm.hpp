@@ -62,15 +62,14 @@ struct Launch {
   int32_t n, total;
 };
 
-// B x B output tile, BK deep k tiles in NB LDS buffers, WM x WN waves, NP
-// planes an operand
-template <int B_, int BK_, int NB_, int WM_, int WN_, int NP_>
+// BM x BN output tile, BK deep k tiles, WM x WN waves, NP planes an operand
+template <int BM_, int BN_, int BK_, int WM_, int WN_, int NP_>
 struct Config {
-  static constexpr int BM = B_, BN = B_, BK = BK_, NB = NB_, WM = WM_, WN = WN_, NP = NP_;
+  static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, NP = NP_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW;
   static constexpr int TM = BM / WM, TN = BN / WN;  // a wave's tile
   static constexpr int MT = TM / 32, NT = TN / 32;
-  static constexpr int BYTES = NP * B_ * BK * 2;    // of one buffer of one operand
+  static constexpr int A = NP * BM * BK * 2, B = NP * BN * BK * 2;  // bytes of a buffer
 };
 
 struct Tile {
@@ -234,20 +233,20 @@ __device__ __forceinline__ V pick(bool c, V a, V b) {
   return c ? a : b;
 }
 
-// all but the wave's last `N` loads have arrived, and every wave says so
+// all but the wave's last `N` loads have arrived, its reads are done, and every
+// wave says so
 template <int N>
 __device__ __forceinline__ void arrive() {
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
 template <class C, bool AT, bool BT, bool DUAL, class Epi>
 __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) {
   static_assert(!DUAL || (C::TN == 64 && !BT), "dual: a wave's columns are 32 of each matrix");
   // (arrays of their own, each named where it is used: so the compiler sees that
-  // the loads in flight go to other buffers than the reads)
-  constexpr int BYTES3 = C::NB == 4 ? C::BYTES : 16;
-  __shared__ __attribute__((aligned(1024))) char a0[C::BYTES], a1[C::BYTES], a2[C::BYTES], a3[BYTES3];
-  __shared__ __attribute__((aligned(1024))) char b0[C::BYTES], b1[C::BYTES], b2[C::BYTES], b3[BYTES3];
+  // the loads in flight go to other arrays than the reads, and waits for none;
+  // with one array for both operands it waited for all in the transposed reads)
+  __shared__ __attribute__((aligned(1024))) char a0[C::A], a1[C::A], b0[C::B], b1[C::B];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / C::WN, wn = w % C::WN;
@@ -321,28 +320,32 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  // NB buffers in turn.  Iteration t's barrier says that tile t + 1 is there
-  // and tile t - 1 is read; then the loads of tile t + NB - 1 start, into the
-  // latter's buffer, and each step's operands are read while the step before
-  // it is in the matrix cores, across the tiles' border too.
+  // Two buffers.  Each step's operands are read while the step before it is in
+  // the matrix cores, also across the tiles' border: the barrier stands before
+  // a tile's last step, where the wave has read that step's operands.  It says
+  // that the next tile is there and that the present one is read, so behind it
+  // the next tile's first step is read and the loads of the tile after that
+  // start, into the present buffer: they have all of a tile's products to arrive.
   constexpr int LPT = Loader<C::BM, C::BK, C::NP, C::NW, AT>::NJ + Loader<C::BN, C::BK, C::NP, C::NW, BT>::NJ;
   constexpr int STEPS = C::BK / 16;
-  static_assert(C::NB == 3 || C::NB == 4, "buffers");
+  static_assert(STEPS % 2 == 0, "the operand registers alternate");
   Step<C, AT, BT> f0, f1;
-  auto iteration = [&](const char* ca, const char* cb, const char* na, const char* nb, char* fa, char* fb,
-                       auto parity)
-                       __attribute__((always_inline)) {
-    arrive<(C::NB - 3) * LPT>();
+  auto iteration = [&](char* ca, char* cb, const char* na, const char* nb) __attribute__((always_inline)) {
     static_for<STEPS>([&](auto step) __attribute__((always_inline)) {
-      constexpr int S = decltype(step)::value, P = (decltype(parity)::value + S) & 1;
-      Step<C, AT, BT>&now = P ? f1 : f0, &next = P ? f0 : f1;
+      constexpr int S = decltype(step)::value;
+      constexpr bool last = S + 1 == STEPS;
+      Step<C, AT, BT>&now = S & 1 ? f1 : f0, &next = S & 1 ? f0 : f1;
+      if constexpr (last) arrive<0>();
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (S == 0) load(fa, fb);
-      if constexpr (S + 1 < STEPS) next.read(ca, cb, S + 1, wm, wn, lane);
-      else next.read(na, nb, 0, wm, wn, lane);
+      if constexpr (last) {
+        load(ca, cb);
+        next.read(na, nb, 0, wm, wn, lane);
+      } else {
+        next.read(ca, cb, S + 1, wm, wn, lane);
+      }
       now.products(acc);
-      // the step's products with the next step's reads, the far tile's loads
-      // and their address work spread between them
+      // the step's products, with the reads, the loads and the loads' address
+      // work spread between them
       constexpr int MF = C::MT * C::NT * (C::NP == 1 ? 1 : 6);
       constexpr int DS = (C::MT * (AT ? 2 : 1) + C::NT * (BT ? 2 : 1)) * C::NP;
       static_for<MF>([&](auto mf) __attribute__((always_inline)) {
@@ -350,8 +353,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
         constexpr int ds = (k + 1) * DS / MF - k * DS / MF, vm = (k + 1) * LPT / MF - k * LPT / MF;
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         if constexpr (ds > 0) __builtin_amdgcn_sched_group_barrier(0x100, ds, 0);
-        if constexpr (S == 0) __builtin_amdgcn_sched_group_barrier(0x006, MF > 8 ? 4 : 6, 0);
-        if constexpr (S == 0 && vm > 0) __builtin_amdgcn_sched_group_barrier(0x010, vm, 0);
+        if constexpr (last) __builtin_amdgcn_sched_group_barrier(0x006, 6, 0);
+        if constexpr (last && vm > 0) __builtin_amdgcn_sched_group_barrier(0x010, vm, 0);
       });
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -359,39 +362,24 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
   if (t < t_end) {
     load(a0, b0);
     load(a1, b1);
-    if constexpr (C::NB == 4) load(a2, b2);
-    arrive<(C::NB - 2) * LPT>();
+    arrive<LPT>();
     f0.read(a0, b0, 0, wm, wn, lane);
-    constexpr std::integral_constant<int, 0> even{};
-    constexpr std::integral_constant<int, STEPS & 1> odd{};
-    // (whole rounds of the buffers: the tiles past the last are zeros)
+    // (in pairs: a tile past the last is zeros)
     int n = t_end - t;
     do {
-      if constexpr (C::NB == 4) iteration(a0, b0, a1, b1, a3, b3, even);
-      else iteration(a0, b0, a1, b1, a2, b2, even);
-      iteration(a1, b1, a2, b2, a0, b0, odd);
-      if constexpr (C::NB == 4) {
-        iteration(a2, b2, a3, b3, a1, b1, even);
-        iteration(a3, b3, a0, b0, a2, b2, odd);
-      } else {
-        iteration(a2, b2, a0, b0, a1, b1, even);
-        if constexpr (STEPS & 1) {  // (odd counts of buffers and steps: the operand registers alternate)
-          iteration(a0, b0, a1, b1, a2, b2, odd);
-          iteration(a1, b1, a2, b2, a0, b0, even);
-          iteration(a2, b2, a0, b0, a1, b1, odd);
-        }
-      }
-      n -= C::NB == 3 && (STEPS & 1) ? 6 : C::NB;
+      iteration(a0, b0, a1, b1);
+      iteration(a1, b1, a0, b0);
+      n -= 2;
     } while (n > 0);
   }
 
   Tile tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr};
   arrive<0>();  // nothing more arrives in LDS, and nobody reads it
   if constexpr (Epi::kStaged) {
-    constexpr int each = C::BYTES / kSlab;
-    static_assert(4 * each >= C::NW, "slabs");
-    char* s = w < each ? a0 : w < 2 * each ? b0 : w < 3 * each ? a1 : b1;
-    tile.slab = s + w % each * kSlab;
+    constexpr int na = C::A / kSlab, nb = C::B / kSlab;
+    static_assert(nb > 0 && 2 * (na + nb) >= C::NW, "slabs");
+    const int i = w < 2 * na ? w : w - 2 * na;
+    tile.slab = w < 2 * na ? (i < na ? a0 : a1) + i % na * kSlab : (i < nb ? b0 : b1) + i % nb * kSlab;
   }
   L.e[pi].template run<C>(acc, tile);
 }

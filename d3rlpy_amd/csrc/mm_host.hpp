@@ -261,22 +261,22 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
 // ---- tile choice --------------------------------------------------------------------
 // Tiles by how many of them a product has: a large one reuses each staged byte
 // most and is taken where its workgroups fill most of the 256 CUs; the small
-// ones keep the chip busy on less.  (Three planes: 128 rows' operands of one
-// step take the registers that 256 rows' take with one.)
+// ones keep the chip busy on less.
 enum TileSize { kLarge, kMid, kSmall };
 
 template <int NP>
 struct Tiles;
 template <>
 struct Tiles<1> {
-  typedef Config<256, 32, 4, 2, 4, 1> Large;
-  typedef Config<128, 32, 4, 2, 2, 1> Mid;
-  typedef Config<64, 64, 4, 2, 1, 1> Small;
+  typedef Config<256, 256, 64, 2, 4, 1> Large;
+  typedef Config<128, 128, 64, 2, 2, 1> Mid;
+  typedef Config<64, 64, 64, 2, 1, 1> Small;
 };
 template <>
 struct Tiles<3> {
-  typedef Config<128, 16, 3, 2, 2, 3> Large, Mid;
-  typedef Config<64, 32, 3, 2, 1, 3> Small;
+  typedef Config<256, 128, 32, 4, 2, 3> Large;
+  typedef Config<128, 128, 32, 2, 2, 3> Mid;
+  typedef Config<64, 64, 32, 2, 1, 3> Small;
 };
 
 template <int NP, class Epi>
@@ -302,8 +302,7 @@ template <int NP, bool AT, bool BT, bool DUAL, class Epi>
 int run(Launch<Epi>& L, TileSize s, hipStream_t stream, const char* what) {
   typedef Tiles<NP> X;
   if (s == kLarge) return launch<typename X::Large, AT, BT, DUAL>(L, stream, what);
-  if constexpr (!std::is_same_v<typename X::Mid, typename X::Large>)
-    if (s == kMid) return launch<typename X::Mid, AT, BT, DUAL>(L, stream, what);
+  if (s == kMid) return launch<typename X::Mid, AT, BT, DUAL>(L, stream, what);
   return launch<typename X::Small, AT, BT, DUAL>(L, stream, what);
 }
 
