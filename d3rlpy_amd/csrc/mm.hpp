@@ -20,6 +20,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -251,54 +252,15 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / C::WN, wn = w % C::WN;
 
-  // workgroups go to the eight XCDs in turn: give each XCD a run of
-  // neighbouring tiles, whose operand rows then meet in its L2
-  int id = blockIdx.x;
-  {
-    const int q = L.total / 8, r = L.total % 8, x = id % 8;
-    id = id / 8 + x * q + (x < r ? x : r);
-  }
-  int pi = 0;
-  while (pi + 1 < L.n && id >= L.p[pi + 1].first) ++pi;
-  const Problem& P = L.p[pi];
-  id -= P.first;
-  const int per = P.tiles_m * P.tiles_n;
-  const int bs = id / per, batch = bs % P.batch, split = bs / P.batch;
-  id %= per;
-  constexpr int GM = 8;  // and the run is a block of GM tile rows
-  const int group = id / (GM * P.tiles_n), in = id % (GM * P.tiles_n);
-  const int gm = min(P.tiles_m - group * GM, GM);
-  const int m0 = (group * GM + in % gm) * C::BM;
-  const int n0 = (in / gm) * (DUAL ? C::BN / 2 : C::BN);
-
+  // The tile being loaded: its operands' pieces, the next k tile's first
+  // elements, the ks its segment has left, its place among the inner segments,
+  // and the k tiles to go.  The loads have no branches: their address work runs
+  // between the matrix instructions of one block.
   Loader<C::BM, C::BK, C::NP, C::NW, AT> la;
   Loader<C::BN, C::BK, C::NP, C::NW, BT> lb;
-  la.template init<false>(w, lane, m0, P.M, P.a.ld);
-  lb.template init<DUAL>(w, lane, n0, P.N, P.b.ld);
-
-  const int kt_seg = max((P.K + C::BK - 1) / C::BK, 1);  // K = 0: one empty tile
-  const int T = kt_seg * P.n_outer * P.n_inner;
-  const int share = T / P.splits, over = T % P.splits;
-  const int t = share * split + min(split, over), t_end = t + share + (split < over ? 1 : 0);
-  int seg = t / kt_seg;
-  const int64_t a_row = AT ? (int64_t)m0 : (int64_t)m0 * P.a.ld;
-  const int64_t b_row = BT ? (int64_t)n0 : (int64_t)n0 * P.b.ld;
-  const int64_t a_k = AT ? P.a.ld * C::BK : (int64_t)C::BK, b_k = BT ? P.b.ld * C::BK : (int64_t)C::BK;
-
-  // the next k tile: its first elements, the ks its segment has left, and its
-  // place among the inner segments.  No branches: the loads' address work runs
-  // between the matrix instructions of one block.
-  const int n_inner = P.n_inner, K = P.K;
-  const int64_t a_part = P.a.s_part, b_part = P.b.s_part, b_up = DUAL ? P.b2 - P.b.p : 0;
-  int inner = seg % n_inner, left = K - t % kt_seg * C::BK, to_load = t_end - t;
-  const __bf16* pa = P.a.p + batch * P.a.s_batch + seg / n_inner * P.a.s_outer + inner * P.a.s_inner + a_row +
-                     t % kt_seg * a_k;
-  const __bf16* pb = P.b.p + batch * P.b.s_batch + seg / n_inner * P.b.s_outer + inner * P.b.s_inner + b_row +
-                     t % kt_seg * b_k;
-  // from a segment's last tile to the next segment's first
-  const int64_t a_in = P.a.s_inner - (kt_seg - 1) * a_k, b_in = P.b.s_inner - (kt_seg - 1) * b_k;
-  const int64_t a_out = a_in + P.a.s_outer - n_inner * P.a.s_inner;
-  const int64_t b_out = b_in + P.b.s_outer - n_inner * P.b.s_inner;
+  const __bf16 *pa, *pb;
+  int64_t a_k, b_k, a_in, b_in, a_out, b_out, a_part, b_part, b_up;
+  int K, n_inner, inner, left, to_load;
   auto load = [&](char* sa, char* sb) __attribute__((always_inline)) {
     const int k_left = to_load > 0 ? left : 0;  // past the last tile: zeros, which the waits count
     la.template load<false>(sa, w, lane, pa, nullptr, a_part, k_left);
@@ -312,13 +274,67 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
     --to_load;
   };
 
-  f32x16 acc[C::MT][C::NT];
-#pragma unroll
-  for (int i = 0; i < C::MT; ++i)
-#pragma unroll
-    for (int j = 0; j < C::NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  // tile `id` of the launch -> the loads' state, and where it lies
+  int pi;
+  auto enter = [&](int id) __attribute__((always_inline)) {
+    // workgroups go to the eight XCDs in turn: give each XCD a run of
+    // neighbouring tiles, whose operand rows then meet in its L2
+    {
+      const int q = L.total / 8, r = L.total % 8, x = id % 8;
+      id = id / 8 + x * q + (x < r ? x : r);
+    }
+    pi = 0;
+    while (pi + 1 < L.n && id >= L.p[pi + 1].first) ++pi;
+    const Problem& P = L.p[pi];
+    id -= P.first;
+    const int per = P.tiles_m * P.tiles_n;
+    int batch = 0, split = 0;
+    if (id >= per) {
+      const int bs = id / per;
+      id -= bs * per;
+      split = bs / P.batch;
+      batch = bs - split * P.batch;
+    }
+    constexpr int GM = 8;  // and the run is a block of GM tile rows
+    const int group = id / (GM * P.tiles_n), in = id - group * (GM * P.tiles_n);
+    const int gm = min(P.tiles_m - group * GM, GM), col = in / gm;
+    const int m0 = (group * GM + in - col * gm) * C::BM, n0 = col * (DUAL ? C::BN / 2 : C::BN);
+    la.template init<false>(w, lane, m0, P.M, P.a.ld);
+    lb.template init<DUAL>(w, lane, n0, P.N, P.b.ld);
+
+    K = P.K;
+    n_inner = P.n_inner;
+    const int kt_seg = max((K + C::BK - 1) / C::BK, 1);  // K = 0: one empty tile
+    int t = 0, seg = 0, kt = 0;
+    to_load = K > 0 ? kt_seg * P.n_outer * n_inner : 0;
+    inner = 0;
+    if (P.splits > 1) {
+      const int share = to_load / P.splits, over = to_load - share * P.splits;
+      t = share * split + min(split, over);
+      to_load = share + (split < over ? 1 : 0);
+      seg = t / kt_seg;
+      kt = t - seg * kt_seg;
+      inner = seg % n_inner;
+    }
+    left = K - kt * C::BK;
+    a_k = AT ? P.a.ld * C::BK : (int64_t)C::BK;
+    b_k = BT ? P.b.ld * C::BK : (int64_t)C::BK;
+    pa = P.a.p + batch * P.a.s_batch + kt * a_k + (AT ? (int64_t)m0 : (int64_t)m0 * P.a.ld);
+    pb = P.b.p + batch * P.b.s_batch + kt * b_k + (BT ? (int64_t)n0 : (int64_t)n0 * P.b.ld);
+    if (seg > 0) {
+      pa += (seg - inner) / n_inner * P.a.s_outer + inner * P.a.s_inner;
+      pb += (seg - inner) / n_inner * P.b.s_outer + inner * P.b.s_inner;
+    }
+    // from a segment's last tile to the next segment's first
+    a_in = P.a.s_inner - (kt_seg - 1) * a_k;
+    b_in = P.b.s_inner - (kt_seg - 1) * b_k;
+    a_out = a_in + P.a.s_outer - n_inner * P.a.s_inner;
+    b_out = b_in + P.b.s_outer - n_inner * P.b.s_inner;
+    a_part = P.a.s_part;
+    b_part = P.b.s_part;
+    b_up = DUAL ? P.b2 - P.b.p : 0;
+    return Tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr};
+  };
 
   // Two buffers.  Each step's operands are read while the step before it is in
   // the matrix cores, also across the tiles' border: the barrier stands before
@@ -330,7 +346,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
   constexpr int STEPS = C::BK / 16;
   static_assert(STEPS % 2 == 0, "the operand registers alternate");
   Step<C, AT, BT> f0, f1;
-  auto iteration = [&](char* ca, char* cb, const char* na, const char* nb) __attribute__((always_inline)) {
+  auto iteration = [&](f32x16 (&acc)[C::MT][C::NT], char* ca, char* cb, const char* na, const char* nb) __attribute__((always_inline)) {
     static_for<STEPS>([&](auto step) __attribute__((always_inline)) {
       constexpr int S = decltype(step)::value;
       constexpr bool last = S + 1 == STEPS;
@@ -359,29 +375,51 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  if (t < t_end) {
-    load(a0, b0);
+  // A workgroup takes tiles gridDim apart; the next one's first loads start
+  // before the epilogue, which has the second buffers to itself.
+  int id = blockIdx.x;
+  Tile tile = enter(id);
+  load(a0, b0);
+  for (;;) {
+    f32x16 acc[C::MT][C::NT];
+#pragma unroll
+    for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+      for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    int n = to_load + 1;  // k tiles
     load(a1, b1);
     arrive<LPT>();
     f0.read(a0, b0, 0, wm, wn, lane);
     // (in pairs: a tile past the last is zeros)
-    int n = t_end - t;
     do {
-      iteration(a0, b0, a1, b1);
-      iteration(a1, b1, a0, b0);
+      iteration(acc, a0, b0, a1, b1);
+      iteration(acc, a1, b1, a0, b0);
       n -= 2;
     } while (n > 0);
-  }
+    arrive<0>();  // nothing more arrives in LDS, and nobody reads it
 
-  Tile tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr};
-  arrive<0>();  // nothing more arrives in LDS, and nobody reads it
-  if constexpr (Epi::kStaged) {
-    constexpr int na = C::A / kSlab, nb = C::B / kSlab;
-    static_assert(nb > 0 && 2 * (na + nb) >= C::NW, "slabs");
-    const int i = w < 2 * na ? w : w - 2 * na;
-    tile.slab = w < 2 * na ? (i < na ? a0 : a1) + i % na * kSlab : (i < nb ? b0 : b1) + i % nb * kSlab;
+    const Epi& epi = L.e[pi];
+    const Tile now = tile;
+    id += gridDim.x;
+    const bool more = id < L.total;
+    if (more) {
+      tile = enter(id);
+      load(a0, b0);
+    }
+    Tile out = now;
+    if constexpr (Epi::kStaged) {
+      constexpr int na = C::A / kSlab, nb = C::B / kSlab;
+      static_assert(na + nb >= C::NW, "slabs");
+      out.slab = w < na ? a1 + w * kSlab : b1 + (w - na) * kSlab;
+    }
+    epi.template run<C>(acc, out);
+    if (!more) break;
+    // every wave is through with its slab
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   }
-  L.e[pi].template run<C>(acc, tile);
 }
 
 // ---- host -------------------------------------------------------------------
@@ -408,7 +446,9 @@ template <class C, bool AT, bool BT, bool DUAL, class Epi>
 int launch(Launch<Epi>& L, hipStream_t stream, const char* what) {
   if (plan<C, DUAL>(L) != 0) return -1;
   if (L.total == 0) return 0;
-  mm_kernel<C, AT, BT, DUAL, Epi><<<L.total, C::THREADS, 0, stream>>>(L);
+  // as many workgroups as the chip holds (a multiple of the XCDs), or fewer
+  constexpr int resident = 256 * (160 * 1024 / (2 * (C::A + C::B)));
+  mm_kernel<C, AT, BT, DUAL, Epi><<<std::min(L.total, resident), C::THREADS, 0, stream>>>(L);
   D3A_LAUNCH_CHECK(what);
   return 0;
 }

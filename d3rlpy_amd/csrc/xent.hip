@@ -26,11 +26,14 @@ using namespace mm;
 
 constexpr int64_t kPieceBytes = 512LL << 20;
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// exp(z - ref), ref2 = ref * log2(e).  With bfloat16 tensors the hardware's
+// exponential and ref2's rounding, |ref| 2^-24 relative, are far below dz's own
+// rounding and no more than the float32 sum's.
 template <int NP>
-__device__ __forceinline__ float exp_(float x) {
-  // (one bfloat16 plane: 2 ulp of the hardware exponential are far below dz's
-  // own rounding, and below the float32 sum's)
-  return NP == 1 ? __expf(x) : expf(x);
+__device__ __forceinline__ float exp_to(float z, float ref, float ref2) {
+  return NP == 1 ? __builtin_amdgcn_exp2f(fmaf(z, kLog2e, -ref2)) : expf(z - ref);
 }
 
 // (max, sum of exp(z - max)) of a + b; an empty side has max -inf, sum 0
@@ -89,12 +92,12 @@ struct LsePartEpi {
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
       // a row of -inf alone: any finite reference gives its sum of 0
-      const float ref = top == -INFINITY ? 0.f : top;
+      const float ref = top == -INFINITY ? 0.f : top, ref2 = ref * kLog2e;
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < C::NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += exp_<NP>(acc[i][j][r] - ref);
+        for (int r = 0; r < 16; ++r) s += exp_to<NP>(acc[i][j][r], ref, ref2);
       const float m2 = __shfl_xor(top, 32), s2 = __shfl_xor(s, 32);
       join(top, s, m2, s2);
       // (a wave past the last column has no part)
@@ -183,15 +186,24 @@ struct DzEpi {
     each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
       if (n >= ld) return;
       const int64_t y = target[m];
-      const bool on = y != ignore;
-      const float l = lse[m];
+      const float l = lse[m], l2 = l * kLog2e;
       const float g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
-      const int64_t want = y - v0;
+      if (bias) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (bias) v[r] += (float)bias[min(n + r, t.N - 1)];
-        const float d = (exp_<NP>(v[r] - l) - (n + r == want ? 1.f : 0.f)) * g;
-        v[r] = on && n + r < t.N ? d : 0.f;
+        for (int r = 0; r < 8; ++r) v[r] += (float)bias[min(n + r, t.N - 1)];
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = exp_to<NP>(v[r], l, l2);
+      const int64_t want = y - v0 - n;
+      if (want >= 0 && want < 8) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] -= r == (int)want ? 1.f : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] *= g;
+      if (y == ignore || n + 8 > t.N) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = y != ignore && n + r < t.N ? v[r] : 0.f;
       }
       store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
     });
