@@ -173,7 +173,7 @@ int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream,
   *bytes = ws.used;
   if (dry || R == 0) return 0;
   if (pack.launch(stream) != 0) return -1;
-  if (run<NP, false, false, true>(L, choose<NP>(L, true), stream, "gated_mlp") != 0) return -1;
+  if (run<NP, false, false, true>(L, choose<NP>(L, true).size, stream, "gated_mlp") != 0) return -1;
   return down.template launch<false, false>(stream, "gated_mlp");
 }
 
@@ -255,7 +255,7 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   if (dry) return 0;
   if (hidden && R > 0) {
     if (pack.launch(stream) != 0) return -1;
-    if (run<NP, false, true, false>(L, choose<NP>(L, false), stream, "gated_mlp_bwd") != 0) return -1;
+    if (run<NP, false, true, false>(L, choose<NP>(L, false).size, stream, "gated_mlp_bwd") != 0) return -1;
     if (dx.template launch<false, true>(stream, "gated_mlp_bwd") != 0) return -1;
   }
   if (dw.template launch<true, true>(stream, "gated_mlp_bwd") != 0) return -1;

@@ -63,6 +63,8 @@ struct Launch {
   int32_t n, total;
 };
 
+constexpr int kSlab = 32 * 64 * 4;  // 32 rows of a wave's 64 columns in float32
+
 // BM x BN output tile, BK deep k tiles, WM x WN waves, NP planes an operand
 template <int BM_, int BN_, int BK_, int WM_, int WN_, int NP_>
 struct Config {
@@ -71,6 +73,10 @@ struct Config {
   static constexpr int TM = BM / WM, TN = BN / WN;  // a wave's tile
   static constexpr int MT = TM / 32, NT = TN / 32;
   static constexpr int A = NP * BM * BK * 2, B = NP * BN * BK * 2;  // bytes of a buffer
+  // the waves' slabs lie in the second buffers, and what is over in an array of its own
+  static constexpr int SLABS_A = A / kSlab, SLABS_B = B / kSlab;
+  static constexpr int MORE = NW > SLABS_A + SLABS_B ? (NW - SLABS_A - SLABS_B) * kSlab : 16;
+  static constexpr int LDS = 2 * (A + B) + MORE;
 };
 
 struct Tile {
@@ -80,7 +86,6 @@ struct Tile {
   char* slab;            // staged epilogues: the wave's own kSlab bytes of LDS
 };
 
-constexpr int kSlab = 32 * 64 * 4;  // 32 rows of a wave's 64 columns in float32
 
 constexpr unsigned kOutside = 0x80000000u;  // = the resource's extent
 
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
   // (arrays of their own, each named where it is used: so the compiler sees that
   // the loads in flight go to other arrays than the reads, and waits for none;
   // with one array for both operands it waited for all in the transposed reads)
-  __shared__ __attribute__((aligned(1024))) char a0[C::A], a1[C::A], b0[C::B], b1[C::B];
+  __shared__ __attribute__((aligned(1024))) char a0[C::A], a1[C::A], b0[C::B], b1[C::B], extra[C::MORE];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / C::WN, wn = w % C::WN;
@@ -411,9 +416,8 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
     }
     Tile out = now;
     if constexpr (Epi::kStaged) {
-      constexpr int na = C::A / kSlab, nb = C::B / kSlab;
-      static_assert(na + nb >= C::NW, "slabs");
-      out.slab = w < na ? a1 + w * kSlab : b1 + (w - na) * kSlab;
+      const int in_b = w - C::SLABS_A, in_extra = in_b - C::SLABS_B;
+      out.slab = in_b < 0 ? a1 + w * kSlab : in_extra < 0 ? b1 + in_b * kSlab : extra + in_extra * kSlab;
     }
     epi.template run<C>(acc, out);
     if (!more) break;
@@ -447,7 +451,7 @@ int launch(Launch<Epi>& L, hipStream_t stream, const char* what) {
   if (plan<C, DUAL>(L) != 0) return -1;
   if (L.total == 0) return 0;
   // as many workgroups as the chip holds (a multiple of the XCDs), or fewer
-  constexpr int resident = 256 * (160 * 1024 / (2 * (C::A + C::B)));
+  constexpr int resident = 256 * (160 * 1024 / C::LDS);
   mm_kernel<C, AT, BT, DUAL, Epi><<<std::min(L.total, resident), C::THREADS, 0, stream>>>(L);
   D3A_LAUNCH_CHECK(what);
   return 0;

@@ -5,6 +5,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 
 #include "mm.hpp"
 
@@ -259,9 +260,8 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
 }
 
 // ---- tile choice --------------------------------------------------------------------
-// Tiles by how many of them a product has: a large one reuses each staged byte
-// most and is taken where its workgroups fill most of the 256 CUs; the small
-// ones keep the chip busy on less.
+// Three tiles: a large one uses each staged byte most, the small ones keep the
+// chip busy on less.
 enum TileSize { kLarge, kMid, kSmall };
 
 template <int NP>
@@ -275,27 +275,68 @@ struct Tiles<1> {
 template <>
 struct Tiles<3> {
   typedef Config<256, 128, 32, 4, 2, 3> Large;
-  typedef Config<128, 128, 32, 2, 2, 3> Mid;
+  typedef Config<128, 128, 32, 4, 2, 3> Mid;
   typedef Config<64, 64, 32, 2, 1, 3> Small;
 };
 
-template <int NP, class Epi>
-int64_t count_tiles(const Launch<Epi>& L, TileSize s, bool dual) {
+// What a tile costs, measured on the products of 8192 x 1024 x 32768 and 1500 x
+// 777 x 10007 and smaller ones: `busy` us a k tile that a CU spends on one where
+// several share it, `alone` us a k tile that one takes by itself (its loads'
+// latency), `ends` us of prologue and epilogue, `resident` workgroups a CU.
+struct Cost {
+  int bm, bn, bk, resident;
+  double busy, alone, ends;
+};
+
+template <int NP>
+Cost cost_of(TileSize s) {
   typedef Tiles<NP> X;
-  const int bm = s == kLarge ? X::Large::BM : s == kMid ? X::Mid::BM : X::Small::BM;
-  int bn = s == kLarge ? X::Large::BN : s == kMid ? X::Mid::BN : X::Small::BN;
-  if (dual) bn /= 2;
-  int64_t n = 0;
-  for (int i = 0; i < L.n; ++i)
-    n += (int64_t)((L.p[i].M + bm - 1) / bm) * ((L.p[i].N + bn - 1) / bn) * L.p[i].batch;
-  return n;
+  if (NP == 1) {
+    if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 1.72, 1.72, 5.0};
+    if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 2, 0.58, 0.75, 4.0};
+    return {X::Small::BM, X::Small::BN, X::Small::BK, 5, 0.22, 0.55, 3.0};
+  }
+  if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 2.5, 2.5, 6.0};
+  if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 1, 1.4, 1.4, 5.0};
+  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.5, 0.95, 4.0};
 }
 
+struct Choice {
+  TileSize size;
+  int splits;
+};
+
+// The tile and, where `may_split`, the cuts of the k axis that the model gives
+// the least time: the fullest CU's tiles, and the partial sums' way out and
+// back in at 4 TB/s plus their pass.
 template <int NP, class Epi>
-TileSize choose(const Launch<Epi>& L, bool dual) {
-  if (count_tiles<NP>(L, kLarge, dual) >= 160) return kLarge;
-  if (count_tiles<NP>(L, kMid, dual) >= 160) return kMid;
-  return kSmall;
+Choice choose(const Launch<Epi>& L, bool dual, bool may_split = false) {
+  Choice best{kSmall, 1};
+  double least = 1e30;
+  for (TileSize s : {kLarge, kMid, kSmall}) {
+    const Cost c = cost_of<NP>(s);
+    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (splits > 1 && !may_split) break;
+      double tiles = 0, steps = 1, partial = 0;
+      for (int i = 0; i < L.n; ++i) {
+        const Problem& p = L.p[i];
+        const int bn = dual ? c.bn / 2 : c.bn;
+        tiles += (double)((p.M + c.bm - 1) / c.bm) * ((p.N + bn - 1) / bn) * p.batch * splits;
+        steps = std::max(steps, (double)((p.K + c.bk - 1) / c.bk) * p.n_outer * p.n_inner);
+        partial += (double)p.M * p.N * p.batch;
+      }
+      if (splits > 1 && steps < 4 * splits) break;
+      steps = std::ceil(steps / splits);
+      const double each = std::ceil(tiles / 256), rounds = std::ceil(each / c.resident);
+      double t = std::max(each * c.busy, rounds * c.alone) * steps + rounds * c.ends;
+      if (splits > 1) t += partial * 4 * (2 * splits) / 4e6 + 4;
+      if (t < least) {
+        least = t;
+        best = Choice{s, splits};
+      }
+    }
+  }
+  return best;
 }
 
 template <int NP, bool AT, bool BT, bool DUAL, class Epi>
@@ -306,13 +347,13 @@ int run(Launch<Epi>& L, TileSize s, hipStream_t stream, const char* what) {
   return launch<typename X::Small, AT, BT, DUAL>(L, stream, what);
 }
 
-// A launch of plain products D -> T (StoreEpi), with the k axis cut where the
-// tiles alone leave CUs idle and each cut keeps `kMinSteps` k tiles.
+// A launch of plain products D -> T (StoreEpi), with the k axis cut where that
+// is the quicker way.
 template <class T, int NP>
 struct Products {
   Launch<StoreEpi<T>> L{};
   SumJobs<T> sums{};
-  TileSize size = kLarge;
+  TileSize size = kSmall;
 
   void add(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, int64_t batch,
            int64_t n_outer, int64_t n_inner, void* out, int64_t ld, int64_t s_batch,
@@ -343,21 +384,15 @@ struct Products {
   // after every add(): the tile, the splits and their partials
   void reserve(Arena& ws, bool may_split) {
     if (L.n == 0) return;
-    size = choose<NP>(L, false);
-    if (!may_split) return;
-    typedef Tiles<NP> X;
-    const int64_t tiles = count_tiles<NP>(L, size, false);
-    const int bk = size == kLarge ? X::Large::BK : size == kMid ? X::Mid::BK : X::Small::BK;
-    constexpr int64_t kMinSteps = 8;
+    const Choice c = choose<NP>(L, false, may_split);
+    size = c.size;
+    if (c.splits == 1) return;
     for (int i = 0; i < L.n; ++i) {
       Problem& p = L.p[i];
-      const int64_t steps = (int64_t)((p.K + bk - 1) / bk) * p.n_outer * p.n_inner;
-      const int64_t s = std::min<int64_t>({256 / std::max<int64_t>(tiles, 1), steps / kMinSteps, 16});
-      if (s < 2) continue;
-      p.splits = (int32_t)s;
+      p.splits = c.splits;
       StoreEpi<T>& e = L.e[i];
       const int64_t n = (int64_t)p.batch * p.M * p.N;
-      e.sum = ws.take<float>(s * n);
+      e.sum = ws.take<float>(c.splits * n);
       e.mode = 1;
       sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits};
       sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + n;

@@ -246,7 +246,7 @@ int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t strea
   p.N = (int32_t)V;
   p.K = (int32_t)D;
   p.batch = p.n_outer = p.n_inner = p.splits = 1;
-  const TileSize size = choose<NP>(L, false);
+  const TileSize size = choose<NP>(L, false).size;
   const int cols = wave_columns<NP>(size);
   const int64_t parts = (V + cols - 1) / cols;
   LsePartEpi<T, NP>& e = L.e[0];
@@ -340,7 +340,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     *bytes = std::max(*bytes, ws.used);
     if (dry) continue;
     if (R > 0) {
-      if (run<NP, false, false, false>(L, choose<NP>(L, false), stream, "linear_cross_entropy_bwd") != 0) return -1;
+      if (run<NP, false, false, false>(L, choose<NP>(L, false).size, stream, "linear_cross_entropy_bwd") != 0) return -1;
       if (dx.template launch<false, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
     }
     if (dw.template launch<true, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
