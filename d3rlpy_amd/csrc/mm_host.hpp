@@ -188,12 +188,20 @@ __global__ __launch_bounds__(256) void colsum_kernel(const ColsumJobs<S> J) {
         ((red[lane] + red[64 + lane]) + red[128 + lane]) + red[192 + lane];
 }
 
+// 64 columns x the chunks over sixteen waves
 template <class T, class S>
-__global__ __launch_bounds__(256) void colsum_finish(const ColsumJobs<S> J) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= J.first[J.n]) return;
+__global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs<S> J) {
+  __shared__ float red[1024];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane, cols = J.first[J.n];
   float s = 0.f;
-  for (int k = 0; k < J.chunks; ++k) s += J.part[(int64_t)k * J.first[J.n] + c];
+  if (c < cols)
+#pragma unroll 4
+    for (int k = w; k < J.chunks; k += 16) s += J.part[k * cols + c];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (w != 0 || c >= cols) return;
+  for (int k = 1; k < 16; ++k) s += red[64 * k + lane];
   int i = 0;
   while (i + 1 < J.n && c >= J.first[i + 1]) ++i;
   const ColsumJob<S>& j = J.j[i];
@@ -223,7 +231,7 @@ struct Colsum {
     if (jobs.n == 0 || cols == 0) return 0;
     colsum_kernel<S, NP><<<dim3((unsigned)((cols + 63) / 64), jobs.chunks), 256, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
-    colsum_finish<T, S><<<(unsigned)((cols + 255) / 256), 256, 0, stream>>>(jobs);
+    colsum_finish<T, S><<<(unsigned)((cols + 63) / 64), 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
     return 0;
   }
@@ -236,12 +244,12 @@ struct SumJob {
   T* out;
   int64_t ld, s_batch;
   int64_t n;          // batch * M * N
-  int32_t M, N, splits;
+  int32_t M, N, splits, vec;  // vec: eight values at a time
 };
 template <class T>
 struct SumJobs {
   SumJob<T> j[kMaxProblems];
-  int64_t end[kMaxProblems];
+  int64_t end[kMaxProblems];  // running count of pieces: a row's eight columns
   int32_t n;
 };
 
@@ -253,10 +261,30 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
   if (i == J.n) return;
   if (i > 0) e -= J.end[i - 1];
   const SumJob<T>& j = J.j[i];
-  float s = 0.f;
-  for (int k = 0; k < j.splits; ++k) s += j.part[k * j.n + e];
-  const int64_t row = e / j.N, n = e - row * j.N, b = row / j.M;
-  j.out[b * j.s_batch + (row - b * j.M) * j.ld + n] = (T)s;
+  const int64_t pieces = (j.N + 7) / 8, row = e / pieces, b = row / j.M;
+  const int n = (int)(e - row * pieces) * 8, left = j.N - n;
+  const float* p = j.part + row * j.N + n;
+  T* o = j.out + b * j.s_batch + (row - b * j.M) * j.ld + n;
+  float s[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s[r] = 0.f;
+  if (j.vec) {
+#pragma unroll 2
+    for (int k = 0; k < j.splits; ++k) {
+      float v[8];
+      load8(p + k * j.n, v);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] += v[r];
+    }
+    store8(o, s);
+    return;
+  }
+  for (int k = 0; k < j.splits; ++k)
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[r] += r < left ? p[k * j.n + r] : 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < left) o[r] = (T)s[r];
 }
 
 // ---- tile choice --------------------------------------------------------------------
@@ -394,8 +422,8 @@ struct Products {
       const int64_t n = (int64_t)p.batch * p.M * p.N;
       e.sum = ws.take<float>(c.splits * n);
       e.mode = 1;
-      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits};
-      sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + n;
+      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits, p.N % 8 == 0 && e.vec};
+      sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + (int64_t)p.batch * p.M * ((p.N + 7) / 8);
       ++sums.n;
     }
   }

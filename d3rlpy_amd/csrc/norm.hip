@@ -238,10 +238,11 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
   }
 }
 
-// dw, db of a member: 64 of its 2 n columns a workgroup, the parts over its waves
+// dw, db of a member: 64 of its 2 n columns a workgroup, the parts over sixteen
+// waves
 template <class W>
-__global__ __launch_bounds__(256) void norm_finish_kernel(const Args A, int32_t parts) {
-  __shared__ float red[256];
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const Args A, int32_t parts) {
+  __shared__ float red[1024];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int64_t col = (int64_t)blockIdx.x * 64 + lane, c = blockIdx.y;
   const int64_t n = A.n;
@@ -249,12 +250,12 @@ __global__ __launch_bounds__(256) void norm_finish_kernel(const Args A, int32_t 
   if (col < 2 * n) {
     const float* p = A.part + c * parts * 2 * n + col;
 #pragma unroll 8
-    for (int k = wid; k < parts; k += 4) s += p[k * 2 * n];
+    for (int k = wid; k < parts; k += 16) s += p[k * 2 * n];
   }
   red[threadIdx.x] = s;
   __syncthreads();
   if (wid != 0 || col >= 2 * n) return;
-  s = ((red[lane] + red[64 + lane]) + red[128 + lane]) + red[192 + lane];
+  for (int k = 1; k < 16; ++k) s += red[64 * k + lane];
   if (col < n) {
     if (A.dw) static_cast<W*>(A.dw)[c * n + col] = (W)s;
   } else {
@@ -470,7 +471,7 @@ int backward(const d3a_layer_norm_desc& d, Arena ws, bool dry, hipStream_t strea
     if (dispatch<T, W>(d, a, true, parts, stream) != 0) return -1;
   }
   if (!cols) return 0;
-  norm_finish_kernel<W><<<dim3((unsigned)((2 * d.n + 63) / 64), (unsigned)d.members), 256, 0, stream>>>(
+  norm_finish_kernel<W><<<dim3((unsigned)((2 * d.n + 63) / 64), (unsigned)d.members), 1024, 0, stream>>>(
       a, (int32_t)parts);
   D3A_LAUNCH_CHECK("layer_norm_bwd");
   return 0;

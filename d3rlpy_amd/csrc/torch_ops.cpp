@@ -57,7 +57,10 @@
 //                                  same for the TD3+BC, BCQ and DiscreteCQL Impls.
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <array>
@@ -1059,6 +1062,207 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backward_met
   return {dx, dW, db};
 }
 
+// ---- autograd of layer_norm, gated_mlp, linear_cross_entropy ---------------------
+// The forward ops are differentiable themselves (Autograd key): one node each,
+// whose backward is the matching _backward op.  In C++ because a pass over a
+// minibatch costs less on the GPU than a Python node costs on the host.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor value(const OptTensor& t) { return given(t) ? *t : at::Tensor(); }
+
+OptTensor optional(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+// Whether a node is needed, and for which inputs.
+template <size_t N>
+bool wants(const std::array<at::Tensor, N>& inputs, std::array<bool, N>& wanted) {
+  bool any = false;
+  for (size_t i = 0; i < N; ++i) {
+    wanted[i] = inputs[i].defined() && inputs[i].requires_grad();
+    any |= wanted[i];
+  }
+  return any && at::GradMode::is_enabled();
+}
+
+template <size_t N>
+int64_t mask_of(const std::array<bool, N>& wanted) {
+  int64_t m = 0;
+  for (size_t i = 0; i < N; ++i) m |= (int64_t)wanted[i] << i;
+  return m;
+}
+
+template <size_t N>
+std::array<bool, N> wanted_of(int64_t mask) {
+  std::array<bool, N> w;
+  for (size_t i = 0; i < N; ++i) w[i] = (mask >> i) & 1;
+  return w;
+}
+
+// the gradients are computed outside autograd: differentiating them raises
+variable_list once(variable_list grads, const char* op) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list defined;
+  for (const at::Tensor& g : grads)
+    if (g.defined()) defined.push_back(g);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("d3rlpy_amd::") + op + " has no second derivative", (int64_t)defined.size());
+  defined = (*error)(std::move(defined));
+  size_t k = 0;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = defined[k++];
+  return grads;
+}
+
+template <class Sig>
+c10::TypedOperatorHandle<Sig> op_handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<Sig>();
+}
+
+using LayerNormSig = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const OptTensor&, const OptTensor&,
+                                                        double);
+
+std::tuple<at::Tensor, at::Tensor> layer_norm_below(const at::Tensor& x, const OptTensor& w, const OptTensor& b,
+                                                    double eps) {
+  static const auto op = op_handle<LayerNormSig>("d3rlpy_amd::layer_norm");
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(x, w, b, eps);
+}
+
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& w, const OptTensor& b,
+                               double eps, int64_t mask) {
+    auto [y, stats] = layer_norm_below(x, w, b, eps);
+    ctx->save_for_backward({x, value(w), value(b), stats});
+    ctx->saved_data["mask"] = mask;
+    ctx->mark_non_differentiable({stats});
+    return {y, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    using Sig = std::tuple<at::Tensor, at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
+                                                               const OptTensor&, const OptTensor&,
+                                                               const at::Tensor&, std::array<bool, 3>);
+    static const auto op = op_handle<Sig>("d3rlpy_amd::layer_norm_backward");
+    const variable_list v = ctx->get_saved_variables();
+    std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
+    {
+      const at::AutoDispatchBelowADInplaceOrView guard;
+      r = op.call(g[0], v[0], optional(v[1]), optional(v[2]), v[3], wanted_of<3>(ctx->saved_data["mask"].toInt()));
+    }
+    return once({std::get<0>(r), std::get<1>(r), std::get<2>(r), at::Tensor(), at::Tensor()}, "layer_norm");
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> layer_norm_autograd(const at::Tensor& x, const OptTensor& w, const OptTensor& b,
+                                                       double eps) {
+  std::array<bool, 3> wanted;
+  if (!wants<3>({x, value(w), value(b)}, wanted)) return layer_norm_below(x, w, b, eps);
+  variable_list r = LayerNormNode::apply(x, w, b, eps, mask_of(wanted));
+  return {r[0], r[1]};
+}
+
+using GatedSig = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                    const at::Tensor&, const OptTensor&, const OptTensor&,
+                                                    const OptTensor&, c10::string_view, bool);
+
+std::tuple<at::Tensor, at::Tensor> gated_mlp_below(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                                                   const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
+                                                   const OptTensor& bd, c10::string_view act, bool keep) {
+  static const auto op = op_handle<GatedSig>("d3rlpy_amd::gated_mlp");
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(x, Wg, Wu, Wd, bg, bu, bd, act, keep);
+}
+
+struct GatedMlpNode : torch::autograd::Function<GatedMlpNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                               const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
+                               const OptTensor& bd, std::string act, int64_t mask) {
+    auto [y, pre] = gated_mlp_below(x, Wg, Wu, Wd, bg, bu, bd, act, true);
+    ctx->save_for_backward({x, Wg, Wu, Wd, value(bg), value(bu), value(bd), pre});
+    ctx->saved_data["mask"] = mask;
+    ctx->saved_data["act"] = act;
+    ctx->mark_non_differentiable({pre});
+    return {y, pre};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    using Sig = Seven(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                      const OptTensor&, const OptTensor&, const OptTensor&, const at::Tensor&, c10::string_view,
+                      std::array<bool, 7>);
+    static const auto op = op_handle<Sig>("d3rlpy_amd::gated_mlp_backward");
+    const variable_list v = ctx->get_saved_variables();
+    const std::string act = ctx->saved_data["act"].toStringRef();
+    Seven r;
+    {
+      const at::AutoDispatchBelowADInplaceOrView guard;
+      r = op.call(g[0], v[0], v[1], v[2], v[3], optional(v[4]), optional(v[5]), optional(v[6]), v[7], act,
+                  wanted_of<7>(ctx->saved_data["mask"].toInt()));
+    }
+    auto [dx, dWg, dWu, dWd, dbg, dbu, dbd] = r;
+    return once({dx, dWg, dWu, dWd, dbg, dbu, dbd, at::Tensor(), at::Tensor()}, "gated_mlp");
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> gated_mlp_autograd(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
+                                                      const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
+                                                      const OptTensor& bd, c10::string_view act, bool keep) {
+  std::array<bool, 7> wanted;
+  if (!wants<7>({x, Wg, Wu, Wd, value(bg), value(bu), value(bd)}, wanted))
+    return gated_mlp_below(x, Wg, Wu, Wd, bg, bu, bd, act, keep);
+  variable_list r = GatedMlpNode::apply(x, Wg, Wu, Wd, bg, bu, bd, std::string(act), mask_of(wanted));
+  return {r[0], r[1]};
+}
+
+using XentSig = std::tuple<at::Tensor, at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
+                                                               const at::Tensor&, const OptTensor&, int64_t,
+                                                               c10::string_view);
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> xent_below(const at::Tensor& x, const at::Tensor& W,
+                                                          const at::Tensor& target, const OptTensor& b,
+                                                          int64_t ignore, c10::string_view reduction) {
+  static const auto op = op_handle<XentSig>("d3rlpy_amd::linear_cross_entropy");
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(x, W, target, b, ignore, reduction);
+}
+
+struct XentNode : torch::autograd::Function<XentNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& W,
+                               const at::Tensor& target, const OptTensor& b, int64_t ignore, std::string reduction,
+                               int64_t mask) {
+    auto [loss, lse, scale] = xent_below(x, W, target, b, ignore, reduction);
+    ctx->save_for_backward({x, W, target, value(b), lse, scale});
+    ctx->saved_data["mask"] = mask;
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->mark_non_differentiable({lse, scale});
+    return {loss, lse, scale};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    using Sig = std::tuple<at::Tensor, at::Tensor, at::Tensor>(
+        const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+        const at::Tensor&, const at::Tensor&, int64_t, c10::string_view, std::array<bool, 3>);
+    static const auto op = op_handle<Sig>("d3rlpy_amd::linear_cross_entropy_backward");
+    const variable_list v = ctx->get_saved_variables();
+    const std::string reduction = ctx->saved_data["reduction"].toStringRef();
+    std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
+    {
+      const at::AutoDispatchBelowADInplaceOrView guard;
+      r = op.call(g[0], v[0], v[1], v[2], optional(v[3]), v[4], v[5], ctx->saved_data["ignore"].toInt(), reduction,
+                  wanted_of<3>(ctx->saved_data["mask"].toInt()));
+    }
+    return once({std::get<0>(r), std::get<1>(r), at::Tensor(), std::get<2>(r), at::Tensor(), at::Tensor(),
+                 at::Tensor()},
+                "linear_cross_entropy");
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> xent_autograd(const at::Tensor& x, const at::Tensor& W,
+                                                             const at::Tensor& target, const OptTensor& b,
+                                                             int64_t ignore, c10::string_view reduction) {
+  std::array<bool, 3> wanted;
+  if (!wants<3>({x, W, value(b)}, wanted)) return xent_below(x, W, target, b, ignore, reduction);
+  variable_list r = XentNode::apply(x, W, target, b, ignore, std::string(reduction), mask_of(wanted));
+  return {r[0], r[1], r[2]};
+}
+
 // the captured update pipeline (a hipGraphExec_t owned by the caller's
 // torch.cuda.CUDAGraph, CUDAGraph.raw_cuda_graph_exec()) launched on the
 // current stream.  The graph draws its noise from the library's own Philox
@@ -1141,6 +1345,12 @@ TORCH_LIBRARY_IMPL(d3rlpy_amd, CUDA, m) {
   m.impl("linear_cross_entropy_backward", &linear_cross_entropy_backward_hip);
   m.impl("cql_update_step", &update_step_hip);
   m.impl("update_step", &update_step_hip);
+}
+
+TORCH_LIBRARY_IMPL(d3rlpy_amd, Autograd, m) {
+  m.impl("layer_norm", &layer_norm_autograd);
+  m.impl("gated_mlp", &gated_mlp_autograd);
+  m.impl("linear_cross_entropy", &xent_autograd);
 }
 
 TORCH_LIBRARY_IMPL(d3rlpy_amd, Meta, m) {

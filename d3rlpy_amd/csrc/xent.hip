@@ -107,26 +107,33 @@ struct LsePartEpi {
   }
 };
 
-// Joins a row's parts: 32 rows x 8 groups of parts a workgroup.
+// Joins the rows' parts: 8 rows x 32 threads a workgroup, first their largest
+// maximum, then the sums that refer to it (the parts again, from the cache).
 __global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32_t parts, int32_t rows,
                                                        const float* ztarget, const int64_t* target,
                                                        int64_t vocab, int64_t ignore, float* lse,
                                                        float* loss) {
-  __shared__ float2 red[256];
-  const int r = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  __shared__ float red[256];
+  const int q = threadIdx.x & 7, g = threadIdx.x >> 3;
+  const int r = blockIdx.x * 8 + q;
   float m = -INFINITY, s = 0.f;
   if (r < rows)
-    for (int p = g; p < parts; p += 8) {
+#pragma unroll 4
+    for (int p = g; p < parts; p += 32) m = fmaxf(m, part[(int64_t)p * rows + r].x);
+  red[threadIdx.x] = m;
+  __syncthreads();
+  for (int k = 0; k < 32; ++k) m = fmaxf(m, red[8 * k + q]);
+  __syncthreads();
+  if (r < rows)
+#pragma unroll 4
+    for (int p = g; p < parts; p += 32) {
       const float2 v = part[(int64_t)p * rows + r];
-      join(m, s, v.x, v.y);
+      s += v.x == m ? v.y : v.y * expf(v.x - m);
     }
-  red[threadIdx.x] = make_float2(m, s);
+  red[threadIdx.x] = s;
   __syncthreads();
   if (g != 0 || r >= rows) return;
-  for (int k = 1; k < 8; ++k) {
-    const float2 v = red[32 * k + threadIdx.x];
-    join(m, s, v.x, v.y);
-  }
+  for (int k = 1; k < 32; ++k) s += red[8 * k + q];
   const float l = m + logf(s);
   const int64_t t = target[r];
   lse[r] = l;
@@ -260,7 +267,7 @@ int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t strea
   if (R > 0) {
     if (pack.launch(stream) != 0) return -1;
     if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy") != 0) return -1;
-    lse_join_kernel<<<(unsigned)((R + 31) / 32), 256, 0, stream>>>(
+    lse_join_kernel<<<(unsigned)((R + 7) / 8), 256, 0, stream>>>(
         e.part, (int32_t)parts, (int32_t)R, e.ztarget, d.target, V, d.ignore_index, d.lse, d.loss);
     D3A_LAUNCH_CHECK("linear_cross_entropy");
   }

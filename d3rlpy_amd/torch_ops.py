@@ -25,7 +25,6 @@ import os
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 _LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libd3rlpy_amd_torch.so")
 _loaded = False
@@ -184,21 +183,12 @@ def squashed_gaussian_sample(mu, logstd, eps, min_logstd: float = -20.0,
     return _SquashedGaussian.apply(mu, logstd, eps, min_logstd, max_logstd)
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps: float):
-        y, stats = load().layer_norm(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, bias, stats)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, weight, bias, stats = ctx.saved_tensors
-        return *load().layer_norm_backward(g, x, weight, bias, stats,
-                                           ctx.needs_input_grad[:3]), None
-
-
+# layer_norm, gated_mlp and linear_cross_entropy carry their gradients in the op
+# library itself (its Autograd kernels), so torch.ops.d3rlpy_amd.layer_norm is
+# differentiable too; the gradients have no second derivative.  A backward pass
+# to capture into a graph is best written with the forward and *_backward ops:
+# autograd's own nodes belong to the stream that ran the forward, and a capture
+# that meets an eager graph's nodes of the same leaves ends the process.
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of ``x``
@@ -207,23 +197,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``x`` [.., n] with ``weight`` / ``bias`` [n], or [members, .., n] with
     [members, n] (every member its own); float32 or bfloat16, the weights in
     ``x``'s dtype or float32 and either may be None.  Statistics are float32."""
-    return _LayerNorm.apply(x, weight, bias, eps)
-
-
-class _GatedMlp(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, Wg, Wu, Wd, bg, bu, bd, activation: str, keep: bool):
-        y, pre = load().gated_mlp(x, Wg, Wu, Wd, bg, bu, bd, activation, keep)
-        ctx.activation = activation
-        ctx.save_for_backward(x, Wg, Wu, Wd, bg, bu, bd, pre)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, Wg, Wu, Wd, bg, bu, bd, pre = ctx.saved_tensors
-        return *load().gated_mlp_backward(g, x, Wg, Wu, Wd, bg, bu, bd, pre, ctx.activation,
-                                          ctx.needs_input_grad[:7]), None, None
+    return load().layer_norm(x, weight, bias, eps)[0]
 
 
 def gated_mlp(x: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, Wd: torch.Tensor,
@@ -238,28 +212,7 @@ def gated_mlp(x: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, Wd: torch.Ten
     'relu'.  float32 (products to float32 accuracy) or bfloat16 (sums in
     float32), one dtype for all.  Where a gradient is wanted the forward keeps
     both pre-activations for the backward."""
-    wants = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, Wg, Wu, Wd, bg, bu, bd))
-    return _GatedMlp.apply(x, Wg, Wu, Wd, bg, bu, bd, activation, wants)
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, W, target, b, ignore_index: int, reduction: str):
-        loss, lse, scale = load().linear_cross_entropy(x, W, target, b, ignore_index, reduction)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        ctx.save_for_backward(x, W, target, b, lse, scale)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        x, W, target, b, lse, scale = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dW, db = load().linear_cross_entropy_backward(
-            g, x, W, target, b, lse, scale, ctx.ignore_index, ctx.reduction,
-            (need[0], need[1], need[3]))
-        return dx, dW, None, db, None, None
+    return load().gated_mlp(x, Wg, Wu, Wd, bg, bu, bd, activation, False)[0]
 
 
 def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, target: torch.Tensor,
@@ -274,4 +227,4 @@ def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, target: torch.Tensor,
     bfloat16; ``target`` [..] int64.  The loss is float32.  A row whose target
     is ``ignore_index`` has loss 0 and no gradient; 'mean' is over the other
     rows (0 where there are none).  A target outside the vocabulary gives NaN."""
-    return _LinearCrossEntropy.apply(x, W, target, b, ignore_index, reduction)
+    return load().linear_cross_entropy(x, W, target, b, ignore_index, reduction)[0]
