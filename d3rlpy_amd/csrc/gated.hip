@@ -183,8 +183,8 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   const bool hidden = d.dx || d.dWg || d.dWu || d.dWd || d.dbg || d.dbu;
   Packer<T, NP> pack(ws);
   Operand dy{}, x{}, wd{}, wg{}, wu{};
+  if (hidden || d.dbd) dy = pack.operand(d.dy, d.lddy, C > 1 ? d.sdy : 0, C, R, O);
   if (hidden) {
-    dy = pack.operand(d.dy, d.lddy, C > 1 ? d.sdy : 0, C, R, O);
     wd = pack.operand(d.Wd, d.ldWd, C > 1 ? d.sWd : 0, C, O, F);
   }
   if (d.dWg || d.dWu) x = pack.operand(d.x, d.ldx, C > 1 ? d.sx : 0, C, R, D);
@@ -244,23 +244,20 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   if (d.dWu) dw.add(du, x, F, D, R, C, 1, 1, d.dWu, D, F * D, nullptr, 0);
   if (d.dWd) dw.add(dy, h, O, F, R, C, 1, 1, d.dWd, F, O * F, nullptr, 0);
   dw.reserve(ws, true);
-  Colsum<T, __bf16, NP> cs;
-  if (d.dbg) cs.add(dg.p, F8, R * F8, plane, R, F, C, d.dbg, F);
-  if (d.dbu) cs.add(du.p, F8, R * F8, plane, R, F, C, d.dbu, F);
+  Colsum<T, NP> cs;
+  if (d.dbg) cs.add(dg, R, F, C, d.dbg);
+  if (d.dbu) cs.add(du, R, F, C, d.dbu);
+  if (d.dbd) cs.add(dy, R, O, C, d.dbd);
   cs.reserve(ws);
-  Colsum<T, T, 1> csd;
-  if (d.dbd) csd.add(static_cast<const T*>(d.dy), d.lddy, C > 1 ? d.sdy : 0, 0, R, O, C, d.dbd, O);
-  csd.reserve(ws);
   *bytes = ws.used;
   if (dry) return 0;
+  if (R > 0 && pack.launch(stream) != 0) return -1;
   if (hidden && R > 0) {
-    if (pack.launch(stream) != 0) return -1;
     if (run<NP, false, true, false>(L, choose<NP>(L, false).size, stream, "gated_mlp_bwd") != 0) return -1;
     if (dx.template launch<false, true>(stream, "gated_mlp_bwd") != 0) return -1;
   }
   if (dw.template launch<true, true>(stream, "gated_mlp_bwd") != 0) return -1;
-  if (cs.launch(stream) != 0) return -1;
-  return csd.launch(stream);
+  return cs.launch(stream);
 }
 
 int call(const d3a_gated_mlp_desc* d, bool bwd, bool dry, hipStream_t stream, int64_t* bytes) {

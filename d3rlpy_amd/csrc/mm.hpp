@@ -560,36 +560,29 @@ struct StoreEpi {
   int64_t ld, s_batch;
   const T* bias;    // [batch][N] or null
   int64_t s_bias;
-  float* sum;       // splits: [split][batch][M][N]; running sum: [M][N]
+  float* sum;       // splits: [split][batch][M], running sum: [M] rows of round8(N)
   int32_t mode;     // 0 out = D, 1 partial, 2 sum = D, 3 sum += D, 4 out = sum + D
   int32_t vec;      // out's rows are 16-byte aligned
   int32_t n_batch;
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
-    const bool whole = t.N % 4 == 0;
+    const int64_t lds = (t.N + 7) / 8 * 8;
     each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
       if (n >= t.N) return;
       const int left = t.N - n;
       if (mode != 0) {
-        float* s = sum + ((mode == 1 ? ((int64_t)t.split * n_batch + t.batch) * t.M : 0) + m) * t.N + n;
-        if (whole && left >= 8) {
-          if (mode >= 3) {
-            float o[8];
-            load8(s, o);
+        float* s = sum + ((mode == 1 ? ((int64_t)t.split * n_batch + t.batch) * t.M : 0) + m) * lds + n;
+        if (mode >= 3) {
+          float o[8];
+          load8(s, o);
 #pragma unroll
-            for (int r = 0; r < 8; ++r) v[r] += o[r];
-          }
-          if (mode <= 3) store8(s, v);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (r < left) {
-              if (mode >= 3) v[r] += s[r];
-              if (mode <= 3) s[r] = v[r];
-            }
+          for (int r = 0; r < 8; ++r) v[r] += o[r];
         }
-        if (mode <= 3) return;
+        if (mode <= 3) {
+          store8(s, v);
+          return;
+        }
       }
       if (bias) {
 #pragma unroll

@@ -137,45 +137,48 @@ struct Packer {
 };
 
 // ---- column sums -----------------------------------------------------------------
-// out[b][c] = sum over rows of the value at [b][r][c]: NP planes added (planes
-// of an exact split), or one array of T.  Rows are cut into chunks whose fp32
-// sums a second pass adds in order, so the result does not depend on timing.
-template <class S>
+// out[b][c] = sum over rows of the value at [b][r][c] of NP operand planes.
+// Rows are cut into chunks whose float32 sums a second pass adds in order, so
+// the result does not depend on timing; few rows are one chunk and one pass.
 struct ColsumJob {
-  const S* src;
+  const __bf16* src;
   int64_t ld, s_batch, s_part;
-  void* out;       // T
-  int64_t s_out;   // elements between batches
+  void* out;       // T [batch][cols]
   int32_t rows, cols, batch;
 };
 constexpr int kMaxColsum = 3;
-template <class S>
 struct ColsumJobs {
-  ColsumJob<S> j[kMaxColsum];
-  float* part;      // [chunks][total columns]
+  ColsumJob j[kMaxColsum];
+  float* part;                    // [chunks][total columns]
   int64_t first[kMaxColsum + 1];  // running count of batch * cols
   int32_t n, chunks;
 };
 
-// a workgroup: 64 columns (one a lane) x its chunk of rows over four waves
-template <class S, int NP>
-__global__ __launch_bounds__(256) void colsum_kernel(const ColsumJobs<S> J) {
-  __shared__ float red[256];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  const bool on = c < J.first[J.n];
+// the job that column c of all belongs to, and its place there
+__device__ __forceinline__ const ColsumJob& colsum_job(const ColsumJobs& J, int64_t c, int64_t& at) {
   int i = 0;
   while (i + 1 < J.n && c >= J.first[i + 1]) ++i;
-  const ColsumJob<S>& j = J.j[i];
-  const int64_t cc = on ? c - J.first[i] : 0;
-  const int64_t b = cc / j.cols, col = cc - b * j.cols;
-  const S* p = j.src + b * j.s_batch + col;
+  at = c - J.first[i];
+  return J.j[i];
+}
+
+// a workgroup: 64 columns (one a lane) x its chunk of rows over sixteen waves
+template <class T, int NP>
+__global__ __launch_bounds__(1024) void colsum_kernel(const ColsumJobs J) {
+  __shared__ float red[1024];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t cols = J.first[J.n], c = (int64_t)blockIdx.x * 64 + lane;
+  const bool on = c < cols;
+  int64_t at;
+  const ColsumJob& j = colsum_job(J, on ? c : 0, at);
+  const int64_t b = at / j.cols;
+  const __bf16* p = j.src + b * j.s_batch + at - b * j.cols;
   const int64_t per = (j.rows + J.chunks - 1) / J.chunks;
   const int64_t r0 = per * blockIdx.y, r1 = min(r0 + per, (int64_t)j.rows);
   float s = 0.f;
   if (on)
-#pragma unroll 4
-    for (int64_t r = r0 + w; r < r1; r += 4) {
+#pragma unroll 8
+    for (int64_t r = r0 + w; r < r1; r += 16) {
       float v = 0.f;
 #pragma unroll
       for (int q = NP - 1; q >= 0; --q) v += (float)p[q * j.s_part + r * j.ld];
@@ -183,14 +186,15 @@ __global__ __launch_bounds__(256) void colsum_kernel(const ColsumJobs<S> J) {
     }
   red[threadIdx.x] = s;
   __syncthreads();
-  if (w == 0 && on)
-    J.part[(int64_t)blockIdx.y * J.first[J.n] + c] =
-        ((red[lane] + red[64 + lane]) + red[128 + lane]) + red[192 + lane];
+  if (w != 0 || !on) return;
+  for (int k = 1; k < 16; ++k) s += red[64 * k + lane];
+  if (J.chunks == 1) static_cast<T*>(j.out)[at] = (T)s;
+  else J.part[blockIdx.y * cols + c] = s;
 }
 
 // 64 columns x the chunks over sixteen waves
-template <class T, class S>
-__global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs<S> J) {
+template <class T>
+__global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs J) {
   __shared__ float red[1024];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane, cols = J.first[J.n];
@@ -202,36 +206,34 @@ __global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs<S> J) {
   __syncthreads();
   if (w != 0 || c >= cols) return;
   for (int k = 1; k < 16; ++k) s += red[64 * k + lane];
-  int i = 0;
-  while (i + 1 < J.n && c >= J.first[i + 1]) ++i;
-  const ColsumJob<S>& j = J.j[i];
-  const int64_t cc = c - J.first[i], b = cc / j.cols;
-  static_cast<T*>(j.out)[b * j.s_out + cc - b * j.cols] = (T)s;
+  int64_t at;
+  const ColsumJob& j = colsum_job(J, c, at);
+  static_cast<T*>(j.out)[at] = (T)s;
 }
 
-template <class T, class S, int NP>
+template <class T, int NP>
 struct Colsum {
-  ColsumJobs<S> jobs{};
-  void add(const S* src, int64_t ld, int64_t s_batch, int64_t s_part, int64_t rows, int64_t cols,
-           int64_t batch, void* out, int64_t s_out) {
-    ColsumJob<S>& j = jobs.j[jobs.n];
-    j = ColsumJob<S>{src, ld, s_batch, s_part, out, s_out, (int32_t)rows, (int32_t)cols, (int32_t)batch};
+  ColsumJobs jobs{};
+  void add(const Operand& o, int64_t rows, int64_t cols, int64_t batch, void* out) {
+    jobs.j[jobs.n] = ColsumJob{o.p, o.ld, o.s_batch, o.s_part, out, (int32_t)rows, (int32_t)cols, (int32_t)batch};
     jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * cols;
     ++jobs.n;
-    // about 1024 workgroups, chunks of at least 32 rows
+    // about 512 workgroups, chunks of at least 128 rows
     const int64_t blocks = (jobs.first[jobs.n] + 63) / 64;
     jobs.chunks = (int32_t)std::max<int64_t>(
-        1, std::min<int64_t>({1024 / std::max<int64_t>(blocks, 1), (rows + 31) / 32, 256}));
+        1, std::min<int64_t>({512 / std::max<int64_t>(blocks, 1), rows / 128, 256}));
+    if (rows <= 512) jobs.chunks = 1;
   }
   void reserve(Arena& ws) {
-    if (jobs.n) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n]);
+    if (jobs.n && jobs.chunks > 1) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n]);
   }
   int launch(hipStream_t stream) {
     const int64_t cols = jobs.first[jobs.n];
     if (jobs.n == 0 || cols == 0) return 0;
-    colsum_kernel<S, NP><<<dim3((unsigned)((cols + 63) / 64), jobs.chunks), 256, 0, stream>>>(jobs);
+    colsum_kernel<T, NP><<<dim3((unsigned)((cols + 63) / 64), jobs.chunks), 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
-    colsum_finish<T, S><<<(unsigned)((cols + 63) / 64), 1024, 0, stream>>>(jobs);
+    if (jobs.chunks == 1) return 0;
+    colsum_finish<T><<<(unsigned)((cols + 63) / 64), 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
     return 0;
   }
@@ -240,11 +242,11 @@ struct Colsum {
 // ---- split-k partials -------------------------------------------------------------
 template <class T>
 struct SumJob {
-  const float* part;  // [splits][batch][M][N]
+  const float* part;  // [splits][batch][M] rows of round8(N)
   T* out;
   int64_t ld, s_batch;
-  int64_t n;          // batch * M * N
-  int32_t M, N, splits, vec;  // vec: eight values at a time
+  int64_t n;          // batch * M * round8(N)
+  int32_t M, N, splits, vec;  // vec: out takes eight values at a time
 };
 template <class T>
 struct SumJobs {
@@ -263,28 +265,25 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
   const SumJob<T>& j = J.j[i];
   const int64_t pieces = (j.N + 7) / 8, row = e / pieces, b = row / j.M;
   const int n = (int)(e - row * pieces) * 8, left = j.N - n;
-  const float* p = j.part + row * j.N + n;
+  const float* p = j.part + (row * pieces) * 8 + n;
   T* o = j.out + b * j.s_batch + (row - b * j.M) * j.ld + n;
   float s[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) s[r] = 0.f;
-  if (j.vec) {
 #pragma unroll 2
-    for (int k = 0; k < j.splits; ++k) {
-      float v[8];
-      load8(p + k * j.n, v);
+  for (int k = 0; k < j.splits; ++k) {
+    float v[8];
+    load8(p + k * j.n, v);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) s[r] += v[r];
-    }
-    store8(o, s);
-    return;
+    for (int r = 0; r < 8; ++r) s[r] += v[r];
   }
-  for (int k = 0; k < j.splits; ++k)
+  if (j.vec && left >= 8) {
+    store8(o, s);
+  } else {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) s[r] += r < left ? p[k * j.n + r] : 0.f;
-#pragma unroll
-  for (int r = 0; r < 8; ++r)
-    if (r < left) o[r] = (T)s[r];
+    for (int r = 0; r < 8; ++r)
+      if (r < left) o[r] = (T)s[r];
+  }
 }
 
 // ---- tile choice --------------------------------------------------------------------
@@ -307,10 +306,14 @@ struct Tiles<3> {
   typedef Config<64, 64, 32, 2, 1, 3> Small;
 };
 
-// What a tile costs, measured on the products of 8192 x 1024 x 32768 and 1500 x
-// 777 x 10007 and smaller ones: `busy` us a k tile that a CU spends on one where
-// several share it, `alone` us a k tile that one takes by itself (its loads'
-// latency), `ends` us of prologue and epilogue, `resident` workgroups a CU.
+// What a tile costs: `busy` us a k tile that a CU spends on one where several
+// share it, `alone` us a k tile that one takes by itself (its loads' latency),
+// `ends` us of prologue and epilogue, `resident` workgroups a CU.  Fitted to
+// measured products, of which (us by large / mid / small tiles, * the best cut
+// of k)  bfloat16: 8192 x 1024 x 4096 82 / 58 / 84, 8192 x 1024 x 32768 415* /
+// 516 / 853, 32768 x 1024 x 8192 373 / 471 / 994, 1024 x 2048 x 1024 28 / 15 /
+// 12;  float32: 1500 x 777 x 10007 134* / 150* / 205*, 1500 x 10007 x 777 152 /
+// 186 / 223, 1999 x 513 x 1366 40* / 39* / 43*, 256 x 512 x 256 19 / 12 / 9.
 struct Cost {
   int bm, bn, bk, resident;
   double busy, alone, ends;
@@ -320,13 +323,13 @@ template <int NP>
 Cost cost_of(TileSize s) {
   typedef Tiles<NP> X;
   if (NP == 1) {
-    if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 1.72, 1.72, 5.0};
-    if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 2, 0.58, 0.75, 4.0};
-    return {X::Small::BM, X::Small::BN, X::Small::BK, 5, 0.22, 0.55, 3.0};
+    if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 1.6, 1.5, 4.0};
+    if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 2, 0.5, 0.65, 4.0};
+    return {X::Small::BM, X::Small::BN, X::Small::BK, 5, 0.22, 0.42, 3.0};
   }
-  if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 2.5, 2.5, 6.0};
-  if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 1, 1.4, 1.4, 5.0};
-  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.5, 0.95, 4.0};
+  if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 2.1, 2.0, 5.0};
+  if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 1, 1.25, 1.2, 4.0};
+  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.47, 0.9, 3.0};
 }
 
 struct Choice {
@@ -336,28 +339,26 @@ struct Choice {
 
 // The tile and, where `may_split`, the cuts of the k axis that the model gives
 // the least time: the fullest CU's tiles, and the partial sums' way out and
-// back in at 4 TB/s plus their pass.
+// back in at 4 TB/s plus 6 us for their pass.
 template <int NP, class Epi>
 Choice choose(const Launch<Epi>& L, bool dual, bool may_split = false) {
   Choice best{kSmall, 1};
   double least = 1e30;
   for (TileSize s : {kLarge, kMid, kSmall}) {
     const Cost c = cost_of<NP>(s);
+    double tiles = 0, steps = 1, partial = 0;
+    for (int i = 0; i < L.n; ++i) {
+      const Problem& p = L.p[i];
+      const int bn = dual ? c.bn / 2 : c.bn;
+      tiles += (double)((p.M + c.bm - 1) / c.bm) * ((p.N + bn - 1) / bn) * p.batch;
+      steps = std::max(steps, (double)((p.K + c.bk - 1) / c.bk) * p.n_outer * p.n_inner);
+      partial += (double)p.M * p.N * p.batch;
+    }
     for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
-      if (splits > 1 && !may_split) break;
-      double tiles = 0, steps = 1, partial = 0;
-      for (int i = 0; i < L.n; ++i) {
-        const Problem& p = L.p[i];
-        const int bn = dual ? c.bn / 2 : c.bn;
-        tiles += (double)((p.M + c.bm - 1) / c.bm) * ((p.N + bn - 1) / bn) * p.batch * splits;
-        steps = std::max(steps, (double)((p.K + c.bk - 1) / c.bk) * p.n_outer * p.n_inner);
-        partial += (double)p.M * p.N * p.batch;
-      }
-      if (splits > 1 && steps < 4 * splits) break;
-      steps = std::ceil(steps / splits);
-      const double each = std::ceil(tiles / 256), rounds = std::ceil(each / c.resident);
-      double t = std::max(each * c.busy, rounds * c.alone) * steps + rounds * c.ends;
-      if (splits > 1) t += partial * 4 * (2 * splits) / 4e6 + 4;
+      if (splits > 1 && (!may_split || steps < 4 * splits || tiles * splits > 1280)) break;
+      const double each = std::ceil(tiles * splits / 256), rounds = std::ceil(each / c.resident);
+      double t = std::max(each * c.busy, rounds * c.alone) * std::ceil(steps / splits) + rounds * c.ends;
+      if (splits > 1) t += partial * 4 * (2 * splits) / 4e6 + 6;
       if (t < least) {
         least = t;
         best = Choice{s, splits};
@@ -419,10 +420,10 @@ struct Products {
       Problem& p = L.p[i];
       p.splits = c.splits;
       StoreEpi<T>& e = L.e[i];
-      const int64_t n = (int64_t)p.batch * p.M * p.N;
+      const int64_t n = (int64_t)p.batch * p.M * round8(p.N);
       e.sum = ws.take<float>(c.splits * n);
       e.mode = 1;
-      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits, p.N % 8 == 0 && e.vec};
+      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits, e.vec};
       sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + (int64_t)p.batch * p.M * ((p.N + 7) / 8);
       ++sums.n;
     }

@@ -141,18 +141,11 @@ __global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32
 }
 
 // The sum of the rows' losses (mean: over the counted rows, at least one), and
-// the factor of each row's gradient.  One workgroup: fixed order, float64.
-__global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* loss, const int64_t* target,
-                                                           int64_t ignore, int32_t rows, int32_t mean,
-                                                           float* out, float* scale) {
+// the factor of each row's gradient.  One workgroup of 1024: fixed order,
+// float64.
+__device__ __forceinline__ void reduce_loss(double s, int n, int32_t mean, float* out, float* scale) {
   __shared__ double ps[16];
   __shared__ int pn[16];
-  double s = 0.0;
-  int n = 0;
-  for (int r = threadIdx.x; r < rows; r += 1024) {
-    s += (double)loss[r];
-    n += target[r] != ignore;
-  }
   for (int o = 32; o > 0; o >>= 1) {
     s += __shfl_xor(s, o);
     n += __shfl_xor(n, o);
@@ -172,6 +165,49 @@ __global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* loss, co
   const double by = mean ? (double)max(n, 1) : 1.0;
   out[0] = (float)(s / by);
   scale[0] = (float)(1.0 / by);
+}
+
+__global__ __launch_bounds__(1024) void loss_reduce_kernel(const float* loss, const int64_t* target,
+                                                           int64_t ignore, int32_t rows, int32_t mean,
+                                                           float* out, float* scale) {
+  double s = 0.0;
+  int n = 0;
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    s += (double)loss[r];
+    n += target[r] != ignore;
+  }
+  reduce_loss(s, n, mean, out, scale);
+}
+
+// Both passes in one workgroup, a thread a row, for few rows and parts (1024 x
+// 16: two launches' 9 us are one of 5).
+constexpr int64_t kJoinSmall = 16384;
+
+__global__ __launch_bounds__(1024) void lse_join_small_kernel(const float2* part, int32_t parts, int32_t rows,
+                                                              const float* ztarget, const int64_t* target,
+                                                              int64_t vocab, int64_t ignore, int32_t mean,
+                                                              float* lse, float* loss, float* out,
+                                                              float* scale) {
+  double sum = 0.0;
+  int n = 0;
+  for (int r = threadIdx.x; r < rows; r += 1024) {
+    float m = -INFINITY, s = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) m = fmaxf(m, part[(int64_t)p * rows + r].x);
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const float2 v = part[(int64_t)p * rows + r];
+      s += v.x == m ? v.y : v.y * expf(v.x - m);
+    }
+    const float l = m + logf(s);
+    const int64_t t = target[r];
+    const float x = t == ignore ? 0.f : t >= 0 && t < vocab ? l - ztarget[r] : NAN;
+    lse[r] = l;
+    loss[r] = x;
+    sum += (double)x;
+    n += t != ignore;
+  }
+  reduce_loss(sum, n, mean, out, scale);
 }
 
 // dz of a piece of the vocabulary, as operand planes
@@ -267,6 +303,13 @@ int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t strea
   if (R > 0) {
     if (pack.launch(stream) != 0) return -1;
     if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy") != 0) return -1;
+    if (d.reduction != 0 && R >= 64 && R * parts <= kJoinSmall) {
+      lse_join_small_kernel<<<1, 1024, 0, stream>>>(e.part, (int32_t)parts, (int32_t)R, e.ztarget, d.target, V,
+                                                    d.ignore_index, d.reduction == 1, d.lse, d.loss, d.out,
+                                                    d.scale);
+      D3A_LAUNCH_CHECK("linear_cross_entropy");
+      return 0;
+    }
     lse_join_kernel<<<(unsigned)((R + 7) / 8), 256, 0, stream>>>(
         e.part, (int32_t)parts, (int32_t)R, e.ztarget, d.target, V, d.ignore_index, d.lse, d.loss);
     D3A_LAUNCH_CHECK("linear_cross_entropy");
@@ -298,7 +341,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
   dz.p = ws.take<__bf16>(NP * R * ld);
   dz.ld = ld;
   dz.s_part = R * ld;
-  float* sum = n_pieces > 1 && d.dx ? ws.take<float>(R * D) : nullptr;
+  float* sum = n_pieces > 1 && d.dx ? ws.take<float>(R * round8(D)) : nullptr;
   const int64_t keep = ws.used;
   if (!dry && R > 0 && pack.launch(stream) != 0) return -1;
   for (int64_t v0 = 0, k = 0; v0 < V; v0 += piece, ++k) {
@@ -341,8 +384,8 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     }
     if (d.dW) dw.add(dz, x, n, D, R, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0);
     dw.reserve(ws, true);
-    Colsum<T, __bf16, NP> cs;
-    if (d.db) cs.add(dz.p, ld, 0, dz.s_part, R, n, 1, static_cast<T*>(d.db) + v0, 0);
+    Colsum<T, NP> cs;
+    if (d.db) cs.add(dz, R, n, 1, static_cast<T*>(d.db) + v0);
     cs.reserve(ws);
     *bytes = std::max(*bytes, ws.used);
     if (dry) continue;
