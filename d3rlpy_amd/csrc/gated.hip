@@ -42,6 +42,7 @@ __device__ __forceinline__ void activation(int act, float g, float& a, float& da
 template <class T, int NP>
 struct GatedEpi {
   static constexpr bool kStaged = true;
+  static constexpr int kRowBytes = 0;
   float *g, *u;    // kept pre-activations, [batch][M] rows of ld, or null
   __bf16* h;       // planes [NP][batch][M] rows of ld
   int64_t ld, s_part;
@@ -51,13 +52,17 @@ struct GatedEpi {
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
-    each8<C, true>(acc, t, [&](int m, int n, float* v, float* up) {
+    float b[8], c[8];
+    load_bias(bg ? bg + t.batch * s_bias : nullptr, first_column<true>(t), t.N, b);
+    load_bias(bu ? bu + t.batch * s_bias : nullptr, first_column<true>(t), t.N, c);
+    auto none = [](int, int) { return Nothing{}; };
+    each8<C, true>(acc, t, none, [&](int m, int n, float* v, float* up, Nothing) {
       if (n >= ld) return;
       float h8[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        if (bg) v[r] += (float)bg[t.batch * s_bias + min(n + r, t.N - 1)];
-        if (bu) up[r] += (float)bu[t.batch * s_bias + min(n + r, t.N - 1)];
+        v[r] += b[r];
+        up[r] += c[r];
         float a, da;
         activation<NP == 1>(act, v[r], a, da);
         h8[r] = n + r < t.N ? a * up[r] : 0.f;
@@ -75,6 +80,7 @@ struct GatedEpi {
 template <int NP>
 struct GatedBwdEpi {
   static constexpr bool kStaged = true;
+  static constexpr int kRowBytes = 0;
   const float *g, *u;
   __bf16 *dg, *du, *h;  // planes, rows of ld
   int64_t ld, s_part;
@@ -82,19 +88,27 @@ struct GatedBwdEpi {
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
-    each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
+    struct Kept {
+      float g[8], u[8];
+    };
+    auto load = [&](int m, int n) {
+      Kept k;
+      const int64_t at = ((int64_t)t.batch * t.M + m) * ld + min((int64_t)n, ld - 8);
+      load8(g + at, k.g);
+      load8(u + at, k.u);
+      return k;
+    };
+    each8<C, false>(acc, t, load, [&](int m, int n, float* v, float*, const Kept& k) {
       if (n >= ld) return;
       const int64_t at = ((int64_t)t.batch * t.M + m) * ld + n;
       float g8[8], u8[8], h8[8];
-      load8(g + at, g8);
-      load8(u + at, u8);
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         float a, da;
-        activation<NP == 1>(act, g8[r], a, da);
+        activation<NP == 1>(act, k.g[r], a, da);
         const bool on = n + r < t.N;
-        h8[r] = on ? a * u8[r] : 0.f;
-        g8[r] = on ? v[r] * u8[r] * da : 0.f;
+        h8[r] = on ? a * k.u[r] : 0.f;
+        g8[r] = on ? v[r] * k.u[r] * da : 0.f;
         u8[r] = on ? v[r] * a : 0.f;
       }
       store_planes<NP>(dg + at, s_part, g8);

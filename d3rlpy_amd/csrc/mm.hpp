@@ -75,15 +75,20 @@ struct Config {
   static constexpr int A = NP * BM * BK * 2, B = NP * BN * BK * 2;  // bytes of a buffer
   // the waves' slabs lie in the second buffers, and what is over in an array of its own
   static constexpr int SLABS_A = A / kSlab, SLABS_B = B / kSlab;
-  static constexpr int MORE = NW > SLABS_A + SLABS_B ? (NW - SLABS_A - SLABS_B) * kSlab : 16;
-  static constexpr int LDS = 2 * (A + B) + MORE;
+  static constexpr int MORE = NW > SLABS_A + SLABS_B ? (NW - SLABS_A - SLABS_B) * kSlab : 0;
 };
+
+// LDS of a workgroup: the buffers, and what the epilogue keeps of a wave's rows
+template <class C, class Epi>
+constexpr int lds_bytes() {
+  return 2 * (C::A + C::B) + (Epi::kStaged ? C::MORE : 0) + C::NW * C::TM * Epi::kRowBytes;
+}
 
 struct Tile {
   int m0, n0;            // first row / column of this wave's part
   int batch, split, lane;
   int M, N;
-  char* slab;            // staged epilogues: the wave's own kSlab bytes of LDS
+  char *slab, *rows;     // the wave's own LDS: kSlab bytes of a staged epilogue, kRowBytes a row
 };
 
 
@@ -252,7 +257,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
   // (arrays of their own, each named where it is used: so the compiler sees that
   // the loads in flight go to other arrays than the reads, and waits for none;
   // with one array for both operands it waited for all in the transposed reads)
-  __shared__ __attribute__((aligned(1024))) char a0[C::A], a1[C::A], b0[C::B], b1[C::B], extra[C::MORE];
+  __shared__ __attribute__((aligned(1024))) char a0[C::A], a1[C::A], b0[C::B], b1[C::B];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / C::WN, wn = w % C::WN;
@@ -338,7 +343,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
     a_part = P.a.s_part;
     b_part = P.b.s_part;
     b_up = DUAL ? P.b2 - P.b.p : 0;
-    return Tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr};
+    return Tile{m0 + wm * C::TM, n0 + wn * (DUAL ? 32 : C::TN), batch, split, lane, P.M, P.N, nullptr, nullptr};
   };
 
   // Two buffers.  Each step's operands are read while the step before it is in
@@ -416,8 +421,16 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
     }
     Tile out = now;
     if constexpr (Epi::kStaged) {
-      const int in_b = w - C::SLABS_A, in_extra = in_b - C::SLABS_B;
-      out.slab = in_b < 0 ? a1 + w * kSlab : in_extra < 0 ? b1 + in_b * kSlab : extra + in_extra * kSlab;
+      const int in_b = w - C::SLABS_A;
+      out.slab = in_b < 0 ? a1 + w * kSlab : b1 + in_b * kSlab;
+      if constexpr (C::MORE > 0) {
+        __shared__ __attribute__((aligned(16))) char more[C::MORE];
+        if (in_b >= C::SLABS_B) out.slab = more + (in_b - C::SLABS_B) * kSlab;
+      }
+    }
+    if constexpr (Epi::kRowBytes > 0) {
+      __shared__ __attribute__((aligned(16))) char rows[C::NW * C::TM * Epi::kRowBytes];
+      out.rows = rows + w * C::TM * Epi::kRowBytes;
     }
     epi.template run<C>(acc, out);
     if (!more) break;
@@ -451,7 +464,7 @@ int launch(Launch<Epi>& L, hipStream_t stream, const char* what) {
   if (plan<C, DUAL>(L) != 0) return -1;
   if (L.total == 0) return 0;
   // as many workgroups as the chip holds (a multiple of the XCDs), or fewer
-  constexpr int resident = 256 * (160 * 1024 / C::LDS);
+  constexpr int resident = 256 * (160 * 1024 / lds_bytes<C, Epi>());
   mm_kernel<C, AT, BT, DUAL, Epi><<<std::min(L.total, resident), C::THREADS, 0, stream>>>(L);
   D3A_LAUNCH_CHECK(what);
   return 0;
@@ -503,59 +516,110 @@ __device__ __forceinline__ void load8(const float* p, float v[8]) {
   load4(p + 4, v + 4);
 }
 
-// A wave's tile, 32 rows at a time, turned in LDS from the matrix
+// ---- staged epilogues ---------------------------------------------------------
+// A wave's tile, 32 rows at a time, is turned in LDS from the matrix
 // instructions' layout (a lane holds one row's runs of four columns, 64 rows
-// apart in memory) to rows: f(m, n, v[8], up[8]) for m < M, with eight
-// consecutive columns n a lane and whole 128-byte rows a group of lanes, so that
-// the epilogue's loads and stores are 16 bytes a lane and contiguous.  Writing
-// straight from the layout cost the 8192 x 32768 x 1024 logits' gradient
-// 1220 us, of 620 without its stores.  DUAL: the wave's 32 columns of both
-// matrices, v and up.  16-byte piece c of row r sits at c ^ (r & 15).
-template <class C, bool DUAL, class F>
-__device__ __forceinline__ void each8(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, F f) {
+// apart in memory) to rows of eight consecutive columns a lane, so that the
+// epilogue's loads and stores are 16 bytes a lane and contiguous.  Writing
+// straight from the layout cost the 8192 x 32768 x 1024 logits' gradient 1220
+// us, of 620 without its stores.  16-byte piece c of row r sits at c ^ (r & 15).
+//
+// Loads and stores finish in order, so a load issued after a store waits for
+// it: what an epilogue loads, it loads before its first store (columns' biases,
+// rows' statistics by way of LDS) or a pass ahead of the stores (load(), below).
+template <class C>
+__device__ __forceinline__ void turn(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, int i) {
   static_assert(C::TN == 64, "slab");
   const int row = t.lane & 31, half = t.lane >> 5;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = 8 * j + 2 * q + half;
+      const f32x16& a = acc[i][j];
+      *reinterpret_cast<f32x4*>(t.slab + row * 256 + ((c ^ (row & 15)) << 4)) =
+          f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// eight columns from piece c on, of row r
+__device__ __forceinline__ void slab8(const Tile& t, int r, int c, float v[8]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(t.slab + r * 256 + (((c + k) ^ (r & 15)) << 4));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * k + e] = x[e];
+  }
+}
+
+// the first of a lane's eight columns (the same in every pass)
+template <bool DUAL>
+__device__ __forceinline__ int first_column(const Tile& t) {
+  return t.n0 + 8 * (t.lane % (DUAL ? 4 : 8));
+}
+
+struct Nothing {};
+
+// load(m, n) -> L, a pass ahead; f(m, n, v[8], up[8], L) for m < M.  DUAL: the
+// wave's 32 columns of both matrices, v and up.
+template <class C, bool DUAL, class G, class F>
+__device__ __forceinline__ void each8(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, G load, F f) {
+  constexpr int LANES = DUAL ? 4 : 8, PASSES = 32 * LANES / 64;  // lanes a row; passes a slab
+  const int n = first_column<DUAL>(t), c = 2 * (t.lane % LANES), r0 = t.lane / LANES;
+  auto row = [&](int pass) __attribute__((always_inline)) {
+    return t.m0 + pass / PASSES * 32 + pass % PASSES * (64 / LANES) + r0;
+  };
+  auto next = load(min(row(0), t.M - 1), n);
 #pragma unroll
   for (int i = 0; i < C::MT; ++i) {
+    turn<C>(acc, t, i);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 8 * j + 2 * q + half;
-        const f32x16& a = acc[i][j];
-        *reinterpret_cast<f32x4*>(t.slab + row * 256 + ((c ^ (row & 15)) << 4)) =
-            f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    constexpr int LANES = DUAL ? 4 : 8;  // lanes a row
-#pragma unroll
-    for (int p = 0; p < 32 * LANES / 64; ++p) {
-      const int r = p * (64 / LANES) + t.lane / LANES, c = 2 * (t.lane % LANES);
+    for (int p = 0; p < PASSES; ++p) {
+      const int pass = i * PASSES + p, r = p * (64 / LANES) + r0, m = row(pass);
+      const auto now = next;
+      if (pass + 1 < C::MT * PASSES) next = load(min(row(pass + 1), t.M - 1), n);
       float v[8], up[8];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(t.slab + r * 256 + (((c + k) ^ (r & 15)) << 4));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * k + e] = x[e];
-        if constexpr (DUAL) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(t.slab + r * 256 + (((8 + c + k) ^ (r & 15)) << 4));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) up[4 * k + e] = y[e];
-        }
-      }
-      const int m = t.m0 + 32 * i + r, n = t.n0 + 4 * c;
-      if (m < t.M) f(m, n, v, up);
+      slab8(t, r, c, v);
+      if constexpr (DUAL) slab8(t, r, c + 8, up);
+      if (m < t.M) f(m, n, v, up, now);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
+}
+
+// f(m, n, v) of one column a lane, whole rows of 64: for outputs whose rows are
+// not 16-byte aligned
+template <class C, class F>
+__device__ __forceinline__ void each1(const f32x16 (&acc)[C::MT][C::NT], const Tile& t, F f) {
+  const int n = t.n0 + t.lane;
+#pragma unroll
+  for (int i = 0; i < C::MT; ++i) {
+    turn<C>(acc, t, i);
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      const float v = *reinterpret_cast<const float*>(t.slab + r * 256 + (((t.lane >> 2) ^ (r & 15)) << 4) +
+                                                      4 * (t.lane & 3));
+      const int m = t.m0 + 32 * i + r;
+      if (m < t.M && n < t.N) f(m, n, v);
+    }
+  }
+}
+
+// a lane's eight columns of a bias (zero past N, or without one)
+template <class T>
+__device__ __forceinline__ void load_bias(const T* bias, int n, int N, float b[8]) {
+#pragma unroll
+  for (int r = 0; r < 8; ++r) b[r] = bias && n + r < N ? (float)bias[n + r] : 0.f;
 }
 
 // D (+ bias) in T, or a float32 partial of a split / running sum over launches
 template <class T>
 struct StoreEpi {
   static constexpr bool kStaged = true;
+  static constexpr int kRowBytes = 0;
   T* out;           // [batch][M] rows of ld
   int64_t ld, s_batch;
   const T* bias;    // [batch][N] or null
@@ -568,33 +632,45 @@ struct StoreEpi {
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
     const int64_t lds = (t.N + 7) / 8 * 8;
-    each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
+    const T* bias_b = bias ? bias + t.batch * s_bias : nullptr;
+    if (mode == 0 && !vec) {
+      const int n = t.n0 + t.lane;
+      const float b = bias_b && n < t.N ? (float)bias_b[n] : 0.f;
+      T* o = out + t.batch * s_batch;
+      each1<C>(acc, t, [&](int m, int n, float v) { o[m * ld + n] = (T)(v + b); });
+      return;
+    }
+    float b[8];
+    load_bias(bias_b, first_column<false>(t), t.N, b);
+    struct Sum {
+      float v[8];
+    };
+    auto load = [&](int m, int n) {
+      Sum o;
+      if (mode >= 3 && n < t.N) {
+        load8(sum + m * lds + n, o.v);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o.v[r] = 0.f;
+      }
+      return o;
+    };
+    each8<C, false>(acc, t, load, [&](int m, int n, float* v, float*, const Sum& o) {
       if (n >= t.N) return;
       const int left = t.N - n;
-      if (mode != 0) {
-        float* s = sum + ((mode == 1 ? ((int64_t)t.split * n_batch + t.batch) * t.M : 0) + m) * lds + n;
-        if (mode >= 3) {
-          float o[8];
-          load8(s, o);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) v[r] += o[r];
-        }
-        if (mode <= 3) {
-          store8(s, v);
-          return;
-        }
+      for (int r = 0; r < 8; ++r) v[r] += mode == 0 ? b[r] : o.v[r];
+      if (mode != 0 && mode <= 3) {
+        store8(sum + ((mode == 1 ? ((int64_t)t.split * n_batch + t.batch) * t.M : 0) + m) * lds + n, v);
+        return;
       }
-      if (bias) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] += (float)bias[t.batch * s_bias + min(n + r, t.N - 1)];
-      }
-      T* o = out + t.batch * s_batch + (int64_t)m * ld + n;
+      T* p = out + t.batch * s_batch + (int64_t)m * ld + n;
       if (vec && left >= 8) {
-        store8(o, v);
+        store8(p, v);
       } else {
 #pragma unroll
         for (int r = 0; r < 8; ++r)
-          if (r < left) o[r] = (T)v[r];
+          if (r < left) p[r] = (T)v[r];
       }
     });
   }

@@ -49,6 +49,7 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 template <class T, int NP>
 struct LsePartEpi {
   static constexpr bool kStaged = false;
+  static constexpr int kRowBytes = 0;
   const T* bias;
   const int64_t* target;
   float2* part;     // [columns of waves][M]
@@ -62,6 +63,13 @@ struct LsePartEpi {
     // have a border or a target in them: the exponentials' 65536 of a 256 x 256
     // tile are already a tenth of its products' time)
     const bool border = t.n0 + C::TN > t.N;
+    int want[C::MT];  // the target's column of the wave's, or -1
+#pragma unroll
+    for (int i = 0; i < C::MT; ++i) {
+      const int m = t.m0 + 32 * i + (t.lane & 31);
+      const int64_t y = m < t.M ? target[m] - v0 - t.n0 : -1;
+      want[i] = y >= 0 && y < min(C::TN, t.N - t.n0) ? (int)y : -1;
+    }
 #pragma unroll
     for (int i = 0; i < C::MT; ++i) {
       const int m = t.m0 + 32 * i + (t.lane & 31);
@@ -76,15 +84,12 @@ struct LsePartEpi {
             acc[i][j][r] = n < t.N ? v : -INFINITY;
           }
       }
-      const int64_t y = m < t.M ? target[m] - v0 : -1;
-      const bool here = y >= t.n0 && y < t.n0 + C::TN && y < t.N;
-      if (__ballot(here)) {
-        const int want = here ? (int)y : -1;
+      if (__ballot(want[i] >= 0)) {
 #pragma unroll
         for (int j = 0; j < C::NT; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (n0 + 32 * j + 8 * (r / 4) + r % 4 == want) ztarget[m] = acc[i][j][r];
+            if (4 * (t.lane >> 5) + 32 * j + 8 * (r / 4) + r % 4 == want[i]) ztarget[m] = acc[i][j][r];
       }
       float top = -INFINITY;
 #pragma unroll
@@ -214,6 +219,7 @@ __global__ __launch_bounds__(1024) void lse_join_small_kernel(const float2* part
 template <class T, int NP>
 struct DzEpi {
   static constexpr bool kStaged = true;
+  static constexpr int kRowBytes = 16;
   const T* bias;
   const int64_t* target;
   const float *lse, *gloss, *scale;  // scale: null = 1
@@ -225,28 +231,37 @@ struct DzEpi {
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
+    // the wave's rows, two a lane: their lse, gradient factor, and target column
+    // (-1: in no column here; -2: the row is ignored)
     const float by = scale ? scale[0] : 1.f;
-    each8<C, false>(acc, t, [&](int m, int n, float* v, float*) {
-      if (n >= ld) return;
+    float4* rows = reinterpret_cast<float4*>(t.rows);
+#pragma unroll
+    for (int k = 0; k < (C::TM + 63) / 64; ++k) {
+      const int i = 64 * k + t.lane, m = min(t.m0 + i, t.M - 1);
       const int64_t y = target[m];
-      const float l = lse[m], l2 = l * kLog2e;
-      const float g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
-      if (bias) {
+      const float l = lse[m], g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
+      const int64_t want = y - v0;
+      const int col = y == ignore ? -2 : want >= 0 && want < t.N ? (int)want : -1;
+      if (i < C::TM) rows[i] = make_float4(l, l * kLog2e, g, __int_as_float(col));
+    }
+    float b[8];
+    load_bias(bias, first_column<false>(t), t.N, b);
+    auto none = [](int, int) { return Nothing{}; };
+    each8<C, false>(acc, t, none, [&](int m, int n, float* v, float*, Nothing) {
+      if (n >= ld) return;
+      const float4 row = rows[m - t.m0];
+      const int col = __float_as_int(row.w), want = col - n;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] += (float)bias[min(n + r, t.N - 1)];
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = exp_to<NP>(v[r], l, l2);
-      const int64_t want = y - v0 - n;
+      for (int r = 0; r < 8; ++r) v[r] = exp_to<NP>(v[r] + b[r], row.x, row.y);
       if (want >= 0 && want < 8) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] -= r == (int)want ? 1.f : 0.f;
+        for (int r = 0; r < 8; ++r) v[r] -= r == want ? 1.f : 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] *= g;
-      if (y == ignore || n + 8 > t.N) {
+      for (int r = 0; r < 8; ++r) v[r] *= row.z;
+      if (col == -2 || n + 8 > t.N) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = y != ignore && n + r < t.N ? v[r] : 0.f;
+        for (int r = 0; r < 8; ++r) v[r] = col != -2 && n + r < t.N ? v[r] : 0.f;
       }
       store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
     });
