@@ -517,7 +517,7 @@ class IqnHeadBwdFusedDesc(C.Structure):
 # name -> (restype, argtypes)
 class GatedMlpDesc(C.Structure):
     _fields_ = (
-        [(f, vp) for f in ("x", "Wg", "Wu", "Wd", "bg", "bu", "bd", "y", "g", "u", "dy",
+        [(f, vp) for f in ("x", "Wg", "Wu", "Wd", "bg", "bu", "bd", "y", "kept", "dy",
                            "dx", "dWg", "dWu", "dWd", "dbg", "dbu", "dbd")]
         + [(f, C.c_int64) for f in ("rows", "n_in", "n_hidden", "n_out", "members", "ldx", "sx",
                                     "ldWg", "sWg", "ldWu", "sWu", "ldWd", "sWd", "lddy", "sdy")]
@@ -644,6 +644,7 @@ _SIGNATURES = {
     "d3a_td3bc_actor_seed": (C.c_int, [C.POINTER(Td3bcActorDesc), vp]),
     "d3a_td3bc_actor_head": (C.c_int, [C.POINTER(Td3bcActorDesc), vp]),
     "d3a_gated_mlp_workspace": (C.c_int, [C.POINTER(GatedMlpDesc), C.c_int32, C.POINTER(C.c_int64)]),
+    "d3a_gated_mlp_kept": (C.c_int, [C.POINTER(GatedMlpDesc), C.POINTER(C.c_int64)]),
     "d3a_gated_mlp": (C.c_int, [C.POINTER(GatedMlpDesc), vp]),
     "d3a_gated_mlp_bwd": (C.c_int, [C.POINTER(GatedMlpDesc), vp]),
     "d3a_linear_xent_workspace": (C.c_int, [C.POINTER(LinearXentDesc), C.c_int32, C.POINTER(C.c_int64)]),

@@ -8,11 +8,12 @@
 // rows.  The first forward launch stages gate and up weights as one B tile
 // whose waves hold the same 32 columns of both, so activation and product
 // happen on the accumulators; the backward's first launch forms dh and, from
-// the kept g and u, dg, du and h in its epilogue.  Kept between the two: g and
-// u in float32.  In bfloat16 they would halve 270 MB of traffic at 8192 x 4096
+// the kept g and u, dg and du in its epilogue.  Kept between the two: h as the
+// down product's operand, and g and u in float32.  In bfloat16 they would halve 270 MB of traffic at 8192 x 4096
 // hidden values, but a second rounding on the way to each gradient takes its
 // error from 1.4 to 2 times that of the result's own rounding.
 #include "mm_host.hpp"
+#include "thin.hpp"
 #include "../../include/d3rlpy_amd.h"
 
 namespace d3a {
@@ -82,38 +83,36 @@ struct GatedBwdEpi {
   static constexpr bool kStaged = true;
   static constexpr int kRowBytes = 0;
   const float *g, *u;
-  __bf16 *dg, *du, *h;  // planes, rows of ld
+  __bf16 *dg, *du;  // planes, rows of ld
   int64_t ld, s_part;
   int32_t act;
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
-    struct Kept {
+    struct Both {
       float g[8], u[8];
     };
     auto load = [&](int m, int n) {
-      Kept k;
+      Both k;
       const int64_t at = ((int64_t)t.batch * t.M + m) * ld + min((int64_t)n, ld - 8);
       load8(g + at, k.g);
       load8(u + at, k.u);
       return k;
     };
-    each8<C, false>(acc, t, load, [&](int m, int n, float* v, float*, const Kept& k) {
+    each8<C, false>(acc, t, load, [&](int m, int n, float* v, float*, const Both& k) {
       if (n >= ld) return;
       const int64_t at = ((int64_t)t.batch * t.M + m) * ld + n;
-      float g8[8], u8[8], h8[8];
+      float g8[8], u8[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         float a, da;
         activation<NP == 1>(act, k.g[r], a, da);
         const bool on = n + r < t.N;
-        h8[r] = on ? a * k.u[r] : 0.f;
         g8[r] = on ? v[r] * k.u[r] * da : 0.f;
         u8[r] = on ? v[r] * a : 0.f;
       }
       store_planes<NP>(dg + at, s_part, g8);
       store_planes<NP>(du + at, s_part, u8);
-      store_planes<NP>(h + at, s_part, h8);
     });
   }
 };
@@ -132,19 +131,105 @@ int check(const d3a_gated_mlp_desc* d, bool bwd) {
                 "gated_mlp: row stride smaller than the row");
   D3A_CHECK_ARG(d->Wg && d->Wu && d->Wd, "gated_mlp: null weight");
   if (d->rows > 0) D3A_CHECK_ARG(d->x && (bwd ? d->dy != nullptr : d->y != nullptr), "gated_mlp: null operand");
-  D3A_CHECK_ARG((d->g == nullptr) == (d->u == nullptr), "gated_mlp: g and u go together");
-  const uintptr_t kept = reinterpret_cast<uintptr_t>(d->g) | reinterpret_cast<uintptr_t>(d->u);
-  D3A_CHECK_ARG((kept & 15) == 0, "gated_mlp: g and u must be 16-byte aligned");
+  D3A_CHECK_ARG((reinterpret_cast<uintptr_t>(d->kept) & 15) == 0, "gated_mlp: kept must be 16-byte aligned");
   if (bwd) {
-    D3A_CHECK_ARG(d->g || d->rows == 0, "gated_mlp: the backward needs the forward's g and u");
+    D3A_CHECK_ARG(d->kept || d->rows == 0, "gated_mlp: the backward needs what the forward kept");
     D3A_CHECK_ARG(d->lddy >= d->n_out, "gated_mlp: row stride smaller than the row");
   }
+  return 0;
+}
+
+// What the forward keeps: g and u, then h's planes, rows of F8 each.
+template <int NP>
+struct Kept {
+  float *g = nullptr, *u = nullptr;
+  Operand h{};
+  explicit Kept(const d3a_gated_mlp_desc& d) {
+    const int64_t F8 = round8(d.n_hidden), n = d.members * d.rows * F8;
+    h.ld = F8;
+    h.s_batch = d.rows * F8;
+    h.s_part = n;
+    if (!d.kept) return;
+    g = static_cast<float*>(d.kept);
+    u = g + n;
+    h.p = reinterpret_cast<const __bf16*>(u + n);
+  }
+  static int64_t bytes(const d3a_gated_mlp_desc& d) {
+    return d.members * d.rows * round8(d.n_hidden) * (2 * 4 + NP * 2);
+  }
+};
+
+struct Activation {
+  __device__ __forceinline__ void operator()(int act, float g, float& a, float& da) const {
+    activation<false>(act, g, a, da);
+  }
+};
+
+// a weight or x whose rows are whole aligned 16-byte pieces
+template <class T>
+bool whole(const void* p, int64_t ld, int64_t s, int64_t n) {
+  constexpr int64_t N = 16 / sizeof(T);
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % N == 0 && s % N == 0 && n % N == 0;
+}
+
+// At most 16 rows: the weights read once.  One row of 2048 x 5632 bfloat16: 9 us
+// and 6, where the tiles take 15 and 13.
+template <class T, int NP>
+int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
+  const Kept<NP> k(d);
+  __bf16* h = d.kept ? const_cast<__bf16*>(k.h.p) : ws.take<__bf16>(NP * C * R * F8);
+  *bytes = ws.used;
+  if (dry || R == 0) return 0;
+  thin::GateArgs<T> a{};
+  a.x = static_cast<const T*>(d.x);
+  a.Wg = static_cast<const T*>(d.Wg);
+  a.Wu = static_cast<const T*>(d.Wu);
+  a.bg = static_cast<const T*>(d.bg);
+  a.bu = static_cast<const T*>(d.bu);
+  a.ldx = d.ldx;
+  a.sx = C > 1 ? d.sx : 0;
+  a.ldg = d.ldWg;
+  a.sg = C > 1 ? d.sWg : 0;
+  a.ldu = d.ldWu;
+  a.su = C > 1 ? d.sWu : 0;
+  a.g = k.g;
+  a.u = k.u;
+  a.h = h;
+  a.ld = F8;
+  a.s_part = C * R * F8;
+  a.R = (int32_t)R;
+  a.D = (int32_t)D;
+  a.F = (int32_t)F;
+  a.act = d.act;
+  const dim3 gate((unsigned)((F + 15) / 16), (unsigned)C), down((unsigned)((O + 15) / 16), (unsigned)C);
+  if (whole<T>(d.x, a.ldx, a.sx, D) && whole<T>(d.Wg, a.ldg, a.sg, D) && whole<T>(d.Wu, a.ldu, a.su, D))
+    thin::gate_kernel<T, NP, true><<<gate, 512, 0, stream>>>(a, Activation{});
+  else
+    thin::gate_kernel<T, NP, false><<<gate, 512, 0, stream>>>(a, Activation{});
+  D3A_LAUNCH_CHECK("gated_mlp");
+  thin::DownArgs<T> b{};
+  b.h = h;
+  b.W = static_cast<const T*>(d.Wd);
+  b.b = static_cast<const T*>(d.bd);
+  b.y = static_cast<T*>(d.y);
+  b.ld = F8;
+  b.s_part = a.s_part;
+  b.ldw = d.ldWd;
+  b.sw = C > 1 ? d.sWd : 0;
+  b.R = (int32_t)R;
+  b.F = (int32_t)F;
+  b.O = (int32_t)O;
+  if (whole<T>(d.Wd, b.ldw, b.sw, F)) thin::down_kernel<T, NP, true><<<down, 1024, 0, stream>>>(b);
+  else thin::down_kernel<T, NP, false><<<down, 1024, 0, stream>>>(b);
+  D3A_LAUNCH_CHECK("gated_mlp");
   return 0;
 }
 
 // run (stream given) or measure (ws null): the same walk over the workspace
 template <class T, int NP>
 int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  if (d.rows <= thin::kRows) return forward_thin<T, NP>(d, ws, dry, stream, bytes);
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
   Packer<T, NP> pack(ws);
   const Operand x = pack.operand(d.x, d.ldx, C > 1 ? d.sx : 0, C, R, D);
@@ -153,11 +238,9 @@ int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream,
   const Operand wg = pack.operand(d.Wg, d.ldWg, C > 1 ? d.sWg : 0, C, F, D, apart);
   const Operand wu = pack.operand(d.Wu, d.ldWu, C > 1 ? d.sWu : 0, C, F, D, apart);
   const Operand wd = pack.operand(d.Wd, d.ldWd, C > 1 ? d.sWd : 0, C, O, F);
-  Operand h{};
-  h.p = ws.take<__bf16>(NP * C * R * F8);
-  h.ld = F8;
-  h.s_batch = R * F8;
-  h.s_part = C * R * F8;
+  const Kept<NP> k(d);
+  Operand h = k.h;
+  if (!d.kept) h.p = ws.take<__bf16>(NP * C * R * F8);
 
   Launch<GatedEpi<T, NP>> L{};
   L.n = 1;
@@ -171,8 +254,8 @@ int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream,
   p.batch = (int32_t)C;
   p.n_outer = p.n_inner = p.splits = 1;
   GatedEpi<T, NP>& e = L.e[0];
-  e.g = d.g;
-  e.u = d.u;
+  e.g = k.g;
+  e.u = k.u;
   e.h = const_cast<__bf16*>(h.p);
   e.ld = F8;
   e.s_part = h.s_part;
@@ -183,9 +266,9 @@ int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream,
 
   Products<T, NP> down;
   down.add(h, wd, R, O, F, C, 1, 1, d.y, O, R * O, d.bd, O);
-  down.reserve(ws, d.bd == nullptr);
+  down.reserve(ws, true);
   *bytes = ws.used;
-  if (dry || R == 0) return 0;
+  if (dry) return 0;
   if (pack.launch(stream) != 0) return -1;
   if (run<NP, false, false, true>(L, choose<NP>(L, true).size, stream, "gated_mlp") != 0) return -1;
   return down.template launch<false, false>(stream, "gated_mlp");
@@ -194,10 +277,10 @@ int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream,
 template <class T, int NP>
 int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
-  const bool hidden = d.dx || d.dWg || d.dWu || d.dWd || d.dbg || d.dbu;
+  const bool hidden = d.dx || d.dWg || d.dWu || d.dbg || d.dbu;  // dg and du are needed
   Packer<T, NP> pack(ws);
   Operand dy{}, x{}, wd{}, wg{}, wu{};
-  if (hidden || d.dbd) dy = pack.operand(d.dy, d.lddy, C > 1 ? d.sdy : 0, C, R, O);
+  if (hidden || d.dWd || d.dbd) dy = pack.operand(d.dy, d.lddy, C > 1 ? d.sdy : 0, C, R, O);
   if (hidden) {
     wd = pack.operand(d.Wd, d.ldWd, C > 1 ? d.sWd : 0, C, O, F);
   }
@@ -210,13 +293,13 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   }
   const int64_t plane = C * R * F8;
   Operand dg{};
-  dg.p = hidden ? ws.take<__bf16>(3 * NP * plane) : nullptr;  // dg, du, h
+  dg.p = hidden ? ws.take<__bf16>(2 * NP * plane) : nullptr;  // dg, du
   dg.ld = F8;
   dg.s_batch = R * F8;
   dg.s_part = plane;
-  Operand du = dg, h = dg;
+  Operand du = dg;
   du.p += NP * plane;
-  h.p += 2 * NP * plane;
+  const Kept<NP> k(d);
 
   Launch<GatedBwdEpi<NP>> L{};
   L.n = 1;
@@ -229,11 +312,10 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   p.batch = (int32_t)C;
   p.n_outer = p.n_inner = p.splits = 1;
   GatedBwdEpi<NP>& e = L.e[0];
-  e.g = d.g;
-  e.u = d.u;
+  e.g = k.g;
+  e.u = k.u;
   e.dg = const_cast<__bf16*>(dg.p);
   e.du = const_cast<__bf16*>(du.p);
-  e.h = const_cast<__bf16*>(h.p);
   e.ld = F8;
   e.s_part = plane;
   e.act = d.act;
@@ -256,7 +338,7 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   }
   if (d.dWg) dw.add(dg, x, F, D, R, C, 1, 1, d.dWg, D, F * D, nullptr, 0);
   if (d.dWu) dw.add(du, x, F, D, R, C, 1, 1, d.dWu, D, F * D, nullptr, 0);
-  if (d.dWd) dw.add(dy, h, O, F, R, C, 1, 1, d.dWd, F, O * F, nullptr, 0);
+  if (d.dWd) dw.add(dy, k.h, O, F, R, C, 1, 1, d.dWd, F, O * F, nullptr, 0);
   dw.reserve(ws, true);
   Colsum<T, NP> cs;
   if (d.dbg) cs.add(dg, R, F, C, d.dbg);
@@ -299,6 +381,12 @@ int d3a_gated_mlp_workspace(const d3a_gated_mlp_desc* d, int32_t backward, int64
   if (d3a::check(d, backward != 0) != 0) return -1;
   D3A_CHECK_ARG(bytes, "gated_mlp: null size");
   return d3a::call(d, backward != 0, true, nullptr, bytes);
+}
+
+int d3a_gated_mlp_kept(const d3a_gated_mlp_desc* d, int64_t* bytes) {
+  D3A_CHECK_ARG(d && bytes, "gated_mlp: null descriptor or size");
+  *bytes = d->dtype == D3A_F32 ? d3a::Kept<3>::bytes(*d) : d3a::Kept<1>::bytes(*d);
+  return 0;
 }
 
 int d3a_gated_mlp(const d3a_gated_mlp_desc* d, void* stream) { return d3a::entry(d, false, stream); }

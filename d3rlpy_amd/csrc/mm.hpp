@@ -390,7 +390,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
   int id = blockIdx.x;
   Tile tile = enter(id);
   load(a0, b0);
-  for (;;) {
+  for (bool first = true;; first = false) {
     f32x16 acc[C::MT][C::NT];
 #pragma unroll
     for (int i = 0; i < C::MT; ++i)
@@ -401,7 +401,9 @@ __global__ __launch_bounds__(C::THREADS, 2) void mm_kernel(const Launch<Epi> L) 
 
     int n = to_load + 1;  // k tiles
     load(a1, b1);
-    arrive<LPT>();
+    // (a later tile's first loads arrived before the epilogue's first store, see
+    // wait_loads: waiting for them here would be waiting for its stores)
+    if (first) arrive<LPT>();
     f0.read(a0, b0, 0, wm, wn, lane);
     // (in pairs: a tile past the last is zeros)
     do {
@@ -564,6 +566,10 @@ __device__ __forceinline__ int first_column(const Tile& t) {
 
 struct Nothing {};
 
+// Every epilogue's, before its first store: the next tile's first loads have
+// arrived, and the main loop need not wait for the stores behind them.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // load(m, n) -> L, a pass ahead; f(m, n, v[8], up[8], L) for m < M.  DUAL: the
 // wave's 32 columns of both matrices, v and up.
 template <class C, bool DUAL, class G, class F>
@@ -577,6 +583,7 @@ __device__ __forceinline__ void each8(const f32x16 (&acc)[C::MT][C::NT], const T
 #pragma unroll
   for (int i = 0; i < C::MT; ++i) {
     turn<C>(acc, t, i);
+    if (i == 0) wait_loads();
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int pass = i * PASSES + p, r = p * (64 / LANES) + r0, m = row(pass);
@@ -598,6 +605,7 @@ __device__ __forceinline__ void each1(const f32x16 (&acc)[C::MT][C::NT], const T
 #pragma unroll
   for (int i = 0; i < C::MT; ++i) {
     turn<C>(acc, t, i);
+    if (i == 0) wait_loads();
 #pragma unroll 8
     for (int r = 0; r < 32; ++r) {
       const float v = *reinterpret_cast<const float*>(t.slab + r * 256 + (((t.lane >> 2) ^ (r & 15)) << 4) +

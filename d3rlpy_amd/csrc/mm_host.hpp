@@ -140,6 +140,7 @@ struct Packer {
 // out[b][c] = sum over rows of the value at [b][r][c] of NP operand planes.
 // Rows are cut into chunks whose float32 sums a second pass adds in order, so
 // the result does not depend on timing; few rows are one chunk and one pass.
+// Memory bound: four columns (8 bytes a plane) a lane.
 struct ColsumJob {
   const __bf16* src;
   int64_t ld, s_batch, s_part;
@@ -149,66 +150,95 @@ struct ColsumJob {
 constexpr int kMaxColsum = 3;
 struct ColsumJobs {
   ColsumJob j[kMaxColsum];
-  float* part;                    // [chunks][total columns]
-  int64_t first[kMaxColsum + 1];  // running count of batch * cols
+  float* part;                    // [chunks][quads][4]
+  int64_t first[kMaxColsum + 1];  // running count of batch * quads of columns
   int32_t n, chunks;
 };
 
-// the job that column c of all belongs to, and its place there
-__device__ __forceinline__ const ColsumJob& colsum_job(const ColsumJobs& J, int64_t c, int64_t& at) {
+// the job that quad q of all belongs to, its batch and its first column there
+__device__ __forceinline__ const ColsumJob& colsum_job(const ColsumJobs& J, int64_t q, int64_t& b, int& col) {
   int i = 0;
-  while (i + 1 < J.n && c >= J.first[i + 1]) ++i;
-  at = c - J.first[i];
-  return J.j[i];
+  while (i + 1 < J.n && q >= J.first[i + 1]) ++i;
+  const ColsumJob& j = J.j[i];
+  const int64_t quads = (j.cols + 3) / 4, at = q - J.first[i];
+  b = at / quads;
+  col = (int)(at - b * quads) * 4;
+  return j;
 }
 
-// a workgroup: 64 columns (one a lane) x its chunk of rows over sixteen waves
+template <class T>
+__device__ __forceinline__ void colsum_store(const ColsumJob& j, int64_t b, int col, const float s[4]) {
+  T* o = static_cast<T*>(j.out) + b * j.cols + col;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (col + k < j.cols) o[k] = (T)s[k];
+}
+
+// a workgroup: 64 quads (one a lane) x its chunk of rows over sixteen waves
 template <class T, int NP>
 __global__ __launch_bounds__(1024) void colsum_kernel(const ColsumJobs J) {
-  __shared__ float red[1024];
+  __shared__ f32x4 red[1024];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t cols = J.first[J.n], c = (int64_t)blockIdx.x * 64 + lane;
-  const bool on = c < cols;
-  int64_t at;
-  const ColsumJob& j = colsum_job(J, on ? c : 0, at);
-  const int64_t b = at / j.cols;
-  const __bf16* p = j.src + b * j.s_batch + at - b * j.cols;
+  const int64_t quads = J.first[J.n], q = (int64_t)blockIdx.x * 64 + lane;
+  const bool on = q < quads;
+  int64_t b;
+  int col;
+  const ColsumJob& j = colsum_job(J, on ? q : 0, b, col);
+  const __bf16* p = j.src + b * j.s_batch + col;
   const int64_t per = (j.rows + J.chunks - 1) / J.chunks;
   const int64_t r0 = per * blockIdx.y, r1 = min(r0 + per, (int64_t)j.rows);
-  float s = 0.f;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (on)
-#pragma unroll 8
+#pragma unroll 4
     for (int64_t r = r0 + w; r < r1; r += 16) {
-      float v = 0.f;
+      bf16x4 x[NP];
 #pragma unroll
-      for (int q = NP - 1; q >= 0; --q) v += (float)p[q * j.s_part + r * j.ld];
-      s += v;
+      for (int k = 0; k < NP; ++k) x[k] = *reinterpret_cast<const bf16x4*>(p + k * j.s_part + r * j.ld);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = (float)x[NP - 1][e];
+#pragma unroll
+        for (int k = NP - 2; k >= 0; --k) v += (float)x[k][e];
+        s[e] += v;
+      }
     }
   red[threadIdx.x] = s;
   __syncthreads();
   if (w != 0 || !on) return;
-  for (int k = 1; k < 16; ++k) s += red[64 * k + lane];
-  if (J.chunks == 1) static_cast<T*>(j.out)[at] = (T)s;
-  else J.part[blockIdx.y * cols + c] = s;
+  for (int k = 1; k < 16; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += red[64 * k + lane][e];
+  const float v[4] = {s[0], s[1], s[2], s[3]};
+  if (J.chunks == 1) colsum_store<T>(j, b, col, v);
+  else store4(J.part + (blockIdx.y * quads + q) * 4, v);
 }
 
-// 64 columns x the chunks over sixteen waves
+// 64 quads x the chunks over sixteen waves
 template <class T>
 __global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs J) {
-  __shared__ float red[1024];
+  __shared__ f32x4 red[1024];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane, cols = J.first[J.n];
-  float s = 0.f;
-  if (c < cols)
+  const int64_t quads = J.first[J.n], q = (int64_t)blockIdx.x * 64 + lane;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (q < quads)
 #pragma unroll 4
-    for (int k = w; k < J.chunks; k += 16) s += J.part[k * cols + c];
+    for (int k = w; k < J.chunks; k += 16) {
+      float v[4];
+      load4(J.part + (k * quads + q) * 4, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
   red[threadIdx.x] = s;
   __syncthreads();
-  if (w != 0 || c >= cols) return;
-  for (int k = 1; k < 16; ++k) s += red[64 * k + lane];
-  int64_t at;
-  const ColsumJob& j = colsum_job(J, c, at);
-  static_cast<T*>(j.out)[at] = (T)s;
+  if (w != 0 || q >= quads) return;
+  for (int k = 1; k < 16; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += red[64 * k + lane][e];
+  int64_t b;
+  int col;
+  const ColsumJob& j = colsum_job(J, q, b, col);
+  const float v[4] = {s[0], s[1], s[2], s[3]};
+  colsum_store<T>(j, b, col, v);
 }
 
 template <class T, int NP>
@@ -216,24 +246,25 @@ struct Colsum {
   ColsumJobs jobs{};
   void add(const Operand& o, int64_t rows, int64_t cols, int64_t batch, void* out) {
     jobs.j[jobs.n] = ColsumJob{o.p, o.ld, o.s_batch, o.s_part, out, (int32_t)rows, (int32_t)cols, (int32_t)batch};
-    jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * cols;
+    jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * ((cols + 3) / 4);
     ++jobs.n;
-    // about 512 workgroups, chunks of at least 128 rows
+    // about 768 workgroups, chunks of at least 64 rows (four a wave)
     const int64_t blocks = (jobs.first[jobs.n] + 63) / 64;
-    jobs.chunks = (int32_t)std::max<int64_t>(
-        1, std::min<int64_t>({512 / std::max<int64_t>(blocks, 1), rows / 128, 256}));
-    if (rows <= 512) jobs.chunks = 1;
+    jobs.chunks = rows <= 512 ? 1
+                              : (int32_t)std::max<int64_t>(
+                                    1, std::min<int64_t>({768 / std::max<int64_t>(blocks, 1), rows / 64, 256}));
   }
   void reserve(Arena& ws) {
-    if (jobs.n && jobs.chunks > 1) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n]);
+    if (jobs.n && jobs.chunks > 1) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n] * 4);
   }
   int launch(hipStream_t stream) {
-    const int64_t cols = jobs.first[jobs.n];
-    if (jobs.n == 0 || cols == 0) return 0;
-    colsum_kernel<T, NP><<<dim3((unsigned)((cols + 63) / 64), jobs.chunks), 1024, 0, stream>>>(jobs);
+    const int64_t quads = jobs.first[jobs.n];
+    if (jobs.n == 0 || quads == 0) return 0;
+    const unsigned blocks = (unsigned)((quads + 63) / 64);
+    colsum_kernel<T, NP><<<dim3(blocks, jobs.chunks), 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
     if (jobs.chunks == 1) return 0;
-    colsum_finish<T><<<(unsigned)((cols + 63) / 64), 1024, 0, stream>>>(jobs);
+    colsum_finish<T><<<blocks, 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
     return 0;
   }
@@ -244,7 +275,8 @@ template <class T>
 struct SumJob {
   const float* part;  // [splits][batch][M] rows of round8(N)
   T* out;
-  int64_t ld, s_batch;
+  const T* bias;      // [batch][N] or null
+  int64_t ld, s_batch, s_bias;
   int64_t n;          // batch * M * round8(N)
   int32_t M, N, splits, vec;  // vec: out takes eight values at a time
 };
@@ -268,8 +300,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
   const float* p = j.part + (row * pieces) * 8 + n;
   T* o = j.out + b * j.s_batch + (row - b * j.M) * j.ld + n;
   float s[8];
-#pragma unroll
-  for (int r = 0; r < 8; ++r) s[r] = 0.f;
+  load_bias(j.bias ? j.bias + b * j.s_bias : nullptr, n, j.N, s);
 #pragma unroll 2
   for (int k = 0; k < j.splits; ++k) {
     float v[8];
@@ -323,13 +354,13 @@ template <int NP>
 Cost cost_of(TileSize s) {
   typedef Tiles<NP> X;
   if (NP == 1) {
-    if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 1.6, 1.5, 4.0};
-    if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 2, 0.5, 0.65, 4.0};
-    return {X::Small::BM, X::Small::BN, X::Small::BK, 5, 0.22, 0.42, 3.0};
+    if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 1.6, 1.4, 6.0};
+    if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 2, 0.5, 0.58, 5.5};
+    return {X::Small::BM, X::Small::BN, X::Small::BK, 5, 0.22, 0.27, 5.5};
   }
-  if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 2.1, 2.0, 5.0};
-  if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 1, 1.25, 1.2, 4.0};
-  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.47, 0.9, 3.0};
+  if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 2.1, 1.9, 6.0};
+  if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 1, 1.25, 1.15, 5.5};
+  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.47, 0.35, 5.5};
 }
 
 struct Choice {
@@ -339,7 +370,7 @@ struct Choice {
 
 // The tile and, where `may_split`, the cuts of the k axis that the model gives
 // the least time: the fullest CU's tiles, and the partial sums' way out and
-// back in at 4 TB/s plus 6 us for their pass.
+// back in at 4 TB/s plus 12 us for their pass (5 of them on the host).
 template <int NP, class Epi>
 Choice choose(const Launch<Epi>& L, bool dual, bool may_split = false) {
   Choice best{kSmall, 1};
@@ -356,9 +387,10 @@ Choice choose(const Launch<Epi>& L, bool dual, bool may_split = false) {
     }
     for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (splits > 1 && (!may_split || steps < 4 * splits || tiles * splits > 1280)) break;
-      const double each = std::ceil(tiles * splits / 256), rounds = std::ceil(each / c.resident);
-      double t = std::max(each * c.busy, rounds * c.alone) * std::ceil(steps / splits) + rounds * c.ends;
-      if (splits > 1) t += partial * 4 * (2 * splits) / 4e6 + 6;
+      const int each = (int)std::ceil(tiles * splits / 256), full = each / c.resident, over = each % c.resident;
+      double t = full * std::max(c.resident * c.busy, c.alone) + (over ? std::max(over * c.busy, c.alone) : 0.0);
+      t = t * std::ceil(steps / splits) + (full + (over > 0)) * c.ends;
+      if (splits > 1) t += partial * 4 * (2 * splits) / 4e6 + 12;
       if (t < least) {
         least = t;
         best = Choice{s, splits};
@@ -423,7 +455,7 @@ struct Products {
       const int64_t n = (int64_t)p.batch * p.M * round8(p.N);
       e.sum = ws.take<float>(c.splits * n);
       e.mode = 1;
-      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.ld, e.s_batch, n, p.M, p.N, p.splits, e.vec};
+      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.bias, e.ld, e.s_batch, e.s_bias, n, p.M, p.N, p.splits, e.vec};
       sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + (int64_t)p.batch * p.M * ((p.N + 7) / 8);
       ++sums.n;
     }

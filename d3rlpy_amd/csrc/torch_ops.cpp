@@ -844,9 +844,7 @@ void gated_call(GatedCall& c, const Gated& s, const at::Tensor& x, const at::Ten
   d.bd = ptr_or_null(c.bd);
 }
 
-int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
-
-// -> (y, pre [2, members, rows, hidden rounded up to 8]: g and u in float32; empty unless `keep`)
+// -> (y, kept: bytes for the backward; empty unless `keep`)
 std::tuple<at::Tensor, at::Tensor> gated_mlp_hip(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
                                                  const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
                                                  const OptTensor& bd, c10::string_view act, bool keep) {
@@ -856,18 +854,16 @@ std::tuple<at::Tensor, at::Tensor> gated_mlp_hip(const at::Tensor& x, const at::
   GatedCall c;
   gated_call(c, s, x, Wg, Wu, Wd, bg, bu, bd, act);
   at::Tensor y = at::empty(s.y_shape, x.options());
-  at::Tensor pre = keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options().dtype(at::kFloat))
-                        : at::empty({0}, x.options().dtype(at::kFloat));
   c.d.y = y.data_ptr();
-  if (pre.numel() > 0) {
-    c.d.g = pre.data_ptr<float>();
-    c.d.u = c.d.g + pre.numel() / 2;
-  }
+  int64_t bytes = 0;
+  if (keep) check_rc(d3a_gated_mlp_kept(&c.d, &bytes), "d3rlpy_amd::gated_mlp");
+  at::Tensor kept = workspace(bytes, x);
+  c.d.kept = bytes > 0 ? kept.data_ptr() : nullptr;
   check_rc(d3a_gated_mlp_workspace(&c.d, 0, &c.d.ws_bytes), "d3rlpy_amd::gated_mlp");
   const at::Tensor ws = workspace(c.d.ws_bytes, x);
   c.d.ws = ws.data_ptr();
   check_rc(d3a_gated_mlp(&c.d, cur_stream()), "d3rlpy_amd::gated_mlp");
-  return {y, pre};
+  return {y, kept};
 }
 
 std::tuple<at::Tensor, at::Tensor> gated_mlp_meta(const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
@@ -875,8 +871,14 @@ std::tuple<at::Tensor, at::Tensor> gated_mlp_meta(const at::Tensor& x, const at:
                                                   const OptTensor& bd, c10::string_view act, bool keep) {
   const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
   activation_code(act);
-  return {at::empty(s.y_shape, x.options()),
-          keep ? at::empty({2, s.members, s.rows, round8(s.n_hidden)}, x.options().dtype(at::kFloat)) : at::empty({0}, x.options().dtype(at::kFloat))};
+  d3a_gated_mlp_desc d{};
+  d.dtype = dtype_code(x, "gated_mlp", "x");
+  d.members = s.members;
+  d.rows = s.rows;
+  d.n_hidden = s.n_hidden;
+  int64_t bytes = 0;
+  if (keep) check_rc(d3a_gated_mlp_kept(&d, &bytes), "d3rlpy_amd::gated_mlp");
+  return {at::empty(s.y_shape, x.options()), at::empty({bytes}, x.options().dtype(at::kByte))};
 }
 
 using Seven = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
@@ -897,15 +899,11 @@ std::array<at::Tensor, 7> gated_grads(const at::Tensor& x, const at::Tensor& Wg,
 // the gradients of x, Wg, Wu, Wd, bg, bu, bd that `wanted` asks for; the others undefined
 Seven gated_mlp_backward_hip(const at::Tensor& g, const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
                              const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
-                             const at::Tensor& pre, c10::string_view act, std::array<bool, 7> wanted) {
+                             const at::Tensor& kept, c10::string_view act, std::array<bool, 7> wanted) {
   check_gpu(x, "gated_mlp_backward");
   const Gated s = gated_shape(x, Wg, Wu, Wd, bg, bu, bd);
   check_like(g, x, "gated_mlp_backward", "grad");
-  check_f32_gpu(pre, "pre");
-  TORCH_CHECK(pre.device() == x.device(), "gated_mlp_backward: pre is on ", pre.device(), ", x on ", x.device());
   TORCH_CHECK(g.sizes() == at::IntArrayRef(s.y_shape), "gated_mlp_backward: grad must have the output's shape");
-  TORCH_CHECK(pre.numel() == 2 * s.members * s.rows * round8(s.n_hidden),
-              "gated_mlp_backward: pre of a forward with keep = True");
   const c10::DeviceGuard guard(x.device());
   GatedCall c;
   gated_call(c, s, x, Wg, Wu, Wd, bg, bu, bd, act);
@@ -913,10 +911,12 @@ Seven gated_mlp_backward_hip(const at::Tensor& g, const at::Tensor& x, const at:
   c.d.dy = c.dy.t.data_ptr();
   c.d.lddy = c.dy.ld;
   c.d.sdy = c.dy.s;
-  if (pre.numel() > 0) {
-    c.d.g = pre.data_ptr<float>();
-    c.d.u = c.d.g + pre.numel() / 2;
-  }
+  int64_t bytes = 0;
+  check_rc(d3a_gated_mlp_kept(&c.d, &bytes), "d3rlpy_amd::gated_mlp_backward");
+  TORCH_CHECK(kept.device() == x.device() && kept.scalar_type() == at::kByte && kept.is_contiguous() &&
+                  kept.numel() == bytes,
+              "gated_mlp_backward: kept of a forward with keep = True");
+  c.d.kept = bytes > 0 ? kept.data_ptr() : nullptr;
   std::array<at::Tensor, 7> o = gated_grads(x, Wg, Wu, Wd, bg, bu, bd, wanted);
   void** to[7] = {&c.d.dx, &c.d.dWg, &c.d.dWu, &c.d.dWd, &c.d.dbg, &c.d.dbu, &c.d.dbd};
   for (int i = 0; i < 7; ++i) *to[i] = ptr_or_null(o[i]);
@@ -1176,12 +1176,12 @@ struct GatedMlpNode : torch::autograd::Function<GatedMlpNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& Wg, const at::Tensor& Wu,
                                const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
                                const OptTensor& bd, std::string act, int64_t mask) {
-    auto [y, pre] = gated_mlp_below(x, Wg, Wu, Wd, bg, bu, bd, act, true);
-    ctx->save_for_backward({x, Wg, Wu, Wd, value(bg), value(bu), value(bd), pre});
+    auto [y, kept] = gated_mlp_below(x, Wg, Wu, Wd, bg, bu, bd, act, true);
+    ctx->save_for_backward({x, Wg, Wu, Wd, value(bg), value(bu), value(bd), kept});
     ctx->saved_data["mask"] = mask;
     ctx->saved_data["act"] = act;
-    ctx->mark_non_differentiable({pre});
-    return {y, pre};
+    ctx->mark_non_differentiable({kept});
+    return {y, kept};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     using Sig = Seven(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
@@ -1307,7 +1307,7 @@ TORCH_LIBRARY(d3rlpy_amd, m) {
   m.def("gated_mlp(Tensor x, Tensor Wg, Tensor Wu, Tensor Wd, Tensor? bg, Tensor? bu, Tensor? bd, "
         "str activation, bool keep) -> (Tensor, Tensor)");
   m.def("gated_mlp_backward(Tensor grad, Tensor x, Tensor Wg, Tensor Wu, Tensor Wd, Tensor? bg, "
-        "Tensor? bu, Tensor? bd, Tensor pre, str activation, bool[7] wanted) -> "
+        "Tensor? bu, Tensor? bd, Tensor kept, str activation, bool[7] wanted) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("linear_cross_entropy(Tensor x, Tensor W, Tensor target, Tensor? b, int ignore_index, "
         "str reduction) -> (Tensor, Tensor, Tensor)");

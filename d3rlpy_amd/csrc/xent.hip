@@ -70,6 +70,7 @@ struct LsePartEpi {
       const int64_t y = m < t.M ? target[m] - v0 - t.n0 : -1;
       want[i] = y >= 0 && y < min(C::TN, t.N - t.n0) ? (int)y : -1;
     }
+    wait_loads();
 #pragma unroll
     for (int i = 0; i < C::MT; ++i) {
       const int m = t.m0 + 32 * i + (t.lane & 31);

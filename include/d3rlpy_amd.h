@@ -1366,16 +1366,16 @@ int d3a_iqn_head_bwd_fused(const d3a_iqn_head_bwd_fused_desc* d, void* stream);
  * x_c rows at x + c * sx + r * ldx (sx = 0 with members > 1: one x for all),
  * Wg / Wu [members][n_hidden][n_in] and Wd [members][n_out][n_hidden] with row
  * strides ldW* and member strides sW*; biases [members][n] contiguous or NULL;
- * y [members][rows][n_out] contiguous.  g, u: NULL, or [members][rows] rows of
- * n_hidden rounded up to 8 in float32, kept for the backward.
- * The backward reads x, the weights, g, u and dy (lddy, sdy) and writes the
+ * y [members][rows][n_out] contiguous.  kept: NULL, or d3a_gated_mlp_kept's
+ * bytes (16-byte aligned) that the forward leaves for the backward: g, u, act(g) u.
+ * The backward reads x, the weights, kept and dy (lddy, sdy) and writes the
  * gradients whose pointers are given, contiguous in their tensor's shape; dx of
  * an x that the members share is the sum over them.  It does not read y. */
 typedef struct d3a_gated_mlp_desc {
   const void *x, *Wg, *Wu, *Wd;
   const void *bg, *bu, *bd;
   void* y;
-  float *g, *u;
+  void* kept;
   const void* dy;
   void *dx, *dWg, *dWu, *dWd, *dbg, *dbu, *dbd;
   int64_t rows, n_in, n_hidden, n_out, members;
@@ -1385,6 +1385,7 @@ typedef struct d3a_gated_mlp_desc {
   int64_t ws_bytes;
 } d3a_gated_mlp_desc;
 int d3a_gated_mlp_workspace(const d3a_gated_mlp_desc* desc, int32_t backward, int64_t* bytes);
+int d3a_gated_mlp_kept(const d3a_gated_mlp_desc* desc, int64_t* bytes);
 int d3a_gated_mlp(const d3a_gated_mlp_desc* desc, void* stream);
 int d3a_gated_mlp_bwd(const d3a_gated_mlp_desc* desc, void* stream);
 

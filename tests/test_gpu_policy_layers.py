@@ -378,7 +378,7 @@ def test_block_is_deterministic_and_replays(T, dtype):
         ops = T.load()
         x = det["emb"][tokens]
         h, s1 = ops.layer_norm(x, det["n1"], det["c1"], 1e-5)
-        y, pre = ops.gated_mlp(h, det["Wg"], det["Wu"], det["Wd"], None, None, None, "silu", True)
+        y, kept = ops.gated_mlp(h, det["Wg"], det["Wu"], det["Wd"], None, None, None, "silu", True)
         r, s2 = ops.layer_norm(x + y, det["n2"], det["c2"], 1e-5)
         loss, lse, scale = ops.linear_cross_entropy(r, det["emb"], target, None, -100, "mean")
         dr, demb, _ = ops.linear_cross_entropy_backward(
@@ -386,7 +386,7 @@ def test_block_is_deterministic_and_replays(T, dtype):
             [True, True, False])
         dxy, dn2, dc2 = ops.layer_norm_backward(dr, x + y, det["n2"], det["c2"], s2, [True] * 3)
         dh, dWg, dWu, dWd = ops.gated_mlp_backward(
-            dxy, h, det["Wg"], det["Wu"], det["Wd"], None, None, None, pre, "silu",
+            dxy, h, det["Wg"], det["Wu"], det["Wd"], None, None, None, kept, "silu",
             [True] * 4 + [False] * 3)[:4]
         return [loss, demb, dn2, dc2, dh, dWg, dWu, dWd]
 
