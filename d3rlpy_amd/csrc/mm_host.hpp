@@ -360,7 +360,7 @@ Cost cost_of(TileSize s) {
   }
   if (s == kLarge) return {X::Large::BM, X::Large::BN, X::Large::BK, 1, 2.1, 1.9, 6.0};
   if (s == kMid) return {X::Mid::BM, X::Mid::BN, X::Mid::BK, 1, 1.25, 1.15, 5.5};
-  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.47, 0.35, 5.5};
+  return {X::Small::BM, X::Small::BN, X::Small::BK, 3, 0.47, 0.6, 5.5};
 }
 
 struct Choice {
