@@ -123,9 +123,8 @@ int check(const d3a_gated_mlp_desc* d, bool bwd) {
   D3A_CHECK_ARG(d->act >= D3A_ACT_SILU && d->act <= D3A_ACT_RELU, "gated_mlp: unknown activation");
   D3A_CHECK_ARG(d->rows >= 0 && d->members >= 1 && d->n_in >= 1 && d->n_hidden >= 1 && d->n_out >= 1,
                 "gated_mlp: sizes must be positive");
-  const int64_t top = (1LL << 31) - 4096;
-  D3A_CHECK_ARG(d->rows < top && d->n_in < top && d->n_hidden < top && d->n_out < top &&
-                    d->members <= 65535,
+  D3A_CHECK_ARG(d->rows <= kMaxRows && d->n_in <= kMaxWidth && d->n_hidden <= kMaxWidth &&
+                    d->n_out <= kMaxWidth && d->members <= 65535,
                 "gated_mlp: size too large");
   D3A_CHECK_ARG(d->ldx >= d->n_in && d->ldWg >= d->n_in && d->ldWu >= d->n_in && d->ldWd >= d->n_hidden,
                 "gated_mlp: row stride smaller than the row");

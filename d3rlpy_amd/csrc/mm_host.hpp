@@ -12,6 +12,10 @@
 namespace d3a {
 namespace mm {
 
+// The longest axes: a tile's rows are addressed within 2 GiB of its first (256
+// rows of kMaxWidth bfloat16 values are 1 GiB), and a row's number is an int.
+constexpr int64_t kMaxWidth = 1LL << 21, kMaxRows = (1LL << 31) - 4096;
+
 inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Bump allocation over the caller's workspace; with a null base it measures.
@@ -104,7 +108,7 @@ struct Packer {
     const int64_t c8 = round8(cols);
     const int64_t nb = s_batch == 0 ? 1 : batch;
     const bool in_place = NP == 1 && !force && cols % 8 == 0 && ld % 8 == 0 && s_batch % 8 == 0 &&
-                          (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld < (1 << 21);
+                          (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld <= kMaxWidth;
     if (in_place) {
       o.p = static_cast<const __bf16*>(p);
       o.ld = ld;

@@ -636,6 +636,9 @@ at::Tensor workspace(int64_t bytes, const at::Tensor& like) {
 // x [.., n] (w [n]) or [members, .., n] (w [members, n]) -> rows, members
 int64_t norm_members(const at::Tensor& x, const OptTensor& w, const OptTensor& b) {
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "layer_norm: empty last dimension");
+  if (given(w) && given(b))
+    TORCH_CHECK(w->sizes() == b->sizes() && w->scalar_type() == b->scalar_type(),
+                "layer_norm: weight and bias of one shape and dtype");
   int64_t members = 1;
   for (const OptTensor* p : {&w, &b}) {
     if (!given(*p)) continue;
@@ -649,9 +652,6 @@ int64_t norm_members(const at::Tensor& x, const OptTensor& w, const OptTensor& b
       members = v.size(0);
     }
   }
-  if (given(w) && given(b))
-    TORCH_CHECK(w->sizes() == b->sizes() && w->scalar_type() == b->scalar_type(),
-                "layer_norm: weight and bias of one shape and dtype");
   return members;
 }
 

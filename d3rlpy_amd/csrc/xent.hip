@@ -26,14 +26,12 @@ using namespace mm;
 
 constexpr int64_t kPieceBytes = 512LL << 20;
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-// exp(z - ref), ref2 = ref * log2(e).  With bfloat16 tensors the hardware's
-// exponential and ref2's rounding, |ref| 2^-24 relative, are far below dz's own
-// rounding and no more than the float32 sum's.
+// exp(z - ref).  (With bfloat16 tensors the hardware's exponential, within 2 ulp
+// and a product's rounding of its argument, is far below dz's own rounding and no
+// more than the float32 sum's.)
 template <int NP>
-__device__ __forceinline__ float exp_to(float z, float ref, float ref2) {
-  return NP == 1 ? __builtin_amdgcn_exp2f(fmaf(z, kLog2e, -ref2)) : expf(z - ref);
+__device__ __forceinline__ float exp_to(float z, float ref) {
+  return NP == 1 ? __expf(z - ref) : expf(z - ref);
 }
 
 // (max, sum of exp(z - max)) of a + b; an empty side has max -inf, sum 0
@@ -98,12 +96,12 @@ struct LsePartEpi {
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
       // a row of -inf alone: any finite reference gives its sum of 0
-      const float ref = top == -INFINITY ? 0.f : top, ref2 = ref * kLog2e;
+      const float ref = top == -INFINITY ? 0.f : top;
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < C::NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += exp_to<NP>(acc[i][j][r], ref, ref2);
+        for (int r = 0; r < 16; ++r) s += exp_to<NP>(acc[i][j][r], ref);
       const float m2 = __shfl_xor(top, 32), s2 = __shfl_xor(s, 32);
       join(top, s, m2, s2);
       // (a wave past the last column has no part)
@@ -243,7 +241,7 @@ struct DzEpi {
       const float l = lse[m], g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
       const int64_t want = y - v0;
       const int col = y == ignore ? -2 : want >= 0 && want < t.N ? (int)want : -1;
-      if (i < C::TM) rows[i] = make_float4(l, l * kLog2e, g, __int_as_float(col));
+      if (i < C::TM) rows[i] = make_float4(l, g, __int_as_float(col), 0.f);
     }
     float b[8];
     load_bias(bias, first_column<false>(t), t.N, b);
@@ -251,15 +249,15 @@ struct DzEpi {
     each8<C, false>(acc, t, none, [&](int m, int n, float* v, float*, Nothing) {
       if (n >= ld) return;
       const float4 row = rows[m - t.m0];
-      const int col = __float_as_int(row.w), want = col - n;
+      const int col = __float_as_int(row.z), want = col - n;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = exp_to<NP>(v[r] + b[r], row.x, row.y);
+      for (int r = 0; r < 8; ++r) v[r] = exp_to<NP>(v[r] + b[r], row.x);
       if (want >= 0 && want < 8) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[r] -= r == want ? 1.f : 0.f;
       }
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] *= row.z;
+      for (int r = 0; r < 8; ++r) v[r] *= row.y;
       if (col == -2 || n + 8 > t.N) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[r] = col != -2 && n + r < t.N ? v[r] : 0.f;
@@ -275,8 +273,8 @@ int check(const d3a_linear_xent_desc* d, bool bwd) {
                 "linear_cross_entropy: dtype must be float32 or bfloat16");
   D3A_CHECK_ARG(d->reduction >= 0 && d->reduction <= 2, "linear_cross_entropy: unknown reduction");
   D3A_CHECK_ARG(d->rows >= 0 && d->n_in >= 1 && d->vocab >= 1, "linear_cross_entropy: sizes must be positive");
-  const int64_t top = (1LL << 31) - 4096;
-  D3A_CHECK_ARG(d->rows < top && d->n_in < top && d->vocab < top, "linear_cross_entropy: size too large");
+  D3A_CHECK_ARG(d->rows <= kMaxRows && d->n_in <= kMaxWidth && d->vocab <= kMaxRows,
+                "linear_cross_entropy: size too large");
   D3A_CHECK_ARG(d->ldx >= d->n_in && d->ldW >= d->n_in, "linear_cross_entropy: row stride smaller than the row");
   D3A_CHECK_ARG(d->W, "linear_cross_entropy: null weight");
   if (d->rows > 0)
@@ -350,6 +348,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
   const Operand w = pack.operand(d.W, d.ldW, 0, 1, V, D);
   // pieces of equal size, multiples of the widest tile
   int64_t piece = std::max<int64_t>(kPieceBytes / (2 * NP * std::max<int64_t>(R, 1)), 256);
+  piece = std::min(piece, kMaxWidth);
   const int64_t n_pieces = (V + piece - 1) / piece;
   piece = std::min<int64_t>(V, ((V + n_pieces - 1) / n_pieces + 255) / 256 * 256);
   const int64_t ld = round8(piece);

@@ -1351,9 +1351,10 @@ int d3a_iqn_head_bwd_fused(const d3a_iqn_head_bwd_fused_desc* d, void* stream);
 /* ---- layers and losses of larger policies: layer norm, the gated feed-forward
  *      block, the softmax cross entropy of a linear head.  Tensors are float32
  *      or bfloat16 (D3A_F32 / D3A_BF16; 16-bit storage, sums and statistics in
- *      float32); `ws` is scratch of at least the size that the matching
- *      *_workspace call reports for the same descriptor (256-byte aligned, owned
- *      by the call until its kernels have run). ------------------------------- */
+ *      float32).  Rows and the vocabulary count up to 2^31 - 4096, the products'
+ *      other axes up to 2^21.  `ws` is scratch of at least the size that the
+ *      matching *_workspace call reports for the same descriptor (256-byte
+ *      aligned, owned by the call until its kernels have run). -------------- */
 #define D3A_F32 0
 #define D3A_BF16 1
 

@@ -316,7 +316,7 @@ def test_linear_cross_entropy_shapes_and_strides(T):
     got = run_xent(T, big[:, 3:43], tied[:, 40:], b, t, "mean", 1.0)
     check(got, ref)
     none = run_xent(T, x[:0], W, b, t[:0], "mean", 1.0)
-    assert float(none["loss"]) == 0 and not none["W"].any() and not none["b"].any()
+    assert not none["loss"].detach().any() and not none["W"].any() and not none["b"].any()
 
 
 # --------------------------------------------------------------- together, replays
@@ -437,3 +437,103 @@ def test_no_second_derivative(T):
     (dx,) = torch.autograd.grad(T.layer_norm(x).sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+# -------------------------------------------------------- refusals, long arrays, memory
+def test_refusals_on_the_gpu(T):
+    x, w = rnd(1, 4, 8), rnd(2, 8)
+    W, Wd, t = rnd(3, 6, 8), rnd(4, 8, 6), torch.zeros(4, dtype=torch.int64, device=DEV)
+    for call, match in (
+            (lambda: T.layer_norm(x.half(), w.half()), "float32 or bfloat16"),
+            (lambda: T.layer_norm(x, w.bfloat16()), "weight and bias must"),
+            (lambda: T.layer_norm(x, w.cpu()), "weight / bias on cpu"),
+            (lambda: T.layer_norm(x, w, eps=-1.0), "eps"),
+            (lambda: T.gated_mlp(x, W, W.bfloat16(), Wd), "Wu is"),
+            (lambda: T.gated_mlp(x, W, W, Wd.cpu()), "Wd is on cpu"),
+            (lambda: T.gated_mlp(x.double(), W.double(), W.double(), Wd.double()),
+             "float32 or bfloat16"),
+            (lambda: T.linear_cross_entropy(x, W, t.cpu()), "target is on cpu"),
+            (lambda: T.linear_cross_entropy(x, W.bfloat16(), t), "W is"),
+            (lambda: T.linear_cross_entropy(x, W, t, rnd(5, 6, dtype=BF16)), "b is")):
+        with pytest.raises(RuntimeError, match=match):
+            call()
+    ops = T.load()
+    y, stats = ops.layer_norm(x, w, None, 1e-5)
+    with pytest.raises(RuntimeError, match="stats of another"):
+        ops.layer_norm_backward(x, x, w, None, stats[:, :, :2].contiguous(), [True] * 3)
+    y, kept = ops.gated_mlp(x, W, W, Wd, None, None, None, "silu", False)
+    with pytest.raises(RuntimeError, match="keep = True"):
+        ops.gated_mlp_backward(y, x, W, W, Wd, None, None, None, kept, "silu", [True] * 7)
+
+
+def test_vocabulary_past_32_bit_offsets(T):
+    """2.2 million classes of 1024 bfloat16 values: W's end lies past 2^32
+    bytes and past 2^31 elements."""
+    V, D, R = 2_200_003, 1024, 5
+    W = torch.empty(V, D, device=DEV, dtype=BF16)
+    W[:] = rnd(1, 1, D, dtype=BF16)
+    W[V - 7] = rnd(2, D, dtype=BF16)
+    x = rnd(3, R, D, dtype=BF16, scale=D ** -0.5)
+    t = torch.tensor([V - 7, V - 1, 0, V - 7, -100], device=DEV)
+    got = T.linear_cross_entropy(x, W, t, reduction="none")
+    z = x.double() @ torch.stack([W[0], W[V - 7]]).double().t()
+    lse = torch.logsumexp(torch.stack([z[:, 0] + torch.log(torch.tensor(V - 1.0, dtype=torch.float64)),
+                                       z[:, 1]]), 0)
+    want = lse - torch.stack([z[0, 1], z[1, 0], z[2, 0], z[3, 1], lse[4]])
+    # lse near 15: sums over some 34000 parts joined 32 ways, each in float32
+    within(got, want, torch.full_like(want, (V / 64 / 32 + 200) * 2.0 ** -24 * 2), "loss")
+
+
+def test_norm_past_32_bit_offsets(T):
+    rows, n = 2_200_001, 1024
+    x = torch.empty(rows, n, device=DEV, dtype=BF16)
+    x[:] = rnd(1, 1, n, dtype=BF16)
+    x[-3:] = rnd(2, 3, n, dtype=BF16, scale=3.0)
+    w, b = rnd(3, n, dtype=BF16), rnd(4, n, dtype=BF16)
+    y = T.layer_norm(x, w, b)
+    for part in (slice(0, 2), slice(rows - 3, rows)):
+        within(y[part], *norm_reference(x[part], w, b, 1e-5, x[part])["y"], "y")
+
+
+def test_logits_all_at_the_lowest_value(T):
+    """A row whose every logit is the type's lowest value: uniform."""
+    for dtype in (F32, BF16):
+        x, W, b, t = xent_inputs(20, 16, 50, dtype, True, pad=0.0)
+        b[:] = torch.finfo(dtype).min
+        got = run_xent(T, torch.zeros_like(x), W, b, t, "sum", 1.0)
+        # lse = lowest + log 50 rounds to lowest (steps of 2e31): the loss is 0,
+        # and every exp(z - lse) is 1, as torch's float32 has it
+        assert not got["loss"].any()
+        p = 20.0 - torch.bincount(t, minlength=50).double()
+        within(got["b"], p, 2.0 ** -8 * p.abs(), "b")
+        dx, dW = got["x"], got["W"]
+        assert torch.isfinite(dx).all() and torch.isfinite(dW).all()
+
+
+def test_nothing_is_left_allocated(T):
+    q, tokens, target = block_inputs(BF16)
+    for _ in range(3):
+        block_step(T, q, tokens, target)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(20):
+        block_step(T, q, tokens, target)
+    assert torch.cuda.memory_allocated() <= before
+
+
+def test_two_streams_at_once(T):
+    """The same calls on two streams at the same time, each with scratch of its
+    own, give what each gives alone."""
+    q, tokens, target = block_inputs(BF16)
+    r = {k: (v.detach() * 0.5).requires_grad_(True) for k, v in q.items()}
+    want = [block_step(T, p, tokens, target) for p in (q, r)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for p, s in zip((q, r), streams):
+            with torch.cuda.stream(s):
+                got.append(block_step(T, p, tokens, target))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and all(torch.equal(u, v) for u, v in zip(a[1], b[1]))
