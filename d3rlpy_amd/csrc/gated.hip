@@ -12,6 +12,7 @@
 // down product's operand, and g and u in float32.  In bfloat16 they would halve 270 MB of traffic at 8192 x 4096
 // hidden values, but a second rounding on the way to each gradient takes its
 // error from 1.4 to 2 times that of the result's own rounding.
+#include "direct.hpp"
 #include "mm_host.hpp"
 #include "thin.hpp"
 #include "../../include/d3rlpy_amd.h"
@@ -138,7 +139,8 @@ int check(const d3a_gated_mlp_desc* d, bool bwd) {
   return 0;
 }
 
-// What the forward keeps: g and u, then h's planes, rows of F8 each.
+// What the forward keeps: g and u, then h, rows of F8 each; h as the operand
+// planes of the tiles, or (is_plain) as an array of T in their place.
 template <int NP>
 struct Kept {
   float *g = nullptr, *u = nullptr;
@@ -158,6 +160,61 @@ struct Kept {
   }
 };
 
+// ---- a minibatch of a small block: direct.hpp ------------------------------------
+// (dg, du and h are plain arrays of T here; h lies where its planes would)
+template <class T>
+struct DirectGateEpi {
+  float *g, *u;
+  T* h;
+  int64_t ld;
+  const T *bg, *bu;
+  int32_t act;
+  __device__ __forceinline__ void run(int batch, int m, int n, int M, int N, const float v[2], const float up[2]) const {
+    if (m >= M) return;
+    const int64_t at = ((int64_t)batch * M + m) * ld;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (n + i >= N) continue;
+      const float x = v[i] + (bg ? (float)bg[(int64_t)batch * N + n + i] : 0.f);
+      const float y = up[i] + (bu ? (float)bu[(int64_t)batch * N + n + i] : 0.f);
+      float a, da;
+      activation<sizeof(T) == 2>(act, x, a, da);
+      if (g) {
+        g[at + n + i] = x;
+        u[at + n + i] = y;
+      }
+      h[at + n + i] = (T)(a * y);
+    }
+  }
+};
+
+template <class T>
+struct DirectGateBwdEpi {
+  const float *g, *u;
+  T *dg, *du;
+  int64_t ld;
+  int32_t act;
+  __device__ __forceinline__ void run(int batch, int m, int n, int M, int N, const float v[2], const float*) const {
+    if (m >= M) return;
+    const int64_t at = ((int64_t)batch * M + m) * ld;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (n + i >= N) continue;
+      float a, da;
+      activation<sizeof(T) == 2>(act, g[at + n + i], a, da);
+      dg[at + n + i] = (T)(v[i] * u[at + n + i] * da);
+      du[at + n + i] = (T)(v[i] * a);
+    }
+  }
+};
+
+bool is_direct(const d3a_gated_mlp_desc& d) {
+  return direct::small((double)d.members * d.rows * d.n_hidden * std::max(d.n_in, d.n_out),
+                       std::max({d.rows, d.n_in, d.n_hidden, d.n_out}));
+}
+
+bool is_plain(const d3a_gated_mlp_desc& d) { return d.rows <= thin::kRows || is_direct(d); }
+
 struct Activation {
   __device__ __forceinline__ void operator()(int act, float g, float& a, float& da) const {
     activation<false>(act, g, a, da);
@@ -171,13 +228,95 @@ bool whole(const void* p, int64_t ld, int64_t s, int64_t n) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % N == 0 && s % N == 0 && n % N == 0;
 }
 
+template <class T, int NP>
+int forward_direct(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
+  const Kept<NP> k(d);
+  T* h = d.kept ? reinterpret_cast<T*>(const_cast<__bf16*>(k.h.p)) : ws.take<T>(C * R * F8);
+  *bytes = ws.used;
+  if (dry || R == 0) return 0;
+  direct::Launch<T, DirectGateEpi<T>> L{};
+  L.n = 1;
+  L.p[0] = direct::problem(direct::operand<T>(d.x, d.ldx, C > 1 ? d.sx : 0, D),
+                           direct::operand<T>(d.Wg, d.ldWg, C > 1 ? d.sWg : 0, D), R, F, D, C);
+  L.p[0].b2 = direct::operand<T>(d.Wu, d.ldWu, C > 1 ? d.sWu : 0, D);
+  L.e[0] = DirectGateEpi<T>{k.g, k.u, h, F8, static_cast<const T*>(d.bg), static_cast<const T*>(d.bu), d.act};
+  if (direct::launch<false, false, true>(L, stream, "gated_mlp") != 0) return -1;
+  direct::Launch<T, direct::StoreEpi<T>> Y{};
+  Y.n = 1;
+  Y.p[0] = direct::problem(direct::operand<T>(h, F8, R * F8, F), direct::operand<T>(d.Wd, d.ldWd, C > 1 ? d.sWd : 0, F),
+                           R, O, F, C);
+  Y.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.y), O, R * O, static_cast<const T*>(d.bd), O};
+  return direct::launch<false, false, false>(Y, stream, "gated_mlp");
+}
+
+template <class T, int NP>
+int backward_direct(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
+  const bool hidden = d.dx || d.dWg || d.dWu || d.dbg || d.dbu;
+  const int64_t plane = C * R * F8;
+  T* dg = hidden ? ws.take<T>(2 * plane) : nullptr;
+  *bytes = ws.used;
+  if (dry) return 0;
+  T* du = dg + plane;
+  const Kept<NP> k(d);
+  const int64_t sdy = C > 1 ? d.sdy : 0, sx = C > 1 ? d.sx : 0, sWd = C > 1 ? d.sWd : 0;
+  if (hidden && R > 0) {
+    direct::Launch<T, DirectGateBwdEpi<T>> L{};
+    L.n = 1;
+    L.p[0] = direct::problem(direct::operand<T>(d.dy, d.lddy, sdy, O), direct::operand<T>(d.Wd, d.ldWd, sWd, O), R, F,
+                             O, C);
+    L.e[0] = DirectGateBwdEpi<T>{k.g, k.u, dg, du, F8, d.act};
+    if (direct::launch<false, true, false>(L, stream, "gated_mlp_bwd") != 0) return -1;
+  }
+  if (d.dx && R > 0) {
+    const bool shared = C > 1 && d.sx == 0;
+    direct::Launch<T, direct::StoreEpi<T>> L{};
+    L.n = 1;
+    direct::Operand<T> a = direct::operand<T>(dg, F8, R * F8, F);
+    direct::Operand<T> b = direct::operand<T>(d.Wg, d.ldWg, C > 1 ? d.sWg : 0, F);
+    direct::Operand<T> b2 = direct::operand<T>(d.Wu, d.ldWu, C > 1 ? d.sWu : 0, F);
+    a.s_inner = plane;
+    if (shared) {
+      for (direct::Operand<T>* o : {&a, &b, &b2}) {
+        o->s_outer = o->s_batch;
+        o->s_batch = 0;
+      }
+    }
+    L.p[0] = direct::problem(a, b, R, D, F, shared ? 1 : C);
+    L.p[0].b2 = b2;
+    L.p[0].n_inner = 2;
+    L.p[0].n_outer = shared ? (int32_t)C : 1;
+    L.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dx), D, R * D, nullptr, 0};
+    if (direct::launch<false, true, false>(L, stream, "gated_mlp_bwd") != 0) return -1;
+  }
+  // the weights' gradients, with the biases' as the sums of their A's rows
+  direct::Launch<T, direct::StoreEpi<T>> W{};
+  auto weight = [&](const direct::Operand<T>& a, const direct::Operand<T>& b, int64_t M, int64_t N, void* dW,
+                    void* db) {
+    // (a bias gradient alone: the product of its first column, written nowhere)
+    if (!dW && !db) return;
+    direct::Problem<T>& p = W.p[W.n];
+    p = direct::problem(a, b, M, dW ? N : 1, R, C);
+    p.rowsum = static_cast<T*>(db);
+    W.e[W.n] = direct::StoreEpi<T>{static_cast<T*>(dW), N, M * N, nullptr, 0};
+    ++W.n;
+  };
+  const direct::Operand<T> x = direct::operand<T>(d.x, d.ldx, sx, R);
+  weight(direct::operand<T>(dg, F8, R * F8, R), x, F, D, d.dWg, d.dbg);
+  weight(direct::operand<T>(du, F8, R * F8, R), x, F, D, d.dWu, d.dbu);
+  weight(direct::operand<T>(d.dy, d.lddy, sdy, R),
+         direct::operand<T>(reinterpret_cast<const T*>(k.h.p), F8, R * F8, R), O, F, d.dWd, d.dbd);
+  return W.n ? direct::launch<true, true, false>(W, stream, "gated_mlp_bwd") : 0;
+}
+
 // At most 16 rows: the weights read once.  One row of 2048 x 5632 bfloat16: 9 us
 // and 6, where the tiles take 15 and 13.
 template <class T, int NP>
 int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
   const Kept<NP> k(d);
-  __bf16* h = d.kept ? const_cast<__bf16*>(k.h.p) : ws.take<__bf16>(NP * C * R * F8);
+  T* h = d.kept ? reinterpret_cast<T*>(const_cast<__bf16*>(k.h.p)) : ws.take<T>(C * R * F8);
   *bytes = ws.used;
   if (dry || R == 0) return 0;
   thin::GateArgs<T> a{};
@@ -196,16 +335,15 @@ int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t st
   a.u = k.u;
   a.h = h;
   a.ld = F8;
-  a.s_part = C * R * F8;
   a.R = (int32_t)R;
   a.D = (int32_t)D;
   a.F = (int32_t)F;
   a.act = d.act;
   const dim3 gate((unsigned)((F + 15) / 16), (unsigned)C), down((unsigned)((O + 15) / 16), (unsigned)C);
   if (whole<T>(d.x, a.ldx, a.sx, D) && whole<T>(d.Wg, a.ldg, a.sg, D) && whole<T>(d.Wu, a.ldu, a.su, D))
-    thin::gate_kernel<T, NP, true><<<gate, 512, 0, stream>>>(a, Activation{});
+    thin::gate_kernel<T, true><<<gate, 512, 0, stream>>>(a, Activation{});
   else
-    thin::gate_kernel<T, NP, false><<<gate, 512, 0, stream>>>(a, Activation{});
+    thin::gate_kernel<T, false><<<gate, 512, 0, stream>>>(a, Activation{});
   D3A_LAUNCH_CHECK("gated_mlp");
   thin::DownArgs<T> b{};
   b.h = h;
@@ -213,14 +351,13 @@ int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t st
   b.b = static_cast<const T*>(d.bd);
   b.y = static_cast<T*>(d.y);
   b.ld = F8;
-  b.s_part = a.s_part;
   b.ldw = d.ldWd;
   b.sw = C > 1 ? d.sWd : 0;
   b.R = (int32_t)R;
   b.F = (int32_t)F;
   b.O = (int32_t)O;
-  if (whole<T>(d.Wd, b.ldw, b.sw, F)) thin::down_kernel<T, NP, true><<<down, 1024, 0, stream>>>(b);
-  else thin::down_kernel<T, NP, false><<<down, 1024, 0, stream>>>(b);
+  if (whole<T>(d.Wd, b.ldw, b.sw, F)) thin::down_kernel<T, true><<<down, 1024, 0, stream>>>(b);
+  else thin::down_kernel<T, false><<<down, 1024, 0, stream>>>(b);
   D3A_LAUNCH_CHECK("gated_mlp");
   return 0;
 }
@@ -229,6 +366,7 @@ int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t st
 template <class T, int NP>
 int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
   if (d.rows <= thin::kRows) return forward_thin<T, NP>(d, ws, dry, stream, bytes);
+  if (is_direct(d)) return forward_direct<T, NP>(d, ws, dry, stream, bytes);
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
   Packer<T, NP> pack(ws);
   const Operand x = pack.operand(d.x, d.ldx, C > 1 ? d.sx : 0, C, R, D);
@@ -275,6 +413,7 @@ int forward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream,
 
 template <class T, int NP>
 int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  if (is_direct(d)) return backward_direct<T, NP>(d, ws, dry, stream, bytes);
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
   const bool hidden = d.dx || d.dWg || d.dWu || d.dbg || d.dbu;  // dg and du are needed
   Packer<T, NP> pack(ws);
@@ -319,6 +458,8 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   e.s_part = plane;
   e.act = d.act;
 
+  Operand h = k.h;
+  if (NP > 1 && is_plain(d) && d.dWd) h = pack.operand(k.h.p, F8, C > 1 ? R * F8 : 0, C, R, F);
   Products<T, NP> dx, dw;
   if (d.dx) {
     // K runs over the gate's and the up's hidden units (and, for an x that the
@@ -337,7 +478,7 @@ int backward(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream
   }
   if (d.dWg) dw.add(dg, x, F, D, R, C, 1, 1, d.dWg, D, F * D, nullptr, 0);
   if (d.dWu) dw.add(du, x, F, D, R, C, 1, 1, d.dWu, D, F * D, nullptr, 0);
-  if (d.dWd) dw.add(dy, k.h, O, F, R, C, 1, 1, d.dWd, F, O * F, nullptr, 0);
+  if (d.dWd) dw.add(dy, h, O, F, R, C, 1, 1, d.dWd, F, O * F, nullptr, 0);
   dw.reserve(ws, true);
   Colsum<T, NP> cs;
   if (d.dbg) cs.add(dg, R, F, C, d.dbg);

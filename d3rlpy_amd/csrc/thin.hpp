@@ -57,27 +57,6 @@ __device__ __forceinline__ Piece<T> load(const T* p, int k, int K, bool on) {
   return o;
 }
 
-// the same of operand planes: a bfloat16 row, or a float32 one's exact split
-template <int NP>
-__device__ __forceinline__ auto load_planes(const __bf16* p, int64_t s_part, int k, int K, bool on) {
-  if constexpr (NP == 1) {
-    return load<__bf16, true>(p, k, K, on);
-  } else {
-    Piece<float> o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = 0.f;
-    if (on && k < K) {
-#pragma unroll
-      for (int q = 2; q >= 0; --q) {
-        const bf16x4 x = *reinterpret_cast<const bf16x4*>(p + q * s_part + k);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o.v[i] += (float)x[i];
-      }
-    }
-    return o;
-  }
-}
-
 // the waves' accumulators, added in order by the first wave
 template <int NACC, int WAVES>
 __device__ __forceinline__ void join(f32x4 (&acc)[NACC], f32x4* red) {
@@ -98,13 +77,13 @@ struct GateArgs {
   const T *x, *Wg, *Wu, *bg, *bu;
   int64_t ldx, sx, ldg, sg, ldu, su;
   float *g, *u;           // kept, or null
-  __bf16* h;              // planes [NP][members][R] rows of ld
-  int64_t ld, s_part;
+  T* h;                   // [members][R] rows of ld, zero past F
+  int64_t ld;
   int32_t R, D, F, act;
 };
 
 // grid (16 hidden units, members), 8 waves
-template <class T, int NP, bool VEC, class Act>
+template <class T, bool VEC, class Act>
 __global__ __launch_bounds__(512) void gate_kernel(const GateArgs<T> A, Act activation) {
   constexpr int WAVES = 8, N = Piece<T>::N, KP = Piece<T>::K;
   __shared__ f32x4 red[WAVES * 2 * 64];
@@ -142,34 +121,22 @@ __global__ __launch_bounds__(512) void gate_kernel(const GateArgs<T> A, Act acti
     *reinterpret_cast<f32x4*>(A.g + at) = acc[0];
     *reinterpret_cast<f32x4*>(A.u + at) = acc[1];
   }
-  if constexpr (NP == 1) {
+  if constexpr (sizeof(T) == 4)
+    mm::store4(A.h + at, h);
+  else
     *reinterpret_cast<bf16x4*>(A.h + at) = bf16x4{(__bf16)h[0], (__bf16)h[1], (__bf16)h[2], (__bf16)h[3]};
-  } else {
-    bf16x4 o[3];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __bf16 p, q, r;
-      mm::split3(h[i], p, q, r);
-      o[0][i] = p;
-      o[1][i] = q;
-      o[2][i] = r;
-    }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x4*>(A.h + q * A.s_part + at) = o[q];
-  }
 }
 
 template <class T>
 struct DownArgs {
-  const __bf16* h;
-  const T *W, *b;
+  const T *h, *W, *b;
   T* y;  // [members][R][O]
-  int64_t ld, s_part, ldw, sw;
+  int64_t ld, ldw, sw;
   int32_t R, F, O;
 };
 
 // grid (16 outputs, members), 16 waves
-template <class T, int NP, bool VEC>
+template <class T, bool VEC>
 __global__ __launch_bounds__(1024) void down_kernel(const DownArgs<T> A) {
   constexpr int WAVES = 16, N = Piece<T>::N, KP = Piece<T>::K;
   __shared__ f32x4 red[WAVES * 64];
@@ -177,12 +144,12 @@ __global__ __launch_bounds__(1024) void down_kernel(const DownArgs<T> A) {
   const int64_t c = blockIdx.y;
   const int n0 = blockIdx.x * 16, row = lane & 15, k0 = (lane >> 4) * N;
   const T* wd = A.W + c * A.sw + (int64_t)min(n0 + row, A.O - 1) * A.ldw;
-  const __bf16* h = A.h + (c * A.R + row) * A.ld;
+  const T* h = A.h + (c * A.R + row) * A.ld;
   f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 4
   for (int k = w * KP; k < A.F; k += WAVES * KP) {
     const Piece<T> a = load<T, VEC>(wd, k + k0, A.F, true);
-    const Piece<T> v = load_planes<NP>(h, A.s_part, k + k0, (int)A.ld, row < A.R);
+    const Piece<T> v = load<T, true>(h, k + k0, (int)A.ld, row < A.R);
     acc[0] = product(a, v, acc[0]);
   }
   join<1, WAVES>(acc, red);

@@ -16,6 +16,7 @@
 // A row whose target is ignore_index has loss 0 and no gradient, whatever its
 // logits are; a row whose target is outside the vocabulary has loss NaN and a
 // NaN gradient.
+#include "direct.hpp"
 #include "mm_host.hpp"
 #include "../../include/d3rlpy_amd.h"
 
@@ -110,6 +111,61 @@ struct LsePartEpi {
     }
   }
 };
+
+// ---- a minibatch and a small vocabulary: direct.hpp -------------------------------
+// One (max, sum) a row and 32 columns: a row's columns lie with 16 threads.
+template <class T>
+struct DirectLseEpi {
+  const T* bias;
+  const int64_t* target;
+  float2* part;
+  float* ztarget;
+  __device__ __forceinline__ void run(int, int m, int n, int M, int N, const float v[2], const float*) const {
+    const int64_t y = m < M ? target[m] : -1;
+    float z[2], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      z[i] = n + i < N ? v[i] + (bias ? (float)bias[n + i] : 0.f) : -INFINITY;
+      if (n + i < N && n + i == y) ztarget[m] = z[i];
+      top = fmaxf(top, z[i]);
+    }
+    const float ref = top == -INFINITY ? 0.f : top;
+    float s = exp_to<3>(z[0], ref) + exp_to<3>(z[1], ref);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor(top, o), s2 = __shfl_xor(s, o);
+      join(top, s, m2, s2);
+    }
+    if ((threadIdx.x & 15) == 0 && m < M) part[(int64_t)(n / 32) * M + m] = make_float2(top, s);
+  }
+};
+
+template <class T>
+struct DirectDzEpi {
+  const T* bias;
+  const int64_t* target;
+  const float *lse, *gloss, *scale;
+  int64_t s_gloss, ignore, vocab;
+  T* dz;
+  int64_t ld;
+  __device__ __forceinline__ void run(int, int m, int n, int M, int N, const float v[2], const float*) const {
+    if (m >= M) return;
+    const int64_t y = target[m];
+    const float by = scale ? scale[0] : 1.f, l = lse[m];
+    const float g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (n + i >= N) continue;
+      const float z = v[i] + (bias ? (float)bias[n + i] : 0.f);
+      const float d = (exp_to<3>(z, l) - (n + i == y ? 1.f : 0.f)) * g;
+      dz[m * ld + n + i] = (T)(y == ignore ? 0.f : d);
+    }
+  }
+};
+
+bool is_direct(const d3a_linear_xent_desc& d) {
+  return direct::small((double)d.rows * d.n_in * d.vocab, std::max({d.rows, d.n_in, d.vocab}));
+}
 
 // Joins the rows' parts: 8 rows x 32 threads a workgroup, first their largest
 // maximum, then the sums that refer to it (the parts again, from the cache).
@@ -290,8 +346,75 @@ int wave_columns(TileSize s) {
   return s == kLarge ? X::Large::TN : s == kMid ? X::Mid::TN : X::Small::TN;
 }
 
+// the rows' lse and loss from their parts, and the reduction
+int finish(const d3a_linear_xent_desc& d, const float2* part, int64_t parts, const float* ztarget,
+           hipStream_t stream) {
+  const int64_t R = d.rows;
+  if (d.reduction != 0 && R >= 64 && R * parts <= kJoinSmall) {
+    lse_join_small_kernel<<<1, 1024, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget, d.target, d.vocab,
+                                                  d.ignore_index, d.reduction == 1, d.lse, d.loss, d.out, d.scale);
+    D3A_LAUNCH_CHECK("linear_cross_entropy");
+    return 0;
+  }
+  if (R > 0) {
+    lse_join_kernel<<<(unsigned)((R + 7) / 8), 256, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget, d.target,
+                                                                d.vocab, d.ignore_index, d.lse, d.loss);
+    D3A_LAUNCH_CHECK("linear_cross_entropy");
+  }
+  if (d.reduction != 0) {
+    loss_reduce_kernel<<<1, 1024, 0, stream>>>(d.loss, d.target, d.ignore_index, (int32_t)R, d.reduction == 1, d.out,
+                                               d.scale);
+    D3A_LAUNCH_CHECK("linear_cross_entropy");
+  }
+  return 0;
+}
+
+template <class T>
+int forward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t R = d.rows, D = d.n_in, V = d.vocab, parts = (V + 31) / 32;
+  direct::Launch<T, DirectLseEpi<T>> L{};
+  L.n = 1;
+  L.p[0] = direct::problem(direct::operand<T>(d.x, d.ldx, 0, D), direct::operand<T>(d.W, d.ldW, 0, D), R, V, D, 1);
+  L.e[0] = DirectLseEpi<T>{static_cast<const T*>(d.b), d.target, ws.take<float2>(parts * R), ws.take<float>(R)};
+  *bytes = ws.used;
+  if (dry) return 0;
+  if (R > 0 && direct::launch<false, false, false>(L, stream, "linear_cross_entropy") != 0) return -1;
+  return finish(d, L.e[0].part, parts, L.e[0].ztarget, stream);
+}
+
+template <class T>
+int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  const int64_t R = d.rows, D = d.n_in, V = d.vocab, ld = round8(V);
+  T* dz = ws.take<T>(R * ld);
+  *bytes = ws.used;
+  if (dry) return 0;
+  if (R > 0) {
+    direct::Launch<T, DirectDzEpi<T>> L{};
+    L.n = 1;
+    L.p[0] = direct::problem(direct::operand<T>(d.x, d.ldx, 0, D), direct::operand<T>(d.W, d.ldW, 0, D), R, V, D, 1);
+    L.e[0] = DirectDzEpi<T>{static_cast<const T*>(d.b), d.target, d.lse, d.gloss,
+                            d.reduction == 1 ? d.scale : nullptr, d.reduction == 0 ? 1 : 0, d.ignore_index, V, dz, ld};
+    if (direct::launch<false, false, false>(L, stream, "linear_cross_entropy_bwd") != 0) return -1;
+    if (d.dx) {
+      direct::Launch<T, direct::StoreEpi<T>> X{};
+      X.n = 1;
+      X.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, V), direct::operand<T>(d.W, d.ldW, 0, V), R, D, V, 1);
+      X.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dx), D, 0, nullptr, 0};
+      if (direct::launch<false, true, false>(X, stream, "linear_cross_entropy_bwd") != 0) return -1;
+    }
+  }
+  if (!d.dW && !d.db) return 0;
+  direct::Launch<T, direct::StoreEpi<T>> W{};
+  W.n = 1;
+  W.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, R), direct::operand<T>(d.x, d.ldx, 0, R), V, d.dW ? D : 1, R, 1);
+  W.p[0].rowsum = static_cast<T*>(d.db);
+  W.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dW), D, 0, nullptr, 0};
+  return direct::launch<true, true, false>(W, stream, "linear_cross_entropy_bwd");
+}
+
 template <class T, int NP>
 int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
+  if (is_direct(d)) return forward_direct<T>(d, ws, dry, stream, bytes);
   const int64_t R = d.rows, D = d.n_in, V = d.vocab;
   Packer<T, NP> pack(ws);
   Launch<LsePartEpi<T, NP>> L{};
@@ -317,23 +440,8 @@ int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t strea
   if (R > 0) {
     if (pack.launch(stream) != 0) return -1;
     if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy") != 0) return -1;
-    if (d.reduction != 0 && R >= 64 && R * parts <= kJoinSmall) {
-      lse_join_small_kernel<<<1, 1024, 0, stream>>>(e.part, (int32_t)parts, (int32_t)R, e.ztarget, d.target, V,
-                                                    d.ignore_index, d.reduction == 1, d.lse, d.loss, d.out,
-                                                    d.scale);
-      D3A_LAUNCH_CHECK("linear_cross_entropy");
-      return 0;
-    }
-    lse_join_kernel<<<(unsigned)((R + 7) / 8), 256, 0, stream>>>(
-        e.part, (int32_t)parts, (int32_t)R, e.ztarget, d.target, V, d.ignore_index, d.lse, d.loss);
-    D3A_LAUNCH_CHECK("linear_cross_entropy");
   }
-  if (d.reduction != 0) {
-    loss_reduce_kernel<<<1, 1024, 0, stream>>>(d.loss, d.target, d.ignore_index, (int32_t)R,
-                                               d.reduction == 1, d.out, d.scale);
-    D3A_LAUNCH_CHECK("linear_cross_entropy");
-  }
-  return 0;
+  return finish(d, e.part, parts, e.ztarget, stream);
 }
 
 template <class T, int NP>
@@ -343,6 +451,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     *bytes = 0;
     return 0;
   }
+  if (is_direct(d)) return backward_direct<T>(d, ws, dry, stream, bytes);
   Packer<T, NP> pack(ws);
   const Operand x = pack.operand(d.x, d.ldx, 0, 1, R, D);
   const Operand w = pack.operand(d.W, d.ldW, 0, 1, V, D);
