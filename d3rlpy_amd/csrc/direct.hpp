@@ -33,6 +33,7 @@ template <class T>
 struct Problem {
   Operand<T> a, b, b2;  // b2: the second B of dual products, or of the second inner segment
   T* rowsum;        // [batch][M]: the sums of A's rows, or null
+  mm::Factor sum_factor;
   int32_t M, N, K, batch, n_outer, n_inner;
   int32_t tiles_m, tiles_n, first;
 };
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void direct_kernel(const Launch<T, 
   if (want_sum && threadIdx.x < 32 && m0 + (int)threadIdx.x < P.M) {
     float s = 0.f;
     for (int v = 0; v < kWaves; ++v) s += sums[v][threadIdx.x];
-    P.rowsum[(int64_t)batch * P.M + m0 + threadIdx.x] = (T)s;
+    P.rowsum[(int64_t)batch * P.M + m0 + threadIdx.x] = (T)(s * P.sum_factor.get());
   }
   // two neighbouring columns a thread, sixteen threads a row
   const int r = threadIdx.x >> 4, c = 2 * (threadIdx.x & 15);
@@ -194,12 +195,14 @@ struct StoreEpi {
   int64_t ld, s_batch;
   const T* bias;
   int64_t s_bias;
+  mm::Factor factor;
   __device__ __forceinline__ void run(int batch, int m, int n, int M, int N, const float v[2], const float*) const {
     if (m >= M || !out) return;
     T* o = out + batch * s_batch + m * ld;
+    const float by = factor.get();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (n + i < N) o[n + i] = (T)(v[i] + (bias ? (float)bias[batch * s_bias + n + i] : 0.f));
+      if (n + i < N) o[n + i] = (T)(v[i] * by + (bias ? (float)bias[batch * s_bias + n + i] : 0.f));
   }
 };
 
@@ -248,10 +251,12 @@ int launch(Launch<T, Epi>& L, hipStream_t stream, const char* what) {
   return 0;
 }
 
-// Whether an operator whose products each have `work` multiply-adds, and axes
-// up to `axis`, runs here: the k steps of a wave stay few, and the tiles'
-// reuse of what they load does not pay yet.
-inline bool small(double work, int64_t axis) { return work <= (double)(1 << 27) && axis <= 2048; }
+// Whether an operator whose products each have `work` multiply-adds and k axes
+// up to `axis` runs here.  Trained in float32 / bfloat16, us here against the
+// tiles: 512 x 256 x 1024 82 / 55 against 100 / 63, 1024 x 512 x 256 69 / 44
+// against 113 / 49 (both 2^27); with a k of 2048, 128 x 512 x 2048, 122 / 90
+// against 111 / 64, since a wave then has sixteen k steps one after another.
+inline bool small(double work, int64_t axis) { return work <= (double)(1 << 27) && axis <= 1024; }
 
 }  // namespace direct
 }  // namespace d3a

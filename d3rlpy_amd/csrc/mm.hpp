@@ -623,6 +623,12 @@ __device__ __forceinline__ void load_bias(const T* bias, int n, int N, float b[8
   for (int r = 0; r < 8; ++r) b[r] = bias && n + r < N ? (float)bias[n + r] : 0.f;
 }
 
+// A factor of a result that is only known on the device: a[0] * b[0] (null: 1).
+struct Factor {
+  const float *a, *b;
+  __device__ __forceinline__ float get() const { return (a ? a[0] : 1.f) * (b ? b[0] : 1.f); }
+};
+
 // D (+ bias) in T, or a float32 partial of a split / running sum over launches
 template <class T>
 struct StoreEpi {
@@ -636,16 +642,18 @@ struct StoreEpi {
   int32_t mode;     // 0 out = D, 1 partial, 2 sum = D, 3 sum += D, 4 out = sum + D
   int32_t vec;      // out's rows are 16-byte aligned
   int32_t n_batch;
+  Factor factor;    // of D, in what goes to out
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
     const int64_t lds = (t.N + 7) / 8 * 8;
     const T* bias_b = bias ? bias + t.batch * s_bias : nullptr;
+    const float by = mode == 0 || mode == 4 ? factor.get() : 1.f;
     if (mode == 0 && !vec) {
       const int n = t.n0 + t.lane;
       const float b = bias_b && n < t.N ? (float)bias_b[n] : 0.f;
       T* o = out + t.batch * s_batch;
-      each1<C>(acc, t, [&](int m, int n, float v) { o[m * ld + n] = (T)(v + b); });
+      each1<C>(acc, t, [&](int m, int n, float v) { o[m * ld + n] = (T)(v * by + b); });
       return;
     }
     float b[8];
@@ -667,7 +675,7 @@ struct StoreEpi {
       if (n >= t.N) return;
       const int left = t.N - n;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] += mode == 0 ? b[r] : o.v[r];
+      for (int r = 0; r < 8; ++r) v[r] = mode == 0 ? v[r] * by + b[r] : (v[r] + o.v[r]) * by;
       if (mode != 0 && mode <= 3) {
         store8(sum + ((mode == 1 ? ((int64_t)t.split * n_batch + t.batch) * t.M : 0) + m) * lds + n, v);
         return;

@@ -150,6 +150,7 @@ struct ColsumJob {
   int64_t ld, s_batch, s_part;
   void* out;       // T [batch][cols]
   int32_t rows, cols, batch;
+  Factor factor;
 };
 constexpr int kMaxColsum = 3;
 struct ColsumJobs {
@@ -173,9 +174,10 @@ __device__ __forceinline__ const ColsumJob& colsum_job(const ColsumJobs& J, int6
 template <class T>
 __device__ __forceinline__ void colsum_store(const ColsumJob& j, int64_t b, int col, const float s[4]) {
   T* o = static_cast<T*>(j.out) + b * j.cols + col;
+  const float by = j.factor.get();
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (col + k < j.cols) o[k] = (T)s[k];
+    if (col + k < j.cols) o[k] = (T)(s[k] * by);
 }
 
 // a workgroup: 64 quads (one a lane) x its chunk of rows over sixteen waves
@@ -248,8 +250,8 @@ __global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs J) {
 template <class T, int NP>
 struct Colsum {
   ColsumJobs jobs{};
-  void add(const Operand& o, int64_t rows, int64_t cols, int64_t batch, void* out) {
-    jobs.j[jobs.n] = ColsumJob{o.p, o.ld, o.s_batch, o.s_part, out, (int32_t)rows, (int32_t)cols, (int32_t)batch};
+  void add(const Operand& o, int64_t rows, int64_t cols, int64_t batch, void* out, Factor factor = {}) {
+    jobs.j[jobs.n] = ColsumJob{o.p, o.ld, o.s_batch, o.s_part, out, (int32_t)rows, (int32_t)cols, (int32_t)batch, factor};
     jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * ((cols + 3) / 4);
     ++jobs.n;
     // about 768 workgroups, chunks of at least 64 rows (four a wave)
@@ -283,6 +285,7 @@ struct SumJob {
   int64_t ld, s_batch, s_bias;
   int64_t n;          // batch * M * round8(N)
   int32_t M, N, splits, vec;  // vec: out takes eight values at a time
+  Factor factor;
 };
 template <class T>
 struct SumJobs {
@@ -303,8 +306,11 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
   const int n = (int)(e - row * pieces) * 8, left = j.N - n;
   const float* p = j.part + (row * pieces) * 8 + n;
   T* o = j.out + b * j.s_batch + (row - b * j.M) * j.ld + n;
-  float s[8];
-  load_bias(j.bias ? j.bias + b * j.s_bias : nullptr, n, j.N, s);
+  float s[8], bias[8];
+  load_bias(j.bias ? j.bias + b * j.s_bias : nullptr, n, j.N, bias);
+  const float by = j.factor.get();
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s[r] = 0.f;
 #pragma unroll 2
   for (int k = 0; k < j.splits; ++k) {
     float v[8];
@@ -312,6 +318,8 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumJobs<T> J) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) s[r] += v[r];
   }
+#pragma unroll
+  for (int r = 0; r < 8; ++r) s[r] = s[r] * by + bias[r];
   if (j.vec && left >= 8) {
     store8(o, s);
   } else {
@@ -422,7 +430,7 @@ struct Products {
 
   void add(const Operand& a, const Operand& b, int64_t M, int64_t N, int64_t K, int64_t batch,
            int64_t n_outer, int64_t n_inner, void* out, int64_t ld, int64_t s_batch,
-           const void* bias, int64_t s_bias) {
+           const void* bias, int64_t s_bias, Factor factor = {}) {
     Problem& p = L.p[L.n];
     p = Problem{};
     p.a = a;
@@ -442,6 +450,7 @@ struct Products {
     e.bias = static_cast<const T*>(bias);
     e.s_bias = s_bias;
     e.n_batch = (int32_t)batch;
+    e.factor = factor;
     e.vec = ld * sizeof(T) % 16 == 0 && s_batch * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
     ++L.n;
   }
@@ -459,7 +468,7 @@ struct Products {
       const int64_t n = (int64_t)p.batch * p.M * round8(p.N);
       e.sum = ws.take<float>(c.splits * n);
       e.mode = 1;
-      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.bias, e.ld, e.s_batch, e.s_bias, n, p.M, p.N, p.splits, e.vec};
+      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.bias, e.ld, e.s_batch, e.s_bias, n, p.M, p.N, p.splits, e.vec, e.factor};
       sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + (int64_t)p.batch * p.M * ((p.N + 7) / 8);
       ++sums.n;
     }

@@ -2,7 +2,8 @@
 // backward, without the logits in memory:
 //
 //   z = x W^T + b,  lse_r = log sum_v exp z_rv,  loss_r = lse_r - z_r,target
-//   dz_rv = (exp(z_rv - lse_r) - [v = target_r]) dloss_r
+//   dz_rv = (exp(z_rv - lse_r) - [v = target_r]) dloss_r  (dloss_r: a row's own;
+//     one for all rows multiplies the products' results instead, see loss_factor)
 //   dx = dz W,  dW = dz^T x,  db_v = sum_r dz_rv
 //
 // Forward: the tiles of mm.hpp over (rows, vocabulary); a tile's epilogue
@@ -144,15 +145,14 @@ template <class T>
 struct DirectDzEpi {
   const T* bias;
   const int64_t* target;
-  const float *lse, *gloss, *scale;
-  int64_t s_gloss, ignore, vocab;
+  const float *lse, *gloss;
+  int64_t ignore, vocab;
   T* dz;
   int64_t ld;
   __device__ __forceinline__ void run(int, int m, int n, int M, int N, const float v[2], const float*) const {
     if (m >= M) return;
     const int64_t y = target[m];
-    const float by = scale ? scale[0] : 1.f, l = lse[m];
-    const float g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
+    const float l = lse[m], g = y >= 0 && y < vocab ? (gloss ? gloss[m] : 1.f) : NAN;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (n + i >= N) continue;
@@ -163,8 +163,17 @@ struct DirectDzEpi {
   }
 };
 
+// What every row's gradient has in common multiplies the products' results and
+// not dz: near a target dz is -1 times it, so that its rounding to bfloat16, up
+// to 2^-8, would be every gradient's.
+Factor loss_factor(const d3a_linear_xent_desc& d) {
+  return d.reduction == 0 ? Factor{} : Factor{d.gloss, d.reduction == 1 ? d.scale : nullptr};
+}
+
 bool is_direct(const d3a_linear_xent_desc& d) {
-  return direct::small((double)d.rows * d.n_in * d.vocab, std::max({d.rows, d.n_in, d.vocab}));
+  // (the vocabulary is a k axis of one product of four: 256 x 256 x 2048 in
+  // float32 takes 61 us here, 70 with tiles)
+  return direct::small((double)d.rows * d.n_in * d.vocab, std::max({d.rows, d.n_in, d.vocab / 2}));
 }
 
 // Joins the rows' parts: 8 rows x 32 threads a workgroup, first their largest
@@ -277,8 +286,7 @@ struct DzEpi {
   static constexpr int kRowBytes = 16;
   const T* bias;
   const int64_t* target;
-  const float *lse, *gloss, *scale;  // scale: null = 1
-  int64_t s_gloss;                   // 1 (a row's own) or 0 (one for all)
+  const float *lse, *gloss;  // gloss: the rows' own, or null (one for all: a factor of the products)
   int64_t ignore, vocab;
   __bf16* dz;                        // planes, rows of ld
   int64_t ld, s_part;
@@ -288,13 +296,12 @@ struct DzEpi {
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
     // the wave's rows, two a lane: their lse, gradient factor, and target column
     // (-1: in no column here; -2: the row is ignored)
-    const float by = scale ? scale[0] : 1.f;
     float4* rows = reinterpret_cast<float4*>(t.rows);
 #pragma unroll
     for (int k = 0; k < (C::TM + 63) / 64; ++k) {
       const int i = 64 * k + t.lane, m = min(t.m0 + i, t.M - 1);
       const int64_t y = target[m];
-      const float l = lse[m], g = y >= 0 && y < vocab ? gloss[m * s_gloss] * by : NAN;
+      const float l = lse[m], g = y >= 0 && y < vocab ? (gloss ? gloss[m] : 1.f) : NAN;
       const int64_t want = y - v0;
       const int col = y == ignore ? -2 : want >= 0 && want < t.N ? (int)want : -1;
       if (i < C::TM) rows[i] = make_float4(l, g, __int_as_float(col), 0.f);
@@ -392,14 +399,14 @@ int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream
     direct::Launch<T, DirectDzEpi<T>> L{};
     L.n = 1;
     L.p[0] = direct::problem(direct::operand<T>(d.x, d.ldx, 0, D), direct::operand<T>(d.W, d.ldW, 0, D), R, V, D, 1);
-    L.e[0] = DirectDzEpi<T>{static_cast<const T*>(d.b), d.target, d.lse, d.gloss,
-                            d.reduction == 1 ? d.scale : nullptr, d.reduction == 0 ? 1 : 0, d.ignore_index, V, dz, ld};
+    L.e[0] = DirectDzEpi<T>{static_cast<const T*>(d.b), d.target, d.lse,
+                            d.reduction == 0 ? d.gloss : nullptr, d.ignore_index, V, dz, ld};
     if (direct::launch<false, false, false>(L, stream, "linear_cross_entropy_bwd") != 0) return -1;
     if (d.dx) {
       direct::Launch<T, direct::StoreEpi<T>> X{};
       X.n = 1;
       X.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, V), direct::operand<T>(d.W, d.ldW, 0, V), R, D, V, 1);
-      X.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dx), D, 0, nullptr, 0};
+      X.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dx), D, 0, nullptr, 0, loss_factor(d)};
       if (direct::launch<false, true, false>(X, stream, "linear_cross_entropy_bwd") != 0) return -1;
     }
   }
@@ -408,7 +415,8 @@ int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream
   W.n = 1;
   W.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, R), direct::operand<T>(d.x, d.ldx, 0, R), V, d.dW ? D : 1, R, 1);
   W.p[0].rowsum = static_cast<T*>(d.db);
-  W.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dW), D, 0, nullptr, 0};
+  W.p[0].sum_factor = loss_factor(d);
+  W.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dW), D, 0, nullptr, 0, loss_factor(d)};
   return direct::launch<true, true, false>(W, stream, "linear_cross_entropy_bwd");
 }
 
@@ -452,6 +460,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     return 0;
   }
   if (is_direct(d)) return backward_direct<T>(d, ws, dry, stream, bytes);
+  const Factor by = loss_factor(d);
   Packer<T, NP> pack(ws);
   const Operand x = pack.operand(d.x, d.ldx, 0, 1, R, D);
   const Operand w = pack.operand(d.W, d.ldW, 0, 1, V, D);
@@ -487,9 +496,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     e.bias = d.b ? static_cast<const T*>(d.b) + v0 : nullptr;
     e.target = d.target;
     e.lse = d.lse;
-    e.gloss = d.gloss;
-    e.scale = d.reduction == 1 ? d.scale : nullptr;
-    e.s_gloss = d.reduction == 0 ? 1 : 0;
+    e.gloss = d.reduction == 0 ? d.gloss : nullptr;
     e.ignore = d.ignore_index;
     e.vocab = V;
     e.dz = const_cast<__bf16*>(dz.p);
@@ -499,17 +506,17 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
 
     Products<T, NP> dx, dw;
     if (d.dx) {
-      dx.add(dz, p.b, R, D, n, 1, 1, 1, d.dx, D, 0, nullptr, 0);
+      dx.add(dz, p.b, R, D, n, 1, 1, 1, d.dx, D, 0, nullptr, 0, by);
       if (n_pieces > 1) {
         dx.L.e[0].sum = sum;
         dx.L.e[0].mode = last ? 4 : k == 0 ? 2 : 3;
       }
       dx.reserve(ws, n_pieces == 1);
     }
-    if (d.dW) dw.add(dz, x, n, D, R, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0);
+    if (d.dW) dw.add(dz, x, n, D, R, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0, by);
     dw.reserve(ws, true);
     Colsum<T, NP> cs;
-    if (d.db) cs.add(dz, R, n, 1, static_cast<T*>(d.db) + v0);
+    if (d.db) cs.add(dz, R, n, 1, static_cast<T*>(d.db) + v0, by);
     cs.reserve(ws);
     *bytes = std::max(*bytes, ws.used);
     if (dry) continue;

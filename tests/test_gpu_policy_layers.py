@@ -137,9 +137,13 @@ def run_gated(T, p, dy, activation):
 SIZES = [(1, 8, 8, 8), (1, 1, 1, 1), (2, 3, 5, 7), (5, 64, 32, 48), (17, 40, 72, 24),
          (33, 129, 100, 65), (64, 256, 130, 256), (65, 72, 520, 71), (200, 256, 512, 256),
          (333, 130, 1000, 129)]
+# an axis past 1024 and few rows: thin forward with the tiles' backward (R <= 16),
+# or the tiles with most of each empty
+THIN_SIZES = [(1, 40, 1100, 24), (7, 24, 1041, 33), (16, 1030, 72, 65), (17, 1030, 72, 24),
+              (40, 33, 1100, 17), (200, 1030, 72, 1100), (1100, 40, 24, 33)]
 
 
-@pytest.mark.parametrize("R,D,F,O", SIZES)
+@pytest.mark.parametrize("R,D,F,O", SIZES + THIN_SIZES)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("activation,bias", [("silu", False), ("gelu", True), ("relu", True)])
 def test_gated_mlp(T, R, D, F, O, dtype, activation, bias):
@@ -157,7 +161,8 @@ def test_gated_mlp_large_tiles(T, R, D, F, O, dtype):
 
 
 @pytest.mark.parametrize("shared", [False, True])
-@pytest.mark.parametrize("R,D,F,O", [(1, 17, 40, 3), (40, 24, 100, 33), (300, 128, 512, 128)])
+@pytest.mark.parametrize("R,D,F,O", [(1, 17, 40, 3), (40, 24, 100, 33), (300, 128, 512, 128),
+                                     (3, 17, 1100, 9), (40, 24, 1100, 33), (33, 1030, 40, 40)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_gated_mlp_members(T, R, D, F, O, dtype, shared):
     p, dy = gated_params(3, R, D, F, O, dtype, True, shared)
@@ -166,8 +171,9 @@ def test_gated_mlp_members(T, R, D, F, O, dtype, shared):
     check(got, gated_reference(p, dy, "silu", shared))
 
 
-def test_gated_mlp_strides(T):
-    R, D, F, O = 50, 64, 96, 40
+@pytest.mark.parametrize("F", [96, 1104])  # products from the tensors, tiles
+def test_gated_mlp_strides(T, F):
+    R, D, O = 50, 64, 40
     p, dy = gated_params(0, R, D, F, O, BF16, False)
     ref = gated_reference(p, dy, "silu")
 
@@ -192,8 +198,10 @@ def test_gated_mlp_strides(T):
     check(run_gated(T, p, one, "silu"), gated_reference(p, one, "silu"))
 
 
-def test_gated_mlp_one_gradient_and_no_rows(T):
-    p, dy = gated_params(0, 20, 24, 40, 16, F32, True)
+@pytest.mark.parametrize("F", [40, 1100])
+@pytest.mark.parametrize("R", [20, 9])
+def test_gated_mlp_one_gradient_and_no_rows(T, R, F):
+    p, dy = gated_params(0, R, 24, F, 16, F32, True)
     ref = gated_reference(p, dy, "silu")
     for k in p:
         q = {n: t.detach().requires_grad_(n == k) for n, t in p.items()}
@@ -239,7 +247,8 @@ def xent_inputs(R, D, V, dtype, bias, pad=0.2):
 
 @pytest.mark.parametrize("R,D,V", [(1, 1, 1), (1, 8, 2), (3, 17, 5), (8, 64, 1000), (33, 100, 257),
                                    (65, 40, 130), (130, 256, 64), (257, 33, 1031),
-                                   (700, 128, 2050)])
+                                   (700, 128, 2050), (1, 8, 2100), (3, 17, 2101), (65, 40, 5003),
+                                   (33, 1030, 257), (1030, 24, 5)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("reduction,bias", [("mean", False), ("sum", True), ("none", True)])
 def test_linear_cross_entropy(T, R, D, V, dtype, reduction, bias):
@@ -262,8 +271,9 @@ def test_linear_cross_entropy_pieces(T):
     check(run_xent(T, x, W, b, t, "mean", 1.0), xent_reference(x, W, b, t, -100, "mean", 1.0))
 
 
-def test_linear_cross_entropy_masked_rows(T):
-    x, W, b, t = xent_inputs(40, 24, 77, F32, True)
+@pytest.mark.parametrize("V", [77, 2201])  # products from the tensors, tiles
+def test_linear_cross_entropy_masked_rows(T, V):
+    x, W, b, t = xent_inputs(40, 24, V, F32, True)
     t[:] = -100
     for reduction in ("mean", "sum", "none"):
         got = run_xent(T, x, W, b, t, reduction, 1.0)
@@ -280,20 +290,21 @@ def test_linear_cross_entropy_masked_rows(T):
     assert torch.equal(got["x"][t == 3], torch.zeros_like(got["x"][t == 3]))
 
 
-def test_linear_cross_entropy_extreme_logits(T):
+@pytest.mark.parametrize("n", [35, 1100])
+def test_linear_cross_entropy_extreme_logits(T, n):
     """Logits of the type's lowest value and of -inf (a masked action), and a
     target outside the vocabulary."""
-    x, W, b, t = xent_inputs(30, 16, 70, F32, True, pad=0.0)
-    t = t % 35
-    b[35:50] = float("-inf")
-    b[50:] = torch.finfo(F32).min
-    cut = xent_reference(x, W[:35], b[:35], t, -100, "mean", 1.0)
+    x, W, b, t = xent_inputs(30, 16, 2 * n, F32, True, pad=0.0)
+    t = t % n
+    b[n:n + 15] = float("-inf")
+    b[n + 15:] = torch.finfo(F32).min
+    cut = xent_reference(x, W[:n], b[:n], t, -100, "mean", 1.0)
     got = run_xent(T, x, W, b, t, "mean", 1.0)
     within(got["loss"], *cut["loss"], "loss")
     within(got["x"], *cut["x"], "x")
-    within(got["W"][:35], *cut["W"], "W")
-    assert not got["W"][35:].any() and not got["b"][35:].any()
-    for wrong in (-1, 70, 1 << 40, -(1 << 40)):
+    within(got["W"][:n], *cut["W"], "W")
+    assert not got["W"][n:].any() and not got["b"][n:].any()
+    for wrong in (-1, 2 * n, 1 << 40, -(1 << 40)):
         u = t.clone()
         u[4] = wrong
         got = run_xent(T, x, W, b, u, "none", 1.0)
@@ -302,8 +313,9 @@ def test_linear_cross_entropy_extreme_logits(T):
         assert torch.isfinite(got["loss"][rest]).all() and torch.isfinite(got["x"][rest]).all()
 
 
-def test_linear_cross_entropy_shapes_and_strides(T):
-    x, W, b, t = xent_inputs(48, 40, 90, BF16, True)
+@pytest.mark.parametrize("V", [90, 2190])
+def test_linear_cross_entropy_shapes_and_strides(T, V):
+    x, W, b, t = xent_inputs(48, 40, V, BF16, True)
     ref = xent_reference(x, W, b, t, -100, "mean", 1.0)
     got = run_xent(T, x.view(4, 12, 40), W, b, t.view(4, 12), "mean", 1.0)
     assert got["x"].shape == (4, 12, 40)
@@ -311,12 +323,27 @@ def test_linear_cross_entropy_shapes_and_strides(T):
     check(got, ref)
     big = torch.full((48, 83), 5.0, device=DEV, dtype=BF16)
     big[:, 3:43] = x
-    tied = rnd(11, 90, 80, dtype=BF16)
+    tied = rnd(11, V, 80, dtype=BF16)
     tied[:, 40:] = W
     got = run_xent(T, big[:, 3:43], tied[:, 40:], b, t, "mean", 1.0)
     check(got, ref)
     none = run_xent(T, x[:0], W, b, t[:0], "mean", 1.0)
     assert not none["loss"].detach().any() and not none["W"].any() and not none["b"].any()
+
+
+@pytest.mark.parametrize("V", [200, 4099])
+def test_linear_cross_entropy_common_factor(T, V):
+    """bfloat16, the mean over 510 rows: 1/510 would round to bfloat16 with
+    2^-8 of it, in every row alike.  The gradients' common error, their
+    component along the exact ones, is at most that of 1 - p at a target, 2^-9
+    (the others' signs vary)."""
+    x, W, _, t = xent_inputs(510, 64, V, BF16, False, pad=0.0)
+    ref = xent_reference(x, W, None, t, -100, "mean", 1.0)
+    got = run_xent(T, x, W, None, t, "mean", 1.0)
+    check(got, ref)
+    for k in ("x", "W"):
+        want = ref[k][0]
+        assert abs(float(((got[k].double() - want) * want).sum() / (want * want).sum())) <= 2.0 ** -9, k
 
 
 # --------------------------------------------------------------- together, replays
