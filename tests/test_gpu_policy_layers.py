@@ -248,7 +248,7 @@ def xent_inputs(R, D, V, dtype, bias, pad=0.2):
 @pytest.mark.parametrize("R,D,V", [(1, 1, 1), (1, 8, 2), (3, 17, 5), (8, 64, 1000), (33, 100, 257),
                                    (65, 40, 130), (130, 256, 64), (257, 33, 1031),
                                    (700, 128, 2050), (1, 8, 2100), (3, 17, 2101), (65, 40, 5003),
-                                   (33, 1030, 257), (1030, 24, 5)])
+                                   (33, 1030, 257), (1030, 24, 5), (9, 40, 33011)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("reduction,bias", [("mean", False), ("sum", True), ("none", True)])
 def test_linear_cross_entropy(T, R, D, V, dtype, reduction, bias):
@@ -311,6 +311,25 @@ def test_linear_cross_entropy_extreme_logits(T, n):
         assert got["loss"][4].isnan() and got["x"][4].isnan().all()
         rest = torch.arange(30, device=DEV) != 4
         assert torch.isfinite(got["loss"][rest]).all() and torch.isfinite(got["x"][rest]).all()
+
+
+@pytest.mark.parametrize("V", [77, 2201, 33011])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_cross_entropy_rows_that_are_not_numbers(T, V, dtype):
+    """NaN in a row, or a logit of +inf: that row's loss and gradient are NaN, no
+    other row's."""
+    x, W, b, t = xent_inputs(70, 24, V, dtype, True)
+    t[5] = t[69] = 1
+    clean = run_xent(T, x, W, b, t, "none", 1.0)
+    bad = x.clone()
+    bad[5, 3] = float("nan")
+    bad[69, 7] = float("inf")
+    got = run_xent(T, bad, W, b, t, "none", 1.0)
+    rest = torch.ones(70, dtype=torch.bool, device=DEV)
+    rest[5] = rest[69] = False
+    assert got["loss"][~rest].isnan().all() and got["x"][~rest].isnan().all()
+    assert torch.equal(got["loss"][rest], clean["loss"][rest])
+    assert torch.equal(got["x"][rest], clean["x"][rest])
 
 
 @pytest.mark.parametrize("V", [90, 2190])
