@@ -226,5 +226,6 @@ def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, target: torch.Tensor,
     ``x`` [.., in], ``W`` [vocab, in], ``b`` [vocab] or None, float32 or
     bfloat16; ``target`` [..] int64.  The loss is float32.  A row whose target
     is ``ignore_index`` has loss 0 and no gradient; 'mean' is over the other
-    rows (0 where there are none).  A target outside the vocabulary gives NaN."""
+    rows (0 where there are none).  A target outside the vocabulary gives NaN.
+    (W's gradient has the ignored rows' x times 0: padding has to be finite.)"""
     return load().linear_cross_entropy(x, W, target, b, ignore_index, reduction)[0]

@@ -1399,8 +1399,10 @@ int d3a_gated_mlp_bwd(const d3a_gated_mlp_desc* desc, void* stream);
  * factor of a row's gradient, read by the backward).  loss and lse [rows] are
  * written always.
  * The backward reads x, W, b, target, lse, scale and gloss ([rows] with
- * reduction 0, else [1]) and writes the gradients whose pointers are given:
- * dx [rows][n_in], dW [vocab][n_in], db [vocab], contiguous. */
+ * reduction 0, else [1], where it multiplies the finished gradients: one that is
+ * not finite spoils the ignored rows' too) and writes the gradients whose
+ * pointers are given: dx [rows][n_in], dW [vocab][n_in], db [vocab], contiguous.
+ * dW has every row's x as a factor, the ignored rows' times 0. */
 typedef struct d3a_linear_xent_desc {
   const void *x, *W, *b;
   const int64_t* target;
