@@ -47,8 +47,8 @@ struct PackJobs {
 
 // One 8-wide piece a thread: 32 bytes (16) in, 48 (16) out; memory bound.
 template <class T, int NP>
-__global__ __launch_bounds__(256) void pack_kernel(const PackJobs J) {
-  int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void pack_kernel(const PackJobs J, int64_t p0) {
+  int64_t p = p0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
   int i = 0;
   while (i < J.n && p >= J.end[i]) ++i;
   if (i == J.n) return;
@@ -129,13 +129,13 @@ struct Packer {
 
   int launch(hipStream_t stream) {
     if (jobs.n == 0 || jobs.end[jobs.n - 1] == 0) return 0;
-    const int64_t blocks = (jobs.end[jobs.n - 1] + 255) / 256;
-    if (blocks >= (1LL << 31)) {
-      set_error("operand too large to pack");
-      return -1;
+    // (a launch holds less than 2^32 threads)
+    constexpr int64_t most = 1LL << 31;
+    const int64_t pieces = jobs.end[jobs.n - 1];
+    for (int64_t p0 = 0; p0 < pieces; p0 += most) {
+      pack_kernel<T, NP><<<(unsigned)((std::min(pieces - p0, most) + 255) / 256), 256, 0, stream>>>(jobs, p0);
+      D3A_LAUNCH_CHECK("pack");
     }
-    pack_kernel<T, NP><<<(unsigned)blocks, 256, 0, stream>>>(jobs);
-    D3A_LAUNCH_CHECK("pack");
     return 0;
   }
 };

@@ -38,6 +38,22 @@ __device__ __forceinline__ void load_vec(const T* p, float* v) {
   }
 }
 
+// the same as it lies in memory, to be converted when it is used
+template <int VEC, class T>
+struct Raw {
+  typedef std::conditional_t<VEC == 1, T, std::conditional_t<sizeof(T) == 4, f32x4, bf16x8>> V;
+  V v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
+  __device__ __forceinline__ void get(float* o) const {
+    if constexpr (VEC == 1) {
+      o[0] = (float)v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o[k] = (float)v[k];
+    }
+  }
+};
+
 template <int VEC, class T>
 __device__ __forceinline__ void store_vec(T* p, const float* v) {
   if constexpr (VEC == 1) {
@@ -69,70 +85,102 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
   return block_sum(v, scratch);
 }
 
-// NCH pieces of VEC values a lane; WPR waves a row (1: four rows a workgroup)
+// NCH pieces of VEC values a lane; WPR waves a row (1: four rows a workgroup).
+// Grid (workgroups, members): workgroup g of a member takes rows g, g + grid, ..
+// (times the rows it holds at once).  Single values (VEC 1) are bound by the
+// loads' number, so w and b stay in registers over 2048 workgroups' rows and the
+// next row is loaded ahead; pieces take a workgroup for every row (up to 2^22, of the
+// 2^24 that a launch holds) and load w and b when they need them: 8192 x 2048 in bfloat16 takes 14 to 15 us, 18 the other way, and 8192
+// x 2047 22, of 38.
+
 template <class T, class W, int VEC, int NCH, int WPR>
 __global__ __launch_bounds__(256) void norm_kernel(const Args A) {
+  constexpr bool kWalk = VEC == 1, kAhead = kWalk && NCH <= 16;
   __shared__ float scratch[4];
   const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wid / WPR;
-  if (row >= A.rows * A.members) return;  // (WPR 4: the whole workgroup or none of it)
-  const int64_t c = row / A.rows, r = row - c * A.rows;
-  const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
   const int l = (wid % WPR) * 64 + lane;
-  float v[NCH][VEC], s = 0.f;
+  const int64_t c = blockIdx.y;
+  Raw<VEC, T> rx[NCH];
+  auto fetch = [&](int64_t r) __attribute__((always_inline)) {
+    const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
 #pragma unroll
-  for (int j = 0; j < NCH; ++j) {
-    const int col = (j * WPR * 64 + l) * VEC;
-    if (col < A.n) {
-      load_vec<VEC>(x + col, v[j]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[j][k] = 0.f;
+    for (int j = 0; j < NCH; ++j) {
+      const int col = (j * WPR * 64 + l) * VEC;
+      if (col < A.n) rx[j].load(x + col);
     }
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) s += v[j][k];
-  }
-  const float mean = row_sum<WPR>(s, scratch) / (float)A.n;
-  s = 0.f;
-#pragma unroll
-  for (int j = 0; j < NCH; ++j) {
-    const int col = (j * WPR * 64 + l) * VEC;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      v[j][k] = col < A.n ? v[j][k] - mean : 0.f;
-      s = fmaf(v[j][k], v[j][k], s);
-    }
-  }
-  const float rstd = 1.f / sqrtf(row_sum<WPR>(s, scratch) / (float)A.n + A.eps);
-  if (A.mean && l == 0) {
-    A.mean[row] = mean;
-    A.rstd[row] = rstd;
-  }
-  T* y = static_cast<T*>(A.y) + row * A.n;
+  };
+  const int64_t step = (int64_t)gridDim.x * (4 / WPR);
+  const int64_t r0 = (int64_t)blockIdx.x * (4 / WPR) + wid / WPR;
+  if (r0 >= A.rows) return;  // (WPR 4: the whole workgroup or none of it)
+  fetch(r0);
   const W* w = static_cast<const W*>(A.w) + c * A.n;
   const W* b = static_cast<const W*>(A.b) + c * A.n;
-#pragma unroll
-  for (int j = 0; j < NCH; ++j) {
+  float wv[NCH][VEC], bv[NCH][VEC];
+  auto affine = [&](int j) __attribute__((always_inline)) {
     const int col = (j * WPR * 64 + l) * VEC;
-    if (col >= A.n) continue;
-    float wv[VEC], bv[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      wv[k] = 1.f;
-      bv[k] = 0.f;
+      wv[j][k] = 1.f;
+      bv[j][k] = 0.f;
     }
-    if (A.w) load_vec<VEC>(w + col, wv);
-    if (A.b) load_vec<VEC>(b + col, bv);
+    if (A.w && col < A.n) load_vec<VEC>(w + col, wv[j]);
+    if (A.b && col < A.n) load_vec<VEC>(b + col, bv[j]);
+  };
+  if (kWalk)
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[j][k] = fmaf(v[j][k] * rstd, wv[k], bv[k]);
-    store_vec<VEC>(y + col, v[j]);
+    for (int j = 0; j < NCH; ++j) affine(j);
+  for (int64_t r = r0; r < A.rows; r += step) {
+    const int64_t row = c * A.rows + r;
+    float v[NCH][VEC], s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      if ((j * WPR * 64 + l) * VEC < A.n) {
+        rx[j].get(v[j]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[j][k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += v[j][k];
+    }
+    if (kAhead && r + step < A.rows) fetch(r + step);
+    const float mean = row_sum<WPR>(s, scratch) / (float)A.n;
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      const int col = (j * WPR * 64 + l) * VEC;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        v[j][k] = col < A.n ? v[j][k] - mean : 0.f;
+        s = fmaf(v[j][k], v[j][k], s);
+      }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<WPR>(s, scratch) / (float)A.n + A.eps);
+    if (A.mean && l == 0) {
+      A.mean[row] = mean;
+      A.rstd[row] = rstd;
+    }
+    T* y = static_cast<T*>(A.y) + row * A.n;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      const int col = (j * WPR * 64 + l) * VEC;
+      if (col >= A.n) continue;
+      if (!kWalk) affine(j);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[j][k] = fmaf(v[j][k] * rstd, wv[j][k], bv[j][k]);
+      store_vec<VEC>(y + col, v[j]);
+    }
+    if (!kAhead && r + step < A.rows) fetch(r + step);
   }
 }
 
-// grid (workgroups, members): workgroup g of a member takes rows g, g + grid, ..
-// (times the rows it holds at once)
+// Grid and rows as the forward's; a row that leaves registers free is loaded one
+// ahead.  Four waves a row from 1025 values on, since a wave that holds 2048 of x, dy,
+// w, dw and db has two neighbours a SIMD at most: 8192 x 2048 in bfloat16 takes 23.5 us
+// (117 MB with the partials, 5 TB/s), of 36; 3001 x 1537 in float32 13.6, of 23.5.
 template <class T, class W, int VEC, int NCH, int WPR>
 __global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
+  constexpr bool kAhead = NCH * VEC <= 16;
   __shared__ float scratch[8];
   __shared__ float cols[WPR == 1 ? 2 * NCH * VEC * 64 : 1];
   const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -151,18 +199,35 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
     if (A.w && col < A.n) load_vec<VEC>(w + col, wv[j]);
   }
   const int64_t step = (int64_t)gridDim.x * (4 / WPR);
-  for (int64_t r = (int64_t)blockIdx.x * (4 / WPR) + wid / WPR; r < A.rows; r += step) {
+  Raw<VEC, T> rx[NCH], ry[NCH];
+  float mean, rstd, next_mean = 0.f, next_rstd = 0.f;
+  auto fetch = [&](int64_t r) __attribute__((always_inline)) {
     const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
     const T* dy = static_cast<const T*>(A.dy) + c * A.sdy + r * A.lddy;
-    const int64_t row = c * A.rows + r;
-    const float mean = A.mean[row], rstd = A.rstd[row];
-    float xh[NCH][VEC], t[NCH][VEC], s[2] = {0.f, 0.f};
+    next_mean = A.mean[c * A.rows + r];
+    next_rstd = A.rstd[c * A.rows + r];
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       const int col = (j * WPR * 64 + l) * VEC;
       if (col < A.n) {
-        load_vec<VEC>(x + col, xh[j]);
-        load_vec<VEC>(dy + col, t[j]);
+        rx[j].load(x + col);
+        ry[j].load(dy + col);
+      }
+    }
+  };
+  const int64_t r0 = (int64_t)blockIdx.x * (4 / WPR) + wid / WPR;
+  if (kAhead && r0 < A.rows) fetch(r0);
+  for (int64_t r = r0; r < A.rows; r += step) {
+    const int64_t row = c * A.rows + r;
+    if (!kAhead) fetch(r);
+    mean = next_mean;
+    rstd = next_rstd;
+    float xh[NCH][VEC], t[NCH][VEC], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      if ((j * WPR * 64 + l) * VEC < A.n) {
+        rx[j].get(xh[j]);
+        ry[j].get(t[j]);
       } else {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -171,6 +236,7 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
         }
       }
     }
+    if (kAhead && r + step < A.rows) fetch(r + step);
 #pragma unroll
     for (int j = 0; j < NCH; ++j)
 #pragma unroll
@@ -230,10 +296,11 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
   for (int j = 0; j < NCH; ++j) {
     const int col = (j * WPR * 64 + l) * VEC;
     if (col >= A.n) continue;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      part[col + k] = dw[j][k];
-      part[A.n + col + k] = db[j][k];
+    store_vec<VEC == 1 ? 1 : 4>(part + col, dw[j]);
+    store_vec<VEC == 1 ? 1 : 4>(part + A.n + col, db[j]);
+    if constexpr (VEC == 8) {
+      store_vec<4>(part + col + 4, dw[j] + 4);
+      store_vec<4>(part + A.n + col + 4, db[j] + 4);
     }
   }
 }
@@ -340,6 +407,7 @@ __global__ __launch_bounds__(256) void norm_long_cols_kernel(const Args A) {
 }
 
 // ---- host -------------------------------------------------------------------
+constexpr int kWave = 1024;  // values that a wave holds
 constexpr int kLong = 8192;  // values that four waves hold
 
 int check(const d3a_layer_norm_desc* d, bool bwd) {
@@ -394,21 +462,22 @@ bool aligned(const d3a_layer_norm_desc& d, bool bwd) {
   return (p & 15) == 0 && s % vec == 0;
 }
 
-// workgroups a member: enough to fill the chip (1024 over the members), each
-// wave at least one row
-int64_t bwd_blocks(const d3a_layer_norm_desc& d) {
-  const int64_t at_once = d.n > 2048 ? 1 : 4;
-  const int64_t most = std::max<int64_t>(1, 1024 / d.members);
-  return std::max<int64_t>(1, std::min((d.rows + at_once - 1) / at_once, most));
+// workgroups a member of a kernel whose waves walk over rows: enough to fill the
+// chip (`all` over the members), each wave at least one row
+int64_t blocks_of(const d3a_layer_norm_desc& d, int64_t at_once, int64_t all) {
+  return std::max<int64_t>(1, std::min((d.rows + at_once - 1) / at_once, std::max<int64_t>(1, all / d.members)));
 }
+// the backward's, each of which writes a partial
+int64_t bwd_blocks(const d3a_layer_norm_desc& d) { return blocks_of(d, d.n > kWave ? 1 : 4, 1024); }
 
 template <class T, class W, int VEC, int NCH, int WPR>
-int launch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, int64_t blocks, hipStream_t stream) {
+int launch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, hipStream_t stream) {
+  constexpr int at_once = 4 / WPR;
   if (bwd) {
-    norm_bwd_kernel<T, W, VEC, NCH, WPR><<<dim3((unsigned)blocks, (unsigned)d.members), 256, 0, stream>>>(a);
+    norm_bwd_kernel<T, W, VEC, NCH, WPR><<<dim3((unsigned)bwd_blocks(d), (unsigned)d.members), 256, 0, stream>>>(a);
   } else {
-    const int64_t rows = d.rows * d.members;
-    norm_kernel<T, W, VEC, NCH, WPR><<<(unsigned)((rows * WPR + 3) / 4), 256, 0, stream>>>(a);
+    const int64_t blocks = blocks_of(d, at_once, VEC == 1 ? 2048 : 1 << 22);
+    norm_kernel<T, W, VEC, NCH, WPR><<<dim3((unsigned)blocks, (unsigned)d.members), 256, 0, stream>>>(a);
   }
   D3A_LAUNCH_CHECK("layer_norm");
   return 0;
@@ -416,29 +485,30 @@ int launch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, int64_t blocks
 
 // pieces of 16 bytes where every row allows them, else single values
 template <class T, class W>
-int dispatch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, int64_t blocks, hipStream_t s) {
+int dispatch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const int64_t n = d.n;
   if (aligned(d, bwd)) {
-    if (n > 4096) return launch<T, W, V, 8192 / (256 * V), 4>(d, a, bwd, blocks, s);
-    if (n > 2048) return launch<T, W, V, 4096 / (256 * V), 4>(d, a, bwd, blocks, s);
-    if (n > 1024) return launch<T, W, V, 2048 / (64 * V), 1>(d, a, bwd, blocks, s);
-    if (n > 512) return launch<T, W, V, 1024 / (64 * V), 1>(d, a, bwd, blocks, s);
-    if (n > 256 || V == 8) return launch<T, W, V, 512 / (64 * V), 1>(d, a, bwd, blocks, s);
-    return launch<T, W, V, V == 8 ? 1 : 256 / (64 * V), 1>(d, a, bwd, blocks, s);
+    if (n > 4096) return launch<T, W, V, 8192 / (256 * V), 4>(d, a, bwd, s);
+    if (n > 2048) return launch<T, W, V, 4096 / (256 * V), 4>(d, a, bwd, s);
+    if (n > kWave && !bwd) return launch<T, W, V, 2048 / (64 * V), 1>(d, a, bwd, s);
+    if (n > kWave) return launch<T, W, V, 2048 / (256 * V), 4>(d, a, bwd, s);
+    if (n > 512) return launch<T, W, V, 1024 / (64 * V), 1>(d, a, bwd, s);
+    if (n > 256 || V == 8) return launch<T, W, V, 512 / (64 * V), 1>(d, a, bwd, s);
+    return launch<T, W, V, V == 8 ? 1 : 256 / (64 * V), 1>(d, a, bwd, s);
   }
-  if (n > 4096) return launch<T, W, 1, 32, 4>(d, a, bwd, blocks, s);
-  if (n > 2048) return launch<T, W, 1, 16, 4>(d, a, bwd, blocks, s);
-  if (n > 1024) return launch<T, W, 1, 32, 1>(d, a, bwd, blocks, s);
-  if (n > 512) return launch<T, W, 1, 16, 1>(d, a, bwd, blocks, s);
-  return launch<T, W, 1, 8, 1>(d, a, bwd, blocks, s);
+  if (n > 4096) return launch<T, W, 1, 32, 4>(d, a, bwd, s);
+  if (n > 2048) return launch<T, W, 1, 16, 4>(d, a, bwd, s);
+  if (n > kWave) return launch<T, W, 1, 8, 4>(d, a, bwd, s);
+  if (n > 512) return launch<T, W, 1, 16, 1>(d, a, bwd, s);
+  return launch<T, W, 1, 8, 1>(d, a, bwd, s);
 }
 
 template <class T, class W>
 int forward(const d3a_layer_norm_desc& d, hipStream_t stream) {
   const Args a = args_of(d);
   if (d.rows == 0) return 0;
-  if (d.n <= kLong) return dispatch<T, W>(d, a, false, 0, stream);
+  if (d.n <= kLong) return dispatch<T, W>(d, a, false, stream);
   norm_long_kernel<T, W><<<(unsigned)(d.rows * d.members), 256, 0, stream>>>(a);
   D3A_LAUNCH_CHECK("layer_norm");
   return 0;
@@ -468,7 +538,7 @@ int backward(const d3a_layer_norm_desc& d, Arena ws, bool dry, hipStream_t strea
       D3A_LAUNCH_CHECK("layer_norm_bwd");
     }
   } else {
-    if (dispatch<T, W>(d, a, true, parts, stream) != 0) return -1;
+    if (dispatch<T, W>(d, a, true, stream) != 0) return -1;
   }
   if (!cols) return 0;
   norm_finish_kernel<W><<<dim3((unsigned)((2 * d.n + 63) / 64), (unsigned)d.members), 1024, 0, stream>>>(

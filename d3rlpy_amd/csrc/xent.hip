@@ -181,10 +181,10 @@ bool is_direct(const d3a_linear_xent_desc& d) {
 __global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32_t parts, int32_t rows,
                                                        const float* ztarget, const int64_t* target,
                                                        int64_t vocab, int64_t ignore, float* lse,
-                                                       float* loss) {
+                                                       float* loss, int32_t r0) {
   __shared__ float red[256];
   const int q = threadIdx.x & 7, g = threadIdx.x >> 3;
-  const int r = blockIdx.x * 8 + q;
+  const int r = r0 + blockIdx.x * 8 + q;
   float m = -INFINITY, s = 0.f;
   if (r < rows)
 #pragma unroll 4
@@ -385,6 +385,8 @@ int wave_columns(TileSize s) {
 }
 
 // the rows' lse and loss from their parts, and the reduction
+// (of kJoinRows at a time: a launch holds less than 2^32 threads)
+constexpr int64_t kJoinRows = 1 << 26;
 int finish(const d3a_linear_xent_desc& d, const float2* part, int64_t parts, const float* ztarget,
            hipStream_t stream) {
   const int64_t R = d.rows;
@@ -399,8 +401,9 @@ int finish(const d3a_linear_xent_desc& d, const float2* part, int64_t parts, con
       lse_join_wide_kernel<<<(unsigned)R, 256, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget, d.target,
                                                             d.vocab, d.ignore_index, d.lse, d.loss);
     else
-      lse_join_kernel<<<(unsigned)((R + 7) / 8), 256, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget,
-                                                                  d.target, d.vocab, d.ignore_index, d.lse, d.loss);
+      for (int64_t r0 = 0; r0 < R; r0 += kJoinRows)
+        lse_join_kernel<<<(unsigned)((std::min(R - r0, kJoinRows) + 7) / 8), 256, 0, stream>>>(
+            part, (int32_t)parts, (int32_t)R, ztarget, d.target, d.vocab, d.ignore_index, d.lse, d.loss, (int32_t)r0);
     D3A_LAUNCH_CHECK("linear_cross_entropy");
   }
   if (d.reduction != 0) {

@@ -101,6 +101,24 @@ def test_layer_norm_without_weight_or_rows(T):
     within(dw, *ref["weight"], "weight")
 
 
+@pytest.mark.parametrize("n", [8, 7])
+def test_layer_norm_more_rows_than_a_launch_has_threads(T, n):
+    """2^26 rows of 64 lanes each would be 2^32 threads."""
+    R = (1 << 26) + 5
+    x = rnd(1, 1 << 12, n, dtype=BF16).repeat((R >> 12) + 1, 1)[:R].requires_grad_(True)
+    w, b = rnd(2, n), rnd(3, n)
+    y = T.layer_norm(x, w, b)
+    dy = torch.ones((), device=DEV, dtype=BF16).expand(R, n)
+    (dx,) = torch.autograd.grad(y, [x], dy)
+    x, y = x.detach(), y.detach()
+    for rows in (slice(0, 9), slice(R - 9, R)):
+        ref = norm_reference(x[rows], w, b, 1e-5, dy[rows])
+        check({"y": y[rows], "x": dx[rows]}, ref, ("y", "x"))
+    # the same rows give the same values, bit by bit
+    for v in (y, dx):
+        assert torch.equal(v[1 << 25:(1 << 25) + (1 << 20)], v[:1 << 20])
+
+
 def test_layer_norm_constant_and_bad_rows(T):
     x = rnd(1, 4, 100)
     x[1] = 3.0
@@ -348,6 +366,19 @@ def test_linear_cross_entropy_shapes_and_strides(T, V):
     check(got, ref)
     none = run_xent(T, x[:0], W, b, t[:0], "mean", 1.0)
     assert not none["loss"].detach().any() and not none["W"].any() and not none["b"].any()
+
+
+def test_linear_cross_entropy_more_rows_than_a_launch_has_threads(T):
+    """2^27 rows, 8 to a workgroup of 256, would be 2^32 threads."""
+    R, D, V = (1 << 27) + 3, 8, 3
+    x = rnd(1, 1 << 12, D, dtype=BF16).repeat((R >> 12) + 1, 1)[:R]
+    W = rnd(2, V, D, dtype=BF16)
+    t = (torch.arange(1 << 12, device=DEV) % V).repeat((R >> 12) + 1)[:R]
+    loss = T.linear_cross_entropy(x, W, t, reduction="none")
+    for rows in (slice(0, 9), slice(R - 9, R)):
+        ref = xent_reference(x[rows], W, None, t[rows], -100, "none", 1.0)
+        within(loss[rows], *ref["loss"], "loss")
+    assert torch.equal(loss[1 << 26:(1 << 26) + (1 << 20)], loss[:1 << 20])
 
 
 @pytest.mark.parametrize("V", [200, 4099])
