@@ -649,6 +649,7 @@ int64_t norm_members(const at::Tensor& x, const OptTensor& w, const OptTensor& b
     TORCH_CHECK(v.device() == x.device(), "layer_norm: weight / bias on ", v.device(), ", x on ", x.device());
     if (v.dim() == 2) {
       TORCH_CHECK(x.dim() >= 2 && x.size(0) == v.size(0), "layer_norm: x [members, .., n] for weight [members, n]");
+      TORCH_CHECK(v.size(0) >= 1, "layer_norm: weight / bias of no member");
       members = v.size(0);
     }
   }

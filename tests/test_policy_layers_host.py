@@ -63,6 +63,7 @@ def test_meta_gradients(T):
 @pytest.mark.parametrize("call,match", [
     (lambda T: T.layer_norm(meta(4, 8), meta(7)), "weight / bias of 7"),
     (lambda T: T.layer_norm(meta(4, 8), meta(3, 8)), "members"),
+    (lambda T: T.layer_norm(meta(0, 4, 8), meta(0, 8)), "no member"),
     (lambda T: T.layer_norm(meta(4, 8), meta(8), meta(1, 8)), "one shape and dtype"),
     (lambda T: T.layer_norm(meta(4, 0)), "empty last"),
     (lambda T: T.gated_mlp(meta(4, 8), meta(5, 7), meta(5, 7), meta(8, 5)), "8 features"),
