@@ -163,14 +163,19 @@ def test_gated_workspaces():
     # aligned bfloat16 operands are read in place: h alone, or nothing with kept
     assert size(gated_desc(kept=None), 0) == 100 * 64 * 2
     assert size(gated_desc(), 0) == 0
-    # unaligned: x and the weights packed beside it
-    assert size(gated_desc(kept=None, x=258), 0) >= 100 * (64 + 32) * 2
+    # a minibatch reads unaligned operands as they lie; tiles have x packed
+    wide = dict(n_hidden=1104, ldWd=1104)
+    assert size(gated_desc(kept=None, x=258), 0) == 100 * 64 * 2
+    assert size(gated_desc(**wide), 0) == 0
+    assert size(gated_desc(kept=None, x=258, **wide), 0) >= 100 * (1104 + 32) * 2
     # the backward's dg and du, and nothing for gradients that nobody wants
     assert size(gated_desc(dx=256), 1) >= 2 * 100 * 64 * 2
     assert size(gated_desc(), 1) == 0
-    # float32: three planes of every operand
+    # float32: three planes of every operand of a tile
+    f = gated_desc(dtype=0, kept=None, **wide)
+    assert size(f, 0) >= 3 * 2 * (100 * 1104 + 100 * 32 + 2 * 1104 * 32 + 48 * 1104)
     f = gated_desc(dtype=0, kept=None)
-    assert size(f, 0) >= 3 * 2 * (100 * 64 + 100 * 32 + 2 * 64 * 32 + 48 * 64)
+    assert size(f, 0) == 4 * 100 * 64
     assert lib.d3a_gated_mlp_kept(ctypes.byref(f), ctypes.byref(n)) == 0
     assert n.value == 100 * 64 * (8 + 6)
 
