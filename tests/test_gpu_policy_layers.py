@@ -488,6 +488,33 @@ def test_block_is_deterministic_and_replays(T, dtype):
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
 
 
+def test_captured_autograd(T):
+    """Loss and torch.autograd.grad captured together, after warm-up passes on
+    the capture's kind of stream whose graphs are gone: every replay, with new
+    parameters between, is the eager pass."""
+    q, tokens, target = block_inputs(F32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            block_step(T, q, tokens, target)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grads = block_step(T, q, tokens, target)
+    for k in range(4):
+        with torch.no_grad():
+            q["Wg"].mul_(1.0 + 0.1 * k)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [loss.detach().clone()] + [g.clone() for g in grads]
+        want = block_step(T, q, tokens, target)
+        assert torch.equal(got[0], want[0].detach())
+        # (the embedding's gradient adds rows of the same token in torch's order)
+        for n, a, b in zip(q, got[1:], want[1]):
+            assert torch.equal(a, b) or n == "emb", n
+
+
 def test_gradients_against_differences(T):
     """The losses' directional derivative, by central differences of the
     float32 loss: steps of 1e-2 leave 1e-4 of curvature and 1e-5 of rounding
