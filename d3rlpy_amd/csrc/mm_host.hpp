@@ -250,6 +250,7 @@ __global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs J) {
 template <class T, int NP>
 struct Colsum {
   ColsumJobs jobs{};
+  bool from_epilogue = false;
   void add(const Operand& o, int64_t rows, int64_t cols, int64_t batch, void* out, Factor factor = {}) {
     jobs.j[jobs.n] = ColsumJob{o.p, o.ld, o.s_batch, o.s_part, out, (int32_t)rows, (int32_t)cols, (int32_t)batch, factor};
     jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * ((cols + 3) / 4);
@@ -260,16 +261,27 @@ struct Colsum {
                               : (int32_t)std::max<int64_t>(
                                     1, std::min<int64_t>({768 / std::max<int64_t>(blocks, 1), rows / 64, 256}));
   }
+  // instead of add(): the chunks' sums come from an epilogue, [chunks][quads][4]
+  float* given(int64_t cols, int32_t chunks, void* out, Factor factor, Arena& ws) {
+    jobs.j[0] = ColsumJob{nullptr, 0, 0, 0, out, 0, (int32_t)cols, 1, factor};
+    jobs.first[1] = (cols + 3) / 4;
+    jobs.n = 1;
+    jobs.chunks = chunks;
+    from_epilogue = true;
+    return jobs.part = ws.take<float>(chunks * jobs.first[1] * 4);
+  }
   void reserve(Arena& ws) {
-    if (jobs.n && jobs.chunks > 1) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n] * 4);
+    if (jobs.n && !from_epilogue && jobs.chunks > 1) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n] * 4);
   }
   int launch(hipStream_t stream) {
     const int64_t quads = jobs.first[jobs.n];
     if (jobs.n == 0 || quads == 0) return 0;
     const unsigned blocks = (unsigned)((quads + 63) / 64);
-    colsum_kernel<T, NP><<<dim3(blocks, jobs.chunks), 1024, 0, stream>>>(jobs);
-    D3A_LAUNCH_CHECK("column sums");
-    if (jobs.chunks == 1) return 0;
+    if (!from_epilogue) {
+      colsum_kernel<T, NP><<<dim3(blocks, jobs.chunks), 1024, 0, stream>>>(jobs);
+      D3A_LAUNCH_CHECK("column sums");
+      if (jobs.chunks == 1) return 0;
+    }
     colsum_finish<T><<<blocks, 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
     return 0;

@@ -322,6 +322,7 @@ struct DzEpi {
   __bf16* dz;                        // planes, rows of ld
   int64_t ld, s_part;
   int32_t v0;
+  float* db;                         // the waves' sums of their rows, [M / C::TM][quads of N][4], or null
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
@@ -339,6 +340,7 @@ struct DzEpi {
     }
     float b[8];
     load_bias(bias, first_column<false>(t), t.N, b);
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     auto none = [](int, int) { return Nothing{}; };
     each8<C, false>(acc, t, none, [&](int m, int n, float* v, float*, Nothing) {
       if (n >= ld) return;
@@ -356,8 +358,23 @@ struct DzEpi {
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[r] = col != -2 && n + r < t.N ? v[r] : 0.f;
       }
+      if (db) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] += v[r];
+      }
       store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
     });
+    if (!db) return;
+    // eight lanes have the same columns
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1)
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] += __shfl_xor(s[r], o);
+    const int n = first_column<false>(t);
+    if (t.lane >= 8 || t.m0 >= t.M) return;
+    float* at = db + (int64_t)(t.m0 / C::TM) * ((t.N + 3) / 4 * 4) + n;
+    if (n < t.N) store4(at, s);
+    if (n + 4 < t.N) store4(at + 4, s + 4);
   }
 };
 
@@ -382,6 +399,11 @@ template <int NP>
 int wave_columns(TileSize s) {
   typedef Tiles<NP> X;
   return s == kLarge ? X::Large::TN : s == kMid ? X::Mid::TN : X::Small::TN;
+}
+template <int NP>
+int wave_rows(TileSize s) {
+  typedef Tiles<NP> X;
+  return s == kLarge ? X::Large::TM : s == kMid ? X::Mid::TM : X::Small::TM;
 }
 
 // the rows' lse and loss from their parts, and the reduction
@@ -553,13 +575,20 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     }
     if (d.dW) dw.add(dz, x, n, D, R, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0, by);
     dw.reserve(ws, true);
+    // db: the waves' sums from the epilogue, up to 256 of a column; of more rows a
+    // pass over dz, whose second part would be the long one.  8192 x 1024 -> 32768 in
+    // bfloat16, both directions: 2195 us, of 2322 with the pass; 1500 x 777 -> 10007 in
+    // float32 651, of 673.
+    const TileSize size = choose<NP>(L, false).size;
+    const int64_t chunks = (R + wave_rows<NP>(size) - 1) / wave_rows<NP>(size);
     Colsum<T, NP> cs;
-    if (d.db) cs.add(dz, R, n, 1, static_cast<T*>(d.db) + v0, by);
+    if (d.db && chunks <= 256) e.db = cs.given(n, (int32_t)chunks, static_cast<T*>(d.db) + v0, by, ws);
+    else if (d.db) cs.add(dz, R, n, 1, static_cast<T*>(d.db) + v0, by);
     cs.reserve(ws);
     *bytes = std::max(*bytes, ws.used);
     if (dry) continue;
     if (R > 0) {
-      if (run<NP, false, false, false>(L, choose<NP>(L, false).size, stream, "linear_cross_entropy_bwd") != 0) return -1;
+      if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy_bwd") != 0) return -1;
       if (dx.template launch<false, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
     }
     if (dw.template launch<true, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
