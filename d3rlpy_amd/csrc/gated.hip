@@ -310,8 +310,9 @@ int backward_direct(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t
   return W.n ? direct::launch<true, true, false>(W, stream, "gated_mlp_bwd") : 0;
 }
 
-// At most 16 rows: the weights read once.  One row of 2048 x 5632 bfloat16: 13.7 us
-// and 8.2 (3.4 and 2.8 TB/s), where the tiles take 20.6 and 14.6.
+// At most 16 rows: the weights read once.  One row of 2048 x 5632 bfloat16: 13.7
+// to 15 us and 8.2 (3.1 to 3.4 and 2.8 TB/s: mostly the launch's ramp; four rows of
+// 4096 x 11008 35 and 18.5, 5 TB/s), where the tiles take 20.6 and 14.6.
 template <class T, int NP>
 int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);

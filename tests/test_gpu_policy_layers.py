@@ -275,7 +275,7 @@ def test_linear_cross_entropy(T, R, D, V, dtype, reduction, bias):
     check(run_xent(T, x, W, b, t, reduction, g), xent_reference(x, W, b, t, -100, reduction, g))
 
 
-@pytest.mark.parametrize("R,D,V", [(4000, 136, 4099), (2049, 72, 10007)])
+@pytest.mark.parametrize("R,D,V", [(4000, 136, 4099), (2049, 72, 10007), (33000, 24, 1100)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_linear_cross_entropy_large_tiles(T, R, D, V, dtype):
     x, W, b, t = xent_inputs(R, D, V, dtype, True)
