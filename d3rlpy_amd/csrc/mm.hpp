@@ -8,9 +8,14 @@
 // row-contiguous (p + k * ld + r); the tile of either goes from memory to LDS
 // without passing registers (16 bytes a lane), and a row-contiguous tile is
 // transposed by the LDS reads.  A bfloat16 operand has one plane; a float32
-// operand is given as its exact three-way bf16 split (three planes, pack.hpp
-// layout), and a k step then takes the six part products that matter, smallest
-// first: fp32 accuracy at six bf16 products a term.
+// operand is given as its exact three-way bf16 split (three planes, see pack_kernel),
+// and a k step then takes the six part products that matter, smallest first: fp32
+// accuracy at six bf16 products a term.  (An infinity, or a value that rounds to one
+// in bfloat16, has NaN parts: its row's or column's results are NaN.)
+//
+// Bound by the matrix cores: 32768 x 1024 x 8192 in bfloat16 takes 373 us (1.47
+// PFLOP/s), 8192 x 1024 x 4096 58 (1.19), 4096 cubed in float32 539 (255 TFLOP/s of
+// terms, 1.53 PFLOP/s of part products).
 //
 // 16-byte pieces outside the operand (rows past its end, ks past K) read as
 // zero through the buffer resource's range check, so M, N and K are free; the

