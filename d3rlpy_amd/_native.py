@@ -529,7 +529,8 @@ class LinearXentDesc(C.Structure):
         [(f, vp) for f in ("x", "W", "b", "target", "loss", "lse", "out", "scale", "gloss",
                            "dx", "dW", "db")]
         + [(f, C.c_int64) for f in ("rows", "n_in", "vocab", "ldx", "ldW", "ignore_index")]
-        + [("dtype", C.c_int32), ("reduction", C.c_int32), ("ws", vp), ("ws_bytes", C.c_int64)])
+        + [("dtype", C.c_int32), ("reduction", C.c_int32), ("ws", vp), ("ws_bytes", C.c_int64),
+           ("low", vp)])
 
 
 class LayerNormDesc(C.Structure):

@@ -985,7 +985,8 @@ void xent_call(XentCall& c, const at::Tensor& x, const at::Tensor& W, const at::
   d.ignore_index = ignore;
 }
 
-// -> (loss [..] or [], lse [..], scale [1]: the factor of a row's gradient)
+// -> (loss [..] or [], lse [..], scale [1 + rows]: the factor of a row's gradient,
+//     and what each lse's rounding left, both for the backward)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_hip(
     const at::Tensor& x, const at::Tensor& W, const at::Tensor& target, const OptTensor& b, int64_t ignore,
     c10::string_view reduction) {
@@ -994,11 +995,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_hip(
   XentCall c;
   xent_call(c, x, W, target, b, ignore, reduction);
   const auto f = x.options().dtype(at::kFloat);
-  at::Tensor rows = at::empty(target.sizes(), f), lse = at::empty(target.sizes(), f), scale = at::empty({1}, f);
+  at::Tensor rows = at::empty(target.sizes(), f), lse = at::empty(target.sizes(), f);
+  at::Tensor scale = at::empty({1 + c.d.rows}, f);
   at::Tensor out = c.d.reduction == 0 ? rows : at::empty({}, f);
   c.d.loss = rows.data_ptr<float>();
   c.d.lse = lse.data_ptr<float>();
   c.d.scale = scale.data_ptr<float>();
+  c.d.low = c.d.scale + 1;
   c.d.out = out.data_ptr<float>();
   check_rc(d3a_linear_xent_workspace(&c.d, 0, &c.d.ws_bytes), "d3rlpy_amd::linear_cross_entropy");
   const at::Tensor ws = workspace(c.d.ws_bytes, x);
@@ -1013,7 +1016,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_meta(
   xent_shape(x, W, target, b);
   const auto f = x.options().dtype(at::kFloat);
   return {reduction_code(reduction) == 0 ? at::empty(target.sizes(), f) : at::empty({}, f),
-          at::empty(target.sizes(), f), at::empty({1}, f)};
+          at::empty(target.sizes(), f), at::empty({1 + target.numel()}, f)};
 }
 
 // the gradients of x, W, b that `wanted` asks for; the others undefined
@@ -1031,11 +1034,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_cross_entropy_backward_hip
   check_f32_gpu(scale, "scale");
   TORCH_CHECK(g.device() == x.device() && lse.device() == x.device() && scale.device() == x.device(),
               "linear_cross_entropy_backward: tensors on several devices");
-  TORCH_CHECK(lse.numel() == c.d.rows && scale.numel() == 1 && g.numel() == (c.d.reduction == 0 ? c.d.rows : 1),
+  TORCH_CHECK(lse.numel() == c.d.rows && scale.numel() == 1 + c.d.rows && g.numel() == (c.d.reduction == 0 ? c.d.rows : 1),
               "linear_cross_entropy_backward: grad of the loss, lse and scale of its forward");
   c.d.gloss = g.data_ptr<float>();
   c.d.lse = lse.data_ptr<float>();
   c.d.scale = scale.data_ptr<float>();
+  c.d.low = c.d.scale + 1;
   // (written by the forward alone)
   c.d.loss = c.d.lse;
   c.d.out = c.d.scale;

@@ -4,6 +4,10 @@
 //   z = x W^T + b,  lse_r = log sum_v exp z_rv,  loss_r = lse_r - z_r,target
 //   dz_rv = (exp(z_rv - lse_r) - [v = target_r]) dloss_r  (dloss_r: a row's own;
 //     one for all rows multiplies the products' results instead, see loss_factor)
+// lse_r = m + log s (m the row's largest logit, s its sum of exp(z - m)) rounds to
+// steps of 2^-24 |m|, which is all of log s where a row's logits share a large value.
+// So the loss is (m - z_target) + log s, and the backward goes by lse and by what its
+// rounding left, low_r = (m - lse_r) + log s.
 //   dx = dz W,  dW = dz^T x,  db_v = sum_r dz_rv
 //
 // Forward: the tiles of mm.hpp over (rows, vocabulary); a tile's epilogue
@@ -36,6 +40,29 @@ constexpr int64_t kPieceBytes = 512LL << 20;
 template <int NP>
 __device__ __forceinline__ float exp_to(float z, float ref) {
   return NP == 1 ? __expf(z - ref) : expf(z - ref);
+}
+
+// exp(z - (lse + low)); `low` as low_factor gives it: with bfloat16 tensors it goes
+// into the product by log2 e that the hardware's exponential takes anyway.
+constexpr float kLog2e = 1.44269504088896341f;
+template <int NP>
+__device__ __forceinline__ float low_factor(float low) {
+  return NP == 1 ? -low * kLog2e : low;
+}
+template <int NP>
+__device__ __forceinline__ float probability(float z, float lse, float low) {
+  return NP == 1 ? __builtin_amdgcn_exp2f(fmaf(z - lse, kLog2e, low)) : expf((z - lse) - low);
+}
+
+// What a row's maximum m and sum s of exp(z - m) give; z: the target's logit.
+struct RowLoss {
+  float lse, low, loss;
+};
+__device__ __forceinline__ RowLoss row_loss(float m, float s, float z, int64_t target, int64_t vocab,
+                                            int64_t ignore) {
+  const float log_s = logf(s), lse = m + log_s;
+  const float loss = target == ignore ? 0.f : target >= 0 && target < vocab ? (m - z) + log_s : NAN;
+  return {lse, (m - lse) + log_s, loss};
 }
 
 // (max, sum of exp(z - max)) of a + b; an empty side has max -inf, sum 0
@@ -147,7 +174,7 @@ template <class T>
 struct DirectDzEpi {
   const T* bias;
   const int64_t* target;
-  const float *lse, *gloss;
+  const float *lse, *low, *gloss;  // low: or null (0)
   int64_t ignore, vocab;
   T* dz;
   int64_t ld;
@@ -155,11 +182,12 @@ struct DirectDzEpi {
     if (m >= M) return;
     const int64_t y = target[m];
     const float l = lse[m], g = y >= 0 && y < vocab ? (gloss ? gloss[m] : 1.f) : NAN;
+    const float lo = low_factor<3>(low ? low[m] : 0.f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (n + i >= N) continue;
       const float z = v[i] + (bias ? (float)bias[n + i] : 0.f);
-      const float d = (exp_to<3>(z, l) - (n + i == y ? 1.f : 0.f)) * g;
+      const float d = (probability<3>(z, l, lo) - (n + i == y ? 1.f : 0.f)) * g;
       dz[m * ld + n + i] = (T)(y == ignore ? 0.f : d);
     }
   }
@@ -183,7 +211,7 @@ bool is_direct(const d3a_linear_xent_desc& d) {
 __global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32_t parts, int32_t rows,
                                                        const float* ztarget, const int64_t* target,
                                                        int64_t vocab, int64_t ignore, float* lse,
-                                                       float* loss, int32_t r0) {
+                                                       float* low, float* loss, int32_t r0) {
   __shared__ float red[256];
   const int q = threadIdx.x & 7, g = threadIdx.x >> 3;
   const int r = r0 + blockIdx.x * 8 + q;
@@ -205,10 +233,10 @@ __global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32
   __syncthreads();
   if (g != 0 || r >= rows) return;
   for (int k = 1; k < 32; ++k) s += red[8 * k + q];
-  const float l = m + logf(s);
-  const int64_t t = target[r];
-  lse[r] = l;
-  loss[r] = t == ignore ? 0.f : t >= 0 && t < vocab ? l - ztarget[r] : NAN;
+  const RowLoss o = row_loss(m, s, ztarget[r], target[r], vocab, ignore);
+  lse[r] = o.lse;
+  if (low) low[r] = o.low;
+  loss[r] = o.loss;
 }
 
 // The same with a workgroup a row, for few rows of many parts: us, 1024 parts
@@ -217,7 +245,7 @@ __global__ __launch_bounds__(256) void lse_join_kernel(const float2* part, int32
 __global__ __launch_bounds__(256) void lse_join_wide_kernel(const float2* part, int32_t parts, int32_t rows,
                                                             const float* ztarget, const int64_t* target,
                                                             int64_t vocab, int64_t ignore, float* lse,
-                                                            float* loss) {
+                                                            float* low, float* loss) {
   __shared__ float red[8];
   const int r = blockIdx.x, w = threadIdx.x >> 6;
   float m = -INFINITY, s = 0.f;
@@ -236,10 +264,10 @@ __global__ __launch_bounds__(256) void lse_join_wide_kernel(const float2* part, 
   if ((threadIdx.x & 63) == 0) red[4 + w] = s;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  const float l = m + logf((red[4] + red[5]) + (red[6] + red[7]));
-  const int64_t t = target[r];
-  lse[r] = l;
-  loss[r] = t == ignore ? 0.f : t >= 0 && t < vocab ? l - ztarget[r] : NAN;
+  const RowLoss o = row_loss(m, (red[4] + red[5]) + (red[6] + red[7]), ztarget[r], target[r], vocab, ignore);
+  lse[r] = o.lse;
+  if (low) low[r] = o.low;
+  loss[r] = o.loss;
 }
 
 // The sum of the rows' losses (mean: over the counted rows, at least one), and
@@ -288,8 +316,8 @@ constexpr int64_t kJoinSmall = 16384;
 __global__ __launch_bounds__(1024) void lse_join_small_kernel(const float2* part, int32_t parts, int32_t rows,
                                                               const float* ztarget, const int64_t* target,
                                                               int64_t vocab, int64_t ignore, int32_t mean,
-                                                              float* lse, float* loss, float* out,
-                                                              float* scale) {
+                                                              float* lse, float* low, float* loss,
+                                                              float* out, float* scale) {
   double sum = 0.0;
   int n = 0;
   for (int r = threadIdx.x; r < rows; r += 1024) {
@@ -301,12 +329,12 @@ __global__ __launch_bounds__(1024) void lse_join_small_kernel(const float2* part
       const float2 v = part[(int64_t)p * rows + r];
       s += v.x == m ? v.y : v.y * expf(v.x - m);
     }
-    const float l = m + logf(s);
     const int64_t t = target[r];
-    const float x = t == ignore ? 0.f : t >= 0 && t < vocab ? l - ztarget[r] : NAN;
-    lse[r] = l;
-    loss[r] = x;
-    sum += (double)x;
+    const RowLoss o = row_loss(m, s, ztarget[r], t, vocab, ignore);
+    lse[r] = o.lse;
+    if (low) low[r] = o.low;
+    loss[r] = o.loss;
+    sum += (double)o.loss;
     n += t != ignore;
   }
   reduce_loss(sum, n, mean, out, scale);
@@ -319,7 +347,8 @@ struct DzEpi {
   static constexpr int kRowBytes = 16;
   const T* bias;
   const int64_t* target;
-  const float *lse, *gloss;  // gloss: the rows' own, or null (one for all: a factor of the products)
+  const float *lse, *low;  // low: or null (0)
+  const float* gloss;      // the rows' own, or null (one for all: a factor of the products)
   int64_t ignore, vocab;
   __bf16* dz;                        // planes, rows of ld
   int64_t ld, s_part;
@@ -328,8 +357,8 @@ struct DzEpi {
 
   template <class C>
   __device__ __forceinline__ void run(f32x16 (&acc)[C::MT][C::NT], const Tile& t) const {
-    // the wave's rows, two a lane: their lse, gradient factor, and target column
-    // (-1: in no column here; -2: the row is ignored)
+    // the wave's rows, two a lane: their lse, gradient factor, target column (-1: in
+    // no column here; -2: the row is ignored) and lse's low part
     float4* rows = reinterpret_cast<float4*>(t.rows);
 #pragma unroll
     for (int k = 0; k < (C::TM + 63) / 64; ++k) {
@@ -338,7 +367,7 @@ struct DzEpi {
       const float l = lse[m], g = y >= 0 && y < vocab ? (gloss ? gloss[m] : 1.f) : NAN;
       const int64_t want = y - v0;
       const int col = y == ignore ? -2 : want >= 0 && want < t.N ? (int)want : -1;
-      if (i < C::TM) rows[i] = make_float4(l, g, __int_as_float(col), 0.f);
+      if (i < C::TM) rows[i] = make_float4(l, g, __int_as_float(col), low_factor<NP>(low ? low[m] : 0.f));
     }
     float b[8];
     load_bias(bias, first_column<false>(t), t.N, b);
@@ -349,7 +378,7 @@ struct DzEpi {
       const float4 row = rows[m - t.m0];
       const int col = __float_as_int(row.z), want = col - n;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) v[r] = exp_to<NP>(v[r] + b[r], row.x);
+      for (int r = 0; r < 8; ++r) v[r] = probability<NP>(v[r] + b[r], row.x, row.w);
       if (want >= 0 && want < 8) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) v[r] -= r == want ? 1.f : 0.f;
@@ -416,18 +445,19 @@ int finish(const d3a_linear_xent_desc& d, const float2* part, int64_t parts, con
   const int64_t R = d.rows;
   if (d.reduction != 0 && R >= 64 && R * parts <= kJoinSmall) {
     lse_join_small_kernel<<<1, 1024, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget, d.target, d.vocab,
-                                                  d.ignore_index, d.reduction == 1, d.lse, d.loss, d.out, d.scale);
+                                                  d.ignore_index, d.reduction == 1, d.lse, d.low, d.loss, d.out, d.scale);
     D3A_LAUNCH_CHECK("linear_cross_entropy");
     return 0;
   }
   if (R > 0) {
     if (R <= 256 && parts >= 512)
       lse_join_wide_kernel<<<(unsigned)R, 256, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget, d.target,
-                                                            d.vocab, d.ignore_index, d.lse, d.loss);
+                                                            d.vocab, d.ignore_index, d.lse, d.low, d.loss);
     else
       for (int64_t r0 = 0; r0 < R; r0 += kJoinRows)
         lse_join_kernel<<<(unsigned)((std::min(R - r0, kJoinRows) + 7) / 8), 256, 0, stream>>>(
-            part, (int32_t)parts, (int32_t)R, ztarget, d.target, d.vocab, d.ignore_index, d.lse, d.loss, (int32_t)r0);
+            part, (int32_t)parts, (int32_t)R, ztarget, d.target, d.vocab, d.ignore_index, d.lse, d.low, d.loss,
+            (int32_t)r0);
     D3A_LAUNCH_CHECK("linear_cross_entropy");
   }
   if (d.reduction != 0) {
@@ -461,7 +491,7 @@ int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream
     direct::Launch<T, DirectDzEpi<T>> L{};
     L.n = 1;
     L.p[0] = direct::problem(direct::operand<T>(d.x, d.ldx, 0, D), direct::operand<T>(d.W, d.ldW, 0, D), R, V, D, 1);
-    L.e[0] = DirectDzEpi<T>{static_cast<const T*>(d.b), d.target, d.lse,
+    L.e[0] = DirectDzEpi<T>{static_cast<const T*>(d.b), d.target, d.lse, d.low,
                             d.reduction == 0 ? d.gloss : nullptr, d.ignore_index, V, dz, ld};
     if (direct::launch<false, false, false>(L, stream, "linear_cross_entropy_bwd") != 0) return -1;
     if (d.dx) {
@@ -558,6 +588,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
     e.bias = d.b ? static_cast<const T*>(d.b) + v0 : nullptr;
     e.target = d.target;
     e.lse = d.lse;
+    e.low = d.low;
     e.gloss = d.reduction == 0 ? d.gloss : nullptr;
     e.ignore = d.ignore_index;
     e.vocab = V;

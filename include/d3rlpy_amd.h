@@ -1397,8 +1397,10 @@ int d3a_gated_mlp_bwd(const d3a_gated_mlp_desc* desc, void* stream);
  * loss and gradient NaN.  reduction 0 none, 1 mean over the rows that are not
  * ignored (0 where there is none), 2 sum; 1 and 2 write out[0] and scale[0] (the
  * factor of a row's gradient, read by the backward).  loss and lse [rows] are
- * written always.
- * The backward reads x, W, b, target, lse, scale and gloss ([rows] with
+ * written always; so is low [rows], if it is given: what lse's rounding to float32
+ * left, without which the backward's probabilities err by a factor of up to
+ * exp(2^-24 |lse|).
+ * The backward reads x, W, b, target, lse, low, scale and gloss ([rows] with
  * reduction 0, else [1], where it multiplies the finished gradients: one that is
  * not finite spoils the ignored rows' too) and writes the gradients whose
  * pointers are given: dx [rows][n_in], dW [vocab][n_in], db [vocab], contiguous.
@@ -1413,6 +1415,7 @@ typedef struct d3a_linear_xent_desc {
   int32_t dtype, reduction;
   void* ws;
   int64_t ws_bytes;
+  float* low;
 } d3a_linear_xent_desc;
 int d3a_linear_xent_workspace(const d3a_linear_xent_desc* desc, int32_t backward, int64_t* bytes);
 int d3a_linear_xent(const d3a_linear_xent_desc* desc, void* stream);

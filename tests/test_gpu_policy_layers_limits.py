@@ -1,0 +1,119 @@
+"""layer_norm, gated_mlp and linear_cross_entropy at the ends of their ranges:
+logits that share a large value, large and long arrays, parts and pieces.  Against
+float64 forms with bounds from the kernels' roundings (policy_layer_helpers)."""
+import ctypes
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from policy_layer_helpers import U, within, xent_reference
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def T():
+    from d3rlpy_amd import torch_ops
+    return torch_ops
+
+
+def rnd(seed, *shape, dtype=F32, scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale + shift).to(dtype).to(DEV)
+
+
+def check(got, ref, keys=None):
+    for k in keys or ref:
+        within(got[k], *ref[k], k)
+
+
+def run_xent(T, x, W, b, target, reduction, g, ignore=-100):
+    q = {"x": x.detach().requires_grad_(True), "W": W.detach().requires_grad_(True)}
+    if b is not None:
+        q["b"] = b.detach().requires_grad_(True)
+    loss = T.linear_cross_entropy(q["x"], q["W"], target, q.get("b"), ignore, reduction)
+    grads = torch.autograd.grad(loss, list(q.values()),
+                                g if torch.is_tensor(g) else torch.full_like(loss, g))
+    return {"loss": loss} | dict(zip(q, grads))
+
+
+# ------------------------------------------------- logits that share a large value
+def common_inputs(V, dtype, common, step):
+    """Logits of ``common`` plus whole multiples of ``step``, exact in float32: x
+    has one feature, which W does not weigh, so a logit is its bias."""
+    R, D = 20, 16
+    x, W = torch.zeros(R, D), torch.randn(V, D, generator=torch.Generator().manual_seed(V))
+    x[:, 0] = torch.arange(1, R + 1)
+    W[:, 0] = 0.0
+    over = torch.randint(0, 8, (V,), generator=torch.Generator().manual_seed(1)) * step
+    b = torch.full((V,), common).to(dtype).double() + over
+    assert torch.equal(b.to(dtype).double(), b)
+    t = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(2))
+    t[3] = -100
+    return x.to(dtype).to(DEV), W.to(dtype).to(DEV), b.to(dtype).to(DEV), over.to(DEV), t.to(DEV)
+
+
+@pytest.mark.parametrize("V", [50, 2201, 33011])  # from the tensors; tiles; many parts a row
+@pytest.mark.parametrize("dtype,common,step", [
+    (F32, 0.0, 0.5), (F32, 1e5, 0.5), (F32, -1e6, 0.5), (F32, -1e9, 0.0),
+    (F32, torch.finfo(F32).min, 0.0), (F32, torch.finfo(F32).max, 0.0),
+    (BF16, -100.0, 0.5), (BF16, 1e6, 0.0), (BF16, torch.finfo(BF16).min, 0.0)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_of_logits_with_a_common_value(T, V, dtype, common, step, reduction):
+    """A value that all of a row's logits share changes neither loss nor gradients:
+    both are those of the logits without it, within the bounds that these have."""
+    x, W, b, over, t = common_inputs(V, dtype, common, step)
+    g = rnd(9, 20) if reduction == "none" else 0.7
+    ref = xent_reference(x, W, over, t, -100, reduction, g)
+    check(run_xent(T, x, W, b, t, reduction, g), ref)
+
+
+def test_cross_entropy_of_uniform_rows_is_torchs(T):
+    """Fifty logits of the lowest value: log 50 and 1/50, as torch has it."""
+    b = torch.full((50,), torch.finfo(F32).min, device=DEV)
+    x, W = torch.zeros(4, 8, device=DEV), torch.zeros(50, 8, device=DEV)
+    t = torch.tensor([0, 7, 49, 7], device=DEV)
+    got = run_xent(T, x, W, b, t, "sum", 1.0)
+    c = b.cpu().requires_grad_(True)
+    loss = torch.nn.functional.cross_entropy(c.expand(4, 50), t.cpu(), reduction="sum")
+    loss.backward()
+    # a logarithm and an exponential of a few steps each, and sums of four
+    within(got["loss"], loss.detach(), 16 * U * loss.detach().abs(), "loss")
+    within(got["b"], c.grad, 64 * U * torch.ones(50), "b")
+
+
+def test_cross_entropy_lse_and_its_low_part(T):
+    """lse is the logsumexp's float32 value, shape and all; the backward of the C
+    entry without the low part goes by lse alone."""
+    from d3rlpy_amd import _native as N
+    x, W, b, over, t = common_inputs(50, F32, 1e5, 0.5)
+    ops = T.load()
+    loss, lse, scale = ops.linear_cross_entropy(x.view(4, 5, 16), W, t.view(4, 5), b, -100, "sum")
+    want = torch.logsumexp(b.double(), 0)
+    assert lse.shape == (4, 5)
+    within(lse, want.expand(4, 5), (U * want.abs()).expand(4, 5), "lse")
+    # and what it left: lse + low is the logarithm of the sum to a few steps of its own
+    low = scale[1:].double()
+    within(lse.flatten().double() + low, want.expand(20), torch.full((20,), 64 * U), "lse + low")
+
+    d = N.LinearXentDesc()
+    d.rows, d.n_in, d.vocab, d.ldx, d.ldW, d.ignore_index, d.reduction = 20, 16, 50, 16, 16, -100, 2
+    one, db = torch.ones(1, device=DEV), torch.empty(50, device=DEV)
+    for k, v in (("x", x), ("W", W), ("b", b), ("target", t), ("loss", loss), ("lse", lse),
+                 ("out", loss), ("scale", scale), ("gloss", one), ("db", db)):
+        setattr(d, k, v.data_ptr())
+    size = ctypes.c_int64()
+    assert N.lib().d3a_linear_xent_workspace(ctypes.byref(d), 1, ctypes.byref(size)) == 0
+    ws = torch.empty(size.value, dtype=torch.uint8, device=DEV)
+    d.ws, d.ws_bytes = ws.data_ptr(), size.value
+    stream = torch.cuda.current_stream().cuda_stream
+    assert N.lib().d3a_linear_xent_bwd(ctypes.byref(d), stream) == 0
+    p = torch.softmax(over.double(), 0)
+    count = torch.bincount(t[t >= 0], minlength=50).double()
+    # every row's p is off by the same factor, exp(2^-24 |lse|) at most
+    within(db, 19 * p - count, 19 * p * (1.1 * U * 1e5) + 64 * U * (19 * p + count), "b")
