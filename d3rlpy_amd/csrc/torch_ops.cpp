@@ -1078,11 +1078,19 @@ at::Tensor value(const OptTensor& t) { return given(t) ? *t : at::Tensor(); }
 
 OptTensor optional(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
+// Forward-mode derivatives are not computed: a tensor that carries one is refused,
+// since the kernels' outputs would come without it.
+void refuse_tangent(const at::Tensor& t, const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "d3rlpy_amd::", op,
+                              " has no forward-mode derivative");
+}
+
 // Whether a node is needed, and for which inputs.
 template <size_t N>
-bool wants(const std::array<at::Tensor, N>& inputs, std::array<bool, N>& wanted) {
+bool wants(const char* op, const std::array<at::Tensor, N>& inputs, std::array<bool, N>& wanted) {
   bool any = false;
   for (size_t i = 0; i < N; ++i) {
+    refuse_tangent(inputs[i], op);
     wanted[i] = inputs[i].defined() && inputs[i].requires_grad();
     any |= wanted[i];
   }
@@ -1147,6 +1155,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
                                                                const OptTensor&, const OptTensor&,
                                                                const at::Tensor&, std::array<bool, 3>);
     static const auto op = op_handle<Sig>("d3rlpy_amd::layer_norm_backward");
+    refuse_tangent(g[0], "layer_norm");
     const variable_list v = ctx->get_saved_variables();
     std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
     {
@@ -1160,7 +1169,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 std::tuple<at::Tensor, at::Tensor> layer_norm_autograd(const at::Tensor& x, const OptTensor& w, const OptTensor& b,
                                                        double eps) {
   std::array<bool, 3> wanted;
-  if (!wants<3>({x, value(w), value(b)}, wanted)) return layer_norm_below(x, w, b, eps);
+  if (!wants<3>("layer_norm", {x, value(w), value(b)}, wanted)) return layer_norm_below(x, w, b, eps);
   variable_list r = LayerNormNode::apply(x, w, b, eps, mask_of(wanted));
   return {r[0], r[1]};
 }
@@ -1193,6 +1202,7 @@ struct GatedMlpNode : torch::autograd::Function<GatedMlpNode> {
                       const OptTensor&, const OptTensor&, const OptTensor&, const at::Tensor&, c10::string_view,
                       std::array<bool, 7>);
     static const auto op = op_handle<Sig>("d3rlpy_amd::gated_mlp_backward");
+    refuse_tangent(g[0], "gated_mlp");
     const variable_list v = ctx->get_saved_variables();
     const std::string act = ctx->saved_data["act"].toStringRef();
     Seven r;
@@ -1210,7 +1220,7 @@ std::tuple<at::Tensor, at::Tensor> gated_mlp_autograd(const at::Tensor& x, const
                                                       const at::Tensor& Wd, const OptTensor& bg, const OptTensor& bu,
                                                       const OptTensor& bd, c10::string_view act, bool keep) {
   std::array<bool, 7> wanted;
-  if (!wants<7>({x, Wg, Wu, Wd, value(bg), value(bu), value(bd)}, wanted))
+  if (!wants<7>("gated_mlp", {x, Wg, Wu, Wd, value(bg), value(bu), value(bd)}, wanted))
     return gated_mlp_below(x, Wg, Wu, Wd, bg, bu, bd, act, keep);
   variable_list r = GatedMlpNode::apply(x, Wg, Wu, Wd, bg, bu, bd, std::string(act), mask_of(wanted));
   return {r[0], r[1]};
@@ -1245,6 +1255,7 @@ struct XentNode : torch::autograd::Function<XentNode> {
         const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
         const at::Tensor&, const at::Tensor&, int64_t, c10::string_view, std::array<bool, 3>);
     static const auto op = op_handle<Sig>("d3rlpy_amd::linear_cross_entropy_backward");
+    refuse_tangent(g[0], "linear_cross_entropy");
     const variable_list v = ctx->get_saved_variables();
     const std::string reduction = ctx->saved_data["reduction"].toStringRef();
     std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
@@ -1263,7 +1274,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> xent_autograd(const at::Tensor& x
                                                              const at::Tensor& target, const OptTensor& b,
                                                              int64_t ignore, c10::string_view reduction) {
   std::array<bool, 3> wanted;
-  if (!wants<3>({x, W, value(b)}, wanted)) return xent_below(x, W, target, b, ignore, reduction);
+  if (!wants<3>("linear_cross_entropy", {x, W, value(b)}, wanted)) return xent_below(x, W, target, b, ignore, reduction);
   variable_list r = XentNode::apply(x, W, target, b, ignore, std::string(reduction), mask_of(wanted));
   return {r[0], r[1], r[2]};
 }

@@ -185,7 +185,8 @@ def squashed_gaussian_sample(mu, logstd, eps, min_logstd: float = -20.0,
 
 # layer_norm, gated_mlp and linear_cross_entropy carry their gradients in the op
 # library itself (its Autograd kernels), so torch.ops.d3rlpy_amd.layer_norm is
-# differentiable too; the gradients have no second derivative.  A backward pass
+# differentiable too; the gradients have no second derivative, and forward-mode
+# (torch.autograd.forward_ad, torch.func.jvp) raises.  A backward pass
 # to capture into a graph is best written with the forward and *_backward ops:
 # autograd's own nodes belong to the stream that ran the forward, and a capture
 # that meets an eager graph's nodes of the same leaves ends the process.
