@@ -313,13 +313,16 @@ int backward_direct(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t
 }
 
 // At most 16 rows: the weights read once.  One row of 2048 x 5632 bfloat16: 13.7
-// to 15 us and 8.2 (3.1 to 3.4 and 2.8 TB/s: mostly the launch's ramp; four rows of
-// 4096 x 11008 35 and 18.5, 5 TB/s), where the tiles take 20.6 and 14.6.
+// to 15 us and 8.2 (3.1 to 3.4 and 2.8 TB/s; four rows of 4096 x 11008 35 and 18.5, 5
+// TB/s), where the tiles take 20.6 and 14.6.  The short ones do not fill the chip: 352
+// and 128 workgroups, one and a half rounds of 256 CUs and half of one.
 template <class T, int NP>
 int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
   const int64_t C = d.members, R = d.rows, D = d.n_in, F = d.n_hidden, O = d.n_out, F8 = round8(F);
   const Kept<NP> k(d);
   T* h = d.kept ? reinterpret_cast<T*>(const_cast<__bf16*>(k.h.p)) : ws.take<T>(C * R * F8);
+  const bool two = NP == 1 && R <= 8;
+  T* lo = two ? ws.take<T>(C * R * F8) : nullptr;
   *bytes = ws.used;
   if (dry || R == 0) return 0;
   thin::GateArgs<T> a{};
@@ -337,6 +340,7 @@ int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t st
   a.g = k.g;
   a.u = k.u;
   a.h = h;
+  a.lo = lo;
   a.ld = F8;
   a.R = (int32_t)R;
   a.D = (int32_t)D;
@@ -350,6 +354,7 @@ int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t st
   D3A_LAUNCH_CHECK("gated_mlp");
   thin::DownArgs<T> b{};
   b.h = h;
+  b.lo = lo;
   b.W = static_cast<const T*>(d.Wd);
   b.b = static_cast<const T*>(d.bd);
   b.y = static_cast<T*>(d.y);
@@ -359,8 +364,14 @@ int forward_thin(const d3a_gated_mlp_desc& d, Arena ws, bool dry, hipStream_t st
   b.R = (int32_t)R;
   b.F = (int32_t)F;
   b.O = (int32_t)O;
-  if (whole<T>(d.Wd, b.ldw, b.sw, F)) thin::down_kernel<T, true><<<down, 1024, 0, stream>>>(b);
-  else thin::down_kernel<T, false><<<down, 1024, 0, stream>>>(b);
+  const bool vec = whole<T>(d.Wd, b.ldw, b.sw, F);
+  if (!two) {
+    if (vec) thin::down_kernel<T, true, 1><<<down, 1024, 0, stream>>>(b);
+    else thin::down_kernel<T, false, 1><<<down, 1024, 0, stream>>>(b);
+  } else if constexpr (NP == 1) {
+    if (vec) thin::down_kernel<T, true, 2><<<down, 1024, 0, stream>>>(b);
+    else thin::down_kernel<T, false, 2><<<down, 1024, 0, stream>>>(b);
+  }
   D3A_LAUNCH_CHECK("gated_mlp");
   return 0;
 }

@@ -6,6 +6,14 @@
 // the instruction's first operand, x's its second; which k a lane group holds
 // is free as long as both agree, so a lane reads 16 bytes of its row.
 // bfloat16 on v_mfma_f32_16x16x32_bf16, float32 on v_mfma_f32_16x16x4_f32.
+//
+// With bfloat16 tensors and at most eight rows h = act(g) u goes to the down product
+// as two bfloat16 parts, to 2^-16 of it: one part alone would be off by up to 2^-8, the
+// largest error of the call.  The second parts are the matrix instruction's other
+// eight rows, where they cost nothing: one row of 2048 x 5632 takes 20.4 us either way,
+// four of 4096 x 11008 53 to 54.  More rows have one part, as a batch has: there h's
+// bytes bound the down product, and two parts take 16 rows from 26.3 us to 31.0, of
+// 4096 x 11008 from 61 to 73.
 #pragma once
 
 #include "mm.hpp"
@@ -77,7 +85,7 @@ struct GateArgs {
   const T *x, *Wg, *Wu, *bg, *bu;
   int64_t ldx, sx, ldg, sg, ldu, su;
   float *g, *u;           // kept, or null
-  T* h;                   // [members][R] rows of ld, zero past F
+  T *h, *lo;              // [members][R] rows of ld, zero past F; lo: the second part, or null
   int64_t ld;
   int32_t R, D, F, act;
 };
@@ -121,22 +129,31 @@ __global__ __launch_bounds__(512) void gate_kernel(const GateArgs<T> A, Act acti
     *reinterpret_cast<f32x4*>(A.g + at) = acc[0];
     *reinterpret_cast<f32x4*>(A.u + at) = acc[1];
   }
-  if constexpr (sizeof(T) == 4)
+  if constexpr (sizeof(T) == 4) {
     mm::store4(A.h + at, h);
-  else
-    *reinterpret_cast<bf16x4*>(A.h + at) = bf16x4{(__bf16)h[0], (__bf16)h[1], (__bf16)h[2], (__bf16)h[3]};
+  } else {
+    bf16x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = (__bf16)h[i];
+      const float left = h[i] - (float)hi[i];
+      lo[i] = (__bf16)(fabsf(left) < INFINITY ? left : 0.f);  // (an infinity is its first part's)
+    }
+    *reinterpret_cast<bf16x4*>(A.h + at) = hi;
+    if (A.lo) *reinterpret_cast<bf16x4*>(A.lo + at) = lo;
+  }
 }
 
 template <class T>
 struct DownArgs {
-  const T *h, *W, *b;
+  const T *h, *lo, *W, *b;
   T* y;  // [members][R][O]
   int64_t ld, ldw, sw;
   int32_t R, F, O;
 };
 
-// grid (16 outputs, members), 16 waves
-template <class T, bool VEC>
+// grid (16 outputs, members), 16 waves; PARTS: h's, two of at most eight rows
+template <class T, bool VEC, int PARTS>
 __global__ __launch_bounds__(1024) void down_kernel(const DownArgs<T> A) {
   constexpr int WAVES = 16, N = Piece<T>::N, KP = Piece<T>::K;
   __shared__ f32x4 red[WAVES * 64];
@@ -144,16 +161,23 @@ __global__ __launch_bounds__(1024) void down_kernel(const DownArgs<T> A) {
   const int64_t c = blockIdx.y;
   const int n0 = blockIdx.x * 16, row = lane & 15, k0 = (lane >> 4) * N;
   const T* wd = A.W + c * A.sw + (int64_t)min(n0 + row, A.O - 1) * A.ldw;
-  const T* h = A.h + (c * A.R + row) * A.ld;
+  const int hrow = PARTS == 2 ? row & 7 : row;
+  const bool on = hrow < A.R;
+  const int64_t at = (c * A.R + hrow) * A.ld;
+  const T* h = (PARTS == 2 && row >= 8 ? A.lo : A.h) + at;
   f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll 4
   for (int k = w * KP; k < A.F; k += WAVES * KP) {
     const Piece<T> a = load<T, VEC>(wd, k + k0, A.F, true);
-    const Piece<T> v = load<T, true>(h, k + k0, (int)A.ld, row < A.R);
+    const Piece<T> v = load<T, true>(h, k + k0, (int)A.ld, on);
     acc[0] = product(a, v, acc[0]);
   }
   join<1, WAVES>(acc, red);
-  if (w != 0 || row >= A.R) return;
+  if (w != 0) return;
+  if constexpr (PARTS == 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[0][i] += __shfl_xor(acc[0][i], 8);
+  if (row >= A.R) return;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int n = n0 + 4 * (lane >> 4) + i;

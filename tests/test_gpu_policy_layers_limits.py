@@ -9,7 +9,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from policy_layer_helpers import U, within, xent_reference
+from policy_layer_helpers import U, acc, within, xent_reference
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -117,3 +117,40 @@ def test_cross_entropy_lse_and_its_low_part(T):
     count = torch.bincount(t[t >= 0], minlength=50).double()
     # every row's p is off by the same factor, exp(2^-24 |lse|) at most
     within(db, 19 * p - count, 19 * p * (1.1 * U * 1e5) + 64 * U * (19 * p + count), "b")
+
+
+# ------------------------------------------------------------- gated block, few rows
+@pytest.mark.parametrize("R,D,F,O", [(1, 64, 512, 48), (1, 256, 2816, 256), (5, 33, 1041, 70),
+                                     (8, 72, 1100, 24)])
+@pytest.mark.parametrize("C", [0, 3])
+@pytest.mark.parametrize("train", [False, True])
+def test_few_rows_are_rounded_once(T, R, D, F, O, C, train):
+    """bfloat16, up to eight rows: y is float32's value rounded to bfloat16, with h held
+    to 2^-16 in between (one bfloat16 h would be 2^-8 off, and sums of it are more than
+    y's own rounding wherever y is small)."""
+    lead = (C,) if C else ()
+    x = rnd(1, *lead, R, D, dtype=BF16)
+    Wg, Wu = (rnd(k, *lead, F, D, dtype=BF16, scale=D ** -0.5) for k in (2, 3))
+    Wd = rnd(4, *lead, O, F, dtype=BF16, scale=F ** -0.5)
+    bd = rnd(5, *lead, O, dtype=BF16)
+    got = T.gated_mlp(x.requires_grad_(train), Wg, Wu, Wd, None, None, bd)
+    x, Wg, Wu, Wd, bd = (t.detach().double() for t in (x, Wg, Wu, Wd, bd))
+    g, u = x @ Wg.mT.contiguous(), x @ Wu.mT.contiguous()
+    e_g = acc(D) * (x.abs() @ Wg.abs().mT.contiguous()) + 2 * U * g.abs()
+    e_u = acc(D) * (x.abs() @ Wu.abs().mT.contiguous()) + 2 * U * u.abs()
+    a = g * torch.sigmoid(g)
+    h = a * u
+    e_h = (1.1 * e_g + 8 * U * (a.abs() + g.abs())) * u.abs() + a.abs() * e_u \
+        + (2 * U + 2.0 ** -16) * h.abs()
+    WdT = Wd.mT.contiguous()
+    y = h @ WdT + bd.unsqueeze(-2)
+    bound = (e_h @ WdT.abs() + 2 * acc(F) * (h.abs() @ WdT.abs()) + (2 * U + 2.0 ** -8) * y.abs())
+    within(got, y, bound, "y")
+
+
+def test_few_rows_with_an_infinite_hidden_value(T):
+    """An infinity of h is one of y, not NaN from its second part."""
+    x = torch.ones(2, 8, device=DEV, dtype=BF16)
+    W = torch.full((16, 8), 1e30, device=DEV, dtype=BF16)
+    Wd = torch.full((8, 16), 0.5, device=DEV, dtype=BF16)
+    assert T.gated_mlp(x, W, W, Wd).isposinf().all()
