@@ -10,8 +10,9 @@
 // transposed by the LDS reads.  A bfloat16 operand has one plane; a float32
 // operand is given as its exact three-way bf16 split (three planes, see pack_kernel),
 // and a k step then takes the six part products that matter, smallest first: fp32
-// accuracy at six bf16 products a term.  (An infinity, or a value that rounds to one
-// in bfloat16, has NaN parts: its row's or column's results are NaN.)
+// accuracy at six bf16 products a term.  (An infinity has NaN parts: its row's or
+// column's results are NaN.  The third part of a value under 2^-110 falls under
+// bfloat16's smallest, 2^-133, and so does what is lost of it.)
 //
 // Bound by the matrix cores: 32768 x 1024 x 8192 in bfloat16 takes 373 us (1.47
 // PFLOP/s), 8192 x 1024 x 4096 58 (1.19), 4096 cubed in float32 539 (255 TFLOP/s of
@@ -477,9 +478,12 @@ int launch(Launch<Epi>& L, hipStream_t stream, const char* what) {
   return 0;
 }
 
-// the exact split of a float32 value in three bfloat16 parts
+// The split of a float32 value in three bfloat16 parts, exact from 2^-110 up.  (Values
+// above the largest bfloat16 would round to an infinity: their first part is the
+// largest.  NaN and infinities have NaN among their parts.)
 __device__ __forceinline__ void split3(float x, __bf16& p0, __bf16& p1, __bf16& p2) {
-  p0 = (__bf16)x;
+  constexpr float kLargest = 3.38953139e38f;  // 2^128 - 2^120
+  p0 = (__bf16)__builtin_amdgcn_fmed3f(x, -kLargest, kLargest);
   const float r = x - (float)p0;
   p1 = (__bf16)r;
   p2 = (__bf16)(r - (float)p1);

@@ -212,7 +212,11 @@ def gated_mlp(x: torch.Tensor, Wg: torch.Tensor, Wu: torch.Tensor, Wd: torch.Ten
     (-> [members, rows, out]).  ``activation``: 'silu', 'gelu' (the erf form) or
     'relu'.  float32 (products to float32 accuracy) or bfloat16 (sums in
     float32), one dtype for all.  Where a gradient is wanted the forward keeps
-    both pre-activations for the backward."""
+    both pre-activations for the backward.
+
+    float32 values are multiplied as three bfloat16 parts: an infinity in ``x`` or a
+    weight gives NaN in the outputs it takes part in (up to 16 rows, forward, what
+    float32 products give)."""
     return load().gated_mlp(x, Wg, Wu, Wd, bg, bu, bd, activation, False)[0]
 
 
@@ -228,5 +232,7 @@ def linear_cross_entropy(x: torch.Tensor, W: torch.Tensor, target: torch.Tensor,
     bfloat16; ``target`` [..] int64.  The loss is float32.  A row whose target
     is ``ignore_index`` has loss 0 and no gradient; 'mean' is over the other
     rows (0 where there are none).  A target outside the vocabulary gives NaN.
-    (W's gradient has the ignored rows' x times 0: padding has to be finite.)"""
+    (W's gradient has the ignored rows' x times 0: padding has to be finite.  float32
+    values are multiplied as three bfloat16 parts: an infinity in ``x`` or ``W`` gives
+    NaN in the rows it takes part in; ``b`` may be infinite.)"""
     return load().linear_cross_entropy(x, W, target, b, ignore_index, reduction)[0]

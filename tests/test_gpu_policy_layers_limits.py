@@ -9,7 +9,7 @@ import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from policy_layer_helpers import U, acc, within, xent_reference
+from policy_layer_helpers import U, acc, gated_reference, within, xent_reference
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -154,3 +154,50 @@ def test_few_rows_with_an_infinite_hidden_value(T):
     W = torch.full((16, 8), 1e30, device=DEV, dtype=BF16)
     Wd = torch.full((8, 16), 0.5, device=DEV, dtype=BF16)
     assert T.gated_mlp(x, W, W, Wd).isposinf().all()
+
+
+# --------------------------------------------------------------- float32's whole range
+def largest_inputs(R, D, N):
+    """x whose first feature is float32's largest value, of either sign, times 2^-125
+    in the weight: 8 in every product, exact, of operands that bfloat16 would round to
+    infinities; the other features are ordinary."""
+    x, W = rnd(1, R, D), rnd(2, N, D, scale=D ** -0.5)
+    x[:, 0] = torch.finfo(F32).max
+    x[1::2, 0] = -torch.finfo(F32).max
+    W[:, 0] = 2.0 ** -125
+    return x, W
+
+
+@pytest.mark.parametrize("F", [72, 1100])  # products from the tensors, tiles
+def test_gated_mlp_of_the_largest_values(T, F):
+    R, D, O = 40, 24, 16
+    x, Wg = largest_inputs(R, D, F)
+    Wu, Wd, dy = rnd(3, F, D, scale=D ** -0.5), rnd(4, O, F, scale=F ** -0.5), rnd(5, R, O)
+    Wu[:, 0] = 2.0 ** -126
+    p = {"x": x, "Wg": Wg, "Wu": Wu, "Wd": Wd}
+    q = {k: v.detach().requires_grad_(k in ("x", "Wd")) for k, v in p.items()}
+    y = T.gated_mlp(*q.values())
+    dx, dWd = torch.autograd.grad(y, [q["x"], q["Wd"]], dy)
+    check({"y": y, "x": dx, "Wd": dWd}, gated_reference(p, dy, "silu"), ("y", "x", "Wd"))
+
+
+@pytest.mark.parametrize("V", [77, 2201])
+def test_cross_entropy_of_the_largest_values(T, V):
+    x, W = largest_inputs(30, 24, V)
+    t = torch.arange(30, device=DEV) % V
+    q = x.detach().requires_grad_(True)
+    loss = T.linear_cross_entropy(q, W, t)
+    (dx,) = torch.autograd.grad(loss, [q])
+    check({"loss": loss, "x": dx}, xent_reference(x, W, None, t, -100, "mean", 1.0), ("loss", "x"))
+
+
+@pytest.mark.parametrize("V", [77, 2201])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_float32_infinities_spoil_their_rows_alone(T, V, bad):
+    x, W, t = rnd(1, 30, 24), rnd(2, V, 24), torch.arange(30, device=DEV)
+    x[7, 3] = bad
+    loss = T.linear_cross_entropy(x, W, t, reduction="none")
+    assert loss[7].isnan()
+    rest = torch.arange(30, device=DEV) != 7
+    want = T.linear_cross_entropy(x[rest], W, t[rest], reduction="none")
+    assert torch.equal(loss[rest], want)
