@@ -308,10 +308,10 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(const Args A) {
 // dw, db of a member: 64 of its 2 n columns a workgroup, the parts over sixteen
 // waves
 template <class W>
-__global__ __launch_bounds__(1024) void norm_finish_kernel(const Args A, int32_t parts) {
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const Args A, int32_t parts, int64_t first) {
   __shared__ float red[1024];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane, c = blockIdx.y;
+  const int64_t col = (first + blockIdx.x) * 64 + lane, c = blockIdx.y;
   const int64_t n = A.n;
   float s = 0.f;
   if (col < 2 * n) {
@@ -332,9 +332,9 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const Args A, int32_t
 
 // rows too long for four waves' registers: a workgroup a row, in passes
 template <class T, class W>
-__global__ __launch_bounds__(256) void norm_long_kernel(const Args A) {
+__global__ __launch_bounds__(256) void norm_long_kernel(const Args A, int64_t first) {
   __shared__ float scratch[4];
-  const int64_t row = blockIdx.x, c = row / A.rows, r = row - c * A.rows;
+  const int64_t row = first + blockIdx.x, c = row / A.rows, r = row - c * A.rows;
   const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
   const W* w = static_cast<const W*>(A.w) + c * A.n;
   const W* b = static_cast<const W*>(A.b) + c * A.n;
@@ -357,9 +357,9 @@ __global__ __launch_bounds__(256) void norm_long_kernel(const Args A) {
 }
 
 template <class T, class W>
-__global__ __launch_bounds__(256) void norm_long_dx_kernel(const Args A) {
+__global__ __launch_bounds__(256) void norm_long_dx_kernel(const Args A, int64_t first) {
   __shared__ float scratch[8];
-  const int64_t row = blockIdx.x, c = row / A.rows, r = row - c * A.rows;
+  const int64_t row = first + blockIdx.x, c = row / A.rows, r = row - c * A.rows;
   const T* x = static_cast<const T*>(A.x) + c * A.sx + r * A.ldx;
   const T* dy = static_cast<const T*>(A.dy) + c * A.sdy + r * A.lddy;
   const W* w = static_cast<const W*>(A.w) + c * A.n;
@@ -381,10 +381,10 @@ __global__ __launch_bounds__(256) void norm_long_dx_kernel(const Args A) {
 
 // partials of dw, db: 64 columns x a chunk of rows (grid x: columns, y: chunks, z: members)
 template <class T>
-__global__ __launch_bounds__(256) void norm_long_cols_kernel(const Args A) {
+__global__ __launch_bounds__(256) void norm_long_cols_kernel(const Args A, int64_t first) {
   __shared__ float red[2][256];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * 64 + lane, c = blockIdx.z;
+  const int64_t col = (first + blockIdx.x) * 64 + lane, c = blockIdx.z;
   const int64_t per = (A.rows + gridDim.y - 1) / gridDim.y, r0 = per * blockIdx.y;
   const int64_t r1 = min(r0 + per, A.rows);
   float dw = 0.f, db = 0.f;
@@ -506,14 +506,26 @@ int dispatch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, hipStream_t 
   return launch<T, W, 1, 8, 1>(d, a, bwd, s);
 }
 
+// f(first, workgroups) over `all` workgroups of `threads`: a launch holds less than
+// 2^32 threads an axis
+template <class F>
+int in_launches(int64_t all, int64_t threads, const char* what, const F& f) {
+  const int64_t most = (1LL << 31) / threads;
+  for (int64_t first = 0; first < all; first += most) {
+    f(first, (unsigned)std::min(all - first, most));
+    D3A_LAUNCH_CHECK(what);
+  }
+  return 0;
+}
+
 template <class T, class W>
 int forward(const d3a_layer_norm_desc& d, hipStream_t stream) {
   const Args a = args_of(d);
   if (d.rows == 0) return 0;
   if (d.n <= kLong) return dispatch<T, W>(d, a, false, stream);
-  norm_long_kernel<T, W><<<(unsigned)(d.rows * d.members), 256, 0, stream>>>(a);
-  D3A_LAUNCH_CHECK("layer_norm");
-  return 0;
+  return in_launches(d.rows * d.members, 256, "layer_norm", [&](int64_t first, unsigned n) {
+    norm_long_kernel<T, W><<<n, 256, 0, stream>>>(a, first);
+  });
 }
 
 int64_t long_chunks(const d3a_layer_norm_desc& d) {
@@ -530,23 +542,21 @@ int backward(const d3a_layer_norm_desc& d, Arena ws, bool dry, hipStream_t strea
   *bytes = ws.used;
   if (dry || (!cols && (!d.dx || d.rows == 0))) return 0;
   if (is_long) {
-    if (d.dx && d.rows > 0) {
-      norm_long_dx_kernel<T, W><<<(unsigned)(d.rows * d.members), 256, 0, stream>>>(a);
-      D3A_LAUNCH_CHECK("layer_norm_bwd");
-    }
-    if (cols) {
-      norm_long_cols_kernel<T><<<dim3((unsigned)((d.n + 63) / 64), (unsigned)parts, (unsigned)d.members), 256, 0,
-                                 stream>>>(a);
-      D3A_LAUNCH_CHECK("layer_norm_bwd");
-    }
+    if (d.dx && in_launches(d.rows * d.members, 256, "layer_norm_bwd", [&](int64_t first, unsigned n) {
+          norm_long_dx_kernel<T, W><<<n, 256, 0, stream>>>(a, first);
+        }) != 0)
+      return -1;
+    if (cols && in_launches((d.n + 63) / 64, 256, "layer_norm_bwd", [&](int64_t first, unsigned n) {
+          norm_long_cols_kernel<T><<<dim3(n, (unsigned)parts, (unsigned)d.members), 256, 0, stream>>>(a, first);
+        }) != 0)
+      return -1;
   } else {
     if (dispatch<T, W>(d, a, true, stream) != 0) return -1;
   }
   if (!cols) return 0;
-  norm_finish_kernel<W><<<dim3((unsigned)((2 * d.n + 63) / 64), (unsigned)d.members), 1024, 0, stream>>>(
-      a, (int32_t)parts);
-  D3A_LAUNCH_CHECK("layer_norm_bwd");
-  return 0;
+  return in_launches((2 * d.n + 63) / 64, 1024, "layer_norm_bwd", [&](int64_t first, unsigned n) {
+    norm_finish_kernel<W><<<dim3(n, (unsigned)d.members), 1024, 0, stream>>>(a, (int32_t)parts, first);
+  });
 }
 
 int call_bwd(const d3a_layer_norm_desc* d, bool dry, hipStream_t stream, int64_t* bytes) {

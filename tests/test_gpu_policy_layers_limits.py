@@ -201,3 +201,33 @@ def test_float32_infinities_spoil_their_rows_alone(T, V, bad):
     rest = torch.arange(30, device=DEV) != 7
     want = T.linear_cross_entropy(x[rest], W, t[rest], reduction="none")
     assert torch.equal(loss[rest], want)
+
+
+# ------------------------------------------------------------------ layer norm, long rows
+def test_layer_norm_of_more_columns_than_a_launch_has_threads(T):
+    """2^27 columns, of which the pass that adds their sums has 32 threads each, are 2^32
+    threads."""
+    n = (1 << 27) + 3
+    x, dy = (torch.randn(1, n, device=DEV, generator=torch.Generator(DEV).manual_seed(k))
+             for k in (1, 2))
+    w, b = (torch.randn(n, device=DEV, generator=torch.Generator(DEV).manual_seed(k))
+            for k in (3, 4))
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = T.layer_norm(*leaves, 1e-5)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    y, x, w, b = (t.detach() for t in (y, x, w, b))
+    # one row: b's gradient is dy itself, w's dy xh; the statistics are sums of 2^19
+    # values a lane, (2^19 + 80) 2^-24 of their mean magnitude
+    assert torch.equal(db, dy[0])
+    mean = x.double().mean()
+    var = ((x - mean) ** 2).double().mean()
+    rstd = 1 / (var + 1e-5).sqrt()
+    u = ((1 << 19) + 80) * U
+    e_mean, e_rstd = u * x.abs().double().mean(), rstd * u * 2
+    for part in (slice(0, 4096), slice((1 << 26) - 2048, (1 << 26) + 2048), slice(n - 4096, n)):
+        xh = (x[0, part].double() - mean) * rstd
+        e_xh = e_mean * rstd + xh.abs() * (e_rstd / rstd + 8 * U)
+        within(dw[part], dy[0, part] * xh, (dy[0, part].abs() * (e_xh + 4 * U * xh.abs())), "weight")
+        want = xh * w[part] + b[part]
+        within(y[0, part], want, e_xh * w[part].abs() + 4 * U * (want.abs() + (xh * w[part]).abs()), "y")
+    assert torch.isfinite(dx).all()
