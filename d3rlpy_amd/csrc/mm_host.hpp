@@ -158,6 +158,7 @@ struct ColsumJobs {
   float* part;                    // [chunks][quads][4]
   int64_t first[kMaxColsum + 1];  // running count of batch * quads of columns
   int32_t n, chunks;
+  int32_t all;                    // chunks of all blocks of rows (chunks: of one)
 };
 
 // the job that quad q of all belongs to, its batch and its first column there
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const ColsumJobs J) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += red[64 * k + lane][e];
   const float v[4] = {s[0], s[1], s[2], s[3]};
-  if (J.chunks == 1) colsum_store<T>(j, b, col, v);
+  if (J.all == 1) colsum_store<T>(j, b, col, v);
   else store4(J.part + (blockIdx.y * quads + q) * 4, v);
 }
 
@@ -228,7 +229,7 @@ __global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs J) {
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (q < quads)
 #pragma unroll 4
-    for (int k = w; k < J.chunks; k += 16) {
+    for (int k = w; k < J.all; k += 16) {
       float v[4];
       load4(J.part + (k * quads + q) * 4, v);
 #pragma unroll
@@ -247,42 +248,50 @@ __global__ __launch_bounds__(1024) void colsum_finish(const ColsumJobs J) {
   colsum_store<T>(j, b, col, v);
 }
 
+// Rows that come in `blocks` of the same buffer: one add() and one reserve(), then a
+// launch(stream, k) for each, the last of which adds them all up.
 template <class T, int NP>
 struct Colsum {
   ColsumJobs jobs{};
   bool from_epilogue = false;
+  int64_t blocks = 1;
   void add(const Operand& o, int64_t rows, int64_t cols, int64_t batch, void* out, Factor factor = {}) {
     jobs.j[jobs.n] = ColsumJob{o.p, o.ld, o.s_batch, o.s_part, out, (int32_t)rows, (int32_t)cols, (int32_t)batch, factor};
     jobs.first[jobs.n + 1] = jobs.first[jobs.n] + batch * ((cols + 3) / 4);
     ++jobs.n;
     // about 768 workgroups, chunks of at least 64 rows (four a wave)
-    const int64_t blocks = (jobs.first[jobs.n] + 63) / 64;
+    const int64_t wide = (jobs.first[jobs.n] + 63) / 64;
     jobs.chunks = rows <= 512 ? 1
                               : (int32_t)std::max<int64_t>(
-                                    1, std::min<int64_t>({768 / std::max<int64_t>(blocks, 1), rows / 64, 256}));
+                                    1, std::min<int64_t>({768 / std::max<int64_t>(wide, 1), rows / 64, 256}));
+    jobs.all = (int32_t)(jobs.chunks * blocks);
   }
   // instead of add(): the chunks' sums come from an epilogue, [chunks][quads][4]
   float* given(int64_t cols, int32_t chunks, void* out, Factor factor, Arena& ws) {
     jobs.j[0] = ColsumJob{nullptr, 0, 0, 0, out, 0, (int32_t)cols, 1, factor};
     jobs.first[1] = (cols + 3) / 4;
     jobs.n = 1;
-    jobs.chunks = chunks;
+    jobs.chunks = jobs.all = chunks;
     from_epilogue = true;
     return jobs.part = ws.take<float>(chunks * jobs.first[1] * 4);
   }
   void reserve(Arena& ws) {
-    if (jobs.n && !from_epilogue && jobs.chunks > 1) jobs.part = ws.take<float>(jobs.chunks * jobs.first[jobs.n] * 4);
+    if (jobs.n && !from_epilogue && jobs.all > 1) jobs.part = ws.take<float>(jobs.all * jobs.first[jobs.n] * 4);
   }
-  int launch(hipStream_t stream) {
+  // the rows of job 0 in this block
+  void set_rows(int64_t rows) { jobs.j[0].rows = (int32_t)rows; }
+  int launch(hipStream_t stream, int64_t k = 0) {
     const int64_t quads = jobs.first[jobs.n];
     if (jobs.n == 0 || quads == 0) return 0;
-    const unsigned blocks = (unsigned)((quads + 63) / 64);
+    const unsigned wide = (unsigned)((quads + 63) / 64);
     if (!from_epilogue) {
-      colsum_kernel<T, NP><<<dim3(blocks, jobs.chunks), 1024, 0, stream>>>(jobs);
+      ColsumJobs block = jobs;
+      if (jobs.all > 1) block.part += k * jobs.chunks * quads * 4;
+      colsum_kernel<T, NP><<<dim3(wide, jobs.chunks), 1024, 0, stream>>>(block);
       D3A_LAUNCH_CHECK("column sums");
-      if (jobs.chunks == 1) return 0;
+      if (jobs.all == 1 || k + 1 < blocks) return 0;
     }
-    colsum_finish<T><<<blocks, 1024, 0, stream>>>(jobs);
+    colsum_finish<T><<<wide, 1024, 0, stream>>>(jobs);
     D3A_LAUNCH_CHECK("column sums");
     return 0;
   }

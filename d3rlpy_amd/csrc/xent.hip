@@ -14,8 +14,11 @@
 // reduces each of its rows to (max, sum of exp(z - max)) and picks the
 // target's logit, and a second pass joins the tiles of a row.  Backward: the
 // logits again, a piece of the vocabulary at a time, whose epilogue writes dz
-// of the piece in the operand layout of the two products that follow; the
-// piece is cut so that dz stays within kPieceBytes.  All products are bound by
+// of the piece in the operand layout of the two products that follow.  Neither grows
+// with rows x vocabulary: the forward's parts and dz stay within kPieceBytes each, by
+// cutting first the vocabulary (backward) and then the rows.  What does grow: the
+// operands' packed copies, with x and W; a float32 sum of dx, with x, where there are
+// several pieces.  All products are bound by
 // the matrix cores, and their epilogues by the exponentials: 8192 x 1024 -> 32768 in
 // bfloat16 takes 510 to 650 us for the logits' sums, 635 to 730 for dz, 475 to 530 for dx and
 // 460 to 505 for dW, of 550 GFLOP each; 1500 x 777 -> 10007 in float32 146, 152, 141, 176.
@@ -33,6 +36,15 @@ namespace {
 using namespace mm;
 
 constexpr int64_t kPieceBytes = 512LL << 20;
+
+// The size of equal parts of `all`: all of it if that is at most `most`, else a multiple
+// of the widest tile's 256, at most `most` (or 256).
+int64_t equal_parts(int64_t all, int64_t most) {
+  if (all <= most) return all;
+  most = std::max<int64_t>(most / 256 * 256, 256);
+  const int64_t n = (all + most - 1) / most;
+  return ((all + n - 1) / n + 255) / 256 * 256;
+}
 
 // exp(z - ref).  (With bfloat16 tensors the hardware's exponential, within 2 ulp
 // and a product's rounding of its argument, is far below dz's own rounding and no
@@ -437,9 +449,33 @@ int wave_rows(TileSize s) {
   return s == kLarge ? X::Large::TM : s == kMid ? X::Mid::TM : X::Small::TM;
 }
 
-// the rows' lse and loss from their parts, and the reduction
+// lse and loss of n rows from r0 on, from their parts
 // (of kJoinRows at a time: a launch holds less than 2^32 threads)
 constexpr int64_t kJoinRows = 1 << 26;
+int join(const d3a_linear_xent_desc& d, int64_t r0, int64_t n, const float2* part, int64_t parts,
+         const float* ztarget, hipStream_t stream) {
+  const int64_t* target = d.target + r0;
+  float *lse = d.lse + r0, *low = d.low ? d.low + r0 : nullptr, *loss = d.loss + r0;
+  if (n <= 256 && parts >= 512)
+    lse_join_wide_kernel<<<(unsigned)n, 256, 0, stream>>>(part, (int32_t)parts, (int32_t)n, ztarget, target, d.vocab,
+                                                          d.ignore_index, lse, low, loss);
+  else
+    for (int64_t at = 0; at < n; at += kJoinRows)
+      lse_join_kernel<<<(unsigned)((std::min(n - at, kJoinRows) + 7) / 8), 256, 0, stream>>>(
+          part, (int32_t)parts, (int32_t)n, ztarget, target, d.vocab, d.ignore_index, lse, low, loss, (int32_t)at);
+  D3A_LAUNCH_CHECK("linear_cross_entropy");
+  return 0;
+}
+
+int reduce(const d3a_linear_xent_desc& d, hipStream_t stream) {
+  if (d.reduction == 0) return 0;
+  loss_reduce_kernel<<<1, 1024, 0, stream>>>(d.loss, d.target, d.ignore_index, (int32_t)d.rows, d.reduction == 1,
+                                             d.out, d.scale);
+  D3A_LAUNCH_CHECK("linear_cross_entropy");
+  return 0;
+}
+
+// both, of all rows
 int finish(const d3a_linear_xent_desc& d, const float2* part, int64_t parts, const float* ztarget,
            hipStream_t stream) {
   const int64_t R = d.rows;
@@ -449,23 +485,8 @@ int finish(const d3a_linear_xent_desc& d, const float2* part, int64_t parts, con
     D3A_LAUNCH_CHECK("linear_cross_entropy");
     return 0;
   }
-  if (R > 0) {
-    if (R <= 256 && parts >= 512)
-      lse_join_wide_kernel<<<(unsigned)R, 256, 0, stream>>>(part, (int32_t)parts, (int32_t)R, ztarget, d.target,
-                                                            d.vocab, d.ignore_index, d.lse, d.low, d.loss);
-    else
-      for (int64_t r0 = 0; r0 < R; r0 += kJoinRows)
-        lse_join_kernel<<<(unsigned)((std::min(R - r0, kJoinRows) + 7) / 8), 256, 0, stream>>>(
-            part, (int32_t)parts, (int32_t)R, ztarget, d.target, d.vocab, d.ignore_index, d.lse, d.low, d.loss,
-            (int32_t)r0);
-    D3A_LAUNCH_CHECK("linear_cross_entropy");
-  }
-  if (d.reduction != 0) {
-    loss_reduce_kernel<<<1, 1024, 0, stream>>>(d.loss, d.target, d.ignore_index, (int32_t)R, d.reduction == 1, d.out,
-                                               d.scale);
-    D3A_LAUNCH_CHECK("linear_cross_entropy");
-  }
-  return 0;
+  if (R > 0 && join(d, 0, R, part, parts, ztarget, stream) != 0) return -1;
+  return reduce(d, stream);
 }
 
 template <class T>
@@ -520,7 +541,7 @@ int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t strea
   Launch<LsePartEpi<T, NP>> L{};
   L.n = 1;
   Problem& p = L.p[0];
-  p.a = pack.operand(d.x, d.ldx, 0, 1, R, D);
+  const Operand x = pack.operand(d.x, d.ldx, 0, 1, R, D);
   p.b = pack.operand(d.W, d.ldW, 0, 1, V, D);
   p.M = (int32_t)R;
   p.N = (int32_t)V;
@@ -529,19 +550,26 @@ int forward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t strea
   const TileSize size = choose<NP>(L, false).size;
   const int cols = wave_columns<NP>(size);
   const int64_t parts = (V + cols - 1) / cols;
+  // (a wave's 64 columns are 8 bytes: rows are cut from 2^32 logits on)
+  const int64_t block = equal_parts(R, kPieceBytes / (parts * (int64_t)sizeof(float2)));
   LsePartEpi<T, NP>& e = L.e[0];
   e.bias = static_cast<const T*>(d.b);
-  e.target = d.target;
-  e.part = ws.take<float2>(parts * R);
-  e.ztarget = ws.take<float>(R);
+  e.part = ws.take<float2>(parts * block);
+  e.ztarget = ws.take<float>(block);
   e.wave_cols = cols;
   *bytes = ws.used;
   if (dry) return 0;
-  if (R > 0) {
-    if (pack.launch(stream) != 0) return -1;
+  if (R > 0 && pack.launch(stream) != 0) return -1;
+  for (int64_t r0 = 0; r0 < R; r0 += block) {
+    // (the blocks reuse one workspace: a stream runs them in order)
+    p.a = x;
+    p.a.p += r0 * x.ld;
+    p.M = (int32_t)std::min(block, R - r0);
+    e.target = d.target + r0;
     if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy") != 0) return -1;
+    if (block < R && join(d, r0, p.M, e.part, parts, e.ztarget, stream) != 0) return -1;
   }
-  return finish(d, e.part, parts, e.ztarget, stream);
+  return block < R ? reduce(d, stream) : finish(d, e.part, parts, e.ztarget, stream);
 }
 
 template <class T, int NP>
@@ -556,76 +584,95 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
   Packer<T, NP> pack(ws);
   const Operand x = pack.operand(d.x, d.ldx, 0, 1, R, D);
   const Operand w = pack.operand(d.W, d.ldW, 0, 1, V, D);
-  // pieces of equal size, multiples of the widest tile
-  int64_t piece = std::max<int64_t>(kPieceBytes / (2 * NP * std::max<int64_t>(R, 1)), 256);
-  piece = std::min(piece, kMaxWidth);
-  const int64_t n_pieces = (V + piece - 1) / piece;
-  piece = std::min<int64_t>(V, ((V + n_pieces - 1) / n_pieces + 255) / 256 * 256);
-  const int64_t ld = round8(piece);
+  // pieces of the vocabulary; where all rows of 256 columns are too much, blocks of rows
+  const int64_t most = kPieceBytes / (2 * NP * std::max<int64_t>(R, 1)) / 256 * 256;
+  const int64_t piece = equal_parts(V, std::min(std::max<int64_t>(most, 256), kMaxWidth));
+  const int64_t ld = round8(piece), block = equal_parts(R, kPieceBytes / (2 * NP * ld));
+  const int64_t n_pieces = (V + piece - 1) / piece, n_blocks = R > 0 ? (R + block - 1) / block : 1;
   Operand dz{};
-  dz.p = ws.take<__bf16>(NP * R * ld);
+  dz.p = ws.take<__bf16>(NP * block * ld);
   dz.ld = ld;
-  dz.s_part = R * ld;
+  dz.s_part = block * ld;
   float* sum = n_pieces > 1 && d.dx ? ws.take<float>(R * round8(D)) : nullptr;
+  float* sum_w = n_blocks > 1 && d.dW ? ws.take<float>(piece * round8(D)) : nullptr;
   const int64_t keep = ws.used;
   if (!dry && R > 0 && pack.launch(stream) != 0) return -1;
   for (int64_t v0 = 0, k = 0; v0 < V; v0 += piece, ++k) {
-    // (the pieces reuse one workspace: a stream runs them in order)
-    ws.used = keep;
     const int64_t n = std::min(piece, V - v0);
-    const bool last = v0 + n == V;
-    Launch<DzEpi<T, NP>> L{};
-    L.n = 1;
-    Problem& p = L.p[0];
-    p.a = x;
-    p.b = w;
-    p.b.p += v0 * w.ld;
-    p.M = (int32_t)R;
-    p.N = (int32_t)n;
-    p.K = (int32_t)D;
-    p.batch = p.n_outer = p.n_inner = p.splits = 1;
-    DzEpi<T, NP>& e = L.e[0];
-    e.bias = d.b ? static_cast<const T*>(d.b) + v0 : nullptr;
-    e.target = d.target;
-    e.lse = d.lse;
-    e.low = d.low;
-    e.gloss = d.reduction == 0 ? d.gloss : nullptr;
-    e.ignore = d.ignore_index;
-    e.vocab = V;
-    e.dz = const_cast<__bf16*>(dz.p);
-    e.ld = ld;
-    e.s_part = dz.s_part;
-    e.v0 = (int32_t)v0;
-
-    Products<T, NP> dx, dw;
-    if (d.dx) {
-      dx.add(dz, p.b, R, D, n, 1, 1, 1, d.dx, D, 0, nullptr, 0, by);
-      if (n_pieces > 1) {
-        dx.L.e[0].sum = sum;
-        dx.L.e[0].mode = last ? 4 : k == 0 ? 2 : 3;
-      }
-      dx.reserve(ws, n_pieces == 1);
-    }
-    if (d.dW) dw.add(dz, x, n, D, R, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0, by);
-    dw.reserve(ws, true);
-    // db: the waves' sums from the epilogue, up to 256 of a column; of more rows a
-    // pass over dz, whose second part would be the long one.  8192 x 1024 -> 32768 in
-    // bfloat16, both directions: 2195 us, of 2322 with the pass; 1500 x 777 -> 10007 in
-    // float32 651, of 673.
-    const TileSize size = choose<NP>(L, false).size;
-    const int64_t chunks = (R + wave_rows<NP>(size) - 1) / wave_rows<NP>(size);
     Colsum<T, NP> cs;
-    if (d.db && chunks <= 256) e.db = cs.given(n, (int32_t)chunks, static_cast<T*>(d.db) + v0, by, ws);
-    else if (d.db) cs.add(dz, R, n, 1, static_cast<T*>(d.db) + v0, by);
-    cs.reserve(ws);
-    *bytes = std::max(*bytes, ws.used);
-    if (dry) continue;
-    if (R > 0) {
-      if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy_bwd") != 0) return -1;
-      if (dx.template launch<false, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
+    int64_t columns = keep;  // what the piece's column sums hold of the workspace
+    for (int64_t b = 0; b < n_blocks; ++b) {
+      // (pieces and blocks reuse one workspace: a stream runs them in order)
+      ws.used = columns;
+      const int64_t r0 = b * block, m = std::min(block, R - r0);
+      Launch<DzEpi<T, NP>> L{};
+      L.n = 1;
+      Problem& p = L.p[0];
+      p.a = x;
+      p.a.p += r0 * x.ld;
+      p.b = w;
+      p.b.p += v0 * w.ld;
+      p.M = (int32_t)m;
+      p.N = (int32_t)n;
+      p.K = (int32_t)D;
+      p.batch = p.n_outer = p.n_inner = p.splits = 1;
+      DzEpi<T, NP>& e = L.e[0];
+      e.bias = d.b ? static_cast<const T*>(d.b) + v0 : nullptr;
+      e.target = d.target + r0;
+      e.lse = d.lse + r0;
+      e.low = d.low ? d.low + r0 : nullptr;
+      e.gloss = d.reduction == 0 ? d.gloss + r0 : nullptr;
+      e.ignore = d.ignore_index;
+      e.vocab = V;
+      e.dz = const_cast<__bf16*>(dz.p);
+      e.ld = ld;
+      e.s_part = dz.s_part;
+      e.v0 = (int32_t)v0;
+
+      // db: the waves' sums from the epilogue, up to 256 of a column; of more rows a
+      // pass over dz, whose second part would be the long one.  8192 x 1024 -> 32768 in
+      // bfloat16, both directions: 2195 us, of 2322 with the pass; 1500 x 777 -> 10007
+      // in float32 651, of 673.
+      const TileSize size = choose<NP>(L, false).size;
+      if (b == 0 && d.db) {
+        const int64_t chunks = (m + wave_rows<NP>(size) - 1) / wave_rows<NP>(size);
+        T* db = static_cast<T*>(d.db) + v0;
+        cs.blocks = n_blocks;
+        if (n_blocks == 1 && chunks <= 256) e.db = cs.given(n, (int32_t)chunks, db, by, ws);
+        else cs.add(dz, m, n, 1, db, by);
+        cs.reserve(ws);
+        columns = ws.used;
+      }
+      if (d.db) cs.set_rows(m);
+      Products<T, NP> dx, dw;
+      if (d.dx) {
+        T* out = static_cast<T*>(d.dx) + r0 * D;
+        dx.add(dz, p.b, m, D, n, 1, 1, 1, out, D, 0, nullptr, 0, by);
+        if (n_pieces > 1) {
+          dx.L.e[0].sum = sum + r0 * round8(D);
+          dx.L.e[0].mode = v0 + n == V ? 4 : k == 0 ? 2 : 3;
+        }
+        dx.reserve(ws, n_pieces == 1);
+      }
+      if (d.dW) {
+        Operand xb = x;
+        xb.p += r0 * x.ld;
+        dw.add(dz, xb, n, D, m, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0, by);
+        if (n_blocks > 1) {
+          dw.L.e[0].sum = sum_w;
+          dw.L.e[0].mode = b + 1 == n_blocks ? 4 : b == 0 ? 2 : 3;
+        }
+        dw.reserve(ws, n_blocks == 1);
+      }
+      *bytes = std::max(*bytes, ws.used);
+      if (dry) continue;
+      if (R > 0) {
+        if (run<NP, false, false, false>(L, size, stream, "linear_cross_entropy_bwd") != 0) return -1;
+        if (dx.template launch<false, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
+      }
+      if (dw.template launch<true, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
+      if (cs.launch(stream, b) != 0) return -1;
     }
-    if (dw.template launch<true, true>(stream, "linear_cross_entropy_bwd") != 0) return -1;
-    if (cs.launch(stream) != 0) return -1;
   }
   return 0;
 }

@@ -231,3 +231,51 @@ def test_layer_norm_of_more_columns_than_a_launch_has_threads(T):
         want = xh * w[part] + b[part]
         within(y[0, part], want, e_xh * w[part].abs() + 4 * U * (want.abs() + (xh * w[part]).abs()), "y")
     assert torch.isfinite(dx).all()
+
+
+# ------------------------------------------- pieces of the vocabulary, blocks of the rows
+def rows_and_classes(R, D, V, dtype, pad=0.2):
+    g = torch.Generator(DEV).manual_seed(R + V)
+    x = torch.randn(R, D, device=DEV, generator=g).to(dtype)
+    W = (torch.randn(V, D, device=DEV, generator=g) * D ** -0.5).to(dtype)
+    b = torch.randn(V, device=DEV, generator=g).to(dtype)
+    t = torch.randint(0, V, (R,), device=DEV, generator=g)
+    t[torch.rand(R, device=DEV, generator=g) < pad] = -100
+    return x, W, b, t
+
+
+@pytest.mark.parametrize("R,D,V,dtype,reduction", [
+    (33000, 24, 9000, BF16, "mean"),    # two pieces, sums of columns by a pass of their own
+    (33000, 24, 9000, BF16, "none"),
+    (8000, 40, 36001, BF16, "none"),    # two pieces, their columns' sums in the epilogue
+    (6000, 24, 33001, F32, "none"),     # three
+    (400003, 24, 300, F32, "mean"),     # two pieces x two blocks of rows
+    (400003, 17, 77, F32, "none"),      # one piece
+    ((1 << 20) + 4099, 8, 264, BF16, "sum"),
+    ((1 << 20) + 4099, 8, 264, BF16, "none")])
+def test_cross_entropy_in_pieces_and_blocks(T, R, D, V, dtype, reduction):
+    x, W, b, t = rows_and_classes(R, D, V, dtype)
+    g = torch.randn(R, device=DEV, generator=torch.Generator(DEV).manual_seed(9)) \
+        if reduction == "none" else 1.0
+    got = run_xent(T, x, W, b, t, reduction, g)
+    again = run_xent(T, x, W, b, t, reduction, g)
+    assert all(torch.equal(got[k], again[k]) for k in got)
+    check(got, xent_reference(x, W, b, t, -100, reduction, g))
+
+
+def test_cross_entropy_forward_in_blocks_of_rows(T):
+    """2^17 rows of 33000 classes: the parts of 516 waves a row are over 512 MiB, so
+    the rows come in two blocks (65792 and the rest)."""
+    R, D, V = (1 << 17) + 3, 8, 33000
+    x, W, b, t = rows_and_classes(R, D, V, BF16)
+    loss = T.linear_cross_entropy(x, W, t, b, reduction="none")
+    for rows in (slice(0, 20), slice(65782, 65802), slice(R - 20, R)):
+        ref = xent_reference(x[rows], W, b, t[rows], -100, "none", 1.0)
+        within(loss[rows], *ref["loss"], "loss")
+    # each block alone gives the same rows, bit by bit, and their sums are all of them's
+    for rows in (slice(0, 65792), slice(65792, R)):
+        assert torch.equal(T.linear_cross_entropy(x[rows], W, t[rows], b, reduction="none"), loss[rows])
+    total, kept = loss.double().sum(), int((t != -100).sum())
+    for reduction, want in (("sum", total), ("mean", total / kept)):
+        got = T.linear_cross_entropy(x, W, t, b, reduction=reduction)
+        within(got, want, 2 * U * want.abs(), reduction)

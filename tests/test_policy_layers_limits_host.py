@@ -75,3 +75,46 @@ def test_calls_without_a_tangent_still_run_in_a_dual_level(T, op):
         y = call(T, *a)
         grads = torch.autograd.grad(y, a, meta(*y.shape))
     assert [g.shape for g in grads] == [t.shape for t in a]
+
+
+def xent_workspace(rows, n_in, vocab, dtype, bwd, reduction=1):
+    import ctypes
+    from d3rlpy_amd import _native as N
+    d = N.LinearXentDesc()
+    d.rows, d.n_in, d.vocab, d.ldx, d.ldW, d.dtype, d.reduction = (rows, n_in, vocab, n_in, n_in,
+                                                                   dtype, reduction)
+    for k in ("x", "W", "b", "target", "loss", "lse", "out", "scale", "gloss", "dx", "dW", "db"):
+        setattr(d, k, 256)
+    n = ctypes.c_int64()
+    assert N.lib().d3a_linear_xent_workspace(ctypes.byref(d), bwd, ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("dtype,planes", [(0, 3), (1, 1)])
+@pytest.mark.parametrize("rows,vocab", [
+    (6000, 29826), (8192, 32768), (8000, 33001), (8192, 1 << 20), (1 << 17, 65536),
+    (1 << 20, 65536), (1 << 20, 300), (1 << 22, 65536), (1 << 23, 40), (1 << 24, 1 << 18),
+    (37, 1 << 26), (1 << 26, 2000)])
+def test_cross_entropy_scratch_does_not_grow_with_the_logits(T, dtype, planes, rows, vocab):
+    """Either direction's scratch is 512 MiB for what has a value a logit (or a wave's
+    64), whatever rows x vocabulary is, and what goes with x and W."""
+    D = 8
+    MiB, pad = 1 << 20, 1 << 16
+    copies = 2 * planes * (rows + vocab) * D  # operands that are packed
+    per_row = 8 * rows  # the targets' logits
+    # partial sums of at most 1280 tiles' rows of D, 256 chunks of column sums a block of rows
+    blocks = rows * planes // (1 << 20) + 2 if rows * planes > 1 << 20 else 1
+    extra = 1280 * 256 * 4 * max(D, 8) + min(vocab, (1 << 21) if blocks == 1 else 256) * 4 * 256 * blocks
+    sums = 4 * rows * D + 4 * 256 * D  # dx over pieces, dW over blocks
+    assert xent_workspace(rows, D, vocab, dtype, 1) <= 512 * MiB + copies + sums + extra + pad
+
+
+def test_cross_entropy_scratch_of_many_rows(T):
+    """The forward's parts of 2^20 rows x 65536 classes are 8 GiB, dz's of 2^22 rows 2
+    GiB a 256 columns: both within 512 MiB, by blocks of rows."""
+    GiB = 1 << 30
+    assert xent_workspace(1 << 20, 8, 65536, 1, 0) < 0.6 * GiB
+    assert xent_workspace(1 << 22, 8, 65536, 1, 1) < 0.8 * GiB
+    assert xent_workspace(1 << 20, 8, 65536, 0, 1) < 0.7 * GiB
+    # and cut down, not up: two pieces of 15104 columns were 518.6 MiB
+    assert xent_workspace(6000, 8, 29826, 0, 1) < 512 * (1 << 20) + 8 * (1 << 20)
