@@ -57,6 +57,7 @@
 //                                  same for the TD3+BC, BCQ and DiscreteCQL Impls.
 #include <ATen/ATen.h>
 #include <ATen/hip/HIPContext.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -1085,6 +1086,31 @@ void refuse_tangent(const at::Tensor& t, const char* op) {
                               " has no forward-mode derivative");
 }
 
+// Autograd waits with each node's own stream for the gradients it is handed, the
+// stream that its forward ran on.  In a capture, a gradient for a node of the default
+// stream (an input computed before the capture, or a leaf whose accumulation node an
+// eager graph of the same leaf keeps alive) is such a wait of the default stream for a
+// capturing one: the capture breaks, and the process has ended by it.  So a backward
+// that would hand on such a gradient raises before it has run.  `inputs`: the
+// forward's tensors in their order.
+void refuse_eager_nodes(const AutogradContext* ctx, at::ArrayRef<at::Tensor> inputs, const char* op) {
+  if (!inputs[0].is_cuda()) return;
+  const c10::DeviceGuard guard(inputs[0].device());
+  // (the default stream is never captured, and not asked: asking may break a capture)
+  const hipStream_t stream = at::hip::getCurrentHIPStream().stream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (!stream || hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  size_t edge = 0;
+  for (const at::Tensor& t : inputs) {
+    if (!t.defined() || !ctx->needs_input_grad(edge++)) continue;
+    const auto to = torch::autograd::impl::gradient_edge(t).function;
+    const auto other = to ? to->stream() : std::nullopt;
+    TORCH_CHECK(!other || c10::hip::HIPStreamMasqueradingAsCUDA(*other).stream(), "d3rlpy_amd::", op,
+                ": a captured backward reaches a tensor whose autograd node belongs to the default stream: "
+                "drop the eager outputs of the same leaves before the capture, and compute its inputs inside it");
+  }
+}
+
 // Whether a node is needed, and for which inputs.
 template <size_t N>
 bool wants(const char* op, const std::array<at::Tensor, N>& inputs, std::array<bool, N>& wanted) {
@@ -1157,6 +1183,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     static const auto op = op_handle<Sig>("d3rlpy_amd::layer_norm_backward");
     refuse_tangent(g[0], "layer_norm");
     const variable_list v = ctx->get_saved_variables();
+    refuse_eager_nodes(ctx, {v[0], v[1], v[2]}, "layer_norm");
     std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
     {
       const at::AutoDispatchBelowADInplaceOrView guard;
@@ -1204,6 +1231,7 @@ struct GatedMlpNode : torch::autograd::Function<GatedMlpNode> {
     static const auto op = op_handle<Sig>("d3rlpy_amd::gated_mlp_backward");
     refuse_tangent(g[0], "gated_mlp");
     const variable_list v = ctx->get_saved_variables();
+    refuse_eager_nodes(ctx, at::ArrayRef<at::Tensor>(v).slice(0, 7), "gated_mlp");
     const std::string act = ctx->saved_data["act"].toStringRef();
     Seven r;
     {
@@ -1257,6 +1285,7 @@ struct XentNode : torch::autograd::Function<XentNode> {
     static const auto op = op_handle<Sig>("d3rlpy_amd::linear_cross_entropy_backward");
     refuse_tangent(g[0], "linear_cross_entropy");
     const variable_list v = ctx->get_saved_variables();
+    refuse_eager_nodes(ctx, at::ArrayRef<at::Tensor>(v).slice(0, 4), "linear_cross_entropy");
     const std::string reduction = ctx->saved_data["reduction"].toStringRef();
     std::tuple<at::Tensor, at::Tensor, at::Tensor> r;
     {

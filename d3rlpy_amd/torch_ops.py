@@ -186,10 +186,16 @@ def squashed_gaussian_sample(mu, logstd, eps, min_logstd: float = -20.0,
 # layer_norm, gated_mlp and linear_cross_entropy carry their gradients in the op
 # library itself (its Autograd kernels), so torch.ops.d3rlpy_amd.layer_norm is
 # differentiable too; the gradients have no second derivative, and forward-mode
-# (torch.autograd.forward_ad, torch.func.jvp) raises.  A backward pass
-# to capture into a graph is best written with the forward and *_backward ops:
-# autograd's own nodes belong to the stream that ran the forward, and a capture
-# that meets an eager graph's nodes of the same leaves ends the process.
+# (torch.autograd.forward_ad, torch.func.jvp) raises.
+#
+# Captured into a graph, a backward pass is best written with the forward and
+# *_backward ops.  Autograd's nodes belong to the stream that ran their forward, a
+# leaf's to the first forward whose graph still lives: a captured gradient that is
+# handed to one of the default stream makes that stream wait for a capturing one,
+# which breaks the capture and has ended the process.  So forward and backward are
+# captured together, after the eager outputs of the same leaves are gone (del loss);
+# the three operators raise where their own gradients would meet such a node, and
+# torch's operators in the same pass do not.
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of ``x``
@@ -197,7 +203,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
     ``x`` [.., n] with ``weight`` / ``bias`` [n], or [members, .., n] with
     [members, n] (every member its own); float32 or bfloat16, the weights in
-    ``x``'s dtype or float32 and either may be None.  Statistics are float32."""
+    ``x``'s dtype or float32 and either may be None.  Statistics are float32.
+
+    To capture a forward and its backward into a graph, drop the eager outputs of the
+    same leaves first: a captured backward that would hand a gradient to the default
+    stream's autograd nodes raises (``gated_mlp`` and ``linear_cross_entropy`` too)."""
     return load().layer_norm(x, weight, bias, eps)[0]
 
 

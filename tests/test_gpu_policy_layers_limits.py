@@ -279,3 +279,45 @@ def test_cross_entropy_forward_in_blocks_of_rows(T):
     for reduction, want in (("sum", total), ("mean", total / kept)):
         got = T.linear_cross_entropy(x, W, t, b, reduction=reduction)
         within(got, want, 2 * U * want.abs(), reduction)
+
+
+# ------------------------------------------------------------- captures and eager graphs
+CAPTURED = {
+    "layer_norm": lambda T, p: T.layer_norm(p["x"], p["w"]),
+    "gated_mlp": lambda T, p: T.gated_mlp(p["x"], p["W"], p["W2"], p["D"]),
+    "linear_cross_entropy": lambda T, p: T.linear_cross_entropy(p["x"], p["W"], p["t"])}
+
+
+@pytest.mark.parametrize("op", CAPTURED)
+def test_capture_that_meets_an_eager_graph_is_refused(T, op):
+    """A captured backward whose leaf has an accumulation node of the default stream,
+    kept alive by an eager output, raises before it hands that node a gradient; with
+    the eager output gone the same capture runs and replays."""
+    call = CAPTURED[op]
+    p = {"x": rnd(1, 20, 8), "w": rnd(2, 8), "W": rnd(3, 12, 8), "W2": rnd(4, 12, 8),
+         "D": rnd(5, 8, 12), "t": torch.arange(20, device=DEV) % 12}
+    leaf = p["w" if op == "layer_norm" else "W"].requires_grad_(True)
+    (want,) = torch.autograd.grad(call(T, p).sum(), [leaf])
+    eager = call(T, p)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match=f"{op}: a captured backward"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(call(T, p).sum(), [leaf])
+    # a gradient that goes elsewhere does not touch that node
+    x = p["x"].requires_grad_(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dx,) = torch.autograd.grad(call(T, p).sum(), [x])
+    graph.replay()
+    del eager
+    (again,) = torch.autograd.grad(call(T, p).sum(), [x])
+    assert torch.equal(dx, again)
+    del again
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(call(T, p).sum(), [leaf])
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
