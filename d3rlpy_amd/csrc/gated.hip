@@ -7,13 +7,16 @@
 // All six products are tiles of mm.hpp for many rows, bound by the matrix cores and
 // the float32 g and u: 8192 x 1024 x 4096 in bfloat16 takes 174 to 203 us for g, u
 // and h (137 GFLOP, 335 MB out), 83 for y, 170 for dg and du, 157 to 173 for dx, 207 to
-// 250 for the three weight gradients (206 GFLOP).  The first forward launch stages gate and up weights as one B tile
-// whose waves hold the same 32 columns of both, so activation and product
-// happen on the accumulators; the backward's first launch forms dh and, from
+// 250 for the three weight gradients (206 GFLOP, 192 tiles for 256 CUs).  The first
+// forward launch stages gate and up weights as one B tile whose waves hold the same 32
+// columns of both, so activation and product happen on the accumulators; the backward's first launch forms dh and, from
 // the kept g and u, dg and du in its epilogue.  Kept between the two: h as the
-// down product's operand, and g and u in float32.  In bfloat16 they would halve 270 MB of traffic at 8192 x 4096
-// hidden values, but a second rounding on the way to each gradient takes its
-// error from 1.4 to 2 times that of the result's own rounding.
+// down product's operand, and g and u in float32.  In bfloat16 they would halve 270 MB
+// of traffic at 8192 x 4096 hidden values, but a second rounding on the way to each
+// gradient takes its error from 1.4 to 2 times that of the result's own rounding.
+// h, dg and du are rounded to bfloat16 where the tensors are, as the operands of one
+// matrix instruction a term; second parts would double the work of y, of dx and of the
+// weights' gradients, six of the nine products.
 #include "direct.hpp"
 #include "mm_host.hpp"
 #include "thin.hpp"
@@ -24,7 +27,8 @@ namespace {
 
 using namespace mm;
 
-// act(g) and act'(g)
+// act(g) and act'(g).  FAST (bfloat16 tensors): the hardware's exponential and
+// reciprocal, good to a few 2^-24, where h is rounded by 2^-8 next.
 template <bool FAST>
 __device__ __forceinline__ void activation(int act, float g, float& a, float& da) {
   if (act == D3A_ACT_RELU) {

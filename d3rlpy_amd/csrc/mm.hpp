@@ -121,7 +121,8 @@ struct Loader {
   // k sits at u ^ unit_swz(k), so that the four ks x two units of half a
   // transposed read do.
   static __device__ __forceinline__ int swz(int r) {
-    return BK == 64 ? ((r >> 1) & 7) : BK == 32 ? ((r >> 2) & 3) : ((r >> 3) & 1);
+    static_assert(BK == 64 || BK == 32, "depth");
+    return BK == 64 ? ((r >> 1) & 7) : ((r >> 2) & 3);
   }
   static __device__ __forceinline__ int unit_swz(int k) {
     return ROWS >= 128 ? (k & 3) << 1 : ((k >> 1) & 1) << 1;

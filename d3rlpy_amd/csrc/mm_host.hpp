@@ -377,7 +377,9 @@ struct Tiles<3> {
 // of k)  bfloat16: 8192 x 1024 x 4096 82 / 58 / 84, 8192 x 1024 x 32768 415* /
 // 516 / 853, 32768 x 1024 x 8192 373 / 471 / 994, 1024 x 2048 x 1024 28 / 15 /
 // 12;  float32: 1500 x 777 x 10007 134* / 150* / 205*, 1500 x 10007 x 777 152 /
-// 186 / 223, 1999 x 513 x 1366 40* / 39* / 43*, 256 x 512 x 256 19 / 12 / 9.
+// 186 / 223, 1999 x 513 x 1366 40* / 39* / 43*, 256 x 512 x 256 19 / 12 / 9.  (Timed
+// alone: inside a block, whose operands come from other kernels, a product can take a
+// fifth longer, as the gated block's dx of 8192 x 1024 x 8192, 157 to 173 us of 134.)
 struct Cost {
   int bm, bn, bk, resident;
   double busy, alone, ends;

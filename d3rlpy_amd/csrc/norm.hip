@@ -90,9 +90,8 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
 // (times the rows it holds at once).  Single values (VEC 1) are bound by the
 // loads' number, so w and b stay in registers over 2048 workgroups' rows and the
 // next row is loaded ahead; pieces take a workgroup for every row (up to 2^22, of the
-// 2^24 that a launch holds) and load w and b when they need them: 8192 x 2048 in bfloat16 takes 14 to 15 us, 18 the other way, and 8192
-// x 2047 22, of 38.
-
+// 2^24 that a launch holds) and load w and b when they need them: 8192 x 2048 in
+// bfloat16 takes 14 to 15 us, 18 the other way, and 8192 x 2047 22, of 38.
 template <class T, class W, int VEC, int NCH, int WPR>
 __global__ __launch_bounds__(256) void norm_kernel(const Args A) {
   constexpr bool kWalk = VEC == 1, kAhead = kWalk && NCH <= 16;
@@ -496,8 +495,10 @@ int dispatch(const d3a_layer_norm_desc& d, const Args& a, bool bwd, hipStream_t 
     if (n > kWave && !bwd) return launch<T, W, V, 2048 / (64 * V), 1>(d, a, bwd, s);
     if (n > kWave) return launch<T, W, V, 2048 / (256 * V), 4>(d, a, bwd, s);
     if (n > 512) return launch<T, W, V, 1024 / (64 * V), 1>(d, a, bwd, s);
-    if (n > 256 || V == 8) return launch<T, W, V, 512 / (64 * V), 1>(d, a, bwd, s);
-    return launch<T, W, V, V == 8 ? 1 : 256 / (64 * V), 1>(d, a, bwd, s);
+    // (one piece a lane: 512 values of bfloat16, 256 of float32)
+    if constexpr (V < 8)
+      if (n > 256) return launch<T, W, V, 512 / (64 * V), 1>(d, a, bwd, s);
+    return launch<T, W, V, 1, 1>(d, a, bwd, s);
   }
   if (n > 4096) return launch<T, W, 1, 32, 4>(d, a, bwd, s);
   if (n > 2048) return launch<T, W, 1, 16, 4>(d, a, bwd, s);
