@@ -321,3 +321,97 @@ def test_capture_that_meets_an_eager_graph_is_refused(T, op):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------- layouts and cuts of the tiled products
+@pytest.mark.parametrize("C", [0, 2])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("by", [8, 3])  # rows that the tiles read in place, and not
+def test_gate_and_up_weights_of_unlike_strides(T, C, dtype, by):
+    """The gate's weights in wider rows (and members further apart) than the up's."""
+    R, D, F, O = 150, 64, 1104, 40
+    lead = (C,) if C else ()
+    p = {"x": rnd(1, *lead, R, D, dtype=dtype),
+         "Wg": rnd(2, *lead, F, D, dtype=dtype, scale=D ** -0.5),
+         "Wu": rnd(3, *lead, F, D, dtype=dtype, scale=D ** -0.5),
+         "Wd": rnd(4, *lead, O, F, dtype=dtype, scale=F ** -0.5)}
+    dy = rnd(5, *lead, R, O, dtype=dtype)
+    ref = gated_reference(p, dy, "silu")
+
+    def spread(t, rows, cols):  # the same values, `rows` and `cols` more around them
+        big = torch.full((*t.shape[:-2], t.shape[-2] + rows, t.shape[-1] + cols), 7.0,
+                         device=DEV, dtype=dtype)
+        big[..., :t.shape[-2], :t.shape[-1]] = t
+        return big[..., :t.shape[-2], :t.shape[-1]]
+
+    for one, other in (((0, by), (0, 0)), ((0, 0), (0, by)), ((8, 0), (0, 0)), ((8, by), (16, 2 * by))):
+        q = p | {"Wg": spread(p["Wg"], *one), "Wu": spread(p["Wu"], *other)}
+        q = {k: v.detach().requires_grad_(True) for k, v in q.items()}
+        y = T.gated_mlp(*q.values())
+        grads = torch.autograd.grad(y, list(q.values()), dy)
+        check({"y": y} | dict(zip(q, grads)), ref)
+
+
+def test_weight_gradients_cut_over_k_with_members(T):
+    """4096 rows are the weight gradients' k axis, cut over workgroups for each of two
+    members: partial sums [split][member]."""
+    from d3rlpy_amd import _native as N
+    C, R, D, F, O = 2, 4096, 64, 1104, 24
+    d = N.GatedMlpDesc()
+    d.rows, d.n_in, d.n_hidden, d.n_out, d.members = R, D, F, O, C
+    d.ldx, d.ldWg, d.ldWu, d.ldWd, d.lddy = D, D, D, F, O
+    d.sx, d.sWg, d.sWu, d.sWd, d.sdy = R * D, F * D, F * D, O * F, R * O
+    for k in ("x", "Wg", "Wu", "Wd", "y", "dy", "kept", "dWd"):
+        setattr(d, k, 256)
+    d.dtype = 1
+    size = ctypes.c_int64()
+    assert N.lib().d3a_gated_mlp_workspace(ctypes.byref(d), 1, ctypes.byref(size)) == 0
+    assert size.value >= 2 * C * O * F * 4  # (all operands in place: the partial sums alone)
+    for dtype in (BF16, F32):
+        p = {"x": rnd(1, C, R, D, dtype=dtype), "Wg": rnd(2, C, F, D, dtype=dtype, scale=D ** -0.5),
+             "Wu": rnd(3, C, F, D, dtype=dtype, scale=D ** -0.5),
+             "Wd": rnd(4, C, O, F, dtype=dtype, scale=F ** -0.5)}
+        dy = rnd(5, C, R, O, dtype=dtype)
+        q = {k: v.detach().requires_grad_(True) for k, v in p.items()}
+        y = T.gated_mlp(*q.values())
+        grads = torch.autograd.grad(y, list(q.values()), dy)
+        check({"y": y} | dict(zip(q, grads)), gated_reference(p, dy, "silu"))
+
+
+@pytest.mark.parametrize("V", [300, 5003])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_head_and_its_gradients_replay(T, V, dtype):
+    """A block with a head of its own, captured through autograd: every gradient of
+    every replay, the head's among them, is the eager pass's bit by bit."""
+    D, F, R = 64, 160, 90
+    q = {"x": rnd(1, R, D), "w": rnd(2, D, scale=0.1, shift=1.0), "c": rnd(3, D, scale=0.1),
+         "Wg": rnd(4, F, D, scale=D ** -0.5), "Wu": rnd(5, F, D, scale=D ** -0.5),
+         "Wd": rnd(6, D, F, scale=F ** -0.5), "head": rnd(7, V, D, scale=D ** -0.5), "b": rnd(8, V)}
+    q = {k: v.to(dtype).requires_grad_(True) for k, v in q.items()}
+    t = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(9)).to(DEV)
+
+    def step():
+        h = T.layer_norm(q["x"], q["w"], q["c"])
+        r = q["x"] + T.gated_mlp(h, q["Wg"], q["Wu"], q["Wd"])
+        loss = T.linear_cross_entropy(r, q["head"], t, q["b"])
+        return [loss.detach()] + list(torch.autograd.grad(loss, list(q.values())))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            q["head"].mul_(1.0 + 0.1 * k)
+            q["x"].add_(0.05 * k)
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got, want = [o.clone() for o in out], step()
+        for name, a, b in zip(["loss"] + list(q), got, want):
+            assert torch.equal(a, b), (k, name)
