@@ -37,13 +37,14 @@ using namespace mm;
 
 constexpr int64_t kPieceBytes = 512LL << 20;
 
-// The size of equal parts of `all`: all of it if that is at most `most`, else a multiple
-// of the widest tile's 256, at most `most` (or 256).
+// The size of equal parts of `all`, at most `most` each: a multiple of the widest tile's
+// 256 where that leaves any.
 int64_t equal_parts(int64_t all, int64_t most) {
   if (all <= most) return all;
-  most = std::max<int64_t>(most / 256 * 256, 256);
+  const int64_t step = most >= 256 ? 256 : 1;
+  most = std::max<int64_t>(most / step, 1) * step;
   const int64_t n = (all + most - 1) / most;
-  return ((all + n - 1) / n + 255) / 256 * 256;
+  return ((all + n - 1) / n + step - 1) / step * step;
 }
 
 // exp(z - ref).  (With bfloat16 tensors the hardware's exponential, within 2 ulp

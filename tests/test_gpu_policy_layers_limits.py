@@ -251,6 +251,7 @@ def rows_and_classes(R, D, V, dtype, pad=0.2):
     (6000, 24, 33001, F32, "none"),     # three
     (400003, 24, 300, F32, "mean"),     # two pieces x two blocks of rows
     (400003, 17, 77, F32, "none"),      # one piece
+    (400003, 17, 300, F32, "sum"),      # rows that are not 16-byte aligned, two x two
     ((1 << 20) + 4099, 8, 264, BF16, "sum"),
     ((1 << 20) + 4099, 8, 264, BF16, "none")])
 def test_cross_entropy_in_pieces_and_blocks(T, R, D, V, dtype, reduction):
@@ -261,6 +262,17 @@ def test_cross_entropy_in_pieces_and_blocks(T, R, D, V, dtype, reduction):
     again = run_xent(T, x, W, b, t, reduction, g)
     assert all(torch.equal(got[k], again[k]) for k in got)
     check(got, xent_reference(x, W, b, t, -100, reduction, g))
+
+
+def test_cross_entropy_single_gradients_in_blocks(T):
+    """A gradient alone is the one that comes with the others, bit by bit."""
+    x, W, b, t = rows_and_classes(400003, 24, 300, F32)
+    want = run_xent(T, x, W, b, t, "mean", 1.0)
+    for k in ("x", "W", "b"):
+        q = {n: v.detach().requires_grad_(n == k) for n, v in (("x", x), ("W", W), ("b", b))}
+        loss = T.linear_cross_entropy(q["x"], q["W"], t, q["b"])
+        (got,) = torch.autograd.grad(loss, [q[k]])
+        assert torch.equal(got, want[k]), k
 
 
 def test_cross_entropy_forward_in_blocks_of_rows(T):

@@ -94,13 +94,13 @@ def xent_workspace(rows, n_in, vocab, dtype, bwd, reduction=1):
 @pytest.mark.parametrize("rows,vocab", [
     (6000, 29826), (8192, 32768), (8000, 33001), (8192, 1 << 20), (1 << 17, 65536),
     (1 << 20, 65536), (1 << 20, 300), (1 << 22, 65536), (1 << 23, 40), (1 << 24, 1 << 18),
-    (37, 1 << 26), (1 << 26, 2000)])
+    (37, 1 << 26), (100, 1 << 26), (300, 1 << 27), (1 << 26, 2000)])
 def test_cross_entropy_scratch_does_not_grow_with_the_logits(T, dtype, planes, rows, vocab):
     """Either direction's scratch is 512 MiB for what has a value a logit (or a wave's
     64), whatever rows x vocabulary is, and what goes with x and W."""
     D = 8
     MiB, pad = 1 << 20, 1 << 16
-    copies = 2 * planes * (rows + vocab) * D  # operands that are packed
+    copies = 6 * (rows + vocab) * D if planes == 3 else 0  # float32 operands are packed
     per_row = 8 * rows  # the targets' logits
     # partial sums of at most 1280 tiles' rows of D, 256 chunks of column sums a block of rows
     blocks = rows * planes // (1 << 20) + 2 if rows * planes > 1 << 20 else 1
