@@ -102,9 +102,11 @@ def test_cross_entropy_scratch_does_not_grow_with_the_logits(T, dtype, planes, r
     MiB, pad = 1 << 20, 1 << 16
     copies = 6 * (rows + vocab) * D if planes == 3 else 0  # float32 operands are packed
     per_row = 8 * rows  # the targets' logits
-    # partial sums of at most 1280 tiles' rows of D, 256 chunks of column sums a block of rows
-    blocks = rows * planes // (1 << 20) + 2 if rows * planes > 1 << 20 else 1
-    extra = 1280 * 256 * 4 * max(D, 8) + min(vocab, (1 << 21) if blocks == 1 else 256) * 4 * 256 * blocks
+    assert xent_workspace(rows, D, vocab, dtype, 0) <= 512 * MiB + copies + per_row + pad
+    # partial sums of at most 1280 tiles' rows of D; the columns' sums, of at least 32 rows
+    # of a piece each, and of 256 columns x 256 chunks a block of rows
+    blocks = rows * planes // (1 << 20) + 2
+    extra = 1280 * 256 * 4 * D + 36 * MiB + blocks * 256 * 256 * 4
     sums = 4 * rows * D + 4 * 256 * D  # dx over pieces, dW over blocks
     assert xent_workspace(rows, D, vocab, dtype, 1) <= 512 * MiB + copies + sums + extra + pad
 
