@@ -335,6 +335,22 @@ def test_capture_that_meets_an_eager_graph_is_refused(T, op):
         assert torch.equal(got, want)
 
 
+def test_cross_entropy_of_few_rows_in_blocks(T):
+    """2^26 classes are 2^20 parts a row, 8 MiB: 100 rows come in two blocks of 50."""
+    R, D, V = 100, 8, (1 << 26) - 5
+    g = torch.Generator(DEV).manual_seed(1)
+    x = torch.randn(R, D, device=DEV, generator=g).to(BF16)
+    W = torch.randn(V, D, device=DEV, generator=g).to(BF16)
+    t = torch.randint(0, V, (R,), device=DEV, generator=g)
+    loss = T.linear_cross_entropy(x, W, t, reduction="none")
+    xd = x.double()
+    lse = torch.stack([torch.logsumexp(xd @ w.double().t(), -1) for w in W.split(1 << 22)]).logsumexp(0)
+    z = (xd * W[t].double()).sum(-1)
+    # a part's 64 terms, then 4096 parts a thread and 256 threads' sums; logits to a few steps
+    bound = U * (4096 + 200 + 64 * (xd.abs().sum(-1) * W.abs().max().double()))
+    within(loss, lse - z, bound, "loss")
+
+
 # ------------------------------------------------- layouts and cuts of the tiled products
 @pytest.mark.parametrize("C", [0, 2])
 @pytest.mark.parametrize("dtype", [F32, BF16])
