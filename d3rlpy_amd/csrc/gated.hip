@@ -4,14 +4,14 @@
 //   dh = dy Wd,  dg = dh * u * act'(g),  du = dh * act(g)
 //   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h
 //
-// All six products are tiles of mm.hpp for many rows, bound by the matrix cores and
-// the float32 g and u: 8192 x 1024 x 4096 in bfloat16 takes 174 to 203 us for g, u
-// and h (137 GFLOP, 335 MB out), 83 for y, 170 for dg and du, 157 to 173 for dx, 207 to
-// 250 for the three weight gradients (206 GFLOP, 192 tiles for 256 CUs).  The first
-// forward launch stages gate and up weights as one B tile whose waves hold the same 32
-// columns of both, so activation and product happen on the accumulators; the backward's first launch forms dh and, from
-// the kept g and u, dg and du in its epilogue.  Kept between the two: h as the
-// down product's operand, and g and u in float32.  In bfloat16 they would halve 270 MB
+// All products are tiles of mm.hpp for many rows, bound by the matrix cores and the
+// float32 g and u: 8192 x 1024 x 4096 in bfloat16 takes 174 to 203 us for g, u and h (137
+// GFLOP, 335 MB out), 81 to 83 for y, 170 for dg and du, 154 to 173 for dx, 207 to 250 for
+// the three weight gradients (206 GFLOP, 192 tiles for 256 CUs).  The first forward launch
+// stages gate and up weights as one B tile whose waves hold the same 32 columns of both,
+// so activation and product happen on the accumulators; the backward's first launch forms
+// dh and, from the kept g and u, dg and du in its epilogue.  Kept between the two: h as
+// the down product's operand, and g and u in float32.  In bfloat16 they would halve 270 MB
 // of traffic at 8192 x 4096 hidden values, but a second rounding on the way to each
 // gradient takes its error from 1.4 to 2 times that of the result's own rounding.
 // h, dg and du are rounded to bfloat16 where the tensors are, as the operands of one

@@ -379,7 +379,7 @@ struct Tiles<3> {
 // 12;  float32: 1500 x 777 x 10007 134* / 150* / 205*, 1500 x 10007 x 777 152 /
 // 186 / 223, 1999 x 513 x 1366 40* / 39* / 43*, 256 x 512 x 256 19 / 12 / 9.  (Timed
 // alone: inside a block, whose operands come from other kernels, a product can take a
-// fifth longer, as the gated block's dx of 8192 x 1024 x 8192, 157 to 173 us of 134.)
+// fifth longer, as the gated block's dx of 8192 x 1024 x 8192, 154 to 173 us of 134.)
 struct Cost {
   int bm, bn, bk, resident;
   double busy, alone, ends;
