@@ -47,9 +47,9 @@ int64_t equal_parts(int64_t all, int64_t most) {
   return ((all + n - 1) / n + step - 1) / step * step;
 }
 
-// exp(z - ref).  (With bfloat16 tensors the hardware's exponential, within 2 ulp
-// and a product's rounding of its argument, is far below dz's own rounding and no
-// more than the float32 sum's.)
+// exp(z - ref), of the forward's sums.  (With bfloat16 tensors the hardware's
+// exponential: within 2 ulp and a product's rounding of its argument it is no more than
+// the float32 sum's own, and in the backward far below dz's rounding.)
 template <int NP>
 __device__ __forceinline__ float exp_to(float z, float ref) {
   return NP == 1 ? __expf(z - ref) : expf(z - ref);
