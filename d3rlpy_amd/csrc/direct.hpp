@@ -36,6 +36,7 @@ struct Problem {
   T* rowsum;        // [batch][M]: the sums of A's rows, or null
   mm::Factor sum_factor;
   int32_t M, N, K, batch, n_outer, n_inner;
+  int32_t fold;     // 0, or up to 16: A has twice as many rows, D is the sum of both halves
   int32_t tiles_m, tiles_n, first;
 };
 
@@ -185,8 +186,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void direct_kernel(const Launch<T, 
       v[i][0] += x.x;
       v[i][1] += x.y;
     }
+    if (P.fold)
+      for (int u = 0; u < kWaves; ++u) {
+        const float2 x = *reinterpret_cast<const float2*>(&red[i][u][((r + P.fold) & 31) * kLine + c]);
+        v[i][0] += x.x;
+        v[i][1] += x.y;
+      }
   }
-  L.e[pi].run(batch, m0 + r, n0 + c, P.M, P.N, v[0], v[NACC - 1]);
+  L.e[pi].run(batch, m0 + r, n0 + c, P.fold ? P.fold : P.M, P.N, v[0], v[NACC - 1]);
 }
 
 // D (+ bias) in T

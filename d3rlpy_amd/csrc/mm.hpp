@@ -528,6 +528,12 @@ __device__ __forceinline__ void load8(const float* p, float v[8]) {
   load4(p + 4, v + 4);
 }
 
+// what v's rounding to bfloat16 left (nothing of an infinity or NaN)
+__device__ __forceinline__ float left_of(float v) {
+  const float left = v - (float)(__bf16)v;
+  return fabsf(left) < INFINITY ? left : 0.f;
+}
+
 // ---- staged epilogues ---------------------------------------------------------
 // A wave's tile, 32 rows at a time, is turned in LDS from the matrix
 // instructions' layout (a lane holds one row's runs of four columns, 64 rows

@@ -478,12 +478,14 @@ struct Products {
     ++L.n;
   }
 
-  // after every add(): the tile, the splits and their partials
-  void reserve(Arena& ws, bool may_split) {
+  // after every add(): the tile, the splits and their partials.  fold: A's rows are this
+  // many times the result's, which is their sum (row m, M / fold + m, ..): in the
+  // partials' layout each split is then `fold` of them
+  void reserve(Arena& ws, bool may_split, int fold = 1) {
     if (L.n == 0) return;
     const Choice c = choose<NP>(L, false, may_split);
     size = c.size;
-    if (c.splits == 1) return;
+    if (c.splits == 1 && fold == 1) return;
     for (int i = 0; i < L.n; ++i) {
       Problem& p = L.p[i];
       p.splits = c.splits;
@@ -491,8 +493,9 @@ struct Products {
       const int64_t n = (int64_t)p.batch * p.M * round8(p.N);
       e.sum = ws.take<float>(c.splits * n);
       e.mode = 1;
-      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.bias, e.ld, e.s_batch, e.s_bias, n, p.M, p.N, p.splits, e.vec, e.factor};
-      sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + (int64_t)p.batch * p.M * ((p.N + 7) / 8);
+      sums.j[sums.n] = SumJob<T>{e.sum, e.out, e.bias, e.ld, e.s_batch, e.s_bias, n / fold, p.M / fold, p.N,
+                                 p.splits * fold, e.vec, e.factor};
+      sums.end[sums.n] = (sums.n ? sums.end[sums.n - 1] : 0) + (int64_t)p.batch * (p.M / fold) * ((p.N + 7) / 8);
       ++sums.n;
     }
   }

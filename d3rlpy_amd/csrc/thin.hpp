@@ -136,8 +136,7 @@ __global__ __launch_bounds__(512) void gate_kernel(const GateArgs<T> A, Act acti
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       hi[i] = (__bf16)h[i];
-      const float left = h[i] - (float)hi[i];
-      lo[i] = (__bf16)(fabsf(left) < INFINITY ? left : 0.f);  // (an infinity is its first part's)
+      lo[i] = (__bf16)mm::left_of(h[i]);
     }
     *reinterpret_cast<bf16x4*>(A.h + at) = hi;
     if (A.lo) *reinterpret_cast<bf16x4*>(A.lo + at) = lo;

@@ -189,7 +189,7 @@ struct DirectDzEpi {
   const int64_t* target;
   const float *lse, *low, *gloss;  // low: or null (0)
   int64_t ignore, vocab;
-  T* dz;
+  T *dz, *second;  // second: dz's second part, or null
   int64_t ld;
   __device__ __forceinline__ void run(int, int m, int n, int M, int N, const float v[2], const float*) const {
     if (m >= M) return;
@@ -201,7 +201,9 @@ struct DirectDzEpi {
       if (n + i >= N) continue;
       const float z = v[i] + (bias ? (float)bias[n + i] : 0.f);
       const float d = (probability<3>(z, l, lo) - (n + i == y ? 1.f : 0.f)) * g;
-      dz[m * ld + n + i] = (T)(y == ignore ? 0.f : d);
+      const float kept = y == ignore ? 0.f : d;
+      dz[m * ld + n + i] = (T)kept;
+      if (second) second[m * ld + n + i] = (T)left_of(kept);
     }
   }
 };
@@ -212,6 +214,15 @@ struct DirectDzEpi {
 Factor loss_factor(const d3a_linear_xent_desc& d) {
   return d.reduction == 0 ? Factor{} : Factor{d.gloss, d.reduction == 1 ? d.scale : nullptr};
 }
+
+// A few bfloat16 rows keep dz in two parts, to 2^-16: with one row the rounding of its
+// target's dz, up to 2^-8, is an error that every gradient shares (1.8 times the plain
+// gradient's own rounding in W's; of many rows these average to 1.2 times).  The second
+// parts cost no product: dx takes them as rows that its tile has free and adds both
+// halves up, dW as a second k segment, of the tile's pair.  Their bytes do: forward and
+// backward of 1 x 112 -> 39680 take 52.1 us, of 47.6 with one part, 16 x 256 -> 1024
+// 27.5 of 26.6, 8 x 1024 -> 65536 151 of 145.
+constexpr int64_t kTwoPartsDirect = 16, kTwoPartsTiles = 32;
 
 bool is_direct(const d3a_linear_xent_desc& d) {
   // (the vocabulary is a k axis of one product of four: 256 x 256 x 2048 in
@@ -363,7 +374,7 @@ struct DzEpi {
   const float *lse, *low;  // low: or null (0)
   const float* gloss;      // the rows' own, or null (one for all: a factor of the products)
   int64_t ignore, vocab;
-  __bf16* dz;                        // planes, rows of ld
+  __bf16 *dz, *second;               // planes, rows of ld; one plane's second part, or null
   int64_t ld, s_part;
   int32_t v0;
   float* db;                         // the waves' sums of their rows, [M / C::TM][quads of N][4], or null
@@ -407,6 +418,13 @@ struct DzEpi {
         for (int r = 0; r < 8; ++r) s[r] += v[r];
       }
       store_planes<NP>(dz + (int64_t)m * ld + n, s_part, v);
+      if constexpr (NP == 1)
+        if (second) {
+          float left[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) left[r] = left_of(v[r]);
+          store8(second + (int64_t)m * ld + n, left);
+        }
     });
     if (!db) return;
     // eight lanes have the same columns
@@ -506,7 +524,8 @@ int forward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_
 template <class T>
 int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stream, int64_t* bytes) {
   const int64_t R = d.rows, D = d.n_in, V = d.vocab, ld = round8(V);
-  T* dz = ws.take<T>(R * ld);
+  const bool two = sizeof(T) == 2 && R <= kTwoPartsDirect;
+  T* dz = ws.take<T>((two ? 2 : 1) * R * ld);
   *bytes = ws.used;
   if (dry) return 0;
   if (R > 0) {
@@ -514,12 +533,15 @@ int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream
     L.n = 1;
     L.p[0] = direct::problem(direct::operand<T>(d.x, d.ldx, 0, D), direct::operand<T>(d.W, d.ldW, 0, D), R, V, D, 1);
     L.e[0] = DirectDzEpi<T>{static_cast<const T*>(d.b), d.target, d.lse, d.low,
-                            d.reduction == 0 ? d.gloss : nullptr, d.ignore_index, V, dz, ld};
+                            d.reduction == 0 ? d.gloss : nullptr, d.ignore_index, V, dz,
+                            two ? dz + R * ld : nullptr, ld};
     if (direct::launch<false, false, false>(L, stream, "linear_cross_entropy_bwd") != 0) return -1;
     if (d.dx) {
       direct::Launch<T, direct::StoreEpi<T>> X{};
       X.n = 1;
-      X.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, V), direct::operand<T>(d.W, d.ldW, 0, V), R, D, V, 1);
+      X.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, V), direct::operand<T>(d.W, d.ldW, 0, V),
+                               two ? 2 * R : R, D, V, 1);
+      X.p[0].fold = two ? (int32_t)R : 0;
       X.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dx), D, 0, nullptr, 0, loss_factor(d)};
       if (direct::launch<false, true, false>(X, stream, "linear_cross_entropy_bwd") != 0) return -1;
     }
@@ -528,6 +550,11 @@ int backward_direct(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream
   direct::Launch<T, direct::StoreEpi<T>> W{};
   W.n = 1;
   W.p[0] = direct::problem(direct::operand<T>(dz, ld, 0, R), direct::operand<T>(d.x, d.ldx, 0, R), V, d.dW ? D : 1, R, 1);
+  if (two) {
+    W.p[0].n_inner = 2;
+    W.p[0].a.s_inner = R * ld;
+    W.p[0].b2 = W.p[0].b;
+  }
   W.p[0].rowsum = static_cast<T*>(d.db);
   W.p[0].sum_factor = loss_factor(d);
   W.e[0] = direct::StoreEpi<T>{static_cast<T*>(d.dW), D, 0, nullptr, 0, loss_factor(d)};
@@ -590,8 +617,9 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
   const int64_t piece = equal_parts(V, std::min(std::max<int64_t>(most, 256), kMaxWidth));
   const int64_t ld = round8(piece), block = equal_parts(R, kPieceBytes / (2 * NP * ld));
   const int64_t n_pieces = (V + piece - 1) / piece, n_blocks = R > 0 ? (R + block - 1) / block : 1;
+  const bool two = NP == 1 && R <= kTwoPartsTiles && n_pieces == 1;
   Operand dz{};
-  dz.p = ws.take<__bf16>(NP * block * ld);
+  dz.p = ws.take<__bf16>((two ? 2 : NP) * block * ld);
   dz.ld = ld;
   dz.s_part = block * ld;
   float* sum = n_pieces > 1 && d.dx ? ws.take<float>(R * round8(D)) : nullptr;
@@ -626,6 +654,7 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
       e.ignore = d.ignore_index;
       e.vocab = V;
       e.dz = const_cast<__bf16*>(dz.p);
+      e.second = two ? e.dz + block * ld : nullptr;
       e.ld = ld;
       e.s_part = dz.s_part;
       e.v0 = (int32_t)v0;
@@ -648,17 +677,19 @@ int backward(const d3a_linear_xent_desc& d, Arena ws, bool dry, hipStream_t stre
       Products<T, NP> dx, dw;
       if (d.dx) {
         T* out = static_cast<T*>(d.dx) + r0 * D;
-        dx.add(dz, p.b, m, D, n, 1, 1, 1, out, D, 0, nullptr, 0, by);
+        dx.add(dz, p.b, two ? 2 * m : m, D, n, 1, 1, 1, out, D, 0, nullptr, 0, by);
         if (n_pieces > 1) {
           dx.L.e[0].sum = sum + r0 * round8(D);
           dx.L.e[0].mode = v0 + n == V ? 4 : k == 0 ? 2 : 3;
         }
-        dx.reserve(ws, n_pieces == 1);
+        dx.reserve(ws, n_pieces == 1, two ? 2 : 1);
       }
       if (d.dW) {
         Operand xb = x;
         xb.p += r0 * x.ld;
-        dw.add(dz, xb, n, D, m, 1, 1, 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0, by);
+        Operand dzb = dz;
+        if (two) dzb.s_inner = block * ld;
+        dw.add(dzb, xb, n, D, m, 1, 1, two ? 2 : 1, static_cast<T*>(d.dW) + v0 * D, D, 0, nullptr, 0, by);
         if (n_blocks > 1) {
           dw.L.e[0].sum = sum_w;
           dw.L.e[0].mode = b + 1 == n_blocks ? 4 : b == 0 ? 2 : 3;

@@ -42,6 +42,16 @@ def run_xent(T, x, W, b, target, reduction, g, ignore=-100):
     return {"loss": loss} | dict(zip(q, grads))
 
 
+def rows_and_classes(R, D, V, dtype, pad=0.2):
+    g = torch.Generator(DEV).manual_seed(R + V)
+    x = torch.randn(R, D, device=DEV, generator=g).to(dtype)
+    W = (torch.randn(V, D, device=DEV, generator=g) * D ** -0.5).to(dtype)
+    b = torch.randn(V, device=DEV, generator=g).to(dtype)
+    t = torch.randint(0, V, (R,), device=DEV, generator=g)
+    t[torch.rand(R, device=DEV, generator=g) < pad] = -100
+    return x, W, b, t
+
+
 # ------------------------------------------------- logits that share a large value
 def common_inputs(V, dtype, common, step):
     """Logits of ``common`` plus whole multiples of ``step``, exact in float32: x
@@ -156,6 +166,31 @@ def test_few_rows_with_an_infinite_hidden_value(T):
     assert T.gated_mlp(x, W, W, Wd).isposinf().all()
 
 
+# ------------------------------------------------------------- cross entropy, few rows
+@pytest.mark.parametrize("R,D,V", [(1, 64, 2), (1, 64, 50), (1, 112, 39680), (3, 33, 77), (16, 40, 2000),
+                                   (1, 17, 2101), (9, 24, 5003), (17, 1030, 40), (32, 72, 4099)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_rows_gradients_are_rounded_once(T, R, D, V, reduction):
+    """bfloat16, up to 16 rows (32 where an axis is too long for the products from the
+    tensors): the gradients are float32's rounded to bfloat16, with dz held to 2^-16 in
+    between.  (One part would be 2^-8 off, an error that all of one row's W gradient
+    shares.)"""
+    x, W, b, t = rows_and_classes(R, D, V, BF16, pad=0.0)
+    W = (W.float() * 1.5).to(BF16)
+    g = rnd(9, R) if reduction == "none" else 0.7
+    got = run_xent(T, x, W, b, t, reduction, g)
+    # float32's bounds on the same values, dz's two parts, the results' rounding
+    ref = xent_reference(x.float(), W.float(), b.float(), t, -100, reduction, g)
+    z = x.double() @ W.double().t() + b.double()
+    d = torch.softmax(z, -1)
+    d[torch.arange(R, device=DEV), t] -= 1.0
+    d = d.abs() * (g.abs().double()[:, None] if reduction == "none" else 0.7 / R)
+    two = {"x": d @ W.double().abs(), "W": d.t() @ x.double().abs(), "b": d.sum(0)}
+    for k, s in two.items():
+        want, bound = ref[k]
+        within(got[k], want, bound + 2.0 ** -16 * s + 2.0 ** -8 * want.abs(), k)
+
+
 # --------------------------------------------------------------- float32's whole range
 def largest_inputs(R, D, N):
     """x whose first feature is float32's largest value, of either sign, times 2^-125
@@ -234,16 +269,6 @@ def test_layer_norm_of_more_columns_than_a_launch_has_threads(T):
 
 
 # ------------------------------------------- pieces of the vocabulary, blocks of the rows
-def rows_and_classes(R, D, V, dtype, pad=0.2):
-    g = torch.Generator(DEV).manual_seed(R + V)
-    x = torch.randn(R, D, device=DEV, generator=g).to(dtype)
-    W = (torch.randn(V, D, device=DEV, generator=g) * D ** -0.5).to(dtype)
-    b = torch.randn(V, device=DEV, generator=g).to(dtype)
-    t = torch.randint(0, V, (R,), device=DEV, generator=g)
-    t[torch.rand(R, device=DEV, generator=g) < pad] = -100
-    return x, W, b, t
-
-
 @pytest.mark.parametrize("R,D,V,dtype,reduction", [
     (33000, 24, 9000, BF16, "mean"),    # two pieces, sums of columns by a pass of their own
     (33000, 24, 9000, BF16, "none"),
